@@ -441,6 +441,126 @@ tvb_status tvb_gguf_tensor(const tvb_gguf* gguf, int i, tvb_cache_tensor* info, 
 tvb_status tvb_gguf_read(tvb_gguf* gguf, const char* name, void* dst, uint64_t capacity);
 tvb_status tvb_gguf_close(tvb_gguf* gguf);
 
+/* ---- serving over a paged KV cache ------------------------------------------
+ * Beyond the reference (one sequence, one merged adapter, a contiguous cache):
+ * the operators of a serving step whose sequences keep their keys and values in
+ * pages and whose requests bring their own LoRA adapters.  The contiguous
+ * counterparts are tvb_rope_inplace + tvb_kv_write, tvb_attention_decode and
+ * tvb_matmul.
+ *
+ * All buffers are device memory of the current device; lengths, tables and
+ * adapter ids are read on the device, so a captured call replays with new ones.
+ * What they hold is checked there: a sequence or token whose numbers are out of
+ * range is skipped (its output rows stay as they were) and a key on a page out
+ * of range is not read; `status` (optional device word, zeroed by the caller)
+ * then gets TVB_DEV_BAD_INPUT, and TVB_DEV_TIMEOUT when a bounded wait gave up.
+ * The calls take workspaces from a pool of this library, ordered on `stream`,
+ * so calls on different streams and captured graphs never share one. */
+#define TVB_DEV_TIMEOUT 1u
+#define TVB_DEV_BAD_INPUT 2u
+
+/* One layer's cache.  Element (page, row, head, d) is at page * page_stride +
+ * row * row_stride + head * head_stride + d, for k and for v alike, so
+ * [page][row][head][d], [page][head][row][d] and pools that interleave k with v
+ * or layers all fit.  Addresses and strides are multiples of 16 bytes. */
+typedef struct {
+    void* k;
+    void* v;
+    tvb_dtype dtype;       /* TVB_F32 or TVB_F16 */
+    int n_pages;
+    int page_size;         /* tokens a page, any number from 1 */
+    int64_t page_stride;   /* in elements */
+    int64_t row_stride;
+    int64_t head_stride;
+} tvb_kv_pages;
+
+/* The sequences of one call.  Rows cu_tokens[b] .. cu_tokens[b + 1] of the
+ * token buffers are the new tokens of sequence b; kv_len[b] is its length with
+ * them, so its row j is at position kv_len[b] - new + j.  Position t of
+ * sequence b lives in row t % page_size of page block_table[b * table_ld +
+ * t / page_size].  Rows from cu_tokens[n_seqs] on belong to nobody and are left
+ * alone. */
+typedef struct {
+    int n_seqs;
+    int n_tokens;            /* rows of the token buffers */
+    int max_new;             /* no sequence brings more new tokens */
+    int max_kv;              /* no sequence is longer */
+    const int* cu_tokens;    /* device [n_seqs + 1] */
+    const int* kv_len;       /* device [n_seqs] */
+    const int* block_table;  /* device [n_seqs][table_ld] */
+    int table_ld;            /* at least max_kv / page_size, rounded up */
+} tvb_paged_batch;
+
+/* Pairs that a rotary position turns together: (i, i + rot_dim / 2), as
+ * tvb_rope_inplace, or (2 i, 2 i + 1). */
+#define TVB_ROPE_HALF 0
+#define TVB_ROPE_INTERLEAVED 1
+/* Frequencies f_i = theta^(-2 i / rot_dim) for contexts `factor` times the
+ * original_len they were trained on: as they are; all divided by factor; by how
+ * many turns a pair makes within original_len (below low_turns divided, above
+ * high_turns kept, blended linearly in the turns between); a linear ramp over
+ * the pairs from the one of fast_turns (kept) to the one of slow_turns
+ * (divided), with cosine and sine times 0.1 ln(factor) + 1. */
+#define TVB_ROPE_PLAIN 0
+#define TVB_ROPE_LINEAR 1
+#define TVB_ROPE_BANDS 2
+#define TVB_ROPE_YARN 3
+
+typedef struct {
+    int rot_dim;          /* dimensions of each head that turn (the first ones), a multiple of 8 */
+    int pairs;            /* TVB_ROPE_HALF, TVB_ROPE_INTERLEAVED */
+    int scaling;          /* TVB_ROPE_PLAIN .. TVB_ROPE_YARN */
+    float theta;
+    float factor;         /* >= 1; the scalings other than TVB_ROPE_PLAIN */
+    int original_len;     /* TVB_ROPE_BANDS, TVB_ROPE_YARN */
+    float low_turns, high_turns;    /* TVB_ROPE_BANDS */
+    float fast_turns, slow_turns;   /* TVB_ROPE_YARN */
+} tvb_rope_config;
+
+/* Rotary positions and cache append of the new tokens: q [n_tokens][ldq]
+ * (n_heads heads of head_dim) rotated into q_out [n_tokens][ldqo] (q_out == q
+ * rotates in place), k [n_tokens][ldk] rotated and v [n_tokens][ldv] copied
+ * into the cache rows of their positions, rounded to its type.  Angles are
+ * reduced in 64 bits, so far positions lose nothing.  head_dim is a multiple of
+ * 8 up to 256; leading dimensions are multiples of 4 floats, buffers 16-byte
+ * aligned. */
+tvb_status tvb_rope_append_paged(float* q_out, int ldqo, const float* q, int ldq, const float* k, int ldk,
+                                 const float* v, int ldv, const tvb_kv_pages* kv, const tvb_paged_batch* batch,
+                                 const tvb_rope_config* rope, int n_heads, int n_kv_heads, int head_dim,
+                                 unsigned* status, void* stream);
+
+/* Attention of the new tokens over the cache (which holds them already): the
+ * token at position p sees keys t with t <= p and, with window > 0, t > p -
+ * window; query head h reads KV head h / (n_heads / n_kv_heads).  out
+ * [n_tokens][ldo] gets softmax(q . k * scale) . v, lse (optional)
+ * [n_tokens][n_heads] the natural logarithm of the sum of exponentials; a row
+ * that sees no key gets zeros and -infinity.  One token a sequence (decode) and
+ * long chunks alike; head_dim 64 or 128.  Values of keys that a row does not
+ * see never reach it, whatever they hold. */
+tvb_status tvb_attention_paged(float* out, int ldo, float* lse, const float* q, int ldq, const tvb_kv_pages* kv,
+                               const tvb_paged_batch* batch, int n_heads, int n_kv_heads, int head_dim, float scale,
+                               int window, unsigned* status, void* stream);
+
+/* The adapters of a projection, all arrays on the device: adapter i adds
+ * scale[i] * B_i (A_i x), A_i = A[i] [rank[i]][K], B_i = B[i] [N][rank[i]]
+ * (16-byte aligned), as tvb_merge_i2s_lora's lora_a and lora_b with scale =
+ * alpha / rank. */
+typedef struct {
+    int n;
+    int max_rank;            /* no rank is larger; at most 256 */
+    tvb_dtype dtype;         /* of A and B: TVB_F32 or TVB_F16 */
+    const void* const* A;    /* [n] */
+    const void* const* B;    /* [n] */
+    const int* rank;         /* [n] */
+    const float* scale;      /* [n] */
+} tvb_lora_table;
+
+/* tvb_matmul with an adapter for each row: y[m] = W x[m] + scale_a B_a A_a x[m],
+ * a = adapter[m] (device [M]; -1: none).  K is a multiple of 8 (16 for INT8
+ * weights), x and y rows are contiguous, x, W 16-byte aligned. */
+tvb_status tvb_matmul_lora(float* y, const float* x, int M, int K, const tvb_weight* w, int N,
+                           const tvb_lora_table* table, const int* adapter, unsigned* status, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -79,6 +79,29 @@ class SamplerConfig(C.Structure):
                 ("repetition_penalty", C.c_float)]
 
 
+class KvPages(C.Structure):
+    _fields_ = [("k", C.c_void_p), ("v", C.c_void_p), ("dtype", C.c_int), ("n_pages", C.c_int),
+                ("page_size", C.c_int), ("page_stride", C.c_int64), ("row_stride", C.c_int64),
+                ("head_stride", C.c_int64)]
+
+
+class PagedBatchDesc(C.Structure):
+    _fields_ = [("n_seqs", C.c_int), ("n_tokens", C.c_int), ("max_new", C.c_int), ("max_kv", C.c_int),
+                ("cu_tokens", C.c_void_p), ("kv_len", C.c_void_p), ("block_table", C.c_void_p),
+                ("table_ld", C.c_int)]
+
+
+class RopeDesc(C.Structure):
+    _fields_ = [("rot_dim", C.c_int), ("pairs", C.c_int), ("scaling", C.c_int), ("theta", C.c_float),
+                ("factor", C.c_float), ("original_len", C.c_int), ("low_turns", C.c_float),
+                ("high_turns", C.c_float), ("fast_turns", C.c_float), ("slow_turns", C.c_float)]
+
+
+class LoraTableDesc(C.Structure):
+    _fields_ = [("n", C.c_int), ("max_rank", C.c_int), ("dtype", C.c_int), ("A", C.c_void_p),
+                ("B", C.c_void_p), ("rank", C.c_void_p), ("scale", C.c_void_p)]
+
+
 class IpcHandle(C.Structure):
     _fields_ = [("bytes", C.c_ubyte * 64)]
 
@@ -149,6 +172,11 @@ _SIGS = {
     "tvb_gguf_read": [_P, C.c_char_p, _P, C.c_uint64],
     "tvb_gguf_close": [_P],
     "tvb_decode_batch": [_P, _P, _P, _I, _P, _P],
+    "tvb_rope_append_paged": [_P, _I, _P, _I, _P, _I, _P, _I, C.POINTER(KvPages), C.POINTER(PagedBatchDesc),
+                              C.POINTER(RopeDesc), _I, _I, _I, _P, _P],
+    "tvb_attention_paged": [_P, _I, _P, _P, _I, C.POINTER(KvPages), C.POINTER(PagedBatchDesc), _I, _I, _I, _F, _I,
+                            _P, _P],
+    "tvb_matmul_lora": [_P, _P, _I, _I, C.POINTER(Weight), _I, C.POINTER(LoraTableDesc), _P, _P, _P],
     "tvb_tp_init": [_P, _I, _I, C.POINTER(C.c_void_p)],
     "tvb_tp_set_peers": [_P, C.POINTER(C.c_void_p)],
     "tvb_ipc_export": [_P, C.POINTER(IpcHandle)],

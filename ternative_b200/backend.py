@@ -22,8 +22,8 @@ from typing import Optional, Sequence
 import numpy as np
 
 from . import _lib
-from ._lib import (TVB_F16, TVB_F32, TVB_I8_ROW, TVB_I8_TENSOR, Buffers, IpcHandle, LayerWeights,
-                   MergeDesc, ModelConfig, Weight, call, load)
+from ._lib import (TVB_F16, TVB_F32, TVB_I8_ROW, TVB_I8_TENSOR, Buffers, IpcHandle, KvPages, LayerWeights,
+                   LoraTableDesc, MergeDesc, ModelConfig, PagedBatchDesc, RopeDesc, Weight, call, load)
 
 
 def _ptr(x) -> Optional[int]:
@@ -73,6 +73,114 @@ class DeviceWeight:
 
     def to_c(self) -> Weight:
         return Weight(self.ptr, self.dtype, self.row_scales, self.tensor_scale)
+
+
+def _tensor(x, name: str, dtype: str, ndim: int):
+    """Checks a torch tensor argument: on the current device, of the type, its
+    last dimension contiguous."""
+    import torch
+    if not x.is_cuda or x.device.index != torch.cuda.current_device():
+        raise ValueError(f"{name} is on {x.device}, not on the current CUDA device")
+    if x.dtype is not getattr(torch, dtype) or x.dim() != ndim:
+        raise ValueError(f"{name}: want a {ndim}-D {dtype} tensor, got {x.dim()}-D {x.dtype}")
+    if x.numel() and x.stride(-1) != 1 and x.shape[-1] != 1:
+        raise ValueError(f"{name}: the last dimension must be contiguous")
+    return x
+
+
+def _heads(x, name: str, rows: int, heads: int, head_dim: int) -> int:
+    """Leading dimension of a token buffer: [rows][>= heads * head_dim] or
+    [rows][heads][head_dim], rows any distance apart."""
+    _tensor(x, name, "float32", x.dim() if x.dim() in (2, 3) else 2)
+    if x.dim() == 3 and (tuple(x.shape[1:]) != (heads, head_dim) or (heads > 1 and x.stride(1) != head_dim)):
+        raise ValueError(f"{name}: shape {tuple(x.shape)}, strides {x.stride()} for {heads} heads of {head_dim}")
+    if x.shape[0] < rows or (x.dim() == 2 and x.shape[1] < heads * head_dim):
+        raise ValueError(f"{name}: shape {tuple(x.shape)} for {rows} rows of {heads} heads of {head_dim}")
+    return x.stride(0) if x.shape[0] > 1 else heads * head_dim
+
+
+class PagedCache:
+    """One layer's paged KV cache (tvb_kv_pages) over two torch tensors of the
+    same type (float32, float16) and strides, indexed [page][row][head][dim];
+    for pools stored [page][head][row][dim] pass ``pool.transpose(1, 2)``."""
+
+    def __init__(self, k, v):
+        import torch
+        for name, x in (("k", k), ("v", v)):
+            if x.dtype not in (torch.float32, torch.float16):
+                raise ValueError(f"{name}: cache type {x.dtype} (float32 or float16)")
+            _tensor(x, name, str(x.dtype).split(".")[1], 4)
+        if k.dtype != v.dtype or k.shape != v.shape or k.stride() != v.stride():
+            raise ValueError("k and v must have the same type, shape and strides")
+        self.k, self.v = k, v
+        n_pages, page_size, self.n_kv_heads, self.head_dim = k.shape
+        ps, rs, hs, _ = k.stride()
+        self.desc = KvPages(k.data_ptr(), v.data_ptr(), TVB_F32 if k.dtype == torch.float32 else TVB_F16, n_pages,
+                            page_size, ps, rs, hs)
+
+
+class PagedBatch:
+    """The sequences of a call (tvb_paged_batch): int32 tensors cu_tokens
+    [n + 1], kv_len [n] (with the new tokens) and block_table [n][pages], and
+    the bounds that hold for them.  The tensors may be rewritten between calls."""
+
+    def __init__(self, cu_tokens, kv_len, block_table, n_tokens: int, max_new: int, max_kv: int):
+        _tensor(cu_tokens, "cu_tokens", "int32", 1)
+        _tensor(kv_len, "kv_len", "int32", 1)
+        _tensor(block_table, "block_table", "int32", 2)
+        n = kv_len.shape[0]
+        if cu_tokens.shape[0] != n + 1 or block_table.shape[0] != n:
+            raise ValueError(f"{n} lengths, {cu_tokens.shape[0]} row offsets, {block_table.shape[0]} tables")
+        self.tensors = (cu_tokens, kv_len, block_table)
+        self.n_tokens = n_tokens
+        self.desc = PagedBatchDesc(n, n_tokens, max_new, max_kv, cu_tokens.data_ptr(), kv_len.data_ptr(),
+                                   block_table.data_ptr(), block_table.stride(0) if n > 1 else block_table.shape[1])
+
+
+class RopeConfig:
+    """Rotary positions (tvb_rope_config): pairs "half" or "interleaved",
+    scaling "none", "linear", "bands" or "yarn"."""
+
+    def __init__(self, rot_dim: int, theta: float = 500000.0, pairs: str = "half", scaling: str = "none",
+                 factor: float = 1.0, original_len: int = 0, low_turns: float = 1.0, high_turns: float = 4.0,
+                 fast_turns: float = 32.0, slow_turns: float = 1.0):
+        kinds, scalings = ("half", "interleaved"), ("none", "linear", "bands", "yarn")
+        if pairs not in kinds or scaling not in scalings:
+            raise ValueError(f"pairs {pairs!r} (of {kinds}), scaling {scaling!r} (of {scalings})")
+        self.desc = RopeDesc(rot_dim, kinds.index(pairs), scalings.index(scaling), theta, factor, original_len,
+                             low_turns, high_turns, fast_turns, slow_turns)
+
+
+class LoraTable:
+    """The adapters of one projection (tvb_lora_table): A [rank][K] and B
+    [N][rank] of each, float32 or float16 alike, with their ranks (int32) and
+    scales alpha / rank (float32) as device tensors.  No rank is above max_rank."""
+
+    def __init__(self, A: Sequence, B: Sequence, rank, scale, max_rank: int):
+        import torch
+        if len(A) != len(B):
+            raise ValueError(f"{len(A)} A and {len(B)} B factors")
+        dtype = A[0].dtype if A else torch.float32
+        if dtype not in (torch.float32, torch.float16):
+            raise ValueError(f"adapter type {dtype} (float32 or float16)")
+        for i, (x, y) in enumerate(zip(A, B)):
+            for name, t in ((f"A[{i}]", x), (f"B[{i}]", y)):
+                _tensor(t, name, str(dtype).split(".")[1], 2)
+                if not t.is_contiguous():
+                    raise ValueError(f"{name} must be contiguous")
+            if x.shape[0] != y.shape[1] or x.shape[0] > max_rank or x.shape[1] != A[0].shape[1] or \
+                    y.shape[0] != B[0].shape[0]:
+                raise ValueError(f"adapter {i}: A {tuple(x.shape)}, B {tuple(y.shape)}, max_rank {max_rank}")
+        self.K = A[0].shape[1] if A else None
+        self.N = B[0].shape[0] if A else None
+        _tensor(rank, "rank", "int32", 1)
+        _tensor(scale, "scale", "float32", 1)
+        if rank.shape[0] != len(A) or scale.shape[0] != len(A):
+            raise ValueError(f"{len(A)} adapters, {rank.shape[0]} ranks, {scale.shape[0]} scales")
+        ptrs = [torch.tensor([t.data_ptr() for t in f], dtype=torch.int64, device=rank.device) for f in (A, B)]
+        self.tensors = (list(A), list(B), rank, scale, ptrs)   # kept alive with the descriptor
+        self.desc = LoraTableDesc(len(A), max_rank, TVB_F32 if dtype == torch.float32 else TVB_F16,
+                                  ptrs[0].data_ptr(), ptrs[1].data_ptr(), rank.data_ptr(), scale.data_ptr())
 
 
 class CUDABackend:
@@ -207,6 +315,49 @@ class CUDABackend:
         out = np.empty(n_floats, np.float32)
         call("tvb_kv_download_slot", self.ctx, layer, pos, n_floats, out.ctypes.data)
         return out
+
+    # ---- serving over a paged KV cache (no counterpart in the reference) --------
+    def rope_append_paged_d(self, d_q_out, d_q, d_k, d_v, cache: PagedCache, batch: PagedBatch, rope: RopeConfig,
+                            n_heads, n_kv_heads, head_dim, status=None, stream=None):
+        """Rotary positions of the new tokens and their append to the cache
+        (tvb_rope_append_paged).  Token buffers are float32 tensors [rows][heads *
+        head_dim] or [rows][heads][head_dim]; rows may be a slice of a wider buffer."""
+        if (cache.n_kv_heads, cache.head_dim) != (n_kv_heads, head_dim):
+            raise ValueError(f"a cache of {cache.n_kv_heads} heads of {cache.head_dim}")
+        T = batch.n_tokens
+        ld = [_heads(x, name, T, h, head_dim) for x, name, h in
+              ((d_q_out, "q_out", n_heads), (d_q, "q", n_heads), (d_k, "k", n_kv_heads), (d_v, "v", n_kv_heads))]
+        call("tvb_rope_append_paged", d_q_out.data_ptr(), ld[0], d_q.data_ptr(), ld[1], d_k.data_ptr(), ld[2],
+             d_v.data_ptr(), ld[3], cache.desc, batch.desc, rope.desc, n_heads, n_kv_heads, head_dim, _ptr(status),
+             self.stream if stream is None else stream)
+
+    def attention_paged_d(self, d_out, d_q, cache: PagedCache, batch: PagedBatch, n_heads, n_kv_heads, head_dim, scale,
+                          window=0, lse=None, status=None, stream=None):
+        """Causal attention of the new tokens over the cache (tvb_attention_paged),
+        window keys back at most when window > 0; lse: float32 [rows][n_heads]."""
+        if (cache.n_kv_heads, cache.head_dim) != (n_kv_heads, head_dim):
+            raise ValueError(f"a cache of {cache.n_kv_heads} heads of {cache.head_dim}")
+        T = batch.n_tokens
+        ldo, ldq = _heads(d_out, "out", T, n_heads, head_dim), _heads(d_q, "q", T, n_heads, head_dim)
+        if lse is not None:
+            _tensor(lse, "lse", "float32", 2)
+            if lse.shape[0] < T or lse.shape[1] != n_heads or not lse.is_contiguous():
+                raise ValueError(f"lse: shape {tuple(lse.shape)} for {T} rows of {n_heads} heads")
+        call("tvb_attention_paged", d_out.data_ptr(), ldo, _ptr(lse), d_q.data_ptr(), ldq, cache.desc, batch.desc,
+             n_heads, n_kv_heads, head_dim, scale, window, _ptr(status), self.stream if stream is None else stream)
+
+    def matmul_lora_d(self, d_y, d_x, M, K, weight: DeviceWeight, N, table: LoraTable, d_adapter, status=None,
+                      stream=None):
+        """y[m] = W x[m] + scale_a B_a A_a x[m], a = adapter[m] (int32, -1: none)
+        (tvb_matmul_lora)."""
+        for x, name, dtype, n in ((d_y, "y", "float32", M * N), (d_x, "x", "float32", M * K), (d_adapter, "adapter", "int32", M)):
+            _tensor(x, name, dtype, x.dim())
+            if x.numel() < n or not x.is_contiguous():
+                raise ValueError(f"{name}: want {n} contiguous values, got shape {tuple(x.shape)}")
+        if table.K is not None and (table.K, table.N) != (K, N):
+            raise ValueError(f"adapters of a projection {table.K} -> {table.N}, not {K} -> {N}")
+        call("tvb_matmul_lora", d_y.data_ptr(), d_x.data_ptr(), M, K, C.byref(weight.to_c()), N, table.desc,
+             d_adapter.data_ptr(), _ptr(status), self.stream if stream is None else stream)
 
     # ---- load-time merge (replaces apply_lora, src/model.cpp:205-258) ----------
     def apply_lora_i2s(self, i2s, scale, K, N, lora_a, lora_b, alpha, out_dtype, dst,

@@ -1,0 +1,455 @@
+// Attention of new tokens over the paged KV cache (tvb_attention_paged).
+//
+//   out = sum_t p_t v_t / sum_t p_t,  p_t = 2^(s_t - m),  s_t = scale log2(e) q . k_t
+//
+// over the keys t in (p - window, p] of the row's position p, in one pass: a
+// running maximum m per row, the sum and the weighted values rescaled by
+// 2^(m_old - m_new) when it grows.
+//
+// paged_rows_kernel: a CTA takes RB query rows of one KV head of one sequence
+// (rows: new token x query head of the group) and one split of the keys; its 8
+// warps take batches of 8 keys in turn and merge at the end.  K and V rows pass
+// through a ring of cp.async stages private to each warp, so no warp waits for
+// another while it streams; each lane owns head_dim / 32 dimensions.  The RB x 8
+// partial dot products of a batch are summed over the lanes by a butterfly that
+// halves the values it carries at each step (31 shuffles for 32 sums).  With
+// more than one split the partial results go to a workspace and
+// paged_merge_kernel joins them in split order.
+#include "attn_paged.h"
+
+#include <algorithm>
+
+namespace tvb {
+
+constexpr int kPrWarps = 8, kPrThreads = 32 * kPrWarps;
+constexpr int kPrKeys = 8;   // keys a batch
+constexpr int kPrMaxSplits = 64;
+
+__device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, bool valid) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(valid ? 16 : 0) : "memory");
+}
+__device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void cp_async_wait() {
+    asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+}
+__device__ __forceinline__ uint32_t pr_smem(const void* p) { return static_cast<uint32_t>(__cvta_generic_to_shared(p)); }
+
+template <typename T, int HD>
+struct PrStage {
+    static constexpr int kRow = HD * (int)sizeof(T);     // bytes of a key
+    static constexpr int kBytes = 2 * kPrKeys * kRow;    // K rows, then V rows
+    static constexpr int kStages = sizeof(T) == 2 ? 4 : 3;
+    static constexpr int kSmem = kPrWarps * kStages * kBytes;
+};
+
+// Sum over the lanes of v[0 .. NV): lane l returns the sum of v[l / (32 / NV)].
+template <int NV>
+__device__ __forceinline__ float pr_reduce(float (&v)[NV], int lane) {
+#pragma unroll
+    for (int n = NV, o = 16; o > 0; o >>= 1) {
+        if (n > 1) {
+            n >>= 1;
+            const bool up = lane & o;
+#pragma unroll
+            for (int i = 0; i < NV / 2; ++i) {
+                if (i < n) {
+                    const float keep = up ? v[i + n] : v[i], send = up ? v[i] : v[i + n];
+                    v[i] = keep + __shfl_xor_sync(0xffffffffu, send, o);
+                }
+            }
+        } else {
+            v[0] += __shfl_xor_sync(0xffffffffu, v[0], o);
+        }
+    }
+    return v[0];
+}
+
+template <typename T, int ND>
+__device__ __forceinline__ void pr_load(const unsigned char* p, float (&f)[ND]) {
+    if constexpr (sizeof(T) == 4) {
+        if constexpr (ND == 4) {
+            const float4 x = *reinterpret_cast<const float4*>(p);
+            f[0] = x.x, f[1] = x.y, f[2] = x.z, f[3] = x.w;
+        } else {
+            const float2 x = *reinterpret_cast<const float2*>(p);
+            f[0] = x.x, f[1] = x.y;
+        }
+    } else {
+        if constexpr (ND == 4) {
+            const uint2 u = *reinterpret_cast<const uint2*>(p);
+            const float2 x = __half22float2(*reinterpret_cast<const __half2*>(&u.x));
+            const float2 y = __half22float2(*reinterpret_cast<const __half2*>(&u.y));
+            f[0] = x.x, f[1] = x.y, f[2] = y.x, f[3] = y.y;
+        } else {
+            const float2 x = __half22float2(*reinterpret_cast<const __half2*>(p));
+            f[0] = x.x, f[1] = x.y;
+        }
+    }
+}
+
+// Sequence and first row of row block x, RB rows a block: block floor(cu[b] g /
+// RB) + b is the first of sequence b, so blocks of neighbours never overlap and
+// floor(T g / RB) + n of them are enough.  Whole CTA; b = n_seqs past the end.
+template <int RB, int NT>
+__device__ __forceinline__ int row_block_seq(const PagedSeqs& s, int group, int x, int* first) {
+    int started = 0;
+    for (int b0 = 0; b0 < s.n_seqs; b0 += NT) {
+        const int b = b0 + (int)threadIdx.x;
+        const bool at = b < s.n_seqs && (int)(((int64_t)__ldg(s.cu + b) * group) / RB) + b <= x;
+        const int n = __syncthreads_count(at);
+        started += n;
+        if (n < NT) break;
+    }
+    const int b = started - 1;
+    if (b < 0) return s.n_seqs;
+    *first = (x - (int)(((int64_t)__ldg(s.cu + b) * group) / RB) - b) * RB;
+    return b;
+}
+
+template <typename T, int HD, int RB>
+__global__ void __launch_bounds__(kPrThreads) paged_rows_kernel(const __grid_constant__ PagedAttnArgs a) {
+    using St = PrStage<T, HD>;
+    constexpr int ND = HD / 32;              // dimensions a lane
+    constexpr int RG = RB < 4 ? RB : 4;      // rows reduced together
+    constexpr int NG = RB / RG;
+    constexpr int NV = RG * kPrKeys;         // sums of one reduction
+    constexpr int LPV = 32 / NV;             // lanes that hold one
+    extern __shared__ __align__(128) unsigned char pr_smem_raw[];
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int kvh = blockIdx.y, split = blockIdx.z;
+
+    int row0 = 0;
+    const int b = row_block_seq<RB, kPrThreads>(a.s, a.group, blockIdx.x, &row0);
+    if (b >= a.s.n_seqs) return;
+    const SeqView sv = seq_view(a.s, b);
+    if (!sv.ok) {
+        if (threadIdx.x == 0) report_bad(a.status);
+        return;
+    }
+    const int rows = min(RB, sv.n * a.group - row0);
+    if (rows <= 0) return;
+    // keys that some row of the block sees, cut to this split
+    const int p_first = sv.pos0 + row0 / a.group, p_last = sv.pos0 + (row0 + rows - 1) / a.group;
+    const int lo = a.window ? max(0, p_first - a.window + 1) : 0;
+    const int k0 = a.nsplit > 1 ? max(lo, split * a.split_len) : lo;
+    const int k1 = a.nsplit > 1 ? min(p_last + 1, (split + 1) * a.split_len) : p_last + 1;
+    if (a.nsplit > 1 && k0 >= k1) return;   // no row of the block takes this split
+
+    // q (times scale log2 e) and positions of the rows
+    float q[RB][ND], acc[RB][ND];
+#pragma unroll
+    for (int r = 0; r < RB; ++r) {
+        const int row = row0 + min(r, rows - 1);
+        const int tok = sv.row0 + row / a.group, head = kvh * a.group + row % a.group;
+        pr_load<float, ND>(reinterpret_cast<const unsigned char*>(a.q + (size_t)tok * a.ldq + head * HD + lane * ND), q[r]);
+#pragma unroll
+        for (int d = 0; d < ND; ++d) q[r][d] *= a.scale2, acc[r][d] = 0.f;
+    }
+    // lane l keeps the score of row group g: row g RG + l / (8 LPV), key (l / LPV) % 8
+    const int lrow = lane / (kPrKeys * LPV), lkey = (lane / LPV) % kPrKeys;
+    int lpos[NG];
+    float m[NG], l[NG];
+#pragma unroll
+    for (int g = 0; g < NG; ++g) {
+        const int r = g * RG + lrow;
+        lpos[g] = r < rows ? sv.pos0 + (row0 + r) / a.group : -1;
+        m[g] = -INFINITY;
+        l[g] = 0.f;
+    }
+
+    unsigned char* ring = pr_smem_raw + warp * St::kStages * St::kBytes;
+    const unsigned char* kb = a.kv.k + (int64_t)kvh * a.kv.head_stride;
+    const unsigned char* vb = a.kv.v + (int64_t)kvh * a.kv.head_stride;
+    const int* table = a.s.table + (size_t)b * a.s.table_ld;
+    bool bad = false;
+
+    // one batch of keys [t, t + 8) into stage st; rows that no query row sees or
+    // whose page does not exist become zeros.  Returns which keys exist (bits).
+    auto request = [&](int t, int st) -> unsigned {
+        int64_t off = -1;
+        if (lane < kPrKeys && t + lane >= k0 && t + lane < k1) {
+            off = paged_offset(a.kv, table, t + lane);
+            bad |= off < 0;
+        }
+        const unsigned have = __ballot_sync(0xffffffffu, off >= 0) & ((1u << kPrKeys) - 1);
+        constexpr int kLanes = St::kRow / 16;        // lanes a row
+        constexpr int kRows = 32 / kLanes;           // rows a pass
+        const uint32_t dst = pr_smem(ring + st * St::kBytes) + lane * 16;
+#pragma unroll
+        for (int j = 0; j < kPrKeys / kRows; ++j) {
+            const int key = j * kRows + lane / kLanes;
+            const int64_t o = __shfl_sync(0xffffffffu, off, key);
+            const int64_t at = (o >= 0 ? o : 0) + (lane % kLanes) * 16;
+            cp_async16(dst + j * 512, kb + at, o >= 0);
+            cp_async16(dst + kPrKeys * St::kRow + j * 512, vb + at, o >= 0);
+        }
+        return have;
+    };
+
+    // batches warp, warp + 8, ... of the keys from k0 on
+    const int step = kPrWarps * kPrKeys;
+    int t = k0 + warp * kPrKeys, tn = t;
+    unsigned have[St::kStages];
+#pragma unroll
+    for (int i = 0; i < St::kStages - 1; ++i, tn += step) {
+        have[i] = tn < k1 ? request(tn, i) : 0u;
+        cp_async_commit();
+    }
+    while (t < k1) {
+#pragma unroll
+        for (int st = 0; st < St::kStages; ++st) {
+            if (t >= k1) break;
+            {
+                constexpr int kAhead = St::kStages - 1;
+                const int ns = (st + kAhead) % St::kStages;
+                __syncwarp();   // every lane is done with the stage that is filled now
+                have[ns] = tn < k1 ? request(tn, ns) : 0u;
+                cp_async_commit();
+                tn += step;
+            }
+            cp_async_wait<St::kStages - 1>();
+            __syncwarp();
+            const unsigned char* stage = ring + st * St::kBytes;
+            const unsigned hv = have[st];
+            float p[NG];
+#pragma unroll
+            for (int g = 0; g < NG; ++g) {
+                float v[NV];
+#pragma unroll
+                for (int key = 0; key < kPrKeys; ++key) {
+                    float kf[ND];
+                    pr_load<T, ND>(stage + key * St::kRow + lane * ND * (int)sizeof(T), kf);
+#pragma unroll
+                    for (int r = 0; r < RG; ++r) {
+                        float x = q[g * RG + r][0] * kf[0];
+#pragma unroll
+                        for (int d = 1; d < ND; ++d) x = fmaf(q[g * RG + r][d], kf[d], x);
+                        v[r * kPrKeys + key] = x;
+                    }
+                }
+                float s = pr_reduce<NV>(v, lane);
+                const int kt = t + lkey;
+                const bool seen = ((hv >> lkey) & 1u) && kt <= lpos[g] && (!a.window || kt > lpos[g] - a.window);
+                if (!seen) s = -INFINITY;
+                float mx = s;
+#pragma unroll
+                for (int o = 16; o > 0; o >>= 1)
+                    if (o >= LPV && o < kPrKeys * LPV) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
+                const float mn = fmaxf(m[g], mx);
+                const float corr = m[g] == mn ? 1.f : exp2f(m[g] - mn);   // m = -inf: 0
+                p[g] = s == -INFINITY ? 0.f : exp2f(s - mn);
+                l[g] = l[g] * corr + p[g];
+                if (__any_sync(0xffffffffu, corr != 1.f)) {
+#pragma unroll
+                    for (int r = 0; r < RG; ++r) {
+                        const float c = __shfl_sync(0xffffffffu, corr, r * kPrKeys * LPV);
+#pragma unroll
+                        for (int d = 0; d < ND; ++d) acc[g * RG + r][d] *= c;
+                    }
+                }
+                m[g] = mn;
+            }
+            // a key that some row does not see adds nothing to that row, even if its value is not finite
+            const bool whole = hv == (1u << kPrKeys) - 1 && t + kPrKeys - 1 <= p_first && (!a.window || t > p_last - a.window);
+#pragma unroll
+            for (int key = 0; key < kPrKeys; ++key) {
+                float vf[ND];
+                pr_load<T, ND>(stage + (kPrKeys + key) * St::kRow + lane * ND * (int)sizeof(T), vf);
+#pragma unroll
+                for (int r = 0; r < RB; ++r) {
+                    const float pr = __shfl_sync(0xffffffffu, p[r / RG], ((r % RG) * kPrKeys + key) * LPV);
+                    if (whole || pr != 0.f) {
+#pragma unroll
+                        for (int d = 0; d < ND; ++d) acc[r][d] = fmaf(pr, vf[d], acc[r][d]);
+                    }
+                }
+            }
+            t += step;
+        }
+    }
+    cp_async_wait<0>();
+    if (bad) report_bad(a.status);
+
+    // merge the warps: [warp][row][HD + 2] in the ring's memory
+    __syncthreads();
+    float* red = reinterpret_cast<float*>(pr_smem_raw);
+    constexpr int kW = HD + 2;
+#pragma unroll
+    for (int g = 0; g < NG; ++g) {
+        // sum over the row's lanes (each sum is held by LPV lanes)
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1)
+            if (o >= LPV && o < kPrKeys * LPV) l[g] += __shfl_xor_sync(0xffffffffu, l[g], o);
+        if (lane % (kPrKeys * LPV) == 0) {
+            float* w = red + (warp * RB + g * RG + lrow) * kW;
+            w[HD] = m[g];
+            w[HD + 1] = l[g];
+        }
+    }
+#pragma unroll
+    for (int r = 0; r < RB; ++r)
+#pragma unroll
+        for (int d = 0; d < ND; ++d) red[(warp * RB + r) * kW + lane * ND + d] = acc[r][d];
+    __syncthreads();
+    for (int r = warp; r < rows; r += kPrWarps) {
+        float M = -INFINITY;
+#pragma unroll
+        for (int w = 0; w < kPrWarps; ++w) M = fmaxf(M, red[(w * RB + r) * kW + HD]);
+        float L = 0.f, o[ND];
+#pragma unroll
+        for (int d = 0; d < ND; ++d) o[d] = 0.f;
+#pragma unroll
+        for (int w = 0; w < kPrWarps; ++w) {
+            const float* x = red + (w * RB + r) * kW;
+            const float c = x[HD] == -INFINITY ? 0.f : exp2f(x[HD] - M);
+            if (c != 0.f) {
+                L = fmaf(x[HD + 1], c, L);
+#pragma unroll
+                for (int d = 0; d < ND; ++d) o[d] = fmaf(x[lane * ND + d], c, o[d]);
+            }
+        }
+        const int row = row0 + r;
+        const int tok = sv.row0 + row / a.group, head = kvh * a.group + row % a.group;
+        if (a.nsplit > 1) {
+            float* pp = a.part + (((size_t)split * a.s.n_tokens + tok) * a.nh + head) * kW;
+            if (lane == 0) *reinterpret_cast<float2*>(pp) = make_float2(L, M);
+#pragma unroll
+            for (int d = 0; d < ND; ++d) pp[2 + lane * ND + d] = o[d];
+        } else {
+            const float inv = L > 0.f ? 1.0f / L : (L == 0.f ? 0.f : L);
+            float* po = a.out + (size_t)tok * a.ldo + head * HD + lane * ND;
+#pragma unroll
+            for (int d = 0; d < ND; ++d) po[d] = o[d] * inv;
+            if (a.lse && lane == 0)
+                a.lse[(size_t)tok * a.nh + head] = L == 0.f ? -INFINITY : (M + log2f(L)) * 0.69314718055994531f;
+        }
+    }
+}
+
+// One warp a (token, head): the partials of the splits that its keys touch,
+// joined in split order.
+template <int HD>
+__global__ void __launch_bounds__(128) paged_merge_kernel(const __grid_constant__ PagedAttnArgs a) {
+    constexpr int ND = HD / 32, kW = HD + 2;
+    const int tok = blockIdx.x, lane = threadIdx.x & 31;
+    int ended = 0;
+    for (int b0 = 0; b0 < a.s.n_seqs; b0 += 128) {
+        const int b = b0 + (int)threadIdx.x;
+        const int n = __syncthreads_count(b < a.s.n_seqs && __ldg(a.s.cu + b + 1) <= tok);
+        ended += n;
+        if (n < 128) break;
+    }
+    if (ended >= a.s.n_seqs) return;
+    const SeqView sv = seq_view(a.s, ended);
+    if (!sv.ok || tok < sv.row0) return;
+    const int pos = sv.pos0 + tok - sv.row0;
+    const int first = (a.window ? max(0, pos - a.window + 1) : 0) / a.split_len, last = pos / a.split_len;
+    pdl_wait();
+    for (int h = blockIdx.y * 4 + (threadIdx.x >> 5); h < a.nh; h += gridDim.y * 4) {
+        const float* base = a.part + ((size_t)tok * a.nh + h) * kW;
+        const size_t stride = (size_t)a.s.n_tokens * a.nh * kW;
+        float M = -INFINITY;
+        for (int sp = first + lane; sp <= last; sp += 32) M = fmaxf(M, base[sp * stride + 1]);
+        M = warp_max(M);
+        float L = 0.f, o[ND];
+#pragma unroll
+        for (int d = 0; d < ND; ++d) o[d] = 0.f;
+        for (int sp = first; sp <= last; ++sp) {
+            const float* x = base + sp * stride;
+            const float2 lm = *reinterpret_cast<const float2*>(x);
+            const float c = lm.y == -INFINITY ? 0.f : exp2f(lm.y - M);
+            if (c != 0.f) {
+                L = fmaf(lm.x, c, L);
+#pragma unroll
+                for (int d = 0; d < ND; ++d) o[d] = fmaf(x[2 + lane * ND + d], c, o[d]);
+            }
+        }
+        const float inv = L > 0.f ? 1.0f / L : (L == 0.f ? 0.f : L);
+        float* po = a.out + (size_t)tok * a.ldo + h * HD + lane * ND;
+#pragma unroll
+        for (int d = 0; d < ND; ++d) po[d] = o[d] * inv;
+        if (a.lse && lane == 0) a.lse[(size_t)tok * a.nh + h] = L == 0.f ? -INFINITY : (M + log2f(L)) * 0.69314718055994531f;
+    }
+}
+
+template <typename T, int HD, int RB>
+static tvb_status launch_rows(const PagedAttnArgs& a, cudaStream_t st) {
+    static int set[kMaxDevices];
+    constexpr int smem = PrStage<T, HD>::kSmem > kPrWarps * RB * (HD + 2) * 4 ? PrStage<T, HD>::kSmem
+                                                                            : kPrWarps * RB * (HD + 2) * 4;
+    TVB_TRY(allow_smem(reinterpret_cast<const void*>(paged_rows_kernel<T, HD, RB>), smem, set));
+    const int64_t blocks = ((int64_t)a.s.n_tokens * a.group) / RB + a.s.n_seqs;
+    paged_rows_kernel<T, HD, RB><<<dim3((unsigned)blocks, (unsigned)a.nkv, (unsigned)a.nsplit), kPrThreads, smem, st>>>(a);
+    return check_launch("paged_rows_kernel");
+}
+
+template <typename T, int HD>
+static tvb_status launch_rows_rb(const PagedAttnArgs& a, int rows, cudaStream_t st) {
+    if (rows <= 1) return launch_rows<T, HD, 1>(a, st);
+    if (rows <= 2) return launch_rows<T, HD, 2>(a, st);
+    if (rows <= 4) return launch_rows<T, HD, 4>(a, st);
+    return launch_rows<T, HD, 8>(a, st);
+}
+
+}  // namespace tvb
+
+extern "C" tvb_status tvb_attention_paged(float* out, int ldo, float* lse, const float* q, int ldq,
+                                          const tvb_kv_pages* kv, const tvb_paged_batch* batch, int nh, int nkv, int hd,
+                                          float scale, int window, unsigned* status, void* stream) {
+    using namespace tvb;
+    TVB_REQUIRE(hd == 64 || hd == 128, "attention_paged: head_dim %d (64 and 128 are built)", hd);
+    TVB_REQUIRE(nh > 0 && nkv > 0 && nh % nkv == 0 && nh <= 65535, "attention_paged: heads %d / kv heads %d", nh, nkv);
+    PagedAttnArgs a = {};
+    TVB_TRY(paged_cache_arg("attention_paged", kv, nkv, hd, &a.kv));
+    TVB_TRY(paged_batch_arg("attention_paged", batch, kv, &a.s));
+    if (!a.s.n_tokens || !a.s.n_seqs || !a.s.max_new) return TVB_OK;   // an empty buffer may have no address
+    TVB_REQUIRE(out && q, "attention_paged: null pointer");
+    TVB_REQUIRE(ldq >= nh * hd && ldo >= nh * hd && ((ldq | ldo) & 3) == 0, "attention_paged: leading dimensions %d, %d",
+                ldq, ldo);
+    TVB_REQUIRE(((reinterpret_cast<uintptr_t>(q) | reinterpret_cast<uintptr_t>(out)) & 15) == 0,
+                "attention_paged: q and out must be 16-byte aligned");
+    TVB_REQUIRE(window >= 0, "attention_paged: window %d", window);
+    TVB_REQUIRE(scale == scale, "attention_paged: scale is NaN");
+    a.q = q;
+    a.out = out;
+    a.lse = lse;
+    a.ldq = ldq;
+    a.ldo = ldo;
+    a.nh = nh;
+    a.nkv = nkv;
+    a.group = nh / nkv;
+    a.scale2 = scale * 1.4426950408889634f;
+    a.window = window;
+    a.status = status;
+    const cudaStream_t st = as_stream(stream);
+    const int rows = std::min(a.s.max_new, a.s.n_tokens) * a.group;
+    const int rb = rows >= 5 ? 8 : rows >= 3 ? 4 : rows;
+    // Splits: enough CTAs for two waves, at least 256 keys each.
+    const int64_t blocks = (((int64_t)a.s.n_tokens * a.group) / rb + a.s.n_seqs) * nkv;
+    const int span = window ? (int)std::min<int64_t>(a.s.max_kv, (int64_t)window + a.s.max_new) : a.s.max_kv;
+    int want = (int)std::min<int64_t>(std::max<int64_t>(1, 2 * num_sms() / blocks), std::max(1, span / 256));
+    want = std::min(want, kPrMaxSplits);
+    a.split_len = ((a.s.max_kv + want - 1) / want + 63) / 64 * 64;
+    if (window && want > 1) a.split_len = ((span + want - 1) / want + 63) / 64 * 64;
+    if (a.split_len < 64) a.split_len = 64;
+    a.nsplit = want > 1 ? (a.s.max_kv + a.split_len - 1) / a.split_len : 1;
+    Workspace ws(st);
+    if (a.nsplit > 1) {
+        TVB_TRY(ws.get((size_t)a.nsplit * a.s.n_tokens * nh * (hd + 2) * 4));
+        a.part = ws.at<float>();
+    }
+    const bool f16 = kv->dtype == TVB_F16;
+    if (hd == 128) {
+        TVB_TRY((f16 ? launch_rows_rb<__half, 128>(a, rows, st) : launch_rows_rb<float, 128>(a, rows, st)));
+    } else {
+        TVB_TRY((f16 ? launch_rows_rb<__half, 64>(a, rows, st) : launch_rows_rb<float, 64>(a, rows, st)));
+    }
+    if (a.nsplit > 1) {
+        const dim3 grid((unsigned)a.s.n_tokens, (unsigned)((nh + 3) / 4));
+        if (hd == 128) paged_merge_kernel<128><<<grid, 128, 0, st>>>(a);
+        else paged_merge_kernel<64><<<grid, 128, 0, st>>>(a);
+        TVB_TRY(check_launch("paged_merge_kernel"));
+    }
+    return TVB_OK;
+}

@@ -1,0 +1,99 @@
+// The paged KV cache and the ragged batch of a serving step, as the device
+// reads them (tvb_kv_pages, tvb_paged_batch), and stream-ordered workspaces.
+#pragma once
+
+#include "common.cuh"
+
+namespace tvb {
+
+// n / d and n % d for 0 <= n < 2^31 by one high multiplication: with s =
+// ceil(log2 d) and m = floor(2^32 (2^s - d) / d) + 1, n / d = (mulhi(n, m) + n)
+// >> s (Granlund and Montgomery's round-up method; the sum stays below 2^32).
+struct FastDiv {
+    uint32_t d, m, s;
+    FastDiv() = default;
+    explicit FastDiv(uint32_t div) : d(div), s(0) {
+        while ((1ull << s) < div) ++s;
+        m = (uint32_t)(((1ull << 32) * ((1ull << s) - div)) / div + 1);
+    }
+    __device__ __forceinline__ uint32_t div(uint32_t n) const { return (__umulhi(n, m) + n) >> s; }
+};
+
+struct PagedKV {
+    unsigned char* k;
+    unsigned char* v;
+    int64_t page_stride, row_stride, head_stride;   // bytes
+    int n_pages;
+    FastDiv page;   // page size
+};
+
+struct PagedSeqs {
+    const int* cu;
+    const int* kv_len;
+    const int* table;
+    int n_seqs, n_tokens, max_new, max_kv, table_ld;
+};
+
+// Bytes from the start of a pool to (position t, head 0) of the sequence whose
+// table row is `table`; -1 where the page does not exist.
+__device__ __forceinline__ int64_t paged_offset(const PagedKV& kv, const int* table, int t) {
+    const uint32_t p = kv.page.div((uint32_t)t);
+    const int page = __ldg(table + p);
+    if ((unsigned)page >= (unsigned)kv.n_pages) return -1;
+    return (int64_t)page * kv.page_stride + (int64_t)((uint32_t)t - p * kv.page.d) * kv.row_stride;
+}
+
+// One sequence of the batch: rows [row0, row0 + n) of the token buffers at
+// positions pos0 ... of a cache of kv tokens.
+struct SeqView {
+    int row0, n, kv, pos0;
+    bool ok;
+};
+
+__device__ __forceinline__ SeqView seq_view(const PagedSeqs& s, int b) {
+    SeqView v;
+    v.row0 = __ldg(s.cu + b);
+    const int end = __ldg(s.cu + b + 1);
+    v.n = end - v.row0;
+    v.kv = __ldg(s.kv_len + b);
+    v.pos0 = v.kv - v.n;
+    v.ok = v.row0 >= 0 && end <= s.n_tokens && v.n >= 0 && v.n <= s.max_new && v.kv <= s.max_kv && v.pos0 >= 0;
+    return v;
+}
+
+__device__ __forceinline__ void report_bad(unsigned* status) {
+    if (status) atomicOr(status, TVB_DEV_BAD_INPUT);
+}
+
+// Host checks and conversion of the descriptors (paged.cu).
+tvb_status paged_cache_arg(const char* who, const tvb_kv_pages* kv, int n_kv_heads, int head_dim, PagedKV* out);
+tvb_status paged_batch_arg(const char* who, const tvb_paged_batch* b, const tvb_kv_pages* kv, PagedSeqs* out);
+
+// A workspace of this call on `st`, from a pool of the library that keeps its
+// memory between calls (the driver orders reuse across streams; inside a
+// capture it becomes the graph's own).  Freed on `st` when it goes out of scope,
+// after the kernels launched until then.
+class Workspace {
+  public:
+    explicit Workspace(cudaStream_t st) : st_(st) {}
+    ~Workspace() {
+        if (p_) cudaFreeAsync(p_, st_);
+    }
+    Workspace(const Workspace&) = delete;
+    Workspace& operator=(const Workspace&) = delete;
+    tvb_status get(size_t bytes);
+    template <class T>
+    T* at(size_t offset = 0) const {
+        return reinterpret_cast<T*>(static_cast<unsigned char*>(p_) + offset);
+    }
+
+  private:
+    cudaStream_t st_;
+    void* p_ = nullptr;
+};
+
+// Raises a kernel's dynamic shared memory limit once per device.
+constexpr int kMaxDevices = 64;
+tvb_status allow_smem(const void* kernel, int bytes, int (&set)[kMaxDevices]);
+
+}  // namespace tvb

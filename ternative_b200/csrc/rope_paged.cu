@@ -1,0 +1,234 @@
+// Rotary positions of a serving step's new tokens with the append to the paged
+// cache (tvb_rope_append_paged).
+//
+//   (a, b) -> m (a cos t - b sin t, b cos t + a sin t),   t = pos f_i
+//
+// for the pairs i of each head's first rot_dim dimensions, f_i = theta^(-2 i /
+// rot_dim) scaled for long contexts.  The host turns f_i into turns a position
+// (f_i / 2 pi, 64 bits); the kernel multiplies by the position, takes the
+// fraction of a turn in [-1/2, 1/2] in 64 bits and only then goes to 32, so the
+// angle's error is 2 pi 2^-26 at any position (an F32 angle at position 30,000
+// is off by 1e-3).
+//
+// Memory bound: q is read and written once, k and v are read once and written
+// in the cache's type.  A CTA takes a few tokens: their cosines and sines go to
+// shared memory once (all heads share them), then every thread moves items of 8
+// dimensions as two float4.
+#include <cmath>
+
+#include "paged.cuh"
+
+namespace tvb {
+
+constexpr int kRpThreads = 256;
+constexpr int kRpMaxPairs = 128;
+constexpr int kRpTokens = 4;   // tokens a CTA, at most
+
+struct RopeArgs {
+    const float *q, *k, *v;
+    float* q_out;
+    int ldq, ldk, ldv, ldqo;
+    int nh, nkv, hd;
+    int rot, interleaved;
+    int tokens;      // a CTA
+    int f16;         // cache type
+    float m;
+    unsigned* status;
+    PagedKV kv;
+    PagedSeqs s;
+    double turns[kRpMaxPairs];   // f_i / 2 pi
+};
+
+__device__ __forceinline__ void rp_store(unsigned char* p, int elem, float4 x, bool f16) {
+    if (f16) {
+        const __half2 a = __floats2half2_rn(x.x, x.y), b = __floats2half2_rn(x.z, x.w);   // the cache's rounding
+        uint2 u;
+        u.x = *reinterpret_cast<const uint32_t*>(&a);
+        u.y = *reinterpret_cast<const uint32_t*>(&b);
+        *reinterpret_cast<uint2*>(p + elem * 2) = u;
+    } else {
+        *reinterpret_cast<float4*>(p + elem * 4) = x;
+    }
+}
+
+__global__ void __launch_bounds__(kRpThreads) rope_append_kernel(const __grid_constant__ RopeArgs a) {
+    __shared__ float2 cs[kRpTokens][kRpMaxPairs];
+    __shared__ int64_t s_off[kRpTokens];   // the token's cache row; -1: skipped
+    __shared__ int s_pos[kRpTokens];
+    const int tid = threadIdx.x;
+    const int t0 = blockIdx.x * a.tokens;
+    const int nt = min(a.tokens, a.s.n_tokens - t0);
+
+    // sequence of each token: how many sequences end at or before it
+    for (int j = 0; j < nt; ++j) {
+        int ended = 0;
+        for (int b0 = 0; b0 < a.s.n_seqs; b0 += kRpThreads) {
+            const int b = b0 + tid;
+            const int n = __syncthreads_count(b < a.s.n_seqs && __ldg(a.s.cu + b + 1) <= t0 + j);
+            ended += n;
+            if (n < kRpThreads) break;
+        }
+        if (tid == 0) {
+            int64_t off = -1;
+            int pos = 0;
+            if (ended < a.s.n_seqs) {   // else: behind the last sequence
+                const SeqView v = seq_view(a.s, ended);
+                pos = v.pos0 + (t0 + j - v.row0);
+                if (v.ok && t0 + j >= v.row0) off = paged_offset(a.kv, a.s.table + (size_t)ended * a.s.table_ld, pos);
+                if (off < 0) report_bad(a.status);
+            }
+            s_off[j] = off;
+            s_pos[j] = pos;
+        }
+    }
+    __syncthreads();
+    const int pairs = a.rot >> 1;
+    for (int i = tid; i < nt * pairs; i += kRpThreads) {
+        const int j = i / pairs, p = i - j * pairs;
+        const double x = (double)s_pos[j] * a.turns[p];
+        float sn, c;
+        sincospif(2.0f * (float)(x - rint(x)), &sn, &c);
+        cs[j][p] = make_float2(c * a.m, sn * a.m);
+    }
+    __syncthreads();
+
+    const int per_head = a.hd >> 3;
+    const int items = (a.nh + 2 * a.nkv) * per_head;
+    for (int i = blockIdx.y * kRpThreads + tid; i < nt * items; i += gridDim.y * kRpThreads) {
+        const int j = i / items, it = i - j * items;
+        const int64_t off = s_off[j];
+        if (off < 0) continue;
+        const int h = it / per_head, c = it - h * per_head;
+        const int row = t0 + j;
+        const bool is_q = h < a.nh, is_k = !is_q && h < a.nh + a.nkv;
+        const bool turn = !(!is_q && !is_k) && c < (a.rot >> 3);
+        const int o0 = turn && !a.interleaved ? 4 * c : 8 * c;
+        const int o1 = turn && !a.interleaved ? 4 * c + (a.rot >> 1) : 8 * c + 4;
+        const int kvh = is_q ? 0 : h - a.nh - (is_k ? 0 : a.nkv);
+        const float* src = is_q ? a.q + (size_t)row * a.ldq + h * a.hd
+                                : (is_k ? a.k + (size_t)row * a.ldk : a.v + (size_t)row * a.ldv) + kvh * a.hd;
+        float4 x = *reinterpret_cast<const float4*>(src + o0);
+        float4 y = *reinterpret_cast<const float4*>(src + o1);
+        if (turn) {
+            const float4 p = *reinterpret_cast<const float4*>(&cs[j][4 * c]);
+            const float4 r = *reinterpret_cast<const float4*>(&cs[j][4 * c + 2]);
+            // cosines p.x p.z r.x r.z, sines p.y p.w r.y r.w of pairs 4c .. 4c + 3
+            if (a.interleaved) {
+                x = make_float4(x.x * p.x - x.y * p.y, x.y * p.x + x.x * p.y, x.z * p.z - x.w * p.w,
+                                x.w * p.z + x.z * p.w);
+                y = make_float4(y.x * r.x - y.y * r.y, y.y * r.x + y.x * r.y, y.z * r.z - y.w * r.w,
+                                y.w * r.z + y.z * r.w);
+            } else {
+                const float4 u = x, w = y;
+                x = make_float4(u.x * p.x - w.x * p.y, u.y * p.z - w.y * p.w, u.z * r.x - w.z * r.y,
+                                u.w * r.z - w.w * r.w);
+                y = make_float4(w.x * p.x + u.x * p.y, w.y * p.z + u.y * p.w, w.z * r.x + u.z * r.y,
+                                w.w * r.z + u.w * r.w);
+            }
+        }
+        if (is_q) {
+            float* dst = a.q_out + (size_t)row * a.ldqo + h * a.hd;
+            *reinterpret_cast<float4*>(dst + o0) = x;
+            *reinterpret_cast<float4*>(dst + o1) = y;
+        } else {
+            unsigned char* dst = (is_k ? a.kv.k : a.kv.v) + off + (int64_t)kvh * a.kv.head_stride;
+            rp_store(dst, o0, x, a.f16);
+            rp_store(dst, o1, y, a.f16);
+        }
+    }
+}
+
+// f_i / 2 pi of every pair, and the factor of cosine and sine.
+static void rope_turns(const tvb_rope_config& r, double* turns, float* m) {
+    const double two_pi = 6.283185307179586476925287;
+    const double ln = std::log((double)r.theta);
+    const double step = std::exp(-2.0 * ln / r.rot_dim);
+    const int pairs = r.rot_dim / 2;
+    *m = 1.0f;
+    double lo = 0.0, width = 1.0;
+    if (r.scaling == TVB_ROPE_YARN) {
+        auto pair = [&](double t) { return r.rot_dim * std::log(r.original_len / (t * two_pi)) / (2.0 * ln); };
+        lo = std::fmax(std::floor(pair(r.fast_turns)), 0.0);
+        width = std::fmax(std::fmin(std::ceil(pair(r.slow_turns)), r.rot_dim - 1.0) - lo, 1e-3);
+        *m = (float)(0.1 * std::log((double)r.factor) + 1.0);
+    }
+    double f = 1.0;
+    for (int i = 0; i < pairs; ++i, f *= step) {
+        double keep = 1.0;   // share of f that is not divided by factor
+        if (r.scaling == TVB_ROPE_LINEAR) {
+            keep = 0.0;
+        } else if (r.scaling == TVB_ROPE_BANDS) {
+            const double t = r.original_len * f / two_pi;
+            keep = std::fmin(std::fmax((t - r.low_turns) / ((double)r.high_turns - r.low_turns), 0.0), 1.0);
+        } else if (r.scaling == TVB_ROPE_YARN) {
+            keep = 1.0 - std::fmin(std::fmax((i - lo) / width, 0.0), 1.0);
+        }
+        turns[i] = (f * keep + (keep < 1.0 ? f / r.factor * (1.0 - keep) : 0.0)) / two_pi;
+    }
+}
+
+}  // namespace tvb
+
+extern "C" tvb_status tvb_rope_append_paged(float* q_out, int ldqo, const float* q, int ldq, const float* k, int ldk,
+                                            const float* v, int ldv, const tvb_kv_pages* kv,
+                                            const tvb_paged_batch* batch, const tvb_rope_config* rope, int nh, int nkv,
+                                            int hd, unsigned* status, void* stream) {
+    using namespace tvb;
+    TVB_REQUIRE(rope, "rope_append_paged: null pointer");
+    TVB_REQUIRE(nh > 0 && nkv > 0 && hd > 0 && hd % 8 == 0 && hd <= 2 * kRpMaxPairs,
+                "rope_append_paged: heads %d/%d, head_dim %d (a multiple of 8 up to %d)", nh, nkv, hd, 2 * kRpMaxPairs);
+    TVB_REQUIRE(nh <= 65536 && nkv <= 65536, "rope_append_paged: heads %d/%d", nh, nkv);
+    RopeArgs a;
+    TVB_TRY(paged_cache_arg("rope_append_paged", kv, nkv, hd, &a.kv));
+    TVB_TRY(paged_batch_arg("rope_append_paged", batch, kv, &a.s));
+    if (!a.s.n_tokens || !a.s.n_seqs) return TVB_OK;   // an empty buffer may have no address
+    TVB_REQUIRE(q_out && q && k && v, "rope_append_paged: null pointer");
+    TVB_REQUIRE(ldq >= nh * hd && ldqo >= nh * hd && ldk >= nkv * hd && ldv >= nkv * hd &&
+                    ((ldq | ldqo | ldk | ldv) & 3) == 0,
+                "rope_append_paged: leading dimensions %d, %d, %d, %d", ldqo, ldq, ldk, ldv);
+    TVB_REQUIRE(q_out != q || ldqo == ldq, "rope_append_paged: in place with leading dimensions %d and %d", ldqo, ldq);
+    TVB_REQUIRE(((reinterpret_cast<uintptr_t>(q_out) | reinterpret_cast<uintptr_t>(q) | reinterpret_cast<uintptr_t>(k) |
+                  reinterpret_cast<uintptr_t>(v)) & 15) == 0,
+                "rope_append_paged: buffers must be 16-byte aligned");
+    TVB_REQUIRE(rope->rot_dim >= 0 && rope->rot_dim <= hd && rope->rot_dim % 8 == 0,
+                "rope_append_paged: rot_dim %d (a multiple of 8 up to head_dim %d)", rope->rot_dim, hd);
+    TVB_REQUIRE(rope->pairs == TVB_ROPE_HALF || rope->pairs == TVB_ROPE_INTERLEAVED, "rope_append_paged: pairs %d",
+                rope->pairs);
+    TVB_REQUIRE(rope->scaling >= TVB_ROPE_PLAIN && rope->scaling <= TVB_ROPE_YARN, "rope_append_paged: scaling %d",
+                rope->scaling);
+    TVB_REQUIRE(rope->theta > 1.0f && std::isfinite(rope->theta), "rope_append_paged: theta %g", rope->theta);
+    if (rope->scaling != TVB_ROPE_PLAIN)
+        TVB_REQUIRE(rope->factor >= 1.0f && std::isfinite(rope->factor), "rope_append_paged: factor %g", rope->factor);
+    if (rope->scaling == TVB_ROPE_BANDS)
+        TVB_REQUIRE(rope->original_len > 0 && rope->low_turns > 0.0f && rope->high_turns > rope->low_turns,
+                    "rope_append_paged: original_len %d, turns %g..%g", rope->original_len, rope->low_turns,
+                    rope->high_turns);
+    if (rope->scaling == TVB_ROPE_YARN)
+        TVB_REQUIRE(rope->original_len > 0 && rope->slow_turns > 0.0f && rope->fast_turns > rope->slow_turns,
+                    "rope_append_paged: original_len %d, turns %g..%g", rope->original_len, rope->slow_turns,
+                    rope->fast_turns);
+    a.q = q;
+    a.k = k;
+    a.v = v;
+    a.q_out = q_out;
+    a.ldq = ldq;
+    a.ldk = ldk;
+    a.ldv = ldv;
+    a.ldqo = ldqo;
+    a.nh = nh;
+    a.nkv = nkv;
+    a.hd = hd;
+    a.rot = rope->rot_dim;
+    a.interleaved = rope->pairs == TVB_ROPE_INTERLEAVED;
+    a.f16 = kv->dtype == TVB_F16;
+    a.status = status;
+    a.m = 1.0f;
+    if (a.rot) rope_turns(*rope, a.turns, &a.m);
+    const int T = a.s.n_tokens;
+    const int items = (nh + 2 * nkv) * (hd / 8);
+    a.tokens = 1;
+    const dim3 grid((unsigned)((T + a.tokens - 1) / a.tokens), 1);
+    (void)items;
+    rope_append_kernel<<<grid, kRpThreads, 0, as_stream(stream)>>>(a);
+    return check_launch("rope_append_kernel");
+}
