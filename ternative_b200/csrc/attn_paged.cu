@@ -24,6 +24,7 @@ namespace tvb {
 constexpr int kPrWarps = 8, kPrThreads = 32 * kPrWarps;
 constexpr int kPrKeys = 8;   // keys a batch
 constexpr int kPrMaxSplits = 64;
+constexpr int kTensorRows = 32;   // rows of a KV head from which F16 caches take the tensor cores
 
 __device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, bool valid) {
     asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(valid ? 16 : 0) : "memory");
@@ -63,48 +64,6 @@ __device__ __forceinline__ float pr_reduce(float (&v)[NV], int lane) {
         }
     }
     return v[0];
-}
-
-template <typename T, int ND>
-__device__ __forceinline__ void pr_load(const unsigned char* p, float (&f)[ND]) {
-    if constexpr (sizeof(T) == 4) {
-        if constexpr (ND == 4) {
-            const float4 x = *reinterpret_cast<const float4*>(p);
-            f[0] = x.x, f[1] = x.y, f[2] = x.z, f[3] = x.w;
-        } else {
-            const float2 x = *reinterpret_cast<const float2*>(p);
-            f[0] = x.x, f[1] = x.y;
-        }
-    } else {
-        if constexpr (ND == 4) {
-            const uint2 u = *reinterpret_cast<const uint2*>(p);
-            const float2 x = __half22float2(*reinterpret_cast<const __half2*>(&u.x));
-            const float2 y = __half22float2(*reinterpret_cast<const __half2*>(&u.y));
-            f[0] = x.x, f[1] = x.y, f[2] = y.x, f[3] = y.y;
-        } else {
-            const float2 x = __half22float2(*reinterpret_cast<const __half2*>(p));
-            f[0] = x.x, f[1] = x.y;
-        }
-    }
-}
-
-// Sequence and first row of row block x, RB rows a block: block floor(cu[b] g /
-// RB) + b is the first of sequence b, so blocks of neighbours never overlap and
-// floor(T g / RB) + n of them are enough.  Whole CTA; b = n_seqs past the end.
-template <int RB, int NT>
-__device__ __forceinline__ int row_block_seq(const PagedSeqs& s, int group, int x, int* first) {
-    int started = 0;
-    for (int b0 = 0; b0 < s.n_seqs; b0 += NT) {
-        const int b = b0 + (int)threadIdx.x;
-        const bool at = b < s.n_seqs && (int)(((int64_t)__ldg(s.cu + b) * group) / RB) + b <= x;
-        const int n = __syncthreads_count(at);
-        started += n;
-        if (n < NT) break;
-    }
-    const int b = started - 1;
-    if (b < 0) return s.n_seqs;
-    *first = (x - (int)(((int64_t)__ldg(s.cu + b) * group) / RB) - b) * RB;
-    return b;
 }
 
 template <typename T, int HD, int RB>
@@ -310,20 +269,7 @@ __global__ void __launch_bounds__(kPrThreads) paged_rows_kernel(const __grid_con
             }
         }
         const int row = row0 + r;
-        const int tok = sv.row0 + row / a.group, head = kvh * a.group + row % a.group;
-        if (a.nsplit > 1) {
-            float* pp = a.part + (((size_t)split * a.s.n_tokens + tok) * a.nh + head) * kW;
-            if (lane == 0) *reinterpret_cast<float2*>(pp) = make_float2(L, M);
-#pragma unroll
-            for (int d = 0; d < ND; ++d) pp[2 + lane * ND + d] = o[d];
-        } else {
-            const float inv = L > 0.f ? 1.0f / L : (L == 0.f ? 0.f : L);
-            float* po = a.out + (size_t)tok * a.ldo + head * HD + lane * ND;
-#pragma unroll
-            for (int d = 0; d < ND; ++d) po[d] = o[d] * inv;
-            if (a.lse && lane == 0)
-                a.lse[(size_t)tok * a.nh + head] = L == 0.f ? -INFINITY : (M + log2f(L)) * 0.69314718055994531f;
-        }
+        paged_row_store<HD, ND>(a, split, sv.row0 + row / a.group, kvh * a.group + row % a.group, lane, L, M, o);
     }
 }
 
@@ -365,11 +311,9 @@ __global__ void __launch_bounds__(128) paged_merge_kernel(const __grid_constant_
                 for (int d = 0; d < ND; ++d) o[d] = fmaf(x[2 + lane * ND + d], c, o[d]);
             }
         }
-        const float inv = L > 0.f ? 1.0f / L : (L == 0.f ? 0.f : L);
-        float* po = a.out + (size_t)tok * a.ldo + h * HD + lane * ND;
-#pragma unroll
-        for (int d = 0; d < ND; ++d) po[d] = o[d] * inv;
-        if (a.lse && lane == 0) a.lse[(size_t)tok * a.nh + h] = L == 0.f ? -INFINITY : (M + log2f(L)) * 0.69314718055994531f;
+        PagedAttnArgs whole = a;
+        whole.nsplit = 1;
+        paged_row_store<HD, ND>(whole, 0, tok, h, lane, L, M, o);
     }
 }
 
@@ -423,24 +367,27 @@ extern "C" tvb_status tvb_attention_paged(float* out, int ldo, float* lse, const
     a.window = window;
     a.status = status;
     const cudaStream_t st = as_stream(stream);
-    const int rows = std::min(a.s.max_new, a.s.n_tokens) * a.group;
-    const int rb = rows >= 5 ? 8 : rows >= 3 ? 4 : rows;
-    // Splits: enough CTAs for two waves, at least 256 keys each.
+    const int64_t rows64 = (int64_t)std::min(a.s.max_new, a.s.n_tokens) * a.group;
+    const int rows = (int)std::min<int64_t>(rows64, 1 << 20);
+    const bool f16 = kv->dtype == TVB_F16;
+    const bool tensor = f16 && rows >= kTensorRows;
+    const int rb = tensor ? 128 : rows >= 5 ? 8 : rows >= 3 ? 4 : rows;
+    // Splits: two waves of CTAs (one wave of the tensor-core kernel's, which fill an SM), at least 256 (1024) keys each.
     const int64_t blocks = (((int64_t)a.s.n_tokens * a.group) / rb + a.s.n_seqs) * nkv;
     const int span = window ? (int)std::min<int64_t>(a.s.max_kv, (int64_t)window + a.s.max_new) : a.s.max_kv;
-    int want = (int)std::min<int64_t>(std::max<int64_t>(1, 2 * num_sms() / blocks), std::max(1, span / 256));
+    int want = (int)std::min<int64_t>(std::max<int64_t>(1, (tensor ? 1 : 2) * num_sms() / blocks),
+                                      std::max(1, span / (tensor ? 1024 : 256)));
     want = std::min(want, kPrMaxSplits);
-    a.split_len = ((a.s.max_kv + want - 1) / want + 63) / 64 * 64;
-    if (window && want > 1) a.split_len = ((span + want - 1) / want + 63) / 64 * 64;
-    if (a.split_len < 64) a.split_len = 64;
+    a.split_len = std::max(64, ((want > 1 ? (span + want - 1) / want : a.s.max_kv) + 63) / 64 * 64);
     a.nsplit = want > 1 ? (a.s.max_kv + a.split_len - 1) / a.split_len : 1;
     Workspace ws(st);
     if (a.nsplit > 1) {
         TVB_TRY(ws.get((size_t)a.nsplit * a.s.n_tokens * nh * (hd + 2) * 4));
         a.part = ws.at<float>();
     }
-    const bool f16 = kv->dtype == TVB_F16;
-    if (hd == 128) {
+    if (tensor) {
+        TVB_TRY(paged_attn_chunk_f16(a, hd, st));
+    } else if (hd == 128) {
         TVB_TRY((f16 ? launch_rows_rb<__half, 128>(a, rows, st) : launch_rows_rb<float, 128>(a, rows, st)));
     } else {
         TVB_TRY((f16 ? launch_rows_rb<__half, 64>(a, rows, st) : launch_rows_rb<float, 64>(a, rows, st)));
