@@ -12,9 +12,10 @@
 //   MMA warp: S = Q K^T (K-major operands) into one of three TMEM buffers a tile
 //     ahead of the softmax, then O = P V with P from TMEM and V as the MN-major
 //     operand it is in memory (no transpose)
-//   softmax warps: thread = row; running maximum, p as hi + lo over its S columns
-//     in TMEM, and O (a fresh product per tile) added to registers with the
-//     rescaling, which also keeps the tensor core's truncating sums short (16
+//   softmax warps: two threads a row, each half of the tile's keys (maxima meet in
+//     shared memory) and half of the dimensions; running maximum, p as hi + lo
+//     over its S columns in TMEM, and O (a fresh product per tile) added to
+//     registers with the rescaling, which also keeps the tensor core's truncating sums short (16
 //     MMAs: 3e-7; a sum over 6000 keys in TMEM would lose 1.4e-5)
 //
 // A masked probability is zero but 0 x inf is not: a loader that finds a
@@ -26,8 +27,8 @@
 namespace tvb {
 
 constexpr int kPcRows = 128, kPcKeys = 128, kPcSlots = 4;
-// Warps 0-3 softmax, 4-6 loaders, 7 MMA: with 8 warps a thread may use 255 registers (a ninth would leave 168).
-constexpr int kPcThreads = 256, kPcLoaders = 3, kPcMmaWarp = 4 + kPcLoaders;
+// Warps 0-7 softmax, 8-10 loaders, 11 MMA: 12 warps leave a thread 168 registers.
+constexpr int kPcThreads = 384, kPcSoft = 8, kPcLoaders = 3, kPcMmaWarp = kPcSoft + kPcLoaders;
 
 template <int HD>
 struct PcSmem {
@@ -36,7 +37,8 @@ struct PcSmem {
     static constexpr int kQ = 0;
     static constexpr int kSlots = 2 * kPlane;
     static constexpr int kBar = kSlots + kPcSlots * kPlane;
-    static constexpr int kBytes = kBar + 256 + 1024;      // barriers, alignment
+    static constexpr int kRed = kBar + 256;                   // row maxima of the two halves, two tiles
+    static constexpr int kBytes = kRed + 2 * 2 * 128 * 4 + 1024;   // alignment
 };
 
 // Shared-memory descriptor of an MN-major operand in 128-byte-swizzled atoms of
@@ -61,14 +63,12 @@ __device__ __forceinline__ void tc_mma_ts(uint32_t tmem_d, uint32_t tmem_a, uint
         : "memory");
 }
 
-__device__ __forceinline__ void tmem_st32(uint32_t taddr, const uint32_t (&r)[32]) {
+__device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t (&r)[16]) {
     asm volatile(
-        "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, "
-        "%15, %16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31, %32};" ::"r"(taddr),
+        "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, "
+        "%15, %16};" ::"r"(taddr),
         "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]),
-        "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(r[16]), "r"(r[17]), "r"(r[18]),
-        "r"(r[19]), "r"(r[20]), "r"(r[21]), "r"(r[22]), "r"(r[23]), "r"(r[24]), "r"(r[25]), "r"(r[26]), "r"(r[27]),
-        "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31])
+        "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
         : "memory");
 }
 __device__ __forceinline__ void tmem_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
@@ -134,10 +134,10 @@ __global__ void __launch_bounds__(kPcThreads, 1) paged_chunk_kernel(const __grid
             mbar_init(empty + i, 1);
         }
         for (int i = 0; i < 3; ++i) mbar_init(s_full + i, 1);
-        for (int i = 0; i < 2; ++i) mbar_init(p_full + i, 128);
+        for (int i = 0; i < 2; ++i) mbar_init(p_full + i, 32 * kPcSoft);
         mbar_init(o_full, 1);
-        mbar_init(o_read, 128);
-        mbar_init(q_full, 128);
+        mbar_init(o_read, 32 * kPcSoft);
+        mbar_init(q_full, 32 * kPcSoft);
         mbar_init(drained, 1);
         *abort_flag = 0;
         *poison = 0;
@@ -154,9 +154,9 @@ __global__ void __launch_bounds__(kPcThreads, 1) paged_chunk_kernel(const __grid
     };
     const int* table = a.s.table + (size_t)b * a.s.table_ld;
 
-    if (warp >= 4 && warp < kPcMmaWarp) {
+    if (warp >= kPcSoft && warp < kPcMmaWarp) {
         // ---- loaders ---------------------------------------------------------------
-        const int w = warp - 4;
+        const int w = warp - kPcSoft;
         constexpr int kLanes = HD / 8;          // 16-byte chunks, lanes a row
         constexpr int kPass = 32 / kLanes;      // rows a warp instruction
         const int c = lane % kLanes;
@@ -254,9 +254,8 @@ __global__ void __launch_bounds__(kPcThreads, 1) paged_chunk_kernel(const __grid
 #pragma unroll
                 for (int kk = 0; kk < kPcKeys / 16; ++kk) {
                     const uint64_t vd = sw128_mn_desc(v_s + kk * 2048, Sm::kAtom);
-                    const uint32_t ph = p + (kk >> 1) * 32 + (kk & 1) * 8;
-                    tc_mma_ts(tmem + kO, ph, vd, idesc_o, kk ? 1u : 0u);
-                    tc_mma_ts(tmem + kO, ph + 16, vd, idesc_o, 1u);
+                    tc_mma_ts(tmem + kO, p + kk * 16, vd, idesc_o, kk ? 1u : 0u);
+                    tc_mma_ts(tmem + kO, p + kk * 16 + 8, vd, idesc_o, 1u);
                 }
                 tc_commit(o_full);
                 tc_commit(empty + item % kPcSlots);
@@ -268,16 +267,19 @@ __global__ void __launch_bounds__(kPcThreads, 1) paged_chunk_kernel(const __grid
         }
         __syncwarp();
     } else {
-        // ---- softmax: thread = row -----------------------------------------------------
-        const int r = threadIdx.x;
+        // ---- softmax: two threads a row, each half of a tile's keys and of the dimensions ----
+        const int r = threadIdx.x & 127, half = warp >> 2;
         const bool live = r < rows;
         const int row = row0 + min(r, rows - 1);
         const int tok = sv.row0 + row / a.group, head = kvh * a.group + row % a.group;
         const int pos = live ? sv.pos0 + row / a.group : -1;
+        float* red = reinterpret_cast<float*>(smem + Sm::kRed);
+        auto pair_sync = [&]() { asm volatile("bar.sync %0, 64;" ::"r"(1 + (warp & 3)) : "memory"); };
         float f = 1.f;   // q = (hi + lo) f / (scale log2 e)
         {
             const float* q = a.q + (size_t)tok * a.ldq + head * HD;
             float mx = 0.f;
+#pragma unroll 4
             for (int d = 0; d < HD; d += 4) {
                 const float4 x = *reinterpret_cast<const float4*>(q + d);
                 mx = fmaxf(mx, fmaxf(fmaxf(fabsf(x.x), fabsf(x.y)), fmaxf(fabsf(x.z), fabsf(x.w))));
@@ -288,7 +290,8 @@ __global__ void __launch_bounds__(kPcThreads, 1) paged_chunk_kernel(const __grid
             if (mx > 0.f && mx < INFINITY) e = max(-100, min(100, (int)((__float_as_uint(mx) >> 23) & 255) - 127 - 13));
             f = __uint_as_float((uint32_t)(127 + e) << 23);
             const float g = a.scale2 * __uint_as_float((uint32_t)(127 - e) << 23);
-            for (int d = 0; d < HD; d += 8) {
+#pragma unroll 2
+            for (int d = half * (HD / 2); d < (half + 1) * (HD / 2); d += 8) {
                 const float4 x = *reinterpret_cast<const float4*>(q + d), y = *reinterpret_cast<const float4*>(q + d + 4);
                 const float v[8] = {x.x * g, x.y * g, x.z * g, x.w * g, y.x * g, y.y * g, y.z * g, y.w * g};
                 __half2 hi[4], lo2[4];
@@ -306,106 +309,97 @@ __global__ void __launch_bounds__(kPcThreads, 1) paged_chunk_kernel(const __grid
             fence_proxy_async_smem_cta();
             mbar_arrive(q_full);
         }
-        float acc[HD];
+        constexpr int kD = HD / 2;   // dimensions of this thread
+        float acc[kD];
 #pragma unroll
-        for (int d = 0; d < HD; ++d) acc[d] = 0.f;
+        for (int d = 0; d < kD; ++d) acc[d] = 0.f;
         float m = -INFINITY, l = 0.f, corr_prev = 1.f;
-        const uint32_t lanes = tmem + ((uint32_t)(32 * warp) << 16);
+        const uint32_t lanes = tmem + ((uint32_t)(32 * (warp & 3)) << 16);
         auto add_o = [&](float c) {   // acc = acc c + O of the last product
 #pragma unroll
-            for (int h = 0; h < HD / 32; ++h) {
+            for (int h = 0; h < kD / 32; ++h) {
                 uint32_t o[32];
-                tmem_ld32(lanes + kO + h * 32, o);
+                tmem_ld32(lanes + kO + half * kD + h * 32, o);
                 tmem_wait_ld();
 #pragma unroll
                 for (int i = 0; i < 32; ++i) acc[h * 32 + i] = fmaf(acc[h * 32 + i], c, __uint_as_float(o[i]));
             }
         };
-        bool ok = true;
         auto landed = [&](uint64_t* bar, int phase) {
             const bool in = mbar_wait_bounded(bar, (uint32_t)(phase & 1));
             return __all_sync(0xffffffffu, in && !*abort_flag) != 0;
         };
+        bool ok = true;
         for (int j = 0; j < nt; ++j) {
-            ok = landed(s_full + j % 3, j / 3);
-            if (!ok) break;
-            tc_fence_after();
-            const uint32_t sb = lanes + (j % 3) * kPcKeys;
+            ok = ok && landed(s_full + j % 3, j / 3);
+            // a warp that gives up tells its partner through the exchange below (a maximum is never NaN), so both leave
+            if (!ok) red[((j & 1) * 2 + half) * 128 + r] = NAN;
+            const uint32_t sb = lanes + (j % 3) * kPcKeys + half * 64;
             const int t0 = k0 + j * kPcKeys;
             const int t1 = min(t0 + kPcKeys, k1);
-            // keys of this tile that the row sees: bits [first, last]
             const bool edge = t1 - t0 < kPcKeys || t1 - 1 > p_first || (a.window && t0 <= p_last - a.window);
-            const int last = min(t1 - 1, pos) - t0, first = a.window ? pos - a.window + 1 - t0 : 0;
-            auto mask = [&](int c) -> uint32_t {
-                uint32_t mk = 0xffffffffu;
-                if (edge) {
-                    const int hi = last - 32 * c, lw = first - 32 * c;
-                    mk = hi < 0 ? 0u : hi >= 31 ? 0xffffffffu : (2u << hi) - 1u;
-                    if (lw > 0) mk &= lw > 31 ? 0u : ~((1u << lw) - 1u);
-                }
-                return mk;
-            };
-            float mx = -INFINITY;
-#pragma unroll
-            for (int c = 0; c < 4; ++c) {
-                uint32_t s[32];
-                tmem_ld32(sb + 32 * c, s);
+            uint32_t s[64];
+            if (ok) {
+                tc_fence_after();
+                tmem_ld32(sb, *reinterpret_cast<uint32_t(*)[32]>(s));
+                tmem_ld32(sb + 32, *reinterpret_cast<uint32_t(*)[32]>(s + 32));
                 tmem_wait_ld();
-                if (edge) {
-                    const uint32_t mk = mask(c);
+                if (edge) {   // keys [first, last] of this half are the row's
+                    const int last = min(t1 - 1, pos) - t0 - half * 64;
+                    const int first = a.window ? pos - a.window + 1 - t0 - half * 64 : 0;
 #pragma unroll
-                    for (int i = 0; i < 32; ++i)
-                        if ((mk >> i) & 1u) mx = fmaxf(mx, __uint_as_float(s[i]));
-                } else {
-#pragma unroll
-                    for (int i = 0; i < 32; ++i) mx = fmaxf(mx, __uint_as_float(s[i]));
+                    for (int i = 0; i < 64; ++i)
+                        if (i > last || i < first) s[i] = 0xff800000u;   // -infinity
                 }
+                float m4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+                for (int i = 0; i < 64; ++i) m4[i & 3] = fmaxf(m4[i & 3], __uint_as_float(s[i]));
+                red[((j & 1) * 2 + half) * 128 + r] = fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3]));
             }
-            const float mn = fmaxf(m, mx * f);
+            pair_sync();
+            const float x0 = red[(j & 1) * 256 + r], x1 = red[(j & 1) * 256 + 128 + r];
+            if (__any_sync(0xffffffffu, x0 != x0 || x1 != x1)) {
+                ok = false;
+                break;
+            }
+            const float mn = fmaxf(m, fmaxf(x0, x1) * f);
             const float corr = m == mn ? 1.f : ex2(m - mn);
             const float mref = mn == -INFINITY ? 0.f : mn;
-            float sum0 = 0.f, sum1 = 0.f;
+            float sum[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-            for (int c = 0; c < 4; ++c) {
-                uint32_t s[32];
-                tmem_ld32(sb + 32 * c, s);
-                tmem_wait_ld();
-                const uint32_t mk = edge ? mask(c) : 0xffffffffu;
-                uint32_t p[32];
+            for (int c = 0; c < 4; ++c) {   // 16 keys: 8 columns of hi, 8 of lo, in place of their scores
+                uint32_t p[16];
 #pragma unroll
-                for (int i = 0; i < 16; ++i) {
-                    float x = ex2(fmaf(__uint_as_float(s[2 * i]), f, -mref));
-                    float y = ex2(fmaf(__uint_as_float(s[2 * i + 1]), f, -mref));
-                    if (edge) {
-                        if (!((mk >> (2 * i)) & 1u)) x = 0.f;
-                        if (!((mk >> (2 * i + 1)) & 1u)) y = 0.f;
-                    }
-                    sum0 += x;
-                    sum1 += y;
+                for (int i = 0; i < 8; ++i) {
+                    const float x = ex2(fmaf(__uint_as_float(s[16 * c + 2 * i]), f, -mref));
+                    const float y = ex2(fmaf(__uint_as_float(s[16 * c + 2 * i + 1]), f, -mref));
+                    sum[(2 * i) & 3] += x;
+                    sum[(2 * i + 1) & 3] += y;
                     const __half2 hi = __floats2half2_rn(x, y);
                     const float2 h = __half22float2(hi);
                     const __half2 lw = __floats2half2_rn(x - h.x, y - h.y);
                     p[i] = *reinterpret_cast<const uint32_t*>(&hi);
-                    p[16 + i] = *reinterpret_cast<const uint32_t*>(&lw);
+                    p[8 + i] = *reinterpret_cast<const uint32_t*>(&lw);
                 }
-                tmem_st32(sb + 32 * c, p);
+                tmem_st16(sb + 16 * c, p);
             }
             tmem_wait_st();
             tc_fence_before();
             mbar_arrive(p_full + (j & 1));
-            l = l * corr + (sum0 + sum1);
+            l = l * corr + ((sum[0] + sum[1]) + (sum[2] + sum[3]));
             m = mn;
             if (j > 0) {
                 ok = landed(o_full, j - 1);
-                if (!ok) break;
-                tc_fence_after();
-                add_o(corr_prev);
-                tc_fence_before();
-                mbar_arrive(o_read);
+                if (ok) {
+                    tc_fence_after();
+                    add_o(corr_prev);
+                    tc_fence_before();
+                    mbar_arrive(o_read);
+                }
             }
             corr_prev = corr;
         }
-        if (ok) ok = landed(o_full, nt - 1);
+        ok = ok && landed(o_full, nt - 1);
         if (ok) {
             tc_fence_after();
             add_o(corr_prev);
@@ -413,20 +407,26 @@ __global__ void __launch_bounds__(kPcThreads, 1) paged_chunk_kernel(const __grid
         } else {
             fail();
         }
+        // the row's sum from its two halves
+        red[half * 128 + r] = l;
+        pair_sync();
+        l = red[r] + red[128 + r];
         if (ok && live && !*poison) {
             if (a.nsplit > 1) {
                 float* pp = a.part + (((size_t)split * a.s.n_tokens + tok) * a.nh + head) * (HD + 2);
-                *reinterpret_cast<float2*>(pp) = make_float2(l, m);
+                if (half == 0) *reinterpret_cast<float2*>(pp) = make_float2(l, m);
+                pp += 2 + half * kD;
 #pragma unroll
-                for (int d = 0; d < HD; d += 2) *reinterpret_cast<float2*>(pp + 2 + d) = make_float2(acc[d], acc[d + 1]);
+                for (int d = 0; d < kD; d += 2) *reinterpret_cast<float2*>(pp + d) = make_float2(acc[d], acc[d + 1]);
             } else {
                 const float inv = l > 0.f ? 1.0f / l : (l == 0.f ? 0.f : l);
-                float* po = a.out + (size_t)tok * a.ldo + head * HD;
+                float* po = a.out + (size_t)tok * a.ldo + head * HD + half * kD;
 #pragma unroll
-                for (int d = 0; d < HD; d += 4)
+                for (int d = 0; d < kD; d += 4)
                     *reinterpret_cast<float4*>(po + d) = make_float4(acc[d] * inv, acc[d + 1] * inv, acc[d + 2] * inv,
                                                                      acc[d + 3] * inv);
-                if (a.lse) a.lse[(size_t)tok * a.nh + head] = l == 0.f ? -INFINITY : (m + log2f(l)) * 0.69314718055994531f;
+                if (a.lse && half == 0)
+                    a.lse[(size_t)tok * a.nh + head] = l == 0.f ? -INFINITY : (m + log2f(l)) * 0.69314718055994531f;
             }
         }
     }
@@ -438,7 +438,7 @@ __global__ void __launch_bounds__(kPcThreads, 1) paged_chunk_kernel(const __grid
     }
     if (*poison && !*abort_flag) {
         // key by key, a warp a row: lane = HD / 32 dimensions
-        for (int r = warp; r < rows; r += 8) paged_row_slow<__half, HD>(a, sv, table, kvh, split, row0 + r, k0, k1);
+        for (int r = warp; r < rows; r += kPcThreads / 32) paged_row_slow<__half, HD>(a, sv, table, kvh, split, row0 + r, k0, k1);
     }
 }
 
