@@ -6,15 +6,13 @@
 // running maximum m per row, the sum and the weighted values rescaled by
 // 2^(m_old - m_new) when it grows.
 //
-// paged_rows_kernel: a CTA takes RB query rows of one KV head of one sequence
-// (rows: new token x query head of the group) and one split of the keys; its 8
-// warps take batches of 8 keys in turn and merge at the end.  K and V rows pass
+// paged_rows_kernel: a CTA takes its run of tiles (attn_schedule: RB query rows of
+// one KV head of one sequence against 64 keys a tile); per piece its 8 warps take
+// batches of 8 keys in turn and merge at the end.  K and V rows pass
 // through a ring of cp.async stages private to each warp, so no warp waits for
 // another while it streams; each lane owns head_dim / 32 dimensions.  The RB x 8
 // partial dot products of a batch are summed over the lanes by a butterfly that
-// halves the values it carries at each step (31 shuffles for 32 sums).  With
-// more than one split the partial results go to a workspace and
-// paged_merge_kernel joins them in split order.
+// halves the values it carries at each step (31 shuffles for 32 sums).
 #include "attn_paged.h"
 
 #include <algorithm>
@@ -23,7 +21,7 @@ namespace tvb {
 
 constexpr int kPrWarps = 8, kPrThreads = 32 * kPrWarps;
 constexpr int kPrKeys = 8;   // keys a batch
-constexpr int kPrMaxSplits = 64;
+constexpr int kPrTile = kPrKeys * kPrWarps;   // keys a tile
 constexpr int kTensorRows = 32;   // rows of a KV head from which F16 caches take the tensor cores
 
 __device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, bool valid) {
@@ -67,40 +65,30 @@ __device__ __forceinline__ float pr_reduce(float (&v)[NV], int lane) {
 }
 
 template <typename T, int HD, int RB>
-__global__ void __launch_bounds__(kPrThreads) paged_rows_kernel(const __grid_constant__ PagedAttnArgs a) {
+__host__ __device__ constexpr int rows_smem() {
+    return PrStage<T, HD>::kSmem > kPrWarps * RB * (HD + 2) * 4 ? PrStage<T, HD>::kSmem : kPrWarps * RB * (HD + 2) * 4;
+}
+
+// One piece; whole CTA.
+template <typename T, int HD, int RB>
+__device__ __forceinline__ void rows_piece(const PagedAttnArgs& a, const AttnPiece& pc, unsigned char* pr_smem_raw) {
     using St = PrStage<T, HD>;
     constexpr int ND = HD / 32;              // dimensions a lane
     constexpr int RG = RB < 4 ? RB : 4;      // rows reduced together
     constexpr int NG = RB / RG;
     constexpr int NV = RG * kPrKeys;         // sums of one reduction
     constexpr int LPV = 32 / NV;             // lanes that hold one
-    extern __shared__ __align__(128) unsigned char pr_smem_raw[];
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const int kvh = blockIdx.y, split = blockIdx.z;
-
-    int row0 = 0;
-    const int b = row_block_seq<RB, kPrThreads>(a.s, a.group, blockIdx.x, &row0);
-    if (b >= a.s.n_seqs) return;
-    const SeqView sv = seq_view(a.s, b);
-    if (!sv.ok) {
-        if (threadIdx.x == 0) report_bad(a.status);
-        return;
-    }
-    const int rows = min(RB, sv.n * a.group - row0);
-    if (rows <= 0) return;
-    // keys that some row of the block sees, cut to this split
-    const int p_first = sv.pos0 + row0 / a.group, p_last = sv.pos0 + (row0 + rows - 1) / a.group;
-    const int lo = a.window ? max(0, p_first - a.window + 1) : 0;
-    const int k0 = a.nsplit > 1 ? max(lo, split * a.split_len) : lo;
-    const int k1 = a.nsplit > 1 ? min(p_last + 1, (split + 1) * a.split_len) : p_last + 1;
-    if (a.nsplit > 1 && k0 >= k1) return;   // no row of the block takes this split
+    const int rows = pc.rows, kvh = pc.kvh, k0 = max(pc.k0, pc.first), k1 = pc.k1;
+    const int p_first = pc.pos0 + (int)a.gdiv.div((uint32_t)pc.row);
+    const int p_last = pc.pos0 + (int)a.gdiv.div((uint32_t)(pc.row + rows - 1));
 
     // q (times scale log2 e) and positions of the rows
     float q[RB][ND], acc[RB][ND];
 #pragma unroll
     for (int r = 0; r < RB; ++r) {
-        const int row = row0 + min(r, rows - 1);
-        const int tok = sv.row0 + row / a.group, head = kvh * a.group + row % a.group;
+        const int row = pc.row + min(r, rows - 1), t = (int)a.gdiv.div((uint32_t)row);
+        const int tok = pc.tok0 + t, head = kvh * a.group + row - t * a.group;
         pr_load<float, ND>(reinterpret_cast<const unsigned char*>(a.q + (size_t)tok * a.ldq + head * HD + lane * ND), q[r]);
 #pragma unroll
         for (int d = 0; d < ND; ++d) q[r][d] *= a.scale2, acc[r][d] = 0.f;
@@ -112,7 +100,7 @@ __global__ void __launch_bounds__(kPrThreads) paged_rows_kernel(const __grid_con
 #pragma unroll
     for (int g = 0; g < NG; ++g) {
         const int r = g * RG + lrow;
-        lpos[g] = r < rows ? sv.pos0 + (row0 + r) / a.group : -1;
+        lpos[g] = r < rows ? pc.pos0 + (int)a.gdiv.div((uint32_t)(pc.row + r)) : -1;
         m[g] = -INFINITY;
         l[g] = 0.f;
     }
@@ -120,7 +108,7 @@ __global__ void __launch_bounds__(kPrThreads) paged_rows_kernel(const __grid_con
     unsigned char* ring = pr_smem_raw + warp * St::kStages * St::kBytes;
     const unsigned char* kb = a.kv.k + (int64_t)kvh * a.kv.head_stride;
     const unsigned char* vb = a.kv.v + (int64_t)kvh * a.kv.head_stride;
-    const int* table = a.s.table + (size_t)b * a.s.table_ld;
+    const int* table = a.s.table + (size_t)pc.b * a.s.table_ld;
     bool bad = false;
 
     // one batch of keys [t, t + 8) into stage st; rows that no query row sees or
@@ -149,28 +137,26 @@ __global__ void __launch_bounds__(kPrThreads) paged_rows_kernel(const __grid_con
     // batches warp, warp + 8, ... of the keys from k0 on
     const int step = kPrWarps * kPrKeys;
     int t = k0 + warp * kPrKeys, tn = t;
-    unsigned have[St::kStages];
-#pragma unroll
+    unsigned have = 0u;
     for (int i = 0; i < St::kStages - 1; ++i, tn += step) {
-        have[i] = tn < k1 ? request(tn, i) : 0u;
+        have |= (tn < k1 ? request(tn, i) : 0u) << (8 * i);
         cp_async_commit();
     }
+    int st = 0;
+#pragma unroll 1   // the loop fits the instruction cache only once
     while (t < k1) {
-#pragma unroll
-        for (int st = 0; st < St::kStages; ++st) {
-            if (t >= k1) break;
-            {
-                constexpr int kAhead = St::kStages - 1;
-                const int ns = (st + kAhead) % St::kStages;
-                __syncwarp();   // every lane is done with the stage that is filled now
-                have[ns] = tn < k1 ? request(tn, ns) : 0u;
-                cp_async_commit();
-                tn += step;
-            }
+        {
+            const int ns = st == 0 ? St::kStages - 1 : st - 1;
+            __syncwarp();   // every lane is done with the stage that is filled now
+            have |= (tn < k1 ? request(tn, ns) : 0u) << (8 * (St::kStages - 1));
+            cp_async_commit();
+            tn += step;
             cp_async_wait<St::kStages - 1>();
             __syncwarp();
             const unsigned char* stage = ring + st * St::kBytes;
-            const unsigned hv = have[st];
+            const unsigned hv = have & 0xffu;   // keys of the stages in order, 8 bits each
+            have >>= 8;
+            st = st == St::kStages - 1 ? 0 : st + 1;
             float p[NG];
 #pragma unroll
             for (int g = 0; g < NG; ++g) {
@@ -268,64 +254,55 @@ __global__ void __launch_bounds__(kPrThreads) paged_rows_kernel(const __grid_con
                 for (int d = 0; d < ND; ++d) o[d] = fmaf(x[lane * ND + d], c, o[d]);
             }
         }
-        const int row = row0 + r;
-        paged_row_store<HD, ND>(a, split, sv.row0 + row / a.group, kvh * a.group + row % a.group, lane, L, M, o);
-    }
-}
-
-// One warp a (token, head): the partials of the splits that its keys touch,
-// joined in split order.
-template <int HD>
-__global__ void __launch_bounds__(128) paged_merge_kernel(const __grid_constant__ PagedAttnArgs a) {
-    constexpr int ND = HD / 32, kW = HD + 2;
-    const int tok = blockIdx.x, lane = threadIdx.x & 31;
-    int ended = 0;
-    for (int b0 = 0; b0 < a.s.n_seqs; b0 += 128) {
-        const int b = b0 + (int)threadIdx.x;
-        const int n = __syncthreads_count(b < a.s.n_seqs && __ldg(a.s.cu + b + 1) <= tok);
-        ended += n;
-        if (n < 128) break;
-    }
-    if (ended >= a.s.n_seqs) return;
-    const SeqView sv = seq_view(a.s, ended);
-    if (!sv.ok || tok < sv.row0) return;
-    const int pos = sv.pos0 + tok - sv.row0;
-    const int first = (a.window ? max(0, pos - a.window + 1) : 0) / a.split_len, last = pos / a.split_len;
-    pdl_wait();
-    for (int h = blockIdx.y * 4 + (threadIdx.x >> 5); h < a.nh; h += gridDim.y * 4) {
-        const float* base = a.part + ((size_t)tok * a.nh + h) * kW;
-        const size_t stride = (size_t)a.s.n_tokens * a.nh * kW;
-        float M = -INFINITY;
-        for (int sp = first + lane; sp <= last; sp += 32) M = fmaxf(M, base[sp * stride + 1]);
-        M = warp_max(M);
-        float L = 0.f, o[ND];
-#pragma unroll
-        for (int d = 0; d < ND; ++d) o[d] = 0.f;
-        for (int sp = first; sp <= last; ++sp) {
-            const float* x = base + sp * stride;
-            const float2 lm = *reinterpret_cast<const float2*>(x);
-            const float c = lm.y == -INFINITY ? 0.f : exp2f(lm.y - M);
-            if (c != 0.f) {
-                L = fmaf(lm.x, c, L);
-#pragma unroll
-                for (int d = 0; d < ND; ++d) o[d] = fmaf(x[2 + lane * ND + d], c, o[d]);
-            }
-        }
-        PagedAttnArgs whole = a;
-        whole.nsplit = 1;
-        paged_row_store<HD, ND>(whole, 0, tok, h, lane, L, M, o);
+        attn_row_store<RB, HD, ND>(a, pc, r, L, M, o);
     }
 }
 
 template <typename T, int HD, int RB>
-static tvb_status launch_rows(const PagedAttnArgs& a, cudaStream_t st) {
+__global__ void __launch_bounds__(kPrThreads) paged_rows_kernel(const __grid_constant__ PagedAttnArgs a) {
+    extern __shared__ __align__(128) unsigned char pr_smem_raw[];
+    __shared__ AttnRun run;
+    __shared__ AttnPiece pieces[kPrWarps];
+    if (!a.balanced) {
+        AttnPiece p;
+        if (attn_block<RB, kPrTile, kPrThreads>(a, 1, &p)) rows_piece<T, HD, RB>(a, p, pr_smem_raw);
+        return;
+    }
+    AttnSchedule& sched = *reinterpret_cast<AttnSchedule*>(pr_smem_raw + rows_smem<T, HD, RB>());
+    const int per_head = attn_schedule<RB, kPrTile, kPrThreads>(a, sched, 1);
+    if (threadIdx.x == 0) run = attn_run(a, per_head);
+    __syncthreads();
+    pdl_launch_dependents();
+    bool begun = false;
+    const AttnPiece& p = pieces[threadIdx.x >> 5];
+    for (int at = run.u, n; (n = attn_next<RB, kPrTile>(a, sched, run, at, 1, &pieces[threadIdx.x >> 5])) != 0; at += n) {
+        rows_piece<T, HD, RB>(a, p, pr_smem_raw);
+        __syncthreads();
+        if (p.slot == 1) {
+            begun = true;
+            if (threadIdx.x == 0) attn_header(a, &p);
+        }
+    }
+    if (!begun && threadIdx.x == 0) attn_header(a, nullptr);
+}
+
+template <typename T, int HD, int RB>
+static tvb_status launch_rows(PagedAttnArgs a, cudaStream_t st) {
     static int set[kMaxDevices];
-    constexpr int smem = PrStage<T, HD>::kSmem > kPrWarps * RB * (HD + 2) * 4 ? PrStage<T, HD>::kSmem
-                                                                            : kPrWarps * RB * (HD + 2) * 4;
+    constexpr int smem = rows_smem<T, HD, RB>() + (int)sizeof(AttnSchedule);
     TVB_TRY(allow_smem(reinterpret_cast<const void*>(paged_rows_kernel<T, HD, RB>), smem, set));
-    const int64_t blocks = ((int64_t)a.s.n_tokens * a.group) / RB + a.s.n_seqs;
-    paged_rows_kernel<T, HD, RB><<<dim3((unsigned)blocks, (unsigned)a.nkv, (unsigned)a.nsplit), kPrThreads, smem, st>>>(a);
-    return check_launch("paged_rows_kernel");
+    a.min_tiles = 1;   // shorter pieces cost more to join than they save
+    Workspace ws(st);
+    dim3 grid;
+    if (a.balanced) {
+        grid = dim3((unsigned)num_sms());
+        TVB_TRY((attn_workspace<RB, HD>(&a, (int)grid.x, &ws)));
+    } else {
+        grid = dim3((unsigned)(((int64_t)a.s.n_tokens * a.group) / RB + a.s.n_seqs), (unsigned)a.nkv);
+    }
+    paged_rows_kernel<T, HD, RB><<<grid, kPrThreads, smem, st>>>(a);
+    TVB_TRY(check_launch("paged_rows_kernel"));
+    return launch_merge<RB, HD>(a, (int)grid.x, st);
 }
 
 template <typename T, int HD>
@@ -363,6 +340,7 @@ extern "C" tvb_status tvb_attention_paged(float* out, int ldo, float* lse, const
     a.nh = nh;
     a.nkv = nkv;
     a.group = nh / nkv;
+    a.gdiv = FastDiv((uint32_t)a.group);
     a.scale2 = scale * 1.4426950408889634f;
     a.window = window;
     a.status = status;
@@ -371,32 +349,13 @@ extern "C" tvb_status tvb_attention_paged(float* out, int ldo, float* lse, const
     const int rows = (int)std::min<int64_t>(rows64, 1 << 20);
     const bool f16 = kv->dtype == TVB_F16;
     const bool tensor = f16 && rows >= kTensorRows;
-    const int rb = tensor ? 128 : rows >= 5 ? 8 : rows >= 3 ? 4 : rows;
-    // Splits: two waves of CTAs (one wave of the tensor-core kernel's, which fill an SM), at least 256 (1024) keys each.
-    const int64_t blocks = (((int64_t)a.s.n_tokens * a.group) / rb + a.s.n_seqs) * nkv;
-    const int span = window ? (int)std::min<int64_t>(a.s.max_kv, (int64_t)window + a.s.max_new) : a.s.max_kv;
-    int want = (int)std::min<int64_t>(std::max<int64_t>(1, (tensor ? 1 : 2) * num_sms() / blocks),
-                                      std::max(1, span / (tensor ? 1024 : 256)));
-    want = std::min(want, kPrMaxSplits);
-    a.split_len = std::max(64, ((want > 1 ? (span + want - 1) / want : a.s.max_kv) + 63) / 64 * 64);
-    a.nsplit = want > 1 ? (a.s.max_kv + a.split_len - 1) / a.split_len : 1;
-    Workspace ws(st);
-    if (a.nsplit > 1) {
-        TVB_TRY(ws.get((size_t)a.nsplit * a.s.n_tokens * nh * (hd + 2) * 4));
-        a.part = ws.at<float>();
-    }
+    a.balanced = a.s.n_seqs <= kAttnSeqs;   // more sequences than that fill the SMs block by block
     if (tensor) {
         TVB_TRY(paged_attn_chunk_f16(a, hd, st));
     } else if (hd == 128) {
         TVB_TRY((f16 ? launch_rows_rb<__half, 128>(a, rows, st) : launch_rows_rb<float, 128>(a, rows, st)));
     } else {
         TVB_TRY((f16 ? launch_rows_rb<__half, 64>(a, rows, st) : launch_rows_rb<float, 64>(a, rows, st)));
-    }
-    if (a.nsplit > 1) {
-        const dim3 grid((unsigned)a.s.n_tokens, (unsigned)((nh + 3) / 4));
-        if (hd == 128) paged_merge_kernel<128><<<grid, 128, 0, st>>>(a);
-        else paged_merge_kernel<64><<<grid, 128, 0, st>>>(a);
-        TVB_TRY(check_launch("paged_merge_kernel"));
     }
     return TVB_OK;
 }

@@ -1,4 +1,6 @@
-// Attention over the paged cache: shared by its kernels (attn_paged.cu).
+// Attention over the paged cache: what its kernels share (attn_paged.cu, one or
+// few rows; attn_paged_tc.cu, chunks on the tensor cores) -- arguments, the
+// split of the work over the SMs, and a row computed key by key.
 #pragma once
 
 #include "paged.cuh"
@@ -11,15 +13,220 @@ struct PagedAttnArgs {
     float* lse;        // may be null
     int ldq, ldo;
     int nh, nkv, group;
+    FastDiv gdiv;      // group
     float scale2;      // scale * log2(e): scores are kept as powers of two
     int window;        // 0: none
-    int split_len;     // keys a split
-    int nsplit;        // splits of the longest sequence; 1: no partials
-    float* part;       // [split][token][head][hd + 2]: sum, max, weighted values
+    int balanced;      // the grid shares the tiles evenly; else a CTA a row block
+    int min_tiles;     // ... but no CTA gets fewer than this
+    float* part;       // [CTA][2]: rows x hd weighted values, rows x (sum, maximum) of cut blocks
+    int* header;       // [CTA][8]: the cut block that the CTA's last piece begins
     unsigned* status;
     PagedKV kv;
     PagedSeqs s;
 };
+
+constexpr int kAttnSeqs = 1024;   // sequences that a balanced grid keeps in shared memory
+
+// The work: row blocks (RB rows -- new token x query head of the group -- of one
+// KV head of one sequence) with the tiles of TK keys that some row of the block
+// sees, tile after tile, block after block, KV head after KV head.  A balanced
+// grid of G CTAs cuts the T tiles into G equal runs, whatever the lengths are; a
+// block that a cut divides leaves partial sums and paged_merge_kernel joins them.
+// Lengths are known on the device only, so every CTA adds up the sequences' tiles
+// first (a few microseconds saved over a launch that does it).
+struct AttnSchedule {
+    int row0[kAttnSeqs], n[kAttnSeqs], kv[kAttnSeqs];
+    int before[kAttnSeqs + 1];   // tiles of the earlier sequences, one KV head
+};
+
+struct AttnPiece {
+    int b;              // sequence
+    int tok0, pos0;     // its first row, its position
+    int kvh;
+    int row, rows;      // first row (token x head) of the block, rows of it
+    int first, k0, k1;  // keys [max(first, k0), k1); tiles start at k0
+    int tiles;
+    int slot;           // -1: the whole block; else the CTA's partial 0 (continues a block) or 1 (begins one)
+    int last_cta;       // slot 1: the CTA that ends the block
+};
+
+// Tiles of block i of a sequence; k0: where they start (multiples of `align`, a
+// power of two, so that boxes of rows stay inside their page).
+template <int RB, int TK>
+__device__ __forceinline__ int attn_tiles(const PagedAttnArgs& a, int n, int pos0, int i, int align, int* first, int* k0,
+                                          int* k1) {
+    const int rows = min(RB, n * a.group - i * RB);
+    const int p_first = pos0 + (int)a.gdiv.div((uint32_t)(i * RB));
+    const int p_last = pos0 + (int)a.gdiv.div((uint32_t)(i * RB + rows - 1));
+    *first = a.window ? max(0, p_first - a.window + 1) : 0;
+    *k0 = *first & ~(align - 1);
+    *k1 = p_last + 1;
+    return (*k1 - *k0 + TK - 1) / TK;
+}
+
+// Whole CTA (NT threads): fills `s` and returns the tiles of one KV head.
+template <int RB, int TK, int NT>
+__device__ __forceinline__ int attn_schedule(const PagedAttnArgs& a, AttnSchedule& s, int align) {
+    const int tid = threadIdx.x, lane = tid & 31;
+    for (int b = tid; b < a.s.n_seqs; b += NT) {
+        const SeqView v = seq_view(a.s, b);
+        if (!v.ok && blockIdx.x == 0) report_bad(a.status);
+        s.row0[b] = v.row0;
+        s.n[b] = v.ok ? v.n : 0;
+        s.kv[b] = v.kv;
+    }
+    __syncthreads();
+    for (int b = tid >> 5; b < a.s.n_seqs; b += NT / 32) {
+        const int n = s.n[b], blocks = (n * a.group + RB - 1) / RB;
+        int t = 0, x, y, z;
+        for (int i = lane; i < blocks; i += 32) t += attn_tiles<RB, TK>(a, n, s.kv[b] - n, i, align, &x, &y, &z);
+        t = __reduce_add_sync(0xffffffffu, t);
+        if (lane == 0) s.before[b + 1] = t;
+    }
+    __syncthreads();
+    if (tid < 32) {
+        int base = 0;
+        for (int b0 = 0; b0 < a.s.n_seqs; b0 += 32) {
+            int t = b0 + lane < a.s.n_seqs ? s.before[b0 + lane + 1] : 0;
+#pragma unroll
+            for (int o = 1; o < 32; o <<= 1) {
+                const int u = __shfl_up_sync(0xffffffffu, t, o);
+                if (lane >= o) t += u;
+            }
+            if (b0 + lane < a.s.n_seqs) s.before[b0 + lane + 1] = base + t;
+            base += __shfl_sync(0xffffffffu, t, 31);
+        }
+        if (lane == 0) s.before[0] = 0;
+    }
+    __syncthreads();
+    return s.before[a.s.n_seqs];
+}
+
+// A CTA's run of tiles.
+struct AttnRun {
+    int64_t total;
+    int per_head, ctas;
+    int u, end;
+};
+
+__device__ __forceinline__ AttnRun attn_run(const PagedAttnArgs& a, int per_head) {
+    AttnRun r;
+    r.per_head = per_head;
+    r.total = (int64_t)per_head * a.nkv;
+    r.ctas = (int)min((int64_t)gridDim.x, max((int64_t)1, r.total / a.min_tiles));
+    r.u = (int)(r.total * min((int)blockIdx.x, r.ctas) / r.ctas);
+    r.end = (int)(r.total * min((int)blockIdx.x + 1, r.ctas) / r.ctas);
+    return r;
+}
+
+// Whole warp: the piece that starts at tile u of the run, into *out (shared
+// memory of this warp); returns its tiles, 0 at the end of the run.  Not inlined:
+// every role of a kernel calls it, and code that fits the instruction cache is
+// worth more than the call.
+template <int RB, int TK>
+__device__ __noinline__ int attn_next(const PagedAttnArgs& a, const AttnSchedule& s, const AttnRun& r, int u, int align,
+                                      AttnPiece* out) {
+    if (u >= r.end) return 0;
+    const int lane = threadIdx.x & 31;
+    AttnPiece p;
+    p.kvh = u / r.per_head;
+    int t = u - p.kvh * r.per_head;
+    int lo = 0, hi = a.s.n_seqs - 1;   // the last sequence that starts at or before t and has tiles
+    while (lo < hi) {
+        const int mid = (lo + hi + 1) >> 1;
+        if (s.before[mid] <= t) lo = mid;
+        else hi = mid - 1;
+    }
+    const int b = lo, n = s.n[b];
+    p.b = b;
+    p.tok0 = s.row0[b];
+    p.pos0 = s.kv[b] - n;
+    t -= s.before[b];
+    const int blocks = (n * a.group + RB - 1) / RB;
+    int i0 = 0, tiles = 0, x, y, z;
+#pragma unroll 1
+    for (;; i0 += 32) {   // the block that holds tile t of the sequence
+        const int nt = i0 + lane < blocks ? attn_tiles<RB, TK>(a, n, p.pos0, i0 + lane, align, &x, &y, &z) : 0;
+        int sum = nt;
+#pragma unroll 1
+        for (int o = 1; o < 32; o <<= 1) {
+            const int v = __shfl_up_sync(0xffffffffu, sum, o);
+            if (lane >= o) sum += v;
+        }
+        const unsigned past = __ballot_sync(0xffffffffu, sum > t);
+        if (past || i0 + 32 >= blocks) {
+            const int l = past ? __ffs(past) - 1 : 31;
+            tiles = __shfl_sync(0xffffffffu, nt, l);
+            t -= __shfl_sync(0xffffffffu, sum, l) - tiles;
+            i0 += l;
+            break;
+        }
+        t -= __shfl_sync(0xffffffffu, sum, 31);
+    }
+    attn_tiles<RB, TK>(a, n, p.pos0, i0, align, &p.first, &p.k0, &p.k1);
+    p.row = i0 * RB;
+    p.rows = min(RB, n * a.group - p.row);
+    p.tiles = min(tiles - t, r.end - u);
+    p.slot = p.tiles == tiles ? -1 : t > 0 ? 0 : 1;
+    p.last_cta = (int)(((u - t + (int64_t)tiles) * r.ctas - 1) / r.total);
+    p.k0 += t * TK;
+    p.k1 = min(p.k1, p.k0 + p.tiles * TK);
+    __syncwarp();
+    if (lane == 0) *out = p;
+    __syncwarp();
+    return p.tiles;
+}
+
+// The piece of a CTA of an unbalanced grid: row block blockIdx.x of the batch,
+// whole.  Block floor(cu[b] g / RB) + b is the first of sequence b, so blocks of
+// neighbours never overlap and floor(T g / RB) + n of them are enough.
+template <int RB, int TK, int NT>
+__device__ __forceinline__ bool attn_block(const PagedAttnArgs& a, int align, AttnPiece* p) {
+    int started = 0;
+    for (int b0 = 0; b0 < a.s.n_seqs; b0 += NT) {
+        const int b = b0 + (int)threadIdx.x;
+        const bool at = b < a.s.n_seqs && (int)(((int64_t)__ldg(a.s.cu + b) * a.group) / RB) + b <= (int)blockIdx.x;
+        const int n = __syncthreads_count(at);
+        started += n;
+        if (n < NT) break;
+    }
+    if (!started) return false;
+    const int b = started - 1;
+    const SeqView v = seq_view(a.s, b);
+    const int i = (int)blockIdx.x - (int)(((int64_t)v.row0 * a.group) / RB) - b;
+    if (!v.ok) {
+        if (threadIdx.x == 0) report_bad(a.status);
+        return false;
+    }
+    if (i * RB >= v.n * a.group) return false;
+    p->b = b;
+    p->tok0 = v.row0;
+    p->pos0 = v.pos0;
+    p->kvh = blockIdx.y;
+    p->row = i * RB;
+    p->rows = min(RB, v.n * a.group - p->row);
+    p->tiles = attn_tiles<RB, TK>(a, v.n, v.pos0, i, align, &p->first, &p->k0, &p->k1);
+    p->slot = -1;
+    return true;
+}
+
+// Partial (CTA, slot) of RB rows: HD weighted values of each, then each row's sum
+// and maximum.
+template <int RB, int HD>
+__device__ __forceinline__ float* attn_part(const PagedAttnArgs& a, int cta, int slot, int r) {
+    return a.part + ((size_t)cta * 2 + slot) * RB * (HD + 2) + (size_t)r * HD;
+}
+template <int RB, int HD>
+__device__ __forceinline__ float* attn_part_sum(const PagedAttnArgs& a, int cta, int slot, int r) {
+    return a.part + (((size_t)cta * 2 + slot) * (HD + 2) + HD) * RB + 2 * r;
+}
+
+// Tells paged_merge_kernel about the cut block that this CTA begins (one thread).
+__device__ __forceinline__ void attn_header(const PagedAttnArgs& a, const AttnPiece* p) {
+    int* h = a.header + blockIdx.x * 8;
+    h[0] = p ? p->rows : 0;
+    if (p) h[1] = p->tok0, h[2] = p->row, h[3] = p->kvh, h[4] = p->last_cta;
+}
 
 template <typename T, int ND>
 __device__ __forceinline__ void pr_load(const unsigned char* p, float (&f)[ND]) {
@@ -44,63 +251,54 @@ __device__ __forceinline__ void pr_load(const unsigned char* p, float (&f)[ND]) 
     }
 }
 
-// Sequence and first row of row block x, RB rows a block: block floor(cu[b] g /
-// RB) + b is the first of sequence b, so blocks of neighbours never overlap and
-// floor(T g / RB) + n of them are enough.  Whole CTA; b = n_seqs past the end.
-template <int RB, int NT>
-__device__ __forceinline__ int row_block_seq(const PagedSeqs& s, int group, int x, int* first) {
-    int started = 0;
-    for (int b0 = 0; b0 < s.n_seqs; b0 += NT) {
-        const int b = b0 + (int)threadIdx.x;
-        const bool at = b < s.n_seqs && (int)(((int64_t)__ldg(s.cu + b) * group) / RB) + b <= x;
-        const int n = __syncthreads_count(at);
-        started += n;
-        if (n < NT) break;
-    }
-    const int b = started - 1;
-    if (b < 0) return s.n_seqs;
-    *first = (x - (int)(((int64_t)__ldg(s.cu + b) * group) / RB) - b) * RB;
-    return b;
+// log of the sum of exponentials from the sum l of powers 2^(s - m)
+__device__ __forceinline__ float attn_lse(float l, float m) {
+    return l == 0.f ? -INFINITY : (m + log2f(l)) * 0.69314718055994531f;
 }
+// What the weighted values are divided by: no key gives zeros, NaN stays.
+__device__ __forceinline__ float attn_inv(float l) { return l > 0.f ? 1.0f / l : (l == 0.f ? 0.f : l); }
 
-// What a row leaves: its sum l, maximum m and weighted values o (ND dimensions a
-// lane) as the partial of `split`, or divided into out and lse.
-template <int HD, int ND>
-__device__ __forceinline__ void paged_row_store(const PagedAttnArgs& a, int split, int tok, int head, int lane, float l,
-                                                float m, const float (&o)[ND]) {
-    if (a.nsplit > 1) {
-        float* pp = a.part + (((size_t)split * a.s.n_tokens + tok) * a.nh + head) * (HD + 2);
-        if (lane == 0) *reinterpret_cast<float2*>(pp) = make_float2(l, m);
+// What a row leaves (one warp, ND dimensions a lane).
+template <int RB, int HD, int ND>
+__device__ __forceinline__ void attn_row_store(const PagedAttnArgs& a, const AttnPiece& p, int r, float l, float m,
+                                               const float (&o)[ND]) {
+    const int lane = threadIdx.x & 31;
+    if (p.slot >= 0) {
+        float* pp = attn_part<RB, HD>(a, blockIdx.x, p.slot, r);
+        if (lane == 0) *reinterpret_cast<float2*>(attn_part_sum<RB, HD>(a, blockIdx.x, p.slot, r)) = make_float2(l, m);
 #pragma unroll
-        for (int d = 0; d < ND; ++d) pp[2 + lane * ND + d] = o[d];
+        for (int d = 0; d < ND; ++d) pp[lane * ND + d] = o[d];
     } else {
-        const float inv = l > 0.f ? 1.0f / l : (l == 0.f ? 0.f : l);   // no key: zeros; NaN stays
+        const int t = (int)a.gdiv.div((uint32_t)(p.row + r)), tok = p.tok0 + t;
+        const int head = p.kvh * a.group + p.row + r - t * a.group;
+        const float inv = attn_inv(l);
         float* po = a.out + (size_t)tok * a.ldo + head * HD + lane * ND;
 #pragma unroll
         for (int d = 0; d < ND; ++d) po[d] = o[d] * inv;
-        if (a.lse && lane == 0)
-            a.lse[(size_t)tok * a.nh + head] = l == 0.f ? -INFINITY : (m + log2f(l)) * 0.69314718055994531f;
+        if (a.lse && lane == 0) a.lse[(size_t)tok * a.nh + head] = attn_lse(l, m);
     }
 }
 
 // One row by one warp, key by key: for tiles whose masked values are not finite
 // or whose pages do not exist, which the tensor cores cannot skip.
-template <typename T, int HD>
-__device__ __noinline__ void paged_row_slow(const PagedAttnArgs& a, const SeqView& sv, const int* table, int kvh, int split,
-                                            int row, int k0, int k1) {
+template <typename T, int RB, int HD>
+__device__ __noinline__ void attn_row_slow(const PagedAttnArgs& a, const AttnPiece& p, int r) {
     constexpr int ND = HD / 32;
     const int lane = threadIdx.x & 31;
-    const int tok = sv.row0 + row / a.group, head = kvh * a.group + row % a.group, pos = sv.pos0 + row / a.group;
+    const int* table = a.s.table + (size_t)p.b * a.s.table_ld;
+    const int t = (int)a.gdiv.div((uint32_t)(p.row + r)), tok = p.tok0 + t, pos = p.pos0 + t;
+    const int head = p.kvh * a.group + p.row + r - t * a.group;
     float q[ND], o[ND], kf[ND], vf[ND];
     pr_load<float, ND>(reinterpret_cast<const unsigned char*>(a.q + (size_t)tok * a.ldq + head * HD + lane * ND), q);
 #pragma unroll
     for (int d = 0; d < ND; ++d) q[d] *= a.scale2, o[d] = 0.f;
     float m = -INFINITY, l = 0.f;
+    int k0 = max(p.k0, p.first);
     if (a.window) k0 = max(k0, pos - a.window + 1);
-    for (int t = k0; t < min(k1, pos + 1); ++t) {
-        const int64_t off = paged_offset(a.kv, table, t);
+    for (int k = k0; k < min(p.k1, pos + 1); ++k) {
+        const int64_t off = paged_offset(a.kv, table, k);
         if (off < 0) continue;
-        const int64_t at = off + (int64_t)kvh * a.kv.head_stride + lane * ND * (int)sizeof(T);
+        const int64_t at = off + (int64_t)p.kvh * a.kv.head_stride + lane * ND * (int)sizeof(T);
         pr_load<T, ND>(a.kv.k + at, kf);
         pr_load<T, ND>(a.kv.v + at, vf);
         float s = 0.f;
@@ -108,13 +306,65 @@ __device__ __noinline__ void paged_row_slow(const PagedAttnArgs& a, const SeqVie
         for (int d = 0; d < ND; ++d) s = fmaf(q[d], kf[d], s);
         s = warp_sum(s);
         const float mn = fmaxf(m, s);
-        const float c = m == mn ? 1.f : exp2f(m - mn), p = s == -INFINITY ? 0.f : exp2f(s - mn);
-        l = l * c + p;
+        const float c = m == mn ? 1.f : exp2f(m - mn), w = s == -INFINITY ? 0.f : exp2f(s - mn);
+        l = l * c + w;
 #pragma unroll
-        for (int d = 0; d < ND; ++d) o[d] = fmaf(o[d], c, p * vf[d]);
+        for (int d = 0; d < ND; ++d) o[d] = fmaf(o[d], c, w * vf[d]);
         m = mn;
     }
-    paged_row_store<HD, ND>(a, split, tok, head, lane, l, m, o);
+    attn_row_store<RB, HD, ND>(a, p, r, l, m, o);
+}
+
+// Joins the pieces of the block that CTA blockIdx.x of the attention kernel
+// began, in key order; a warp a row.
+template <int RB, int HD>
+__global__ void __launch_bounds__(256) paged_merge_kernel(const __grid_constant__ PagedAttnArgs a) {
+    constexpr int ND = HD / 32;
+    pdl_wait();
+    const int c0 = blockIdx.x, lane = threadIdx.x & 31;
+    const int* h = a.header + c0 * 8;
+    const int rows = h[0];
+    if (!rows) return;
+    AttnPiece p;
+    p.tok0 = h[1], p.row = h[2], p.kvh = h[3];
+    p.slot = -1;
+    const int last = h[4];
+    for (int r = blockIdx.y * 8 + (threadIdx.x >> 5); r < rows; r += gridDim.y * 8) {
+        float M = -INFINITY;
+        for (int c = c0 + lane; c <= last; c += 32) M = fmaxf(M, attn_part_sum<RB, HD>(a, c, c == c0, r)[1]);
+        M = warp_max(M);
+        float L = 0.f, o[ND];
+#pragma unroll
+        for (int d = 0; d < ND; ++d) o[d] = 0.f;
+        for (int c = c0; c <= last; ++c) {
+            const float* x = attn_part<RB, HD>(a, c, c == c0, r);
+            const float2 lm = *reinterpret_cast<const float2*>(attn_part_sum<RB, HD>(a, c, c == c0, r));
+            const float w = lm.y == -INFINITY ? 0.f : exp2f(lm.y - M);
+            if (w != 0.f) {
+                L = fmaf(lm.x, w, L);
+#pragma unroll
+                for (int d = 0; d < ND; ++d) o[d] = fmaf(x[lane * ND + d], w, o[d]);
+            }
+        }
+        attn_row_store<RB, HD, ND>(a, p, r, L, M, o);
+    }
+}
+
+template <int RB, int HD>
+tvb_status launch_merge(const PagedAttnArgs& a, int ctas, cudaStream_t st) {
+    if (!a.balanced) return TVB_OK;
+    TVB_CUDA(launch_maybe_pdl(paged_merge_kernel<RB, HD>, dim3((unsigned)ctas, (unsigned)((RB + 7) / 8)), dim3(256), 0, st, true, a));
+    return check_launch("paged_merge_kernel");
+}
+
+// Workspace of a balanced grid.
+template <int RB, int HD>
+tvb_status attn_workspace(PagedAttnArgs* a, int ctas, Workspace* ws) {
+    const size_t part = (size_t)ctas * 2 * RB * (HD + 2) * 4;
+    TVB_TRY(ws->get(part + (size_t)ctas * 32));
+    a->part = ws->at<float>();
+    a->header = ws->at<int>(part);
+    return TVB_OK;
 }
 
 tvb_status paged_attn_chunk_f16(const PagedAttnArgs& a, int hd, cudaStream_t st);   // attn_paged_tc.cu

@@ -1,34 +1,56 @@
 // Attention of chunks of new tokens over an F16 paged cache on the tensor cores
-// (tvb_attention_paged; attn_paged.cu has the formula and the split).
+// (tvb_attention_paged; attn_paged.cu has the formula).
 //
-// paged_chunk_kernel: a CTA takes 128 query rows (new token x query head of the
-// group) of one KV head of one sequence, and one split of its keys in tiles of
-// 128.  Products in F32 accuracy from F16 operands: q (times scale log2 e, with
-// a power-of-two exponent a row) and p are split into F16 hi + lo planes, K and
-// V are F16 as they are, so every product takes two MMAs.
+// paged_chunk_kernel: one CTA an SM takes its run of tiles (attn_schedule):
+// blocks of 128 query rows (new token x query head of the group) of one KV head
+// of one sequence against tiles of 128 keys.  Products in F32 accuracy from F16
+// operands: q (times scale log2 e, with a power-of-two exponent a row) and p are
+// split into F16 hi + lo planes, K and V are F16 as they are, so every product
+// takes two MMAs and the bound is the tensor pipe at twice the algorithmic FLOPs.
 //
-//   loader warps (a slot of shared memory at a time each): rows of K or V by 16-byte cp.async,
-//     page by page, into the 128-byte swizzle; rows without a key become zeros
-//   MMA warp: S = Q K^T (K-major operands) into one of three TMEM buffers a tile
-//     ahead of the softmax, then O = P V with P from TMEM and V as the MN-major
-//     operand it is in memory (no transpose)
-//   softmax warps: two threads a row, each half of the tile's keys (maxima meet in
-//     shared memory) and half of the dimensions; running maximum, p as hi + lo
-//     over its S columns in TMEM, and O (a fresh product per tile) added to
-//     registers with the rescaling, which also keeps the tensor core's truncating sums short (16
-//     MMAs: 3e-7; a sum over 6000 keys in TMEM would lose 1.4e-5)
+//   loader warps (a slot of shared memory at a time each): K or V by TMA, a box of
+//     rows a lane, page by page (pages that no box of 8 rows divides: by 16-byte
+//     cp.async); in V rows behind the last key become zeros
+//   MMA warp: S = Q K^T (K-major operands) into one of two TMEM buffers, then O =
+//     P V with P from TMEM and V as the MN-major operand it is in memory (no
+//     transpose): PV(j), S(j + 2), PV(j + 1), S(j + 3), ...
+//   softmax warps, two groups of 128 threads, thread = row: a group takes every
+//     other tile (its own running maximum and sum, p as hi + lo over the S columns
+//     in TMEM), so that one group's exponentials run under the other's MMAs.  Both
+//     add every tile's O, half of the dimensions each, to registers with the
+//     rescaling; a fresh product per tile also keeps the tensor core's truncating
+//     sums short (16 MMAs: 3e-7; a sum over 6000 keys in TMEM would lose 1.4e-5)
 //
 // A masked probability is zero but 0 x inf is not: a loader that finds a
 // non-finite value in a V tile that some row does not see whole, or a page that
-// does not exist, flags the CTA, which then computes its rows key by key instead.
+// does not exist, marks the piece, whose rows are then computed key by key.
 #include "attn_paged.h"
+#include "prefill.h"
 #include "tcgen05.cuh"
 
 namespace tvb {
 
 constexpr int kPcRows = 128, kPcKeys = 128, kPcSlots = 4;
 // Warps 0-7 softmax, 8-10 loaders, 11 MMA: 12 warps leave a thread 168 registers.
-constexpr int kPcThreads = 384, kPcSoft = 8, kPcLoaders = 3, kPcMmaWarp = kPcSoft + kPcLoaders;
+constexpr int kPcSoft = 8, kPcLoaders = 3, kPcMmaWarp = kPcSoft + kPcLoaders, kPcThreads = 32 * (kPcMmaWarp + 1);
+
+// Barriers and flags of a CTA.
+struct PcShared {
+    uint64_t full[kPcSlots], empty[kPcSlots];
+    uint64_t s_full[2], p_full[2], o_full[2], o_read[2];
+    uint64_t q_full, drained;
+    uint64_t fix[kPcLoaders];   // a V tile that its loader looks over
+    uint32_t tmem;
+    int abort;
+    int slow, slow_done;        // warps that compute rows key by key now; how many have done so
+    int gone[4];                // a warp of the pair gave up
+    int poison[8];              // [piece % 8] = piece + 1: marked
+    float f[128];               // q scale log2 e = (hi + lo) f
+    float m[4][128];            // row maxima that a tile's p refer to
+    AttnRun run;
+    AttnPiece piece[kPcMmaWarp + 1];   // of each warp
+    float sum[2][2][128];       // a row's sum and maximum in each group, at the end of a piece
+};
 
 template <int HD>
 struct PcSmem {
@@ -36,9 +58,9 @@ struct PcSmem {
     static constexpr int kPlane = kAtom * (HD / 64);      // Q plane, K or V tile
     static constexpr int kQ = 0;
     static constexpr int kSlots = 2 * kPlane;
-    static constexpr int kBar = kSlots + kPcSlots * kPlane;
-    static constexpr int kRed = kBar + 256;                   // row maxima of the two halves, two tiles
-    static constexpr int kBytes = kRed + 2 * 2 * 128 * 4 + 1024;   // alignment
+    static constexpr int kShared = kSlots + kPcSlots * kPlane;
+    static constexpr int kSched = kShared + (int)((sizeof(PcShared) + 127) / 128 * 128);
+    static constexpr int kBytes = kSched + (int)sizeof(AttnSchedule) + 1024;   // alignment
 };
 
 // Shared-memory descriptor of an MN-major operand in 128-byte-swizzled atoms of
@@ -63,6 +85,14 @@ __device__ __forceinline__ void tc_mma_ts(uint32_t tmem_d, uint32_t tmem_a, uint
         : "memory");
 }
 
+__device__ __forceinline__ void tmem_ld16(uint32_t taddr, uint32_t (&r)[16]) {
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, "
+        "%15}, [%16];"
+        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
+          "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+        : "r"(taddr));
+}
 __device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t (&r)[16]) {
     asm volatile(
         "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, "
@@ -83,352 +113,554 @@ __device__ __forceinline__ float ex2(float x) {
     return y;
 }
 
+// Two F32 operations an instruction.
+__device__ __forceinline__ uint64_t pack2(float x, float y) {
+    uint64_t r;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(x), "f"(y));
+    return r;
+}
+__device__ __forceinline__ float2 unpack2(uint64_t v) {
+    float2 r;
+    asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(v));
+    return r;
+}
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+    uint64_t r;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+    return r;
+}
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
+    uint64_t r;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+}
+
+__device__ __forceinline__ void tma_load_4d(uint32_t dst, const CUtensorMap* map, int x, int y, int z, int w, uint64_t* bar) {
+    asm volatile(
+        "cp.async.bulk.tensor.4d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5}], [%6];" ::"r"(
+            dst),
+        "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y), "r"(z), "r"(w), "r"(smem_u32(bar))
+        : "memory");
+}
+
+// K and V pools as [page][row][head][dim], boxes of `box` rows of one head and 64
+// dimensions; box 0: no maps (cp.async).
+struct PcMaps {
+    CUtensorMap k, v;
+};
+
 __device__ __forceinline__ void pc_cp_async16(uint32_t dst, const void* src, bool valid) {
     asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(valid ? 16 : 0) : "memory");
 }
 
 template <int HD>
-__global__ void __launch_bounds__(kPcThreads, 1) paged_chunk_kernel(const __grid_constant__ PagedAttnArgs a) {
+__global__ void __launch_bounds__(kPcThreads, 1)
+paged_chunk_kernel(const __grid_constant__ PcMaps maps, const __grid_constant__ PagedAttnArgs a, int box) {
     using Sm = PcSmem<HD>;
-    constexpr int kO = 3 * kPcKeys;   // TMEM: S/P buffers in columns [0, 384), O behind
+    constexpr int kO = 2 * kPcKeys;   // TMEM: two S/P buffers in columns [0, 256), two O buffers behind
     extern __shared__ unsigned char pc_smem_raw[];
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const int kvh = blockIdx.y, split = blockIdx.z;
-
-    int row0 = 0;
-    const int b = row_block_seq<kPcRows, kPcThreads>(a.s, a.group, blockIdx.x, &row0);
-    if (b >= a.s.n_seqs) return;
-    const SeqView sv = seq_view(a.s, b);
-    if (!sv.ok) {
-        if (threadIdx.x == 0) report_bad(a.status);
-        return;
-    }
-    const int rows = min(kPcRows, sv.n * a.group - row0);
-    if (rows <= 0) return;
-    const int p_first = sv.pos0 + row0 / a.group, p_last = sv.pos0 + (row0 + rows - 1) / a.group;
-    const int lo = a.window ? max(0, p_first - a.window + 1) : 0;
-    const int k0 = a.nsplit > 1 ? max(lo, split * a.split_len) : lo;
-    const int k1 = a.nsplit > 1 ? min(p_last + 1, (split + 1) * a.split_len) : p_last + 1;
-    if (k0 >= k1) return;   // no row of the block takes this split
-    const int nt = (k1 - k0 + kPcKeys - 1) / kPcKeys;
-    const int nitems = 2 * nt;   // K0, then K(j + 1), V(j) for every tile j
-
     const uint32_t raw = smem_u32(pc_smem_raw);
     const uint32_t base = (raw + 1023u) & ~1023u;
     unsigned char* smem = pc_smem_raw + (base - raw);
-    uint64_t* full = reinterpret_cast<uint64_t*>(smem + Sm::kBar);
-    uint64_t* empty = full + kPcSlots;
-    uint64_t* s_full = empty + kPcSlots;   // [3]
-    uint64_t* p_full = s_full + 3;         // [2]
-    uint64_t* o_full = p_full + 2;
-    uint64_t* o_read = o_full + 1;
-    uint64_t* q_full = o_read + 1;
-    uint64_t* drained = q_full + 1;
-    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(drained + 1);
-    volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
-    volatile int* poison = abort_flag + 1;
+    PcShared& sh = *reinterpret_cast<PcShared*>(smem + Sm::kShared);
+    AttnSchedule& sched = *reinterpret_cast<AttnSchedule*>(smem + Sm::kSched);
+    const int align = box ? box : 1;
+
+    // the CTA's pieces: a run of tiles, or the one block of an unbalanced grid
+    AttnPiece only;
+    bool any = true;
+    if (a.balanced) {
+        const AttnRun run = attn_run(a, attn_schedule<kPcRows, kPcKeys, kPcThreads>(a, sched, align));
+        pdl_launch_dependents();
+        any = run.u < run.end;
+        if (threadIdx.x == 0) sh.run = run;
+    } else {
+        any = attn_block<kPcRows, kPcKeys, kPcThreads>(a, align, &only);
+        if (lane == 0 && any) sh.piece[warp] = only;
+    }
+    if (!any) {
+        if (a.balanced && threadIdx.x == 0) attn_header(a, nullptr);
+        return;
+    }
+    int at = 0;   // tiles of this warp's earlier pieces
+    auto next = [&](int i) -> bool {   // whole warp: piece i
+        if (!a.balanced) return i == 0;
+        const int n = attn_next<kPcRows, kPcKeys>(a, sched, sh.run, sh.run.u + at, align, &sh.piece[warp]);
+        at += n;
+        return n != 0;
+    };
 
     if (threadIdx.x == 0) {
         for (int i = 0; i < kPcSlots; ++i) {
-            mbar_init(full + i, 1);
-            mbar_init(empty + i, 1);
+            mbar_init(sh.full + i, 1);
+            mbar_init(sh.empty + i, 1);
         }
-        for (int i = 0; i < 3; ++i) mbar_init(s_full + i, 1);
-        for (int i = 0; i < 2; ++i) mbar_init(p_full + i, 32 * kPcSoft);
-        mbar_init(o_full, 1);
-        mbar_init(o_read, 32 * kPcSoft);
-        mbar_init(q_full, 32 * kPcSoft);
-        mbar_init(drained, 1);
-        *abort_flag = 0;
-        *poison = 0;
+        for (int i = 0; i < 2; ++i) {
+            mbar_init(sh.s_full + i, 1);
+            mbar_init(sh.p_full + i, kPcSoft / 2);
+            mbar_init(sh.o_full + i, 1);
+            mbar_init(sh.o_read + i, kPcSoft);
+        }
+        mbar_init(&sh.q_full, kPcSoft);
+        mbar_init(&sh.drained, 1);
+        for (int i = 0; i < kPcLoaders; ++i) mbar_init(sh.fix + i, 1);
+        sh.abort = 0;
+        sh.slow = sh.slow_done = 0;
+        for (int i = 0; i < 4; ++i) sh.gone[i] = 0;
+        for (int i = 0; i < 8; ++i) sh.poison[i] = 0;
         fence_barrier_init();
     }
-    if (warp == kPcMmaWarp) tmem_alloc(tmem_slot, 512);
+    if (warp == kPcMmaWarp) tmem_alloc(&sh.tmem, 512);
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
-    const uint32_t tmem = *tmem_slot;
+    const uint32_t tmem = sh.tmem;
+    volatile int* abort_flag = &sh.abort;
+    volatile int *slow = &sh.slow, *slow_done = &sh.slow_done;
     auto fail = [&]() {
         *abort_flag = 1;
         if (a.status) atomicOr(a.status, TVB_DEV_TIMEOUT);
     };
-    const int* table = a.s.table + (size_t)b * a.s.table_ld;
+    // bounded wait; rows computed key by key may take longer than its limit
+    auto landed = [&](uint64_t* bar, int phase) -> bool {
+        if (mbar_try_wait(bar, (uint32_t)(phase & 1))) return true;
+        int seen = *slow_done;
+        while (!mbar_wait_bounded(bar, (uint32_t)(phase & 1))) {
+            const int done = *slow_done;
+            if (*abort_flag || (done == seen && !*slow)) return false;
+            seen = done;
+        }
+        return true;
+    };
 
-    if (warp >= kPcSoft && warp < kPcMmaWarp) {
+    // the softmax warps' registers: 128 x (200 + 200 + 104) = 384 x 168, what the CTA was launched with
+    if (warp >= kPcSoft) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 104;");
+    if (warp < kPcMmaWarp) {
         // ---- loaders ---------------------------------------------------------------
         const int w = warp - kPcSoft;
-        constexpr int kLanes = HD / 8;          // 16-byte chunks, lanes a row
+        constexpr int kLanes = HD / 8;          // 16-byte chunks, lanes a row (cp.async)
         constexpr int kPass = 32 / kLanes;      // rows a warp instruction
         const int c = lane % kLanes;
-        for (int i = w; i < nitems; i += kPcLoaders) {
-            const int sl = i % kPcSlots;
-            const uint32_t slot = base + Sm::kSlots + sl * Sm::kPlane;
-            const bool is_k = i == 0 || ((i & 1) && i != nitems - 1);
-            const int tile = i == 0 ? 0 : is_k ? (i + 1) >> 1 : i == nitems - 1 ? nt - 1 : (i >> 1) - 1;
-            const bool free_slot = mbar_wait_bounded(empty + sl, (uint32_t)((i / kPcSlots + 1) & 1));
-            if (__any_sync(0xffffffffu, !free_slot || *abort_flag)) {
-                fail();
-                break;
-            }
-            const unsigned char* src = (is_k ? a.kv.k : a.kv.v) + (int64_t)kvh * a.kv.head_stride + c * 16;
-            const int t0 = k0 + tile * kPcKeys;
-            bool bad = false;
-#pragma unroll
-            for (int r0 = 0; r0 < kPcKeys; r0 += 32) {
-                int64_t off = -1;
-                if (t0 + r0 + lane < k1) {
-                    off = paged_offset(a.kv, table, t0 + r0 + lane);
-                    bad |= off < 0;
+        int fixes = 0;
+        int issued = -1;   // last item whose boxes were requested on `full`
+        if (box && w == 0 && lane == 0) {
+            prefetch_tmap(&maps.k);
+            prefetch_tmap(&maps.v);
+        }
+        const AttnPiece& p = sh.piece[warp];
+        bool ok = true;
+        int item0 = 0;   // items of earlier pieces: K0, K1, then V(j), K(j + 2) for every tile j
+        for (int pi = 0; ok && next(pi); item0 += 2 * p.tiles, ++pi) {
+            const int nt = p.tiles, nitems = 2 * nt;
+            const int* table = a.s.table + (size_t)p.b * a.s.table_ld;
+            const int p_first = p.pos0 + (int)a.gdiv.div((uint32_t)p.row);
+            const int p_last = p.pos0 + (int)a.gdiv.div((uint32_t)(p.row + p.rows - 1));
+            for (int i = 0; i < nitems; ++i) {
+                const int gi = item0 + i;
+                if (gi % kPcLoaders != w) continue;
+                const int sl = gi % kPcSlots;
+                const uint32_t slot = base + Sm::kSlots + sl * Sm::kPlane;
+                const bool is_k = i != nitems - 1 && (i == 0 || (i & 1));
+                const int tile = i == 0 ? 0 : is_k ? (i + 1) >> 1 : i == nitems - 1 ? nt - 1 : (i >> 1) - 1;
+                const bool free_slot = landed(sh.empty + sl, gi / kPcSlots + 1);
+                if (__any_sync(0xffffffffu, !free_slot || *abort_flag)) {
+                    fail();
+                    ok = false;
+                    break;
                 }
-#pragma unroll
-                for (int r = 0; r < 32; r += kPass) {
-                    const int64_t o = __shfl_sync(0xffffffffu, off, r + lane / kLanes);
-                    const int row = r0 + r + lane / kLanes;
-                    pc_cp_async16(slot + (c >> 3) * Sm::kAtom + sw128_offset(row, c & 7), src + (o >= 0 ? o : 0), o >= 0);
+                const int t0 = p.k0 + tile * kPcKeys, t1 = min(t0 + kPcKeys, p.k1);
+                // V rows that some query row does not see must be finite, those behind the last key zero
+                const bool look = !is_k && (t1 - t0 < kPcKeys || t1 - 1 > p_first || t0 < p.first ||
+                                            (a.window && t0 <= p_last - a.window));
+                bool bad = false;
+                if (box) {
+                    // one box a lane: `box` rows x 64 dimensions
+                    const int per = kPcKeys / box, n = per * (HD / 64), row = (lane % per) * box, at = lane / per;
+                    int page = -1, in = 0;
+                    if (lane < n && t0 + row < p.k1) {
+                        const uint32_t t = (uint32_t)(t0 + row), pg = a.kv.page.div(t);
+                        in = (int)(t - pg * a.kv.page.d);
+                        page = __ldg(table + pg);
+                        if ((unsigned)page >= (unsigned)a.kv.n_pages) {
+                            page = -1;
+                            bad = true;
+                        }
+                    }
+                    const unsigned go = __ballot_sync(0xffffffffu, page >= 0);
+                    uint64_t* bar = look ? sh.fix + w : sh.full + sl;
+                    if (bad) {
+                        *reinterpret_cast<volatile int*>(&sh.poison[pi & 7]) = pi + 1;
+                        report_bad(a.status);
+                    }
+                    __syncwarp();
+                    if (lane == 0) mbar_expect_tx(bar, (uint32_t)(__popc(go) * box * 128));
+                    __syncwarp();
+                    if (page >= 0)
+                        tma_load_4d(slot + at * Sm::kAtom + row * 128, is_k ? &maps.k : &maps.v, at * 64, p.kvh, in, page, bar);
+                    if (!look) {
+                        issued = gi;
+                        continue;
+                    }
+                    const bool in_time = mbar_wait_bounded(bar, (uint32_t)(fixes++ & 1));
+                    if (__any_sync(0xffffffffu, !in_time)) {
+                        fail();
+                        ok = false;
+                        break;
+                    }
+                } else {
+                    const unsigned char* src = (is_k ? a.kv.k : a.kv.v) + (int64_t)p.kvh * a.kv.head_stride + c * 16;
+#pragma unroll 1
+                    for (int r0 = 0; r0 < kPcKeys; r0 += 32) {
+                        int64_t off = -1;
+                        if (t0 + r0 + lane < p.k1) {
+                            off = paged_offset(a.kv, table, t0 + r0 + lane);
+                            bad |= off < 0;
+                        }
+#pragma unroll 4
+                        for (int r = 0; r < 32; r += kPass) {
+                            const int64_t o = __shfl_sync(0xffffffffu, off, r + lane / kLanes);
+                            const int row = r0 + r + lane / kLanes;
+                            pc_cp_async16(slot + (c >> 3) * Sm::kAtom + sw128_offset(row, c & 7), src + (o >= 0 ? o : 0), o >= 0);
+                        }
+                    }
+                    asm volatile("cp.async.commit_group;" ::: "memory");
+                    asm volatile("cp.async.wait_group 0;" ::: "memory");
+                    if (bad) {
+                        *reinterpret_cast<volatile int*>(&sh.poison[pi & 7]) = pi + 1;
+                        report_bad(a.status);
+                    }
                 }
-            }
-            asm volatile("cp.async.commit_group;" ::: "memory");
-            if (bad) {
-                *poison = 1;
-                report_bad(a.status);
-            }
-            asm volatile("cp.async.wait_group 0;" ::: "memory");
-            // V rows that some query row does not see must be finite
-            const int t1 = min(t0 + kPcKeys, k1);
-            if (!is_k && (t1 - 1 > p_first || (a.window && t0 <= p_last - a.window))) {
+                if (look) {
+                    __syncwarp();
+                    uint32_t nonfinite = 0;
+                    for (int j = lane; j < Sm::kPlane / 16; j += 32) {
+                        const int key = (j * 16 % Sm::kAtom) / 128;
+                        uint4* at = reinterpret_cast<uint4*>(smem + Sm::kSlots + sl * Sm::kPlane + j * 16);
+                        if (t0 + key >= p.k1) {
+                            *at = make_uint4(0u, 0u, 0u, 0u);
+                        } else {
+                            const uint4 v = *at;
+                            const uint32_t u[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+                            for (int e = 0; e < 4; ++e)
+                                nonfinite |= (uint32_t)((u[e] & 0x7C00u) == 0x7C00u) | (uint32_t)((u[e] & 0x7C000000u) == 0x7C000000u);
+                        }
+                    }
+                    if (nonfinite) *reinterpret_cast<volatile int*>(&sh.poison[pi & 7]) = pi + 1;
+                }
+                fence_proxy_async_smem_cta();
                 __syncwarp();
-                uint32_t nonfinite = 0;
-                for (int j = lane; j < Sm::kPlane / 4; j += 32) {
-                    const uint32_t v = *reinterpret_cast<const volatile uint32_t*>(smem + Sm::kSlots + sl * Sm::kPlane + j * 4);
-                    nonfinite |= (uint32_t)((v & 0x7C00u) == 0x7C00u) | (uint32_t)((v & 0x7C000000u) == 0x7C000000u);
-                }
-                if (nonfinite) *poison = 1;
+                if (lane == 0) mbar_arrive(sh.full + sl);
             }
-            fence_proxy_async_smem_cta();
-            __syncwarp();
-            if (lane == 0) mbar_arrive(full + sl);
         }
         asm volatile("cp.async.wait_all;" ::: "memory");
-    } else if (warp == kPcMmaWarp) {
+        if (box && *abort_flag) {   // no TMA write may outlive the CTA: the last two items cover every slot still in flight
+            for (int i = max(w, issued - kPcLoaders); i <= issued; i += kPcLoaders)
+                mbar_wait_bounded(sh.full + i % kPcSlots, (uint32_t)((i / kPcSlots) & 1));
+        }
+    } else {
         // ---- MMA issuer --------------------------------------------------------------
-        if (lane == 0) {
-            constexpr uint32_t idesc_s = umma_idesc_f16(kPcRows, kPcKeys);
-            constexpr uint32_t idesc_o = umma_idesc_f16(kPcRows, HD) | (1u << 16);   // B is MN-major
-            int item = 0;
-            auto ready = [&](int i) {
-                if (!mbar_wait_bounded(full + i % kPcSlots, (uint32_t)((i / kPcSlots) & 1))) return false;
-                tc_fence_after();
-                return true;
-            };
-            auto mma_s = [&](int j) {
-                const uint32_t k_s = base + Sm::kSlots + (item % kPcSlots) * Sm::kPlane, d = tmem + (j % 3) * kPcKeys;
-#pragma unroll
-                for (int kk = 0; kk < HD / 16; ++kk) {
-                    const uint32_t o = (kk >> 2) * Sm::kAtom + (kk & 3) * 32;
-                    const uint64_t kd = sw128_desc(k_s + o);
-                    tc_mma(d, sw128_desc(base + Sm::kQ + o), kd, idesc_s, kk ? 1u : 0u);
-                    tc_mma(d, sw128_desc(base + Sm::kQ + Sm::kPlane + o), kd, idesc_s, 1u);
-                }
-                tc_commit(s_full + j % 3);
-            };
-            bool ok = mbar_wait_bounded(q_full, 0u) && ready(0);
-            if (ok) {
-                tc_fence_after();
-                mma_s(0);
-                tc_commit(empty + 0);
-                ++item;
-            }
-            for (int j = 0; ok && j < nt && !*abort_flag; ++j) {
-                if (j + 1 < nt) {
-                    ok = ready(item);
-                    if (!ok) break;
-                    mma_s(j + 1);
-                    tc_commit(empty + item % kPcSlots);
+        constexpr uint32_t idesc_s = umma_idesc_f16(kPcRows, kPcKeys);
+        constexpr uint32_t idesc_o = umma_idesc_f16(kPcRows, HD) | (1u << 16);   // B is MN-major
+        int item = 0, tile = 0;   // over all pieces
+        const AttnPiece& p = sh.piece[warp];
+        bool ok = true;
+        for (int pi = 0; ok && next(pi); ++pi) {
+            if (lane == 0) {
+                auto ready = [&]() { return landed(sh.full + item % kPcSlots, item / kPcSlots); };
+                auto mma_s = [&](int j) {   // tile j (of all) takes the buffer of P(j - 2)
+                    const uint32_t k_s = base + Sm::kSlots + (item % kPcSlots) * Sm::kPlane, d = tmem + (j & 1) * kPcKeys;
+                    tc_fence_after();
+#pragma unroll 1
+                    for (int kk = 0; kk < HD / 16; ++kk) {
+                        const uint32_t o = (kk >> 2) * Sm::kAtom + (kk & 3) * 32;
+                        const uint64_t kd = sw128_desc(k_s + o);
+                        tc_mma(d, sw128_desc(base + Sm::kQ + o), kd, idesc_s, kk ? 1u : 0u);
+                        tc_mma(d, sw128_desc(base + Sm::kQ + Sm::kPlane + o), kd, idesc_s, 1u);
+                    }
+                    tc_commit(sh.s_full + (j & 1));
+                    tc_commit(sh.empty + item % kPcSlots);
                     ++item;
+                };
+                const int end = tile + p.tiles;
+                ok = landed(&sh.q_full, pi);
+                for (int j = tile; ok && j < min(end, tile + 2); ++j) {
+                    ok = ready() && (j < 2 || landed(sh.o_full + (j & 1), (j - 2) >> 1));
+                    if (ok) mma_s(j);
                 }
-                ok = mbar_wait_bounded(p_full + (j & 1), (uint32_t)((j >> 1) & 1)) && ready(item) &&
-                     (j == 0 || mbar_wait_bounded(o_read, (uint32_t)((j - 1) & 1)));
-                if (!ok) break;
-                tc_fence_after();
-                const uint32_t v_s = base + Sm::kSlots + (item % kPcSlots) * Sm::kPlane, p = tmem + (j % 3) * kPcKeys;
-#pragma unroll
-                for (int kk = 0; kk < kPcKeys / 16; ++kk) {
-                    const uint64_t vd = sw128_mn_desc(v_s + kk * 2048, Sm::kAtom);
-                    tc_mma_ts(tmem + kO, p + kk * 16, vd, idesc_o, kk ? 1u : 0u);
-                    tc_mma_ts(tmem + kO, p + kk * 16 + 8, vd, idesc_o, 1u);
+                for (int j = tile; ok && j < end; ++j) {
+                    ok = ready() && (j < 2 || landed(sh.o_read + (j & 1), (j - 2) >> 1)) && landed(sh.p_full + (j & 1), j >> 1);
+                    if (!ok) break;
+                    tc_fence_after();
+                    const uint32_t v_s = base + Sm::kSlots + (item % kPcSlots) * Sm::kPlane;
+                    const uint32_t pt = tmem + (j & 1) * kPcKeys, ot = tmem + kO + (j & 1) * HD;
+#pragma unroll 1
+                    for (int kk = 0; kk < kPcKeys / 16; ++kk) {
+                        const uint64_t vd = sw128_mn_desc(v_s + kk * 2048, Sm::kAtom);
+                        tc_mma_ts(ot, pt + kk * 16, vd, idesc_o, kk ? 1u : 0u);
+                        tc_mma_ts(ot, pt + kk * 16 + 8, vd, idesc_o, 1u);
+                    }
+                    tc_commit(sh.o_full + (j & 1));
+                    tc_commit(sh.empty + item % kPcSlots);
+                    ++item;
+                    if (j + 2 < end) {
+                        ok = ready() && landed(sh.o_full + (j & 1), j >> 1);   // S(j + 2) takes the place of P(j)
+                        if (ok) mma_s(j + 2);
+                    }
                 }
-                tc_commit(o_full);
-                tc_commit(empty + item % kPcSlots);
-                ++item;
+                if (!ok) fail();
             }
-            if (!ok) fail();
-            tc_commit(drained);   // every MMA issued above
-            mbar_wait_bounded(drained, 0u);
+            ok = __shfl_sync(0xffffffffu, (int)ok, 0) != 0;
+            tile += p.tiles;
+        }
+        if (lane == 0) {
+            tc_commit(&sh.drained);   // every MMA issued above
+            mbar_wait_bounded(&sh.drained, 0u);
         }
         __syncwarp();
+    }
     } else {
-        // ---- softmax: two threads a row, each half of a tile's keys and of the dimensions ----
-        const int r = threadIdx.x & 127, half = warp >> 2;
-        const bool live = r < rows;
-        const int row = row0 + min(r, rows - 1);
-        const int tok = sv.row0 + row / a.group, head = kvh * a.group + row % a.group;
-        const int pos = live ? sv.pos0 + row / a.group : -1;
-        float* red = reinterpret_cast<float*>(smem + Sm::kRed);
-        auto pair_sync = [&]() { asm volatile("bar.sync %0, 64;" ::"r"(1 + (warp & 3)) : "memory"); };
-        float f = 1.f;   // q = (hi + lo) f / (scale log2 e)
-        {
-            const float* q = a.q + (size_t)tok * a.ldq + head * HD;
-            float mx = 0.f;
-#pragma unroll 4
-            for (int d = 0; d < HD; d += 4) {
-                const float4 x = *reinterpret_cast<const float4*>(q + d);
-                mx = fmaxf(mx, fmaxf(fmaxf(fabsf(x.x), fabsf(x.y)), fmaxf(fabsf(x.z), fabsf(x.w))));
-            }
-            mx *= fabsf(a.scale2);
-            // 2^e with mx / 2^e in [2^13, 2^14): both planes of every value that matters are normal F16
-            int e = 0;
-            if (mx > 0.f && mx < INFINITY) e = max(-100, min(100, (int)((__float_as_uint(mx) >> 23) & 255) - 127 - 13));
-            f = __uint_as_float((uint32_t)(127 + e) << 23);
-            const float g = a.scale2 * __uint_as_float((uint32_t)(127 - e) << 23);
-#pragma unroll 2
-            for (int d = half * (HD / 2); d < (half + 1) * (HD / 2); d += 8) {
-                const float4 x = *reinterpret_cast<const float4*>(q + d), y = *reinterpret_cast<const float4*>(q + d + 4);
-                const float v[8] = {x.x * g, x.y * g, x.z * g, x.w * g, y.x * g, y.y * g, y.z * g, y.w * g};
-                __half2 hi[4], lo2[4];
-#pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    hi[i] = __floats2half2_rn(v[2 * i], v[2 * i + 1]);
-                    const float2 h = __half22float2(hi[i]);
-                    lo2[i] = __floats2half2_rn(v[2 * i] - h.x, v[2 * i + 1] - h.y);
-                }
-                const int c = d >> 3;
-                unsigned char* dst = smem + Sm::kQ + (c >> 3) * Sm::kAtom + sw128_offset(r, c & 7);
-                *reinterpret_cast<uint4*>(dst) = *reinterpret_cast<const uint4*>(hi);
-                *reinterpret_cast<uint4*>(dst + Sm::kPlane) = *reinterpret_cast<const uint4*>(lo2);
-            }
-            fence_proxy_async_smem_cta();
-            mbar_arrive(q_full);
-        }
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 200;");
+        // ---- softmax: thread = row; group `half` takes the tiles of its parity, and half of the dimensions ----
         constexpr int kD = HD / 2;   // dimensions of this thread
-        float acc[kD];
-#pragma unroll
-        for (int d = 0; d < kD; ++d) acc[d] = 0.f;
-        float m = -INFINITY, l = 0.f, corr_prev = 1.f;
+        const int r = threadIdx.x & 127, half = warp >> 2;
         const uint32_t lanes = tmem + ((uint32_t)(32 * (warp & 3)) << 16);
-        auto add_o = [&](float c) {   // acc = acc c + O of the last product
-#pragma unroll
-            for (int h = 0; h < kD / 32; ++h) {
-                uint32_t o[32];
-                tmem_ld32(lanes + kO + half * kD + h * 32, o);
-                tmem_wait_ld();
-#pragma unroll
-                for (int i = 0; i < 32; ++i) acc[h * 32 + i] = fmaf(acc[h * 32 + i], c, __uint_as_float(o[i]));
-            }
+        auto pair_sync = [&]() { asm volatile("bar.sync %0, 64;" ::"r"(1 + (warp & 3)) : "memory"); };
+        // one arrival a warp: 32 on one word would take the shared-memory pipe 32 cycles
+        auto warp_arrive = [&](uint64_t* bar) {
+            __syncwarp();
+            if (lane == 0) mbar_arrive(bar);
         };
-        auto landed = [&](uint64_t* bar, int phase) {
-            const bool in = mbar_wait_bounded(bar, (uint32_t)(phase & 1));
-            return __all_sync(0xffffffffu, in && !*abort_flag) != 0;
+        auto all_landed = [&](uint64_t* bar, int phase) -> bool {
+            return __all_sync(0xffffffffu, landed(bar, phase) && !*abort_flag) != 0;
         };
+        const AttnPiece& p = sh.piece[warp];
         bool ok = true;
-        for (int j = 0; j < nt; ++j) {
-            ok = ok && landed(s_full + j % 3, j / 3);
-            // a warp that gives up tells its partner through the exchange below (a maximum is never NaN), so both leave
-            if (!ok) red[((j & 1) * 2 + half) * 128 + r] = NAN;
-            const uint32_t sb = lanes + (j % 3) * kPcKeys + half * 64;
-            const int t0 = k0 + j * kPcKeys;
-            const int t1 = min(t0 + kPcKeys, k1);
-            const bool edge = t1 - t0 < kPcKeys || t1 - 1 > p_first || (a.window && t0 <= p_last - a.window);
-            uint32_t s[64];
-            if (ok) {
-                tc_fence_after();
-                tmem_ld32(sb, *reinterpret_cast<uint32_t(*)[32]>(s));
-                tmem_ld32(sb + 32, *reinterpret_cast<uint32_t(*)[32]>(s + 32));
-                tmem_wait_ld();
-                if (edge) {   // keys [first, last] of this half are the row's
-                    const int last = min(t1 - 1, pos) - t0 - half * 64;
-                    const int first = a.window ? pos - a.window + 1 - t0 - half * 64 : 0;
+        bool begun = false;   // a cut block that this CTA begins
+        int tile = 0;
+        for (int pi = 0; ok && next(pi); tile += p.tiles, ++pi) {
+            const bool live = r < p.rows;
+            const int row = p.row + min(r, p.rows - 1);
+            const int t = (int)a.gdiv.div((uint32_t)row);
+            const int tok = p.tok0 + t, head = p.kvh * a.group + row - t * a.group;
+            const int pos = live ? p.pos0 + t : -1;
+            const int p_first = p.pos0 + (int)a.gdiv.div((uint32_t)p.row);
+            const int p_last = p.pos0 + (int)a.gdiv.div((uint32_t)(p.row + p.rows - 1));
+            {
+                // q times scale log2 e as hi + lo planes with a power-of-two factor a row.  A warp takes 16 rows, all
+                // requested before the first is used; lane = 4 dimensions (HD 64: two rows a pass).
+                constexpr int kPer = 128 / HD, kLoads = 16 / kPer;   // rows a pass, passes
+                const int sub = lane / (HD / 4), d = lane % (HD / 4) * 4;
+                float4 x[kLoads];
 #pragma unroll
-                    for (int i = 0; i < 64; ++i)
-                        if (i > last || i < first) s[i] = 0xff800000u;   // -infinity
+                for (int k = 0; k < kLoads; ++k) {
+                    const int qr = p.row + min(warp * 16 + k * kPer + sub, p.rows - 1), qt = (int)a.gdiv.div((uint32_t)qr);
+                    x[k] = __ldg(reinterpret_cast<const float4*>(a.q + (size_t)(p.tok0 + qt) * a.ldq +
+                                                                 (p.kvh * a.group + qr - qt * a.group) * HD + d));
                 }
-                float m4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
-                for (int i = 0; i < 64; ++i) m4[i & 3] = fmaxf(m4[i & 3], __uint_as_float(s[i]));
-                red[((j & 1) * 2 + half) * 128 + r] = fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3]));
-            }
-            pair_sync();
-            const float x0 = red[(j & 1) * 256 + r], x1 = red[(j & 1) * 256 + 128 + r];
-            if (__any_sync(0xffffffffu, x0 != x0 || x1 != x1)) {
-                ok = false;
-                break;
-            }
-            const float mn = fmaxf(m, fmaxf(x0, x1) * f);
-            const float corr = m == mn ? 1.f : ex2(m - mn);
-            const float mref = mn == -INFINITY ? 0.f : mn;
-            float sum[4] = {0.f, 0.f, 0.f, 0.f};
+                for (int k = 0; k < kLoads; ++k) {
+                    const int qr = warp * 16 + k * kPer + sub;
+                    const float4 y = make_float4(x[k].x * a.scale2, x[k].y * a.scale2, x[k].z * a.scale2, x[k].w * a.scale2);
+                    // the largest magnitude by its bits, infinities and NaN apart
+                    uint32_t mx = max(max(__float_as_uint(fabsf(y.x)), __float_as_uint(fabsf(y.y))),
+                                      max(__float_as_uint(fabsf(y.z)), __float_as_uint(fabsf(y.w))));
+                    if constexpr (HD == 128) {
+                        mx = __reduce_max_sync(0xffffffffu, mx);
+                    } else {
 #pragma unroll
-            for (int c = 0; c < 4; ++c) {   // 16 keys: 8 columns of hi, 8 of lo, in place of their scores
-                uint32_t p[16];
+                        for (int o = 8; o > 0; o >>= 1) mx = max(mx, __shfl_xor_sync(0xffffffffu, mx, o));
+                    }
+                    // 2^e with the largest / 2^e in [2^13, 2^14): both planes of every value that matters are normal F16
+                    const int e = mx > 0u && mx < 0x7f800000u ? max(-100, min(100, (int)(mx >> 23) - 127 - 13)) : 0;
+                    const float g = __uint_as_float((uint32_t)(127 - e) << 23);
+                    const float v[4] = {y.x * g, y.y * g, y.z * g, y.w * g};
+                    __half2 hi[2], lo[2];
 #pragma unroll
-                for (int i = 0; i < 8; ++i) {
-                    const float x = ex2(fmaf(__uint_as_float(s[16 * c + 2 * i]), f, -mref));
-                    const float y = ex2(fmaf(__uint_as_float(s[16 * c + 2 * i + 1]), f, -mref));
-                    sum[(2 * i) & 3] += x;
-                    sum[(2 * i + 1) & 3] += y;
-                    const __half2 hi = __floats2half2_rn(x, y);
-                    const float2 h = __half22float2(hi);
-                    const __half2 lw = __floats2half2_rn(x - h.x, y - h.y);
-                    p[i] = *reinterpret_cast<const uint32_t*>(&hi);
-                    p[8 + i] = *reinterpret_cast<const uint32_t*>(&lw);
+                    for (int i = 0; i < 2; ++i) {
+                        hi[i] = __floats2half2_rn(v[2 * i], v[2 * i + 1]);
+                        const float2 h = __half22float2(hi[i]);
+                        lo[i] = __floats2half2_rn(v[2 * i] - h.x, v[2 * i + 1] - h.y);
+                    }
+                    unsigned char* dst = smem + Sm::kQ + (d >> 6) * Sm::kAtom + sw128_offset(qr, (d >> 3) & 7) + (d & 4) * 2;
+                    *reinterpret_cast<uint2*>(dst) = *reinterpret_cast<const uint2*>(hi);
+                    *reinterpret_cast<uint2*>(dst + Sm::kPlane) = *reinterpret_cast<const uint2*>(lo);
+                    if (d == 0) sh.f[qr] = __uint_as_float((uint32_t)(127 + e) << 23);
                 }
-                tmem_st16(sb + 16 * c, p);
+                fence_proxy_async_smem_cta();
+                warp_arrive(&sh.q_full);
             }
-            tmem_wait_st();
-            tc_fence_before();
-            mbar_arrive(p_full + (j & 1));
-            l = l * corr + ((sum[0] + sum[1]) + (sum[2] + sum[3]));
-            m = mn;
-            if (j > 0) {
-                ok = landed(o_full, j - 1);
-                if (ok) {
+            uint64_t acc[kD / 2];   // pairs of dimensions
+#pragma unroll
+            for (int d = 0; d < kD / 2; ++d) acc[d] = 0ull;
+            float m = -INFINITY, l = 0.f;   // of this group's tiles
+            float mo = -INFINITY;           // what acc refers to
+            int added = tile;
+            auto add_o = [&](int upto) -> bool {   // acc += O of the tiles before `upto`
+                for (; added < upto; ++added) {
+                    if (!all_landed(sh.o_full + (added & 1), added >> 1)) return false;
                     tc_fence_after();
-                    add_o(corr_prev);
+                    const float mj = sh.m[added & 3][r], mn = fmaxf(mo, mj);
+                    const float c = mo == mn ? 1.f : ex2(mo - mn), e = mj == mn ? 1.f : ex2(mj - mn);
+                    mo = mn;
+                    const bool plain = __all_sync(0xffffffffu, c == 1.f && e == 1.f);
+                    const uint64_t c2 = pack2(c, c), e2 = pack2(e, e);
+#pragma unroll
+                    for (int h = 0; h < kD / 32; ++h) {
+                        uint32_t o[32];
+                        tmem_ld32(lanes + kO + (added & 1) * HD + half * kD + h * 32, o);
+                        if (!plain) {
+#pragma unroll
+                            for (int i = 0; i < 16; ++i) acc[16 * h + i] = fma2(acc[16 * h + i], c2, 0ull);
+                        }
+                        tmem_wait_ld();
+#pragma unroll
+                        for (int i = 0; i < 16; ++i)
+                            acc[16 * h + i] = fma2(pack2(__uint_as_float(o[2 * i]), __uint_as_float(o[2 * i + 1])), e2, acc[16 * h + i]);
+                    }
                     tc_fence_before();
-                    mbar_arrive(o_read);
+                    warp_arrive(sh.o_read + (added & 1));
+                }
+                return true;
+            };
+            const int end = tile + p.tiles;
+            for (int j = tile + ((tile ^ half) & 1); ok && j < end; j += 2) {
+                ok = add_o(j - 1) && all_landed(sh.s_full + (j & 1), j >> 1);
+                if (!ok) break;
+                const float f = sh.f[r];   // written before the row's scores were
+                tc_fence_after();
+                const uint32_t sb = lanes + (j & 1) * kPcKeys;
+                const int t0 = p.k0 + (j - tile) * kPcKeys, t1 = min(t0 + kPcKeys, p.k1);
+                const bool edge = t1 - t0 < kPcKeys || t0 < p.first || t1 - 1 > p_first || (a.window && t0 <= p_last - a.window);
+                // keys [first, last] of the tile are the row's
+                const int last = min(t1 - 1, pos) - t0, first = max(p.first, a.window ? pos - a.window + 1 : 0) - t0;
+                float m4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+                // loops rolled on purpose: what the three roles run between tiles fits the instruction cache
+#pragma unroll 1
+                for (int c = 0; c < kPcKeys; c += 32) {
+                    uint32_t s[32];
+                    tmem_ld32(sb + c, s);
+                    tmem_wait_ld();
+                    if (edge) {
+#pragma unroll
+                        for (int k = 0; k < 32; ++k)
+                            if (c + k > last || c + k < first) s[k] = 0xff800000u;   // -infinity
+                    }
+#pragma unroll
+                    for (int k = 0; k < 32; ++k) m4[k & 3] = fmaxf(m4[k & 3], __uint_as_float(s[k]));
+                }
+                const float mn = fmaxf(m, fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3])) * f);
+                const float corr = m == mn ? 1.f : ex2(m - mn);
+                const float mref = mn == -INFINITY ? 0.f : mn;
+                const uint64_t f2 = pack2(f, f), m2 = pack2(-mref, -mref);
+                const uint64_t minus1 = pack2(-1.f, -1.f);
+                uint64_t sum[2] = {0ull, 0ull};
+#pragma unroll 1
+                for (int c = 0; c < kPcKeys; c += 16) {   // 16 keys: 8 columns of hi, 8 of lo, in place of their scores
+                    uint32_t zc[16];
+                    tmem_ld16(sb + c, zc);
+                    tmem_wait_ld();
+                    if (edge) {
+#pragma unroll
+                        for (int k = 0; k < 16; ++k)
+                            if (c + k > last || c + k < first) zc[k] = 0xff800000u;
+                    }
+                    uint64_t x[8];
+                    uint32_t pl[16];
+#pragma unroll
+                    for (int k = 0; k < 8; ++k)
+                        x[k] = fma2(pack2(__uint_as_float(zc[2 * k]), __uint_as_float(zc[2 * k + 1])), f2, m2);
+#pragma unroll
+                    for (int k = 0; k < 8; ++k) {
+                        const float2 y = unpack2(x[k]);
+                        x[k] = pack2(ex2(y.x), ex2(y.y));
+                    }
+#pragma unroll
+                    for (int k = 0; k < 8; ++k) sum[k & 1] = add2(sum[k & 1], x[k]);
+                    // hi: the upper 11 bits as they are; lo: the rest, rounded to F16
+#pragma unroll
+                    for (int k = 0; k < 8; ++k) {
+                        const uint64_t h = x[k] & 0xffffe000ffffe000ull;
+                        const float2 y = unpack2(h), w = unpack2(fma2(h, minus1, x[k]));
+                        const __half2 hi = __floats2half2_rn(y.x, y.y), lo = __floats2half2_rn(w.x, w.y);
+                        pl[k] = *reinterpret_cast<const uint32_t*>(&hi);
+                        pl[8 + k] = *reinterpret_cast<const uint32_t*>(&lo);
+                    }
+                    tmem_st16(sb + c, pl);
+                }
+                sh.m[j & 3][r] = mn;
+                tmem_wait_st();
+                tc_fence_before();
+                warp_arrive(sh.p_full + (j & 1));
+                const float2 both = unpack2(add2(sum[0], sum[1]));
+                l = l * corr + (both.x + both.y);
+                m = mn;
+                ok = add_o(j);
+            }
+            ok = ok && add_o(end);
+            if (!ok) fail();
+            // the row's sum from its two groups
+            sh.sum[half][0][r] = l;
+            sh.sum[half][1][r] = m;
+            if (!ok) *reinterpret_cast<volatile int*>(&sh.gone[warp & 3]) = 1;
+            pair_sync();
+            ok = !*reinterpret_cast<volatile int*>(&sh.gone[warp & 3]);   // both go on or both leave
+            l = 0.f;
+#pragma unroll
+            for (int g = 0; g < 2; ++g) {
+                const float mg = sh.sum[g][1][r];
+                l += mg == -INFINITY ? sh.sum[g][0][r] : sh.sum[g][0][r] * ex2(mg - mo);   // (0 or NaN) : rescaled
+            }
+            m = mo;
+            begun = begun || p.slot == 1;
+            const bool poisoned = *reinterpret_cast<volatile int*>(&sh.poison[pi & 7]) == pi + 1;
+            if (ok && !poisoned) {
+                // rows through shared memory (the planes of q, all read), so that a warp stores whole rows: chunk c of row
+                // r (16 bytes) at c ^ (r % 32), without bank conflicts either way
+                const float scale = p.slot >= 0 ? 1.f : attn_inv(l);
+                unsigned char* st = smem + Sm::kQ + r * (HD * 4);
+#pragma unroll
+                for (int c = 0; c < kD / 4; ++c) {
+                    const float2 u = unpack2(acc[2 * c]), v = unpack2(acc[2 * c + 1]);
+                    *reinterpret_cast<float4*>(st + (((half * (kD / 4) + c) ^ (r & (HD / 4 - 1))) * 16)) =
+                        make_float4(u.x * scale, u.y * scale, v.x * scale, v.y * scale);
+                }
+                if (half == 0 && live) {
+                    if (p.slot >= 0) *reinterpret_cast<float2*>(attn_part_sum<kPcRows, HD>(a, blockIdx.x, p.slot, r)) = make_float2(l, m);
+                    else if (a.lse) a.lse[(size_t)tok * a.nh + head] = attn_lse(l, m);
+                }
+                pair_sync();
+                constexpr int kPer = 128 / HD;   // rows a pass
+                const int sub = lane / (HD / 4), c = lane % (HD / 4);
+#pragma unroll 4
+                for (int k = 0; k < 16; k += kPer) {
+                    const int rr = (warp & 3) * 32 + half * 16 + k + sub;
+                    if (rr < p.rows) {
+                        const float4 v = *reinterpret_cast<const float4*>(smem + Sm::kQ + rr * (HD * 4) + ((c ^ (rr & (HD / 4 - 1))) * 16));
+                        const int rt = (int)a.gdiv.div((uint32_t)(p.row + rr));
+                        float* to = p.slot >= 0 ? attn_part<kPcRows, HD>(a, blockIdx.x, p.slot, rr)
+                                                : a.out + (size_t)(p.tok0 + rt) * a.ldo + (p.kvh * a.group + p.row + rr - rt * a.group) * HD;
+                        *reinterpret_cast<float4*>(to + c * 4) = v;
+                    }
                 }
             }
-            corr_prev = corr;
-        }
-        ok = ok && landed(o_full, nt - 1);
-        if (ok) {
-            tc_fence_after();
-            add_o(corr_prev);
-            tc_fence_before();
-        } else {
-            fail();
-        }
-        // the row's sum from its two halves
-        red[half * 128 + r] = l;
-        pair_sync();
-        l = red[r] + red[128 + r];
-        if (ok && live && !*poison) {
-            if (a.nsplit > 1) {
-                float* pp = a.part + (((size_t)split * a.s.n_tokens + tok) * a.nh + head) * (HD + 2);
-                if (half == 0) *reinterpret_cast<float2*>(pp) = make_float2(l, m);
-                pp += 2 + half * kD;
-#pragma unroll
-                for (int d = 0; d < kD; d += 2) *reinterpret_cast<float2*>(pp + d) = make_float2(acc[d], acc[d + 1]);
-            } else {
-                const float inv = l > 0.f ? 1.0f / l : (l == 0.f ? 0.f : l);
-                float* po = a.out + (size_t)tok * a.ldo + head * HD + half * kD;
-#pragma unroll
-                for (int d = 0; d < kD; d += 4)
-                    *reinterpret_cast<float4*>(po + d) = make_float4(acc[d] * inv, acc[d + 1] * inv, acc[d + 2] * inv,
-                                                                     acc[d + 3] * inv);
-                if (a.lse && half == 0)
-                    a.lse[(size_t)tok * a.nh + head] = l == 0.f ? -INFINITY : (m + log2f(l)) * 0.69314718055994531f;
+            if (ok && poisoned) {
+                if (lane == 0) atomicAdd(&sh.slow, 1);
+                for (int k = warp; k < p.rows; k += kPcSoft) attn_row_slow<__half, kPcRows, HD>(a, p, k);
+                if (lane == 0) {
+                    atomicAdd(&sh.slow_done, 1);
+                    atomicSub(&sh.slow, 1);
+                }
             }
+            if (p.slot == 1 && threadIdx.x == 0) attn_header(a, &p);
+            // every row has left (and every sum was read) before the next piece's queries come
+            asm volatile("bar.sync 5, %0;" ::"n"(32 * kPcSoft) : "memory");
+            volatile int* gone = sh.gone;
+            ok = !(gone[0] | gone[1] | gone[2] | gone[3]);   // all go on or all leave: the barrier above counts on it
         }
+        if (a.balanced && !begun && threadIdx.x == 0) attn_header(a, nullptr);
     }
     tc_fence_before();
     __syncthreads();
@@ -436,19 +668,39 @@ __global__ void __launch_bounds__(kPcThreads, 1) paged_chunk_kernel(const __grid
         tc_fence_after();
         tmem_dealloc(tmem, 512);
     }
-    if (*poison && !*abort_flag) {
-        // key by key, a warp a row: lane = HD / 32 dimensions
-        for (int r = warp; r < rows; r += kPcThreads / 32) paged_row_slow<__half, HD>(a, sv, table, kvh, split, row0 + r, k0, k1);
-    }
+}
+
+// Pool as a tensor map, or false where its strides do not make one.
+static bool pool_map(CUtensorMap* m, const void* p, const PagedKV& kv, int nkv, int hd, int box) {
+    const uint64_t dims[4] = {(uint64_t)hd, (uint64_t)nkv, kv.page.d, (uint64_t)kv.n_pages};
+    const uint64_t strides[3] = {(uint64_t)(nkv > 1 ? kv.head_stride : kv.row_stride), (uint64_t)kv.row_stride,
+                                 (uint64_t)kv.page_stride};
+    const uint32_t b[4] = {64u, 1u, (uint32_t)box, 1u};
+    return encode_f16_tiled(m, p, 4, dims, strides, b) == TVB_OK;
 }
 
 template <int HD>
-static tvb_status launch_chunk(const PagedAttnArgs& a, cudaStream_t st) {
+static tvb_status launch_chunk(PagedAttnArgs a, cudaStream_t st) {
     static int set[kMaxDevices];
     TVB_TRY(allow_smem(reinterpret_cast<const void*>(paged_chunk_kernel<HD>), PcSmem<HD>::kBytes, set));
-    const int64_t blocks = ((int64_t)a.s.n_tokens * a.group) / kPcRows + a.s.n_seqs;
-    paged_chunk_kernel<HD><<<dim3((unsigned)blocks, (unsigned)a.nkv, (unsigned)a.nsplit), kPcThreads, PcSmem<HD>::kBytes, st>>>(a);
-    return check_launch("paged_chunk_kernel");
+    // boxes: the largest power of two that divides a page, up to a tile; pages that leave less than 8 rows go by cp.async
+    int box = 1;
+    while (box < kPcKeys && a.kv.page.d % (2u * box) == 0) box *= 2;
+    PcMaps maps;
+    if (box < 8 || !pool_map(&maps.k, a.kv.k, a.kv, a.nkv, HD, box) || !pool_map(&maps.v, a.kv.v, a.kv, a.nkv, HD, box)) box = 0;
+    // a piece of two tiles still pays for its start (the block's queries) and its partial sums
+    a.min_tiles = 2;
+    Workspace ws(st);
+    dim3 grid;
+    if (a.balanced) {
+        grid = dim3((unsigned)num_sms());
+        TVB_TRY((attn_workspace<kPcRows, HD>(&a, (int)grid.x, &ws)));
+    } else {
+        grid = dim3((unsigned)(((int64_t)a.s.n_tokens * a.group) / kPcRows + a.s.n_seqs), (unsigned)a.nkv);
+    }
+    paged_chunk_kernel<HD><<<grid, kPcThreads, PcSmem<HD>::kBytes, st>>>(maps, a, box);
+    TVB_TRY(check_launch("paged_chunk_kernel"));
+    return launch_merge<kPcRows, HD>(a, (int)grid.x, st);
 }
 
 tvb_status paged_attn_chunk_f16(const PagedAttnArgs& a, int hd, cudaStream_t st) {
