@@ -22,6 +22,7 @@ namespace tvb {
 constexpr int kPrWarps = 8, kPrThreads = 32 * kPrWarps;
 constexpr int kPrKeys = 8;   // keys a batch
 constexpr int kPrTile = kPrKeys * kPrWarps;   // keys a tile
+constexpr int kPrExtra = 1;   // what starting and leaving a block costs, in tiles
 constexpr int kTensorRows = 32;   // rows of a KV head from which F16 caches take the tensor cores
 
 __device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, bool valid) {
@@ -269,13 +270,13 @@ __global__ void __launch_bounds__(kPrThreads) paged_rows_kernel(const __grid_con
         return;
     }
     AttnSchedule& sched = *reinterpret_cast<AttnSchedule*>(pr_smem_raw + rows_smem<T, HD, RB>());
-    const int per_head = attn_schedule<RB, kPrTile, kPrThreads>(a, sched, 1);
+    const int per_head = attn_schedule<RB, kPrTile, kPrExtra, kPrThreads>(a, sched, 1);
     if (threadIdx.x == 0) run = attn_run(a, per_head);
     __syncthreads();
     pdl_launch_dependents();
     bool begun = false;
     const AttnPiece& p = pieces[threadIdx.x >> 5];
-    for (int at = run.u, n; (n = attn_next<RB, kPrTile>(a, sched, run, at, 1, &pieces[threadIdx.x >> 5])) != 0; at += n) {
+    for (int at = run.u; (at = attn_next<RB, kPrTile, kPrExtra>(a, sched, run, at, 1, &pieces[threadIdx.x >> 5])) != 0;) {
         rows_piece<T, HD, RB>(a, p, pr_smem_raw);
         __syncthreads();
         if (p.slot == 1) {
@@ -291,7 +292,7 @@ static tvb_status launch_rows(PagedAttnArgs a, cudaStream_t st) {
     static int set[kMaxDevices];
     constexpr int smem = rows_smem<T, HD, RB>() + (int)sizeof(AttnSchedule);
     TVB_TRY(allow_smem(reinterpret_cast<const void*>(paged_rows_kernel<T, HD, RB>), smem, set));
-    a.min_tiles = 1;   // shorter pieces cost more to join than they save
+    a.min_units = 1 + kPrExtra;
     Workspace ws(st);
     dim3 grid;
     if (a.balanced) {

@@ -17,7 +17,7 @@ struct PagedAttnArgs {
     float scale2;      // scale * log2(e): scores are kept as powers of two
     int window;        // 0: none
     int balanced;      // the grid shares the tiles evenly; else a CTA a row block
-    int min_tiles;     // ... but no CTA gets fewer than this
+    int min_units;     // ... but no CTA gets fewer than this (tiles and blocks' extra)
     float* part;       // [CTA][2]: rows x hd weighted values, rows x (sum, maximum) of cut blocks
     int* header;       // [CTA][8]: the cut block that the CTA's last piece begins
     unsigned* status;
@@ -29,14 +29,15 @@ constexpr int kAttnSeqs = 1024;   // sequences that a balanced grid keeps in sha
 
 // The work: row blocks (RB rows -- new token x query head of the group -- of one
 // KV head of one sequence) with the tiles of TK keys that some row of the block
-// sees, tile after tile, block after block, KV head after KV head.  A balanced
-// grid of G CTAs cuts the T tiles into G equal runs, whatever the lengths are; a
-// block that a cut divides leaves partial sums and paged_merge_kernel joins them.
+// sees, tile after tile, block after block, KV head after KV head; a block counts
+// EX units more, before its tiles, for its start and end.  A balanced grid of G
+// CTAs cuts the T units into G equal runs, whatever the lengths are; a block whose
+// tiles a cut divides leaves partial sums and paged_merge_kernel joins them.
 // Lengths are known on the device only, so every CTA adds up the sequences' tiles
 // first (a few microseconds saved over a launch that does it).
 struct AttnSchedule {
     int row0[kAttnSeqs], n[kAttnSeqs], kv[kAttnSeqs];
-    int before[kAttnSeqs + 1];   // tiles of the earlier sequences, one KV head
+    int before[kAttnSeqs + 1];   // units of the earlier sequences, one KV head
 };
 
 struct AttnPiece {
@@ -64,8 +65,8 @@ __device__ __forceinline__ int attn_tiles(const PagedAttnArgs& a, int n, int pos
     return (*k1 - *k0 + TK - 1) / TK;
 }
 
-// Whole CTA (NT threads): fills `s` and returns the tiles of one KV head.
-template <int RB, int TK, int NT>
+// Whole CTA (NT threads): fills `s` and returns the units of one KV head.
+template <int RB, int TK, int EX, int NT>
 __device__ __forceinline__ int attn_schedule(const PagedAttnArgs& a, AttnSchedule& s, int align) {
     const int tid = threadIdx.x, lane = tid & 31;
     for (int b = tid; b < a.s.n_seqs; b += NT) {
@@ -79,7 +80,7 @@ __device__ __forceinline__ int attn_schedule(const PagedAttnArgs& a, AttnSchedul
     for (int b = tid >> 5; b < a.s.n_seqs; b += NT / 32) {
         const int n = s.n[b], blocks = (n * a.group + RB - 1) / RB;
         int t = 0, x, y, z;
-        for (int i = lane; i < blocks; i += 32) t += attn_tiles<RB, TK>(a, n, s.kv[b] - n, i, align, &x, &y, &z);
+        for (int i = lane; i < blocks; i += 32) t += attn_tiles<RB, TK>(a, n, s.kv[b] - n, i, align, &x, &y, &z) + EX;
         t = __reduce_add_sync(0xffffffffu, t);
         if (lane == 0) s.before[b + 1] = t;
     }
@@ -102,7 +103,7 @@ __device__ __forceinline__ int attn_schedule(const PagedAttnArgs& a, AttnSchedul
     return s.before[a.s.n_seqs];
 }
 
-// A CTA's run of tiles.
+// A CTA's run of units.
 struct AttnRun {
     int64_t total;
     int per_head, ctas;
@@ -113,25 +114,25 @@ __device__ __forceinline__ AttnRun attn_run(const PagedAttnArgs& a, int per_head
     AttnRun r;
     r.per_head = per_head;
     r.total = (int64_t)per_head * a.nkv;
-    r.ctas = (int)min((int64_t)gridDim.x, max((int64_t)1, r.total / a.min_tiles));
+    r.ctas = (int)min((int64_t)gridDim.x, max((int64_t)1, r.total / a.min_units));
     r.u = (int)(r.total * min((int)blockIdx.x, r.ctas) / r.ctas);
     r.end = (int)(r.total * min((int)blockIdx.x + 1, r.ctas) / r.ctas);
     return r;
 }
 
-// Whole warp: the piece that starts at tile u of the run, into *out (shared
-// memory of this warp); returns its tiles, 0 at the end of the run.  Not inlined:
-// every role of a kernel calls it, and code that fits the instruction cache is
-// worth more than the call.
-template <int RB, int TK>
+// Whole warp: the next piece from unit u of the run on, into *out (shared memory
+// of this warp); returns the unit after it, 0 when the run has no more.  Not
+// inlined, for the instruction cache's sake.
+template <int RB, int TK, int EX>
 __device__ __noinline__ int attn_next(const PagedAttnArgs& a, const AttnSchedule& s, const AttnRun& r, int u, int align,
                                       AttnPiece* out) {
-    if (u >= r.end) return 0;
     const int lane = threadIdx.x & 31;
     AttnPiece p;
+again:
+    if (u >= r.end) return 0;
     p.kvh = u / r.per_head;
     int t = u - p.kvh * r.per_head;
-    int lo = 0, hi = a.s.n_seqs - 1;   // the last sequence that starts at or before t and has tiles
+    int lo = 0, hi = a.s.n_seqs - 1;   // the last sequence that starts at or before t
     while (lo < hi) {
         const int mid = (lo + hi + 1) >> 1;
         if (s.before[mid] <= t) lo = mid;
@@ -145,8 +146,8 @@ __device__ __noinline__ int attn_next(const PagedAttnArgs& a, const AttnSchedule
     const int blocks = (n * a.group + RB - 1) / RB;
     int i0 = 0, tiles = 0, x, y, z;
 #pragma unroll 1
-    for (;; i0 += 32) {   // the block that holds tile t of the sequence
-        const int nt = i0 + lane < blocks ? attn_tiles<RB, TK>(a, n, p.pos0, i0 + lane, align, &x, &y, &z) : 0;
+    for (;; i0 += 32) {   // the block that holds unit t of the sequence
+        const int nt = i0 + lane < blocks ? attn_tiles<RB, TK>(a, n, p.pos0, i0 + lane, align, &x, &y, &z) + EX : 0;
         int sum = nt;
 #pragma unroll 1
         for (int o = 1; o < 32; o <<= 1) {
@@ -163,18 +164,23 @@ __device__ __noinline__ int attn_next(const PagedAttnArgs& a, const AttnSchedule
         }
         t -= __shfl_sync(0xffffffffu, sum, 31);
     }
+    // t: unit of the block, `tiles` of them; the tiles are those from EX on
+    const int begin = max(t, EX), end = min(tiles, t + r.end - u);
+    const int first_unit = u - t;
+    u = first_unit + end;
+    if (begin >= end) goto again;   // the run ends, or begins, before the block's first tile
     attn_tiles<RB, TK>(a, n, p.pos0, i0, align, &p.first, &p.k0, &p.k1);
     p.row = i0 * RB;
     p.rows = min(RB, n * a.group - p.row);
-    p.tiles = min(tiles - t, r.end - u);
-    p.slot = p.tiles == tiles ? -1 : t > 0 ? 0 : 1;
-    p.last_cta = (int)(((u - t + (int64_t)tiles) * r.ctas - 1) / r.total);
-    p.k0 += t * TK;
+    p.tiles = end - begin;
+    p.slot = p.tiles == tiles - EX ? -1 : begin > EX ? 0 : 1;
+    p.last_cta = (int)(((int64_t)(first_unit + tiles) * r.ctas - 1) / r.total);
+    p.k0 += (begin - EX) * TK;
     p.k1 = min(p.k1, p.k0 + p.tiles * TK);
     __syncwarp();
     if (lane == 0) *out = p;
     __syncwarp();
-    return p.tiles;
+    return u;
 }
 
 // The piece of a CTA of an unbalanced grid: row block blockIdx.x of the batch,

@@ -31,8 +31,10 @@
 namespace tvb {
 
 constexpr int kPcRows = 128, kPcKeys = 128, kPcSlots = 4;
-// Warps 0-7 softmax, 8-10 loaders, 11 MMA: 12 warps leave a thread 168 registers.
-constexpr int kPcSoft = 8, kPcLoaders = 3, kPcMmaWarp = kPcSoft + kPcLoaders, kPcThreads = 32 * (kPcMmaWarp + 1);
+// Warps 0-7 softmax, 8-9 loaders, 10 pieces, 11 MMA.
+constexpr int kPcSoft = 8, kPcLoaders = 2, kPcPieceWarp = kPcSoft + kPcLoaders, kPcMmaWarp = kPcPieceWarp + 1;
+constexpr int kPcThreads = 32 * (kPcMmaWarp + 1);
+constexpr int kPcExtra = 3;   // what starting and leaving a block costs, in tiles
 
 // Barriers and flags of a CTA.
 struct PcShared {
@@ -48,7 +50,8 @@ struct PcShared {
     float f[128];               // q scale log2 e = (hi + lo) f
     float m[4][128];            // row maxima that a tile's p refer to
     AttnRun run;
-    AttnPiece piece[kPcMmaWarp + 1];   // of each warp
+    uint64_t piece_full[4], piece_empty[4];
+    AttnPiece piece[4];         // the pieces to come; tiles 0: no more
     float sum[2][2][128];       // a row's sum and maximum in each group, at the end of a piece
 };
 
@@ -171,26 +174,17 @@ paged_chunk_kernel(const __grid_constant__ PcMaps maps, const __grid_constant__ 
     AttnPiece only;
     bool any = true;
     if (a.balanced) {
-        const AttnRun run = attn_run(a, attn_schedule<kPcRows, kPcKeys, kPcThreads>(a, sched, align));
+        const AttnRun run = attn_run(a, attn_schedule<kPcRows, kPcKeys, kPcExtra, kPcThreads>(a, sched, align));
         pdl_launch_dependents();
         any = run.u < run.end;
         if (threadIdx.x == 0) sh.run = run;
     } else {
         any = attn_block<kPcRows, kPcKeys, kPcThreads>(a, align, &only);
-        if (lane == 0 && any) sh.piece[warp] = only;
     }
     if (!any) {
         if (a.balanced && threadIdx.x == 0) attn_header(a, nullptr);
         return;
     }
-    int at = 0;   // tiles of this warp's earlier pieces
-    auto next = [&](int i) -> bool {   // whole warp: piece i
-        if (!a.balanced) return i == 0;
-        const int n = attn_next<kPcRows, kPcKeys>(a, sched, sh.run, sh.run.u + at, align, &sh.piece[warp]);
-        at += n;
-        return n != 0;
-    };
-
     if (threadIdx.x == 0) {
         for (int i = 0; i < kPcSlots; ++i) {
             mbar_init(sh.full + i, 1);
@@ -201,6 +195,10 @@ paged_chunk_kernel(const __grid_constant__ PcMaps maps, const __grid_constant__ 
             mbar_init(sh.p_full + i, kPcSoft / 2);
             mbar_init(sh.o_full + i, 1);
             mbar_init(sh.o_read + i, kPcSoft);
+        }
+        for (int i = 0; i < 4; ++i) {
+            mbar_init(sh.piece_full + i, 1);
+            mbar_init(sh.piece_empty + i, kPcSoft + kPcLoaders + 1);
         }
         mbar_init(&sh.q_full, kPcSoft);
         mbar_init(&sh.drained, 1);
@@ -234,10 +232,20 @@ paged_chunk_kernel(const __grid_constant__ PcMaps maps, const __grid_constant__ 
         return true;
     };
 
+    // whole warp: piece i is in sh.piece[i % 4], until done(i)
+    auto next = [&](int i) -> bool {
+        const bool in = landed(sh.piece_full + (i & 3), i >> 2);
+        return __all_sync(0xffffffffu, in) && sh.piece[i & 3].tiles != 0;
+    };
+    auto done = [&](int i) {
+        __syncwarp();
+        if (lane == 0) mbar_arrive(sh.piece_empty + (i & 3));
+    };
+
     // the softmax warps' registers: 128 x (200 + 200 + 104) = 384 x 168, what the CTA was launched with
     if (warp >= kPcSoft) {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 104;");
-    if (warp < kPcMmaWarp) {
+    if (warp < kPcPieceWarp) {
         // ---- loaders ---------------------------------------------------------------
         const int w = warp - kPcSoft;
         constexpr int kLanes = HD / 8;          // 16-byte chunks, lanes a row (cp.async)
@@ -249,10 +257,10 @@ paged_chunk_kernel(const __grid_constant__ PcMaps maps, const __grid_constant__ 
             prefetch_tmap(&maps.k);
             prefetch_tmap(&maps.v);
         }
-        const AttnPiece& p = sh.piece[warp];
         bool ok = true;
         int item0 = 0;   // items of earlier pieces: K0, K1, then V(j), K(j + 2) for every tile j
-        for (int pi = 0; ok && next(pi); item0 += 2 * p.tiles, ++pi) {
+        for (int pi = 0; ok && next(pi); ++pi) {
+            const AttnPiece& p = sh.piece[pi & 3];
             const int nt = p.tiles, nitems = 2 * nt;
             const int* table = a.s.table + (size_t)p.b * a.s.table_ld;
             const int p_first = p.pos0 + (int)a.gdiv.div((uint32_t)p.row);
@@ -354,31 +362,52 @@ paged_chunk_kernel(const __grid_constant__ PcMaps maps, const __grid_constant__ 
                 __syncwarp();
                 if (lane == 0) mbar_arrive(sh.full + sl);
             }
+            item0 += nitems;
+            done(pi);
         }
         asm volatile("cp.async.wait_all;" ::: "memory");
         if (box && *abort_flag) {   // no TMA write may outlive the CTA: the last two items cover every slot still in flight
             for (int i = max(w, issued - kPcLoaders); i <= issued; i += kPcLoaders)
                 mbar_wait_bounded(sh.full + i % kPcSlots, (uint32_t)((i / kPcSlots) & 1));
         }
+    } else if (warp == kPcPieceWarp) {
+        // ---- the pieces, ahead of the others ------------------------------------------
+        for (int pi = 0, at = a.balanced ? sh.run.u : 0;; ++pi) {
+            if (pi >= 4 && !__all_sync(0xffffffffu, landed(sh.piece_empty + (pi & 3), (pi >> 2) - 1))) break;
+            AttnPiece* out = sh.piece + (pi & 3);
+            int n = 0;
+            if (a.balanced) {
+                at = attn_next<kPcRows, kPcKeys, kPcExtra>(a, sched, sh.run, at, align, out);
+                n = at != 0;
+            } else if (pi == 0) {
+                n = only.tiles;
+                if (lane == 0) *out = only;
+            }
+            if (n == 0 && lane == 0) out->tiles = 0;
+            __syncwarp();
+            if (lane == 0) mbar_arrive(sh.piece_full + (pi & 3));
+            if (n == 0) break;
+        }
     } else {
         // ---- MMA issuer --------------------------------------------------------------
         constexpr uint32_t idesc_s = umma_idesc_f16(kPcRows, kPcKeys);
         constexpr uint32_t idesc_o = umma_idesc_f16(kPcRows, HD) | (1u << 16);   // B is MN-major
         int item = 0, tile = 0;   // over all pieces
-        const AttnPiece& p = sh.piece[warp];
         bool ok = true;
         for (int pi = 0; ok && next(pi); ++pi) {
+            const AttnPiece& p = sh.piece[pi & 3];
             if (lane == 0) {
                 auto ready = [&]() { return landed(sh.full + item % kPcSlots, item / kPcSlots); };
                 auto mma_s = [&](int j) {   // tile j (of all) takes the buffer of P(j - 2)
-                    const uint32_t k_s = base + Sm::kSlots + (item % kPcSlots) * Sm::kPlane, d = tmem + (j & 1) * kPcKeys;
+                    const uint32_t d = tmem + (j & 1) * kPcKeys;
+                    const uint64_t qd = sw128_desc(base + Sm::kQ), kd = sw128_desc(base + Sm::kSlots + (item % kPcSlots) * Sm::kPlane);
                     tc_fence_after();
-#pragma unroll 1
-                    for (int kk = 0; kk < HD / 16; ++kk) {
-                        const uint32_t o = (kk >> 2) * Sm::kAtom + (kk & 3) * 32;
-                        const uint64_t kd = sw128_desc(k_s + o);
-                        tc_mma(d, sw128_desc(base + Sm::kQ + o), kd, idesc_s, kk ? 1u : 0u);
-                        tc_mma(d, sw128_desc(base + Sm::kQ + Sm::kPlane + o), kd, idesc_s, 1u);
+#pragma unroll
+                    for (int kk = 0; kk < HD / 16; ++kk) {   // addresses in a descriptor count 16 bytes
+                        constexpr uint64_t kLo = Sm::kPlane >> 4;
+                        const uint64_t o = (kk >> 2) * (Sm::kAtom >> 4) + (kk & 3) * 2;
+                        tc_mma(d, qd + o, kd + o, idesc_s, kk ? 1u : 0u);
+                        tc_mma(d, qd + (o + kLo), kd + o, idesc_s, 1u);
                     }
                     tc_commit(sh.s_full + (j & 1));
                     tc_commit(sh.empty + item % kPcSlots);
@@ -394,13 +423,12 @@ paged_chunk_kernel(const __grid_constant__ PcMaps maps, const __grid_constant__ 
                     ok = ready() && (j < 2 || landed(sh.o_read + (j & 1), (j - 2) >> 1)) && landed(sh.p_full + (j & 1), j >> 1);
                     if (!ok) break;
                     tc_fence_after();
-                    const uint32_t v_s = base + Sm::kSlots + (item % kPcSlots) * Sm::kPlane;
+                    const uint64_t vd = sw128_mn_desc(base + Sm::kSlots + (item % kPcSlots) * Sm::kPlane, Sm::kAtom);
                     const uint32_t pt = tmem + (j & 1) * kPcKeys, ot = tmem + kO + (j & 1) * HD;
-#pragma unroll 1
+#pragma unroll
                     for (int kk = 0; kk < kPcKeys / 16; ++kk) {
-                        const uint64_t vd = sw128_mn_desc(v_s + kk * 2048, Sm::kAtom);
-                        tc_mma_ts(ot, pt + kk * 16, vd, idesc_o, kk ? 1u : 0u);
-                        tc_mma_ts(ot, pt + kk * 16 + 8, vd, idesc_o, 1u);
+                        tc_mma_ts(ot, pt + kk * 16, vd + kk * (2048 >> 4), idesc_o, kk ? 1u : 0u);
+                        tc_mma_ts(ot, pt + kk * 16 + 8, vd + kk * (2048 >> 4), idesc_o, 1u);
                     }
                     tc_commit(sh.o_full + (j & 1));
                     tc_commit(sh.empty + item % kPcSlots);
@@ -414,6 +442,7 @@ paged_chunk_kernel(const __grid_constant__ PcMaps maps, const __grid_constant__ 
             }
             ok = __shfl_sync(0xffffffffu, (int)ok, 0) != 0;
             tile += p.tiles;
+            done(pi);
         }
         if (lane == 0) {
             tc_commit(&sh.drained);   // every MMA issued above
@@ -436,11 +465,11 @@ paged_chunk_kernel(const __grid_constant__ PcMaps maps, const __grid_constant__ 
         auto all_landed = [&](uint64_t* bar, int phase) -> bool {
             return __all_sync(0xffffffffu, landed(bar, phase) && !*abort_flag) != 0;
         };
-        const AttnPiece& p = sh.piece[warp];
         bool ok = true;
         bool begun = false;   // a cut block that this CTA begins
         int tile = 0;
-        for (int pi = 0; ok && next(pi); tile += p.tiles, ++pi) {
+        for (int pi = 0; ok && next(pi); ++pi) {
+            const AttnPiece& p = sh.piece[pi & 3];
             const bool live = r < p.rows;
             const int row = p.row + min(r, p.rows - 1);
             const int t = (int)a.gdiv.div((uint32_t)row);
@@ -534,8 +563,12 @@ paged_chunk_kernel(const __grid_constant__ PcMaps maps, const __grid_constant__ 
                 const uint32_t sb = lanes + (j & 1) * kPcKeys;
                 const int t0 = p.k0 + (j - tile) * kPcKeys, t1 = min(t0 + kPcKeys, p.k1);
                 const bool edge = t1 - t0 < kPcKeys || t0 < p.first || t1 - 1 > p_first || (a.window && t0 <= p_last - a.window);
-                // keys [first, last] of the tile are the row's
+                // keys [first, last] of the tile are the row's: bits of the 32 (or 16) from key c on
                 const int last = min(t1 - 1, pos) - t0, first = max(p.first, a.window ? pos - a.window + 1 : 0) - t0;
+                auto seen = [&](int c) -> uint32_t {
+                    const int hi = min(last - c, 31), lo = max(first - c, 0);
+                    return hi < lo ? 0u : (0xffffffffu >> (31 - hi)) & (0xffffffffu << lo);
+                };
                 float m4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
                 // loops rolled on purpose: what the three roles run between tiles fits the instruction cache
 #pragma unroll 1
@@ -544,9 +577,10 @@ paged_chunk_kernel(const __grid_constant__ PcMaps maps, const __grid_constant__ 
                     tmem_ld32(sb + c, s);
                     tmem_wait_ld();
                     if (edge) {
+                        const uint32_t mk = seen(c);
 #pragma unroll
                         for (int k = 0; k < 32; ++k)
-                            if (c + k > last || c + k < first) s[k] = 0xff800000u;   // -infinity
+                            if (!(mk & (1u << k))) s[k] = 0xff800000u;   // -infinity
                     }
 #pragma unroll
                     for (int k = 0; k < 32; ++k) m4[k & 3] = fmaxf(m4[k & 3], __uint_as_float(s[k]));
@@ -563,9 +597,10 @@ paged_chunk_kernel(const __grid_constant__ PcMaps maps, const __grid_constant__ 
                     tmem_ld16(sb + c, zc);
                     tmem_wait_ld();
                     if (edge) {
+                        const uint32_t mk = seen(c);
 #pragma unroll
                         for (int k = 0; k < 16; ++k)
-                            if (c + k > last || c + k < first) zc[k] = 0xff800000u;
+                            if (!(mk & (1u << k))) zc[k] = 0xff800000u;
                     }
                     uint64_t x[8];
                     uint32_t pl[16];
@@ -659,6 +694,8 @@ paged_chunk_kernel(const __grid_constant__ PcMaps maps, const __grid_constant__ 
             asm volatile("bar.sync 5, %0;" ::"n"(32 * kPcSoft) : "memory");
             volatile int* gone = sh.gone;
             ok = !(gone[0] | gone[1] | gone[2] | gone[3]);   // all go on or all leave: the barrier above counts on it
+            tile += p.tiles;
+            done(pi);
         }
         if (a.balanced && !begun && threadIdx.x == 0) attn_header(a, nullptr);
     }
@@ -689,7 +726,7 @@ static tvb_status launch_chunk(PagedAttnArgs a, cudaStream_t st) {
     PcMaps maps;
     if (box < 8 || !pool_map(&maps.k, a.kv.k, a.kv, a.nkv, HD, box) || !pool_map(&maps.v, a.kv.v, a.kv, a.nkv, HD, box)) box = 0;
     // a piece of two tiles still pays for its start (the block's queries) and its partial sums
-    a.min_tiles = 2;
+    a.min_units = 2 + kPcExtra;
     Workspace ws(st);
     dim3 grid;
     if (a.balanced) {
