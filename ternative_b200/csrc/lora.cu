@@ -1,68 +1,304 @@
 // Adapters of many requests beside a shared projection (tvb_matmul_lora):
 //   y[m] = W x[m] + scale_a B_a (A_a x[m]),  a = adapter[m]
-#include <algorithm>
+//
+// Up to 16 rows (a decode batch) the call is bound by the bytes of W and of the
+// adapters in use, each read once:
+//
+// lora_shrink_kernel: t[m] = scale_a A_a x[m], a warp a (row, rank index).
+// lora_rows_kernel: W streamed once for all rows through mma.sync m16n8k16 (rows
+// of x are the 16-row operand, 8 weight rows the other; a memory-bound product
+// that needs no more than the legacy tensor path).  x is split into F16 hi + lo
+// planes with a power-of-two factor a row, so products are F32-faithful; each
+// warp keeps its K slice of x in registers for the whole kernel and weights come
+// straight from global memory in the operand's layout: with k permuted so that a
+// thread's fragments of 2 or 4 steps are 16 contiguous bytes of a weight row.
+// The CTA's warps cut K, and the CTAs of a cluster cut it further; partial sums
+// meet in shared memory (distributed over the cluster), then the epilogue scales
+// INT8 rows and adds t . B_a.  It is launched as the shrink kernel's dependent
+// and waits for t only there, so both stream together.
+#include "lora.h"
 
-#include "paged.cuh"
+#include <algorithm>
+#include <cooperative_groups.h>
+
+namespace cg = cooperative_groups;
 
 namespace tvb {
 
-constexpr int kLoraMaxRank = 256;
+constexpr int kLrWarps = 8, kLrThreads = 32 * kLrWarps;
+constexpr int kLrCols = 16;        // weight rows a tile
+constexpr int kLrSlice = 160;      // largest K slice of a warp (F16; INT8: 192, a multiple of 64)
+constexpr int kLrMaxSplit = 8;     // CTAs of a cluster
+constexpr int kLrMaxRows = 16;
 
-struct LoraArgs {
-    const float* x;
-    float* y;
-    float* t;   // [M][max_rank]: scale_a A_a x
-    int M, K, N, n, max_rank, f16;
-    const void* const* A;
-    const void* const* B;
-    const int* rank;
-    const float* scale;
-    const int* adapter;
-    unsigned* status;
-};
-
-// The adapter of row m, or -1 where it has none (or none that can be used).
-__device__ __forceinline__ int lora_of(const LoraArgs& a, int m, int* rank) {
-    const int i = __ldg(a.adapter + m);
-    *rank = 0;
-    if (i == -1) return -1;
-    if ((unsigned)i >= (unsigned)a.n) {
-        report_bad(a.status);
-        return -1;
-    }
-    const int r = __ldg(a.rank + i);
-    if (r < 0 || r > a.max_rank) {
-        report_bad(a.status);
-        return -1;
-    }
-    *rank = r;
-    return i;
-}
-
-__device__ __forceinline__ float lora_elem(const void* p, size_t i, bool f16) {
-    return f16 ? __half2float(static_cast<const __half*>(p)[i]) : static_cast<const float*>(p)[i];
-}
-
-// Warp per (row, rank index).
+// Warp per (row, rank index): K in float4 (or 8 halves) a lane.
 __global__ void __launch_bounds__(256) lora_shrink_kernel(const __grid_constant__ LoraArgs a) {
+    pdl_launch_dependents();
     const int m = blockIdx.x, lane = threadIdx.x & 31;
     int rank;
-    const int ad = lora_of(a, m, &rank);
+    const int ad = lora_of(a, m, &rank, blockIdx.y == 0 && threadIdx.x == 0);
+    const int j = blockIdx.y * 8 + (threadIdx.x >> 5);
+    if (j >= rank) return;
     const float* x = a.x + (size_t)m * a.K;
-    for (int j = blockIdx.y * 8 + (threadIdx.x >> 5); j < rank; j += gridDim.y * 8) {
-        const void* A = a.A[ad];
-        float s = 0.f;
-        for (int k = lane; k < a.K; k += 32) s = fmaf(x[k], lora_elem(A, (size_t)j * a.K + k, a.f16), s);
-        s = warp_sum(s);
-        if (lane == 0) a.t[(size_t)m * a.max_rank + j] = s * __ldg(a.scale + ad);
+    float s0 = 0.f, s1 = 0.f;
+    if (a.f16) {
+        const __half* A = static_cast<const __half*>(a.A[ad]) + (size_t)j * a.K;
+#pragma unroll 4
+        for (int k = lane * 8; k < a.K; k += 256) {
+            const uint4 u = __ldg(reinterpret_cast<const uint4*>(A + k));
+            float f[8];
+            h8_to_f8(u, f);
+            const float4 v = __ldg(reinterpret_cast<const float4*>(x + k)), w = __ldg(reinterpret_cast<const float4*>(x + k + 4));
+            s0 = fmaf(f[0], v.x, fmaf(f[1], v.y, fmaf(f[2], v.z, fmaf(f[3], v.w, s0))));
+            s1 = fmaf(f[4], w.x, fmaf(f[5], w.y, fmaf(f[6], w.z, fmaf(f[7], w.w, s1))));
+        }
+    } else {
+        const float* A = static_cast<const float*>(a.A[ad]) + (size_t)j * a.K;
+#pragma unroll 4
+        for (int k = lane * 8; k < a.K; k += 256) {
+            const float4 p = __ldg(reinterpret_cast<const float4*>(A + k)), q = __ldg(reinterpret_cast<const float4*>(A + k + 4));
+            const float4 v = __ldg(reinterpret_cast<const float4*>(x + k)), w = __ldg(reinterpret_cast<const float4*>(x + k + 4));
+            s0 = fmaf(p.x, v.x, fmaf(p.y, v.y, fmaf(p.z, v.z, fmaf(p.w, v.w, s0))));
+            s1 = fmaf(q.x, w.x, fmaf(q.y, w.y, fmaf(q.z, w.z, fmaf(q.w, w.w, s1))));
+        }
     }
+    const float s = warp_sum(s0 + s1);
+    if (lane == 0) a.t[(size_t)m * a.max_rank + j] = s * __ldg(a.scale + ad);
 }
 
-// Thread per (row, output).
+__device__ __forceinline__ void mma_f16(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+    asm volatile(
+        "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+        : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+
+// Four int8 as two pairs of F16, exactly: the biased byte b + 128 in the low bits
+// of 1024, less 1152.
+__device__ __forceinline__ void i8x4_to_h2(uint32_t w, uint32_t* lo, uint32_t* hi) {
+    const uint32_t u = w ^ 0x80808080u;
+    uint32_t p = __byte_perm(u, 0x64646464u, 0x4140), q = __byte_perm(u, 0x64646464u, 0x4342);
+    const __half2 bias = __half2half2(__ushort_as_half(0x6480));   // 1152
+    const __half2 x = __hsub2(*reinterpret_cast<const __half2*>(&p), bias), y = __hsub2(*reinterpret_cast<const __half2*>(&q), bias);
+    *lo = *reinterpret_cast<const uint32_t*>(&x);
+    *hi = *reinterpret_cast<const uint32_t*>(&y);
+}
+
+struct LoraRowsPlan {
+    int slice;   // K of a warp
+    int tiles;   // tiles of weight rows
+};
+
+// W8: INT8 weights.  WIDE: 9 to 16 rows (else the upper half of the operand is
+// zero and takes no registers).
+template <bool W8, bool WIDE>
+__global__ void __launch_bounds__(kLrThreads, WIDE ? 1 : 2)
+lora_rows_kernel(const __grid_constant__ LoraArgs a, const __grid_constant__ LoraRowsPlan plan) {
+    constexpr int E = W8 ? 16 : 8;                     // weights in 16 bytes
+    constexpr int kBlock = 4 * E;                      // k a load of the warp
+    constexpr int kBlocks = W8 ? 3 : kLrSlice / kBlock;   // loads a weight row
+    constexpr int kSteps = E / 4;                      // MMA steps a load
+    constexpr int kHalves = WIDE ? 2 : 1;
+    extern __shared__ __align__(16) float lr_smem[];   // [tile][16 rows][16 weight rows], then the warps' sums
+    cg::cluster_group cl = cg::this_cluster();
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, q = lane & 3;
+    const int rank = (int)cl.block_rank(), nsplit = (int)cl.num_blocks();
+    const int group = (int)(blockIdx.x / nsplit), groups = (int)(gridDim.x / nsplit);
+    const int k0 = (rank * kLrWarps + warp) * plan.slice;
+    const int my_tiles = plan.tiles > group ? (plan.tiles - group + groups - 1) / groups : 0;
+    float* warps = lr_smem + ((plan.tiles + groups - 1) / groups) * 256;   // [2][8 warps][16][16 + 1]
+    const unsigned char* W = static_cast<const unsigned char*>(a.w);
+
+    // this warp's weights of rows [n0, n0 + 16): 16 bytes of row g (and g + 8) a load
+    uint4 w[2][kBlocks];
+    auto request = [&](int tile) {
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            const int n = tile * kLrCols + h * 8 + g;
+#pragma unroll
+            for (int i = 0; i < kBlocks; ++i) {
+                const int k = k0 + i * kBlock + q * E;
+                w[h][i] = n < a.N && i * kBlock < plan.slice && k < a.K
+                              ? ld_stream16(W + ((size_t)n * a.K + k) * (W8 ? 1 : 2))
+                              : make_uint4(0u, 0u, 0u, 0u);
+            }
+        }
+    };
+    if (my_tiles) request(group);
+
+    // x of rows g (and g + 8), this thread's k, as hi + lo with a factor a row
+    uint32_t xh[kBlocks][kSteps][2 * kHalves], xl[kBlocks][kSteps][2 * kHalves];
+    float f[2] = {0.f, 0.f};
+#pragma unroll
+    for (int hf = 0; hf < kHalves; ++hf) {
+        const int m = g + 8 * hf;
+        float v[kBlocks][E];
+        float mx = 0.f;
+#pragma unroll
+        for (int i = 0; i < kBlocks; ++i) {
+            const int k = k0 + i * kBlock + q * E;
+            const bool in = m < a.M && i * kBlock < plan.slice && k < a.K;
+#pragma unroll
+            for (int e = 0; e < E; e += 4) {
+                const float4 x = in ? __ldg(reinterpret_cast<const float4*>(a.x + (size_t)m * a.K + k + e)) : make_float4(0.f, 0.f, 0.f, 0.f);
+                v[i][e] = x.x, v[i][e + 1] = x.y, v[i][e + 2] = x.z, v[i][e + 3] = x.w;
+                mx = fmaxf(mx, fmaxf(fmaxf(fabsf(x.x), fabsf(x.y)), fmaxf(fabsf(x.z), fabsf(x.w))));
+            }
+        }
+        mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
+        mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
+        int e2 = 0;   // the largest / 2^e2 in [2^13, 2^14)
+        if (mx > 0.f && mx < INFINITY) e2 = max(-100, min(100, (int)((__float_as_uint(mx) >> 23) & 255) - 127 - 13));
+        f[hf] = __uint_as_float((uint32_t)(127 + e2) << 23);
+        const float inv = __uint_as_float((uint32_t)(127 - e2) << 23);
+#pragma unroll
+        for (int i = 0; i < kBlocks; ++i)
+#pragma unroll
+            for (int s = 0; s < kSteps; ++s)
+#pragma unroll
+                for (int p = 0; p < 2; ++p) {
+                    const float x0 = v[i][4 * s + 2 * p] * inv, x1 = v[i][4 * s + 2 * p + 1] * inv;
+                    const __half2 hi = __floats2half2_rn(x0, x1);
+                    const float2 h = __half22float2(hi);
+                    const __half2 lo = __floats2half2_rn(x0 - h.x, x1 - h.y);
+                    xh[i][s][p * kHalves + hf] = *reinterpret_cast<const uint32_t*>(&hi);
+                    xl[i][s][p * kHalves + hf] = *reinterpret_cast<const uint32_t*>(&lo);
+                }
+    }
+
+    for (int it = 0; it < my_tiles; ++it) {
+        const int tile = group + it * groups;
+        float hi[2][4] = {}, lo[2][4] = {};   // sums of the two planes apart: shorter chains
+        auto steps = [&](int h, int i) {
+            const uint4 u = w[h][i];
+            const uint32_t ww[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+            for (int s = 0; s < kSteps; ++s) {
+                uint32_t b0, b1;
+                if constexpr (W8) i8x4_to_h2(ww[s], &b0, &b1);
+                else b0 = ww[2 * s], b1 = ww[2 * s + 1];
+                uint32_t ah[4], al[4];
+                if constexpr (WIDE) {
+                    ah[0] = xh[i][s][0], ah[1] = xh[i][s][1], ah[2] = xh[i][s][2], ah[3] = xh[i][s][3];
+                    al[0] = xl[i][s][0], al[1] = xl[i][s][1], al[2] = xl[i][s][2], al[3] = xl[i][s][3];
+                } else {
+                    ah[0] = xh[i][s][0], ah[1] = 0u, ah[2] = xh[i][s][1], ah[3] = 0u;
+                    al[0] = xl[i][s][0], al[1] = 0u, al[2] = xl[i][s][1], al[3] = 0u;
+                }
+                mma_f16(hi[h], ah, b0, b1);
+                mma_f16(lo[h], al, b0, b1);
+            }
+        };
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+#pragma unroll
+            for (int i = 0; i < kBlocks; ++i) steps(h, i);
+        if (it + 1 < my_tiles) request(tile + groups);
+        // D: rows g, g + 8; weight rows 2q, 2q + 1 of each 8
+        float* red = warps + (it & 1) * (kLrWarps * 272) + warp * 272;
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+                if (WIDE || e < 2) red[(g + 8 * (e >> 1)) * 17 + h * 8 + 2 * q + (e & 1)] = (hi[h][e] + lo[h][e]) * f[e >> 1];
+        __syncthreads();
+        if (WIDE || threadIdx.x < 128) {
+            const int m = threadIdx.x >> 4, c = threadIdx.x & 15;
+            const float* r = warps + (it & 1) * (kLrWarps * 272) + m * 17 + c;
+            float s = r[0];
+#pragma unroll
+            for (int v = 1; v < kLrWarps; ++v) s += r[v * 272];
+            lr_smem[it * 256 + threadIdx.x] = s;
+        }
+    }
+    if (nsplit > 1) cl.sync();
+    else __syncthreads();
+    if (a.n) pdl_wait();   // t of the shrink kernel
+
+    // epilogue: the cluster's CTAs share its tiles; partial sums in rank order
+    const int m = threadIdx.x >> 4, c = threadIdx.x & 15;
+    if (m < a.M) {
+        int r;
+        const int ad = lora_of(a, m, &r, false);
+        const float* t = a.t + (size_t)m * a.max_rank;
+        const void* Bp = ad >= 0 ? a.B[ad] : nullptr;
+        for (int it = rank; it < my_tiles; it += nsplit) {
+            const int n = (group + it * groups) * kLrCols + c;
+            if (n >= a.N) continue;
+            float s = 0.f;
+            for (int p = 0; p < nsplit; ++p) s += *(cl.map_shared_rank(lr_smem, p) + it * 256 + threadIdx.x);
+            s *= a.row_scales ? __ldg(a.row_scales + n) : a.tscale;
+            float d = 0.f;
+            if (a.f16 && (r & 7) == 0) {
+                const __half* B = static_cast<const __half*>(Bp) + (size_t)n * r;
+#pragma unroll 2
+                for (int j = 0; j < r; j += 8) {
+                    float b[8];
+                    h8_to_f8(__ldg(reinterpret_cast<const uint4*>(B + j)), b);
+                    const float4 u = *reinterpret_cast<const float4*>(t + j), v = *reinterpret_cast<const float4*>(t + j + 4);
+                    d = fmaf(b[0], u.x, fmaf(b[1], u.y, fmaf(b[2], u.z, fmaf(b[3], u.w, d))));
+                    d = fmaf(b[4], v.x, fmaf(b[5], v.y, fmaf(b[6], v.z, fmaf(b[7], v.w, d))));
+                }
+            } else if (!a.f16 && (r & 3) == 0) {
+                const float* B = static_cast<const float*>(Bp) + (size_t)n * r;
+#pragma unroll 4
+                for (int j = 0; j < r; j += 4) {
+                    const float4 b = __ldg(reinterpret_cast<const float4*>(B + j)), u = *reinterpret_cast<const float4*>(t + j);
+                    d = fmaf(b.x, u.x, fmaf(b.y, u.y, fmaf(b.z, u.z, fmaf(b.w, u.w, d))));
+                }
+            } else {
+#pragma unroll 4
+                for (int j = 0; j < r; ++j) d = fmaf(lora_elem(Bp, (size_t)n * r + j, a.f16), t[j], d);
+            }
+            a.y[(size_t)m * a.N + n] = s + d;
+        }
+    }
+    if (nsplit > 1) cl.sync();   // no CTA leaves while another reads its sums
+}
+
+template <bool W8, bool WIDE>
+static tvb_status launch_rows_kernel(const LoraArgs& a, bool dependent, cudaStream_t st) {
+    constexpr int kBlock = W8 ? 64 : 32, kMax = W8 ? 192 : kLrSlice;
+    LoraRowsPlan plan;
+    plan.tiles = (a.N + kLrCols - 1) / kLrCols;
+    // the fewest CTAs a cluster whose warps' slices hold K, slices as even as blocks of the load allow
+    const int nsplit = (a.K + kLrWarps * kMax - 1) / (kLrWarps * kMax);
+    const int per = (a.K + nsplit * kLrWarps - 1) / (nsplit * kLrWarps);
+    plan.slice = (per + kBlock - 1) / kBlock * kBlock;
+    int groups = std::max(1, std::min(plan.tiles, num_sms() * (WIDE ? 1 : 2) / nsplit));
+    const int smem = ((plan.tiles + groups - 1) / groups * 256 + 2 * kLrWarps * 272) * 4;
+    static int set[kMaxDevices];
+    TVB_TRY(allow_smem(reinterpret_cast<const void*>(lora_rows_kernel<W8, WIDE>), smem, set));
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned)(groups * nsplit));
+    cfg.blockDim = dim3(kLrThreads);
+    cfg.dynamicSmemBytes = (size_t)smem;
+    cfg.stream = st;
+    cudaLaunchAttribute attr[2];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = (unsigned)nsplit;
+    attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+    attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[1].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = dependent ? 2 : 1;
+    TVB_CUDA(cudaLaunchKernelEx(&cfg, lora_rows_kernel<W8, WIDE>, a, plan));
+    return check_launch("lora_rows_kernel");
+}
+
+// Whether the few-rows kernel takes a call: its rows fit one operand and a
+// cluster's warps hold K.
+static bool lora_few_rows(const LoraArgs& a) {
+    const int most = kLrMaxSplit * kLrWarps * (a.w8 ? 192 : kLrSlice);
+    const int tiles = (a.N + kLrCols - 1) / kLrCols;
+    return a.M <= kLrMaxRows && a.K <= most && tiles <= 148 * 100;
+}
+
+// Thread per (row, output): t . B_a added to y.
 __global__ void __launch_bounds__(256) lora_expand_kernel(const __grid_constant__ LoraArgs a) {
     const int m = blockIdx.y, n = blockIdx.x * 256 + threadIdx.x;
     int rank;
-    const int ad = lora_of(a, m, &rank);
+    const int ad = lora_of(a, m, &rank, false);
     if (ad < 0 || n >= a.N) return;
     const void* B = a.B[ad];
     float s = 0.f;
@@ -91,8 +327,6 @@ extern "C" tvb_status tvb_matmul_lora(float* y, const float* x, int M, int K, co
                 "matmul_lora: null adapter pointer");
     TVB_REQUIRE(table->dtype == TVB_F32 || table->dtype == TVB_F16, "matmul_lora: adapter dtype %d", (int)table->dtype);
     if (!M) return TVB_OK;
-    TVB_TRY(tvb_matmul(y, x, M, K, w, N, stream));
-    if (!table->n || !table->max_rank) return TVB_OK;
     const cudaStream_t st = as_stream(stream);
     LoraArgs a = {};
     a.x = x;
@@ -100,8 +334,12 @@ extern "C" tvb_status tvb_matmul_lora(float* y, const float* x, int M, int K, co
     a.M = M;
     a.K = K;
     a.N = N;
-    a.n = table->n;
-    a.max_rank = table->max_rank;
+    a.w = w->w;
+    a.w8 = w->dtype != TVB_F16;
+    a.row_scales = w->dtype == TVB_I8_ROW ? w->row_scales : nullptr;
+    a.tscale = w->dtype == TVB_I8_TENSOR ? w->tensor_scale : 1.0f;
+    a.n = table->max_rank ? table->n : 0;
+    a.max_rank = (table->max_rank + 3) & ~3;   // rows of t stay 16-byte aligned
     a.f16 = table->dtype == TVB_F16;
     a.A = table->A;
     a.B = table->B;
@@ -110,10 +348,19 @@ extern "C" tvb_status tvb_matmul_lora(float* y, const float* x, int M, int K, co
     a.adapter = adapter;
     a.status = status;
     Workspace ws(st);
-    TVB_TRY(ws.get((size_t)M * a.max_rank * 4));
-    a.t = ws.at<float>();
-    lora_shrink_kernel<<<dim3((unsigned)M, (unsigned)((a.max_rank + 7) / 8)), 256, 0, st>>>(a);
-    TVB_TRY(check_launch("lora_shrink_kernel"));
+    if (a.n) {
+        TVB_TRY(ws.get((size_t)M * a.max_rank * 4));
+        a.t = ws.at<float>();
+        lora_shrink_kernel<<<dim3((unsigned)M, (unsigned)((a.max_rank + 7) / 8)), 256, 0, st>>>(a);
+        TVB_TRY(check_launch("lora_shrink_kernel"));
+    }
+    if (lora_few_rows(a)) {
+        const bool wide = M > 8, dep = a.n > 0;
+        if (a.w8) return wide ? launch_rows_kernel<true, true>(a, dep, st) : launch_rows_kernel<true, false>(a, dep, st);
+        return wide ? launch_rows_kernel<false, true>(a, dep, st) : launch_rows_kernel<false, false>(a, dep, st);
+    }
+    TVB_TRY(tvb_matmul(y, x, M, K, w, N, stream));
+    if (!a.n) return TVB_OK;
     lora_expand_kernel<<<dim3((unsigned)((N + 255) / 256), (unsigned)M), 256, 0, st>>>(a);
     return check_launch("lora_expand_kernel");
 }
