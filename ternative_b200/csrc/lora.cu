@@ -14,8 +14,10 @@
 // thread's fragments of 2 or 4 steps are 16 contiguous bytes of a weight row.
 // The CTA's warps cut K, and the CTAs of a cluster cut it further; partial sums
 // meet in shared memory (distributed over the cluster), then the epilogue scales
-// INT8 rows and adds t . B_a.  It is launched as the shrink kernel's dependent
-// and waits for t only there, so both stream together.
+// INT8 rows and adds t . B_a.  It is launched as the shrink kernel's dependent,
+// which hides its launch; letting it start beside the shrink's CTAs was slower: the
+// clusters that then found no room ran as a second wave (8 rows 4096 -> 14336: 48 us
+// against 33).
 #include "lora.h"
 
 #include <algorithm>
@@ -27,43 +29,61 @@ namespace tvb {
 
 constexpr int kLrWarps = 8, kLrThreads = 32 * kLrWarps;
 constexpr int kLrCols = 16;        // weight rows a tile
-constexpr int kLrSlice = 160;      // largest K slice of a warp (F16; INT8: 192, a multiple of 64)
+// Largest K slice of a warp: what two CTAs an SM (one, when WIDE) have registers for.
+__host__ __device__ constexpr int lr_slice(bool w8, bool wide) { return !wide ? 128 : w8 ? 192 : 160; }
+constexpr int kLrBatch = 4;        // tiles between two barriers of the CTA
 constexpr int kLrMaxSplit = 8;     // CTAs of a cluster
 constexpr int kLrMaxRows = 16;
 
-// Warp per (row, rank index): K in float4 (or 8 halves) a lane.
+// A CTA takes 4 rank indexes of a row; its 8 warps cut K (8 k a lane), so that all
+// loads of a short K are in flight at once.
+constexpr int kLsRanks = 4;
+
+template <bool F16>
+__device__ __forceinline__ void lora_load8(const void* p, size_t at, float (&f)[8]) {
+    if constexpr (F16) {
+        h8_to_f8(__ldg(reinterpret_cast<const uint4*>(static_cast<const __half*>(p) + at)), f);
+    } else {
+        const float4* q = reinterpret_cast<const float4*>(static_cast<const float*>(p) + at);
+        const float4 x = __ldg(q), y = __ldg(q + 1);
+        f[0] = x.x, f[1] = x.y, f[2] = x.z, f[3] = x.w, f[4] = y.x, f[5] = y.y, f[6] = y.z, f[7] = y.w;
+    }
+}
+
+template <bool F16>
 __global__ void __launch_bounds__(256) lora_shrink_kernel(const __grid_constant__ LoraArgs a) {
-    pdl_launch_dependents();
-    const int m = blockIdx.x, lane = threadIdx.x & 31;
+    __shared__ float part[8][kLsRanks];
+    const int m = blockIdx.x, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     int rank;
     const int ad = lora_of(a, m, &rank, blockIdx.y == 0 && threadIdx.x == 0);
-    const int j = blockIdx.y * 8 + (threadIdx.x >> 5);
+    const int j = blockIdx.y * kLsRanks;
     if (j >= rank) return;
     const float* x = a.x + (size_t)m * a.K;
-    float s0 = 0.f, s1 = 0.f;
-    if (a.f16) {
-        const __half* A = static_cast<const __half*>(a.A[ad]) + (size_t)j * a.K;
-#pragma unroll 4
-        for (int k = lane * 8; k < a.K; k += 256) {
-            const uint4 u = __ldg(reinterpret_cast<const uint4*>(A + k));
-            float f[8];
-            h8_to_f8(u, f);
-            const float4 v = __ldg(reinterpret_cast<const float4*>(x + k)), w = __ldg(reinterpret_cast<const float4*>(x + k + 4));
-            s0 = fmaf(f[0], v.x, fmaf(f[1], v.y, fmaf(f[2], v.z, fmaf(f[3], v.w, s0))));
-            s1 = fmaf(f[4], w.x, fmaf(f[5], w.y, fmaf(f[6], w.z, fmaf(f[7], w.w, s1))));
-        }
-    } else {
-        const float* A = static_cast<const float*>(a.A[ad]) + (size_t)j * a.K;
-#pragma unroll 4
-        for (int k = lane * 8; k < a.K; k += 256) {
-            const float4 p = __ldg(reinterpret_cast<const float4*>(A + k)), q = __ldg(reinterpret_cast<const float4*>(A + k + 4));
-            const float4 v = __ldg(reinterpret_cast<const float4*>(x + k)), w = __ldg(reinterpret_cast<const float4*>(x + k + 4));
-            s0 = fmaf(p.x, v.x, fmaf(p.y, v.y, fmaf(p.z, v.z, fmaf(p.w, v.w, s0))));
-            s1 = fmaf(q.x, w.x, fmaf(q.y, w.y, fmaf(q.z, w.z, fmaf(q.w, w.w, s1))));
-        }
+    const void* A = a.A[ad];
+    float s[kLsRanks] = {};
+#pragma unroll 2
+    for (int k = (int)threadIdx.x * 8; k < a.K; k += 2048) {
+        float v[8], f[kLsRanks][8];
+#pragma unroll
+        for (int i = 0; i < kLsRanks; ++i) lora_load8<F16>(A, (size_t)min(j + i, rank - 1) * a.K + k, f[i]);
+        lora_load8<false>(x, k, v);
+#pragma unroll
+        for (int i = 0; i < kLsRanks; ++i)
+#pragma unroll
+            for (int e = 0; e < 8; ++e) s[i] = fmaf(f[i][e], v[e], s[i]);
     }
-    const float s = warp_sum(s0 + s1);
-    if (lane == 0) a.t[(size_t)m * a.max_rank + j] = s * __ldg(a.scale + ad);
+#pragma unroll
+    for (int i = 0; i < kLsRanks; ++i) {
+        s[i] = warp_sum(s[i]);
+        if (lane == 0) part[warp][i] = s[i];
+    }
+    __syncthreads();
+    if (threadIdx.x < kLsRanks && j + (int)threadIdx.x < rank) {
+        float t = 0.f;
+#pragma unroll
+        for (int w = 0; w < 8; ++w) t += part[w][threadIdx.x];
+        a.t[(size_t)m * a.max_rank + j + threadIdx.x] = t * __ldg(a.scale + ad);
+    }
 }
 
 __device__ __forceinline__ void mma_f16(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
@@ -84,9 +104,38 @@ __device__ __forceinline__ void i8x4_to_h2(uint32_t w, uint32_t* lo, uint32_t* h
     *hi = *reinterpret_cast<const uint32_t*>(&y);
 }
 
+// t . row of B from element `at` on
+__device__ __forceinline__ float lora_dot(const void* Bp, size_t at, const float* t, int r, bool f16) {
+    float d = 0.f;
+    if (f16 && (r & 7) == 0) {
+        const __half* B = static_cast<const __half*>(Bp) + at;
+#pragma unroll 2
+        for (int j = 0; j < r; j += 8) {
+            float b[8];
+            h8_to_f8(__ldg(reinterpret_cast<const uint4*>(B + j)), b);
+            const float4 u = *reinterpret_cast<const float4*>(t + j), v = *reinterpret_cast<const float4*>(t + j + 4);
+            d = fmaf(b[0], u.x, fmaf(b[1], u.y, fmaf(b[2], u.z, fmaf(b[3], u.w, d))));
+            d = fmaf(b[4], v.x, fmaf(b[5], v.y, fmaf(b[6], v.z, fmaf(b[7], v.w, d))));
+        }
+    } else if (!f16 && (r & 3) == 0) {
+        const float* B = static_cast<const float*>(Bp) + at;
+#pragma unroll 4
+        for (int j = 0; j < r; j += 4) {
+            const float4 b = __ldg(reinterpret_cast<const float4*>(B + j)), u = *reinterpret_cast<const float4*>(t + j);
+            d = fmaf(b.x, u.x, fmaf(b.y, u.y, fmaf(b.z, u.z, fmaf(b.w, u.w, d))));
+        }
+    } else {
+#pragma unroll 4
+        for (int j = 0; j < r; ++j) d = fmaf(lora_elem(Bp, at + j, f16), t[j], d);
+    }
+    return d;
+}
+
 struct LoraRowsPlan {
-    int slice;   // K of a warp
-    int tiles;   // tiles of weight rows
+    int slice;    // K of a warp in a pass
+    int passes;
+    int tiles;    // tiles of weight rows
+    int most;     // tiles of a cluster, at most
 };
 
 // W8: INT8 weights.  WIDE: 9 to 16 rows (else the upper half of the operand is
@@ -96,119 +145,136 @@ __global__ void __launch_bounds__(kLrThreads, WIDE ? 1 : 2)
 lora_rows_kernel(const __grid_constant__ LoraArgs a, const __grid_constant__ LoraRowsPlan plan) {
     constexpr int E = W8 ? 16 : 8;                     // weights in 16 bytes
     constexpr int kBlock = 4 * E;                      // k a load of the warp
-    constexpr int kBlocks = W8 ? 3 : kLrSlice / kBlock;   // loads a weight row
+    constexpr int kBlocks = lr_slice(W8, WIDE) / kBlock;     // loads a weight row
     constexpr int kSteps = E / 4;                      // MMA steps a load
     constexpr int kHalves = WIDE ? 2 : 1;
+    constexpr int kRed = kLrMaxRows * 17;              // a warp's sums of a tile
     extern __shared__ __align__(16) float lr_smem[];   // [tile][16 rows][16 weight rows], then the warps' sums
     cg::cluster_group cl = cg::this_cluster();
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, q = lane & 3;
     const int rank = (int)cl.block_rank(), nsplit = (int)cl.num_blocks();
     const int group = (int)(blockIdx.x / nsplit), groups = (int)(gridDim.x / nsplit);
-    const int k0 = (rank * kLrWarps + warp) * plan.slice;
     const int my_tiles = plan.tiles > group ? (plan.tiles - group + groups - 1) / groups : 0;
-    float* warps = lr_smem + ((plan.tiles + groups - 1) / groups) * 256;   // [2][8 warps][16][16 + 1]
-    const unsigned char* W = static_cast<const unsigned char*>(a.w);
+    float* warps = lr_smem + plan.most * 256;          // [2][kLrBatch tiles][8 warps][16][16 + 1]
+    const int64_t row_bytes = (int64_t)a.K * (W8 ? 1 : 2);
+    int batch = 0;
 
-    // this warp's weights of rows [n0, n0 + 16): 16 bytes of row g (and g + 8) a load
-    uint4 w[2][kBlocks];
-    auto request = [&](int tile) {
+#pragma unroll 1
+    for (int pass = 0; pass < plan.passes; ++pass) {
+        const int k0 = ((pass * nsplit + rank) * kLrWarps + warp) * plan.slice + q * E;   // this thread's first k
+        unsigned in_k = 0;   // its loads that lie inside K and the slice
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
-            const int n = tile * kLrCols + h * 8 + g;
+        for (int i = 0; i < kBlocks; ++i) in_k |= (unsigned)(i * kBlock < plan.slice && k0 + i * kBlock < a.K) << i;
+
+        // this warp's weights of 16 rows: 16 bytes of row g and of row g + 8 a load
+        uint4 w[2][kBlocks];
+        int n = group * kLrCols + g;
+        const unsigned char* wp = static_cast<const unsigned char*>(a.w) + n * row_bytes + (int64_t)k0 * (W8 ? 1 : 2);
+        auto request = [&]() {
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                const bool row = n + 8 * h < a.N;
+                const unsigned char* p = wp + 8 * h * row_bytes;
+#pragma unroll
+                for (int i = 0; i < kBlocks; ++i)
+                    w[h][i] = row && ((in_k >> i) & 1u) ? ld_stream16(p + i * 64) : make_uint4(0u, 0u, 0u, 0u);
+            }
+            n += groups * kLrCols;
+            wp += groups * kLrCols * row_bytes;
+        };
+        if (my_tiles) request();
+
+        // x of rows g (and g + 8), this thread's k, as hi + lo with a factor a row
+        uint32_t xh[kBlocks][kSteps][2 * kHalves], xl[kBlocks][kSteps][2 * kHalves];
+        float f[2] = {0.f, 0.f};
+#pragma unroll
+        for (int hf = 0; hf < kHalves; ++hf) {
+            const int m = g + 8 * hf;
+            float v[kBlocks][E];
+            float mx = 0.f;
 #pragma unroll
             for (int i = 0; i < kBlocks; ++i) {
-                const int k = k0 + i * kBlock + q * E;
-                w[h][i] = n < a.N && i * kBlock < plan.slice && k < a.K
-                              ? ld_stream16(W + ((size_t)n * a.K + k) * (W8 ? 1 : 2))
-                              : make_uint4(0u, 0u, 0u, 0u);
-            }
-        }
-    };
-    if (my_tiles) request(group);
-
-    // x of rows g (and g + 8), this thread's k, as hi + lo with a factor a row
-    uint32_t xh[kBlocks][kSteps][2 * kHalves], xl[kBlocks][kSteps][2 * kHalves];
-    float f[2] = {0.f, 0.f};
+                const bool in = m < a.M && ((in_k >> i) & 1u);
 #pragma unroll
-    for (int hf = 0; hf < kHalves; ++hf) {
-        const int m = g + 8 * hf;
-        float v[kBlocks][E];
-        float mx = 0.f;
-#pragma unroll
-        for (int i = 0; i < kBlocks; ++i) {
-            const int k = k0 + i * kBlock + q * E;
-            const bool in = m < a.M && i * kBlock < plan.slice && k < a.K;
-#pragma unroll
-            for (int e = 0; e < E; e += 4) {
-                const float4 x = in ? __ldg(reinterpret_cast<const float4*>(a.x + (size_t)m * a.K + k + e)) : make_float4(0.f, 0.f, 0.f, 0.f);
-                v[i][e] = x.x, v[i][e + 1] = x.y, v[i][e + 2] = x.z, v[i][e + 3] = x.w;
-                mx = fmaxf(mx, fmaxf(fmaxf(fabsf(x.x), fabsf(x.y)), fmaxf(fabsf(x.z), fabsf(x.w))));
-            }
-        }
-        mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
-        mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
-        int e2 = 0;   // the largest / 2^e2 in [2^13, 2^14)
-        if (mx > 0.f && mx < INFINITY) e2 = max(-100, min(100, (int)((__float_as_uint(mx) >> 23) & 255) - 127 - 13));
-        f[hf] = __uint_as_float((uint32_t)(127 + e2) << 23);
-        const float inv = __uint_as_float((uint32_t)(127 - e2) << 23);
-#pragma unroll
-        for (int i = 0; i < kBlocks; ++i)
-#pragma unroll
-            for (int s = 0; s < kSteps; ++s)
-#pragma unroll
-                for (int p = 0; p < 2; ++p) {
-                    const float x0 = v[i][4 * s + 2 * p] * inv, x1 = v[i][4 * s + 2 * p + 1] * inv;
-                    const __half2 hi = __floats2half2_rn(x0, x1);
-                    const float2 h = __half22float2(hi);
-                    const __half2 lo = __floats2half2_rn(x0 - h.x, x1 - h.y);
-                    xh[i][s][p * kHalves + hf] = *reinterpret_cast<const uint32_t*>(&hi);
-                    xl[i][s][p * kHalves + hf] = *reinterpret_cast<const uint32_t*>(&lo);
+                for (int e = 0; e < E; e += 4) {
+                    const float4 x = in ? __ldg(reinterpret_cast<const float4*>(a.x + (size_t)m * a.K + k0 + i * kBlock + e))
+                                        : make_float4(0.f, 0.f, 0.f, 0.f);
+                    v[i][e] = x.x, v[i][e + 1] = x.y, v[i][e + 2] = x.z, v[i][e + 3] = x.w;
+                    mx = fmaxf(mx, fmaxf(fmaxf(fabsf(x.x), fabsf(x.y)), fmaxf(fabsf(x.z), fabsf(x.w))));
                 }
-    }
-
-    for (int it = 0; it < my_tiles; ++it) {
-        const int tile = group + it * groups;
-        float hi[2][4] = {}, lo[2][4] = {};   // sums of the two planes apart: shorter chains
-        auto steps = [&](int h, int i) {
-            const uint4 u = w[h][i];
-            const uint32_t ww[4] = {u.x, u.y, u.z, u.w};
-#pragma unroll
-            for (int s = 0; s < kSteps; ++s) {
-                uint32_t b0, b1;
-                if constexpr (W8) i8x4_to_h2(ww[s], &b0, &b1);
-                else b0 = ww[2 * s], b1 = ww[2 * s + 1];
-                uint32_t ah[4], al[4];
-                if constexpr (WIDE) {
-                    ah[0] = xh[i][s][0], ah[1] = xh[i][s][1], ah[2] = xh[i][s][2], ah[3] = xh[i][s][3];
-                    al[0] = xl[i][s][0], al[1] = xl[i][s][1], al[2] = xl[i][s][2], al[3] = xl[i][s][3];
-                } else {
-                    ah[0] = xh[i][s][0], ah[1] = 0u, ah[2] = xh[i][s][1], ah[3] = 0u;
-                    al[0] = xl[i][s][0], al[1] = 0u, al[2] = xl[i][s][1], al[3] = 0u;
-                }
-                mma_f16(hi[h], ah, b0, b1);
-                mma_f16(lo[h], al, b0, b1);
             }
-        };
+            mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
+            mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
+            int e2 = 0;   // the largest / 2^e2 in [2^13, 2^14)
+            if (mx > 0.f && mx < INFINITY) e2 = max(-100, min(100, (int)((__float_as_uint(mx) >> 23) & 255) - 127 - 13));
+            f[hf] = __uint_as_float((uint32_t)(127 + e2) << 23);
+            const float inv = __uint_as_float((uint32_t)(127 - e2) << 23);
 #pragma unroll
-        for (int h = 0; h < 2; ++h)
+            for (int i = 0; i < kBlocks; ++i)
 #pragma unroll
-            for (int i = 0; i < kBlocks; ++i) steps(h, i);
-        if (it + 1 < my_tiles) request(tile + groups);
-        // D: rows g, g + 8; weight rows 2q, 2q + 1 of each 8
-        float* red = warps + (it & 1) * (kLrWarps * 272) + warp * 272;
+                for (int s = 0; s < kSteps; ++s)
 #pragma unroll
-        for (int h = 0; h < 2; ++h)
+                    for (int p = 0; p < 2; ++p) {
+                        const float x0 = v[i][4 * s + 2 * p] * inv, x1 = v[i][4 * s + 2 * p + 1] * inv;
+                        const __half2 hi = __floats2half2_rn(x0, x1);
+                        const float2 h = __half22float2(hi);
+                        const __half2 lo = __floats2half2_rn(x0 - h.x, x1 - h.y);
+                        xh[i][s][p * kHalves + hf] = *reinterpret_cast<const uint32_t*>(&hi);
+                        xl[i][s][p * kHalves + hf] = *reinterpret_cast<const uint32_t*>(&lo);
+                    }
+        }
+
+        // kLrBatch tiles between barriers: the warps run apart as far as that
+#pragma unroll 1
+        for (int it = 0; it < my_tiles; it += kLrBatch, ++batch) {
+            float* half = warps + (batch & 1) * (kLrBatch * kLrWarps * kRed);
+            const int nb = min(kLrBatch, my_tiles - it);
+#pragma unroll 1
+            for (int b = 0; b < nb; ++b) {
+                float hi[2][4] = {}, lo[2][4] = {};   // sums of the two planes apart: shorter chains
 #pragma unroll
-            for (int e = 0; e < 4; ++e)
-                if (WIDE || e < 2) red[(g + 8 * (e >> 1)) * 17 + h * 8 + 2 * q + (e & 1)] = (hi[h][e] + lo[h][e]) * f[e >> 1];
-        __syncthreads();
-        if (WIDE || threadIdx.x < 128) {
-            const int m = threadIdx.x >> 4, c = threadIdx.x & 15;
-            const float* r = warps + (it & 1) * (kLrWarps * 272) + m * 17 + c;
-            float s = r[0];
+                for (int h = 0; h < 2; ++h)
 #pragma unroll
-            for (int v = 1; v < kLrWarps; ++v) s += r[v * 272];
-            lr_smem[it * 256 + threadIdx.x] = s;
+                    for (int i = 0; i < kBlocks; ++i) {
+                        const uint32_t ww[4] = {w[h][i].x, w[h][i].y, w[h][i].z, w[h][i].w};
+#pragma unroll
+                        for (int s = 0; s < kSteps; ++s) {
+                            uint32_t b0, b1;
+                            if constexpr (W8) i8x4_to_h2(ww[s], &b0, &b1);
+                            else b0 = ww[2 * s], b1 = ww[2 * s + 1];
+                            uint32_t ah[4], al[4];
+                            if constexpr (WIDE) {
+                                ah[0] = xh[i][s][0], ah[1] = xh[i][s][1], ah[2] = xh[i][s][2], ah[3] = xh[i][s][3];
+                                al[0] = xl[i][s][0], al[1] = xl[i][s][1], al[2] = xl[i][s][2], al[3] = xl[i][s][3];
+                            } else {
+                                ah[0] = xh[i][s][0], ah[1] = 0u, ah[2] = xh[i][s][1], ah[3] = 0u;
+                                al[0] = xl[i][s][0], al[1] = 0u, al[2] = xl[i][s][1], al[3] = 0u;
+                            }
+                            mma_f16(hi[h], ah, b0, b1);
+                            mma_f16(lo[h], al, b0, b1);
+                        }
+                    }
+                if (it + b + 1 < my_tiles) request();
+                // D: rows g, g + 8; weight rows 2q, 2q + 1 of each 8
+                float* red = half + (b * kLrWarps + warp) * kRed;
+#pragma unroll
+                for (int h = 0; h < 2; ++h)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e)
+                        if (WIDE || e < 2) red[(g + 8 * (e >> 1)) * 17 + h * 8 + 2 * q + (e & 1)] = (hi[h][e] + lo[h][e]) * f[e >> 1];
+            }
+            __syncthreads();
+            if (WIDE || threadIdx.x < 128) {
+                const int at = (threadIdx.x >> 4) * 17 + (threadIdx.x & 15);
+                for (int b = 0; b < nb; ++b) {
+                    const float* r = half + b * kLrWarps * kRed + at;
+                    float s = r[0];
+#pragma unroll
+                    for (int v = 1; v < kLrWarps; ++v) s += r[v * kRed];
+                    float* sum = lr_smem + (it + b) * 256 + threadIdx.x;
+                    *sum = pass ? *sum + s : s;
+                }
+            }
         }
     }
     if (nsplit > 1) cl.sync();
@@ -222,35 +288,14 @@ lora_rows_kernel(const __grid_constant__ LoraArgs a, const __grid_constant__ Lor
         const int ad = lora_of(a, m, &r, false);
         const float* t = a.t + (size_t)m * a.max_rank;
         const void* Bp = ad >= 0 ? a.B[ad] : nullptr;
+#pragma unroll 1
         for (int it = rank; it < my_tiles; it += nsplit) {
             const int n = (group + it * groups) * kLrCols + c;
             if (n >= a.N) continue;
             float s = 0.f;
             for (int p = 0; p < nsplit; ++p) s += *(cl.map_shared_rank(lr_smem, p) + it * 256 + threadIdx.x);
             s *= a.row_scales ? __ldg(a.row_scales + n) : a.tscale;
-            float d = 0.f;
-            if (a.f16 && (r & 7) == 0) {
-                const __half* B = static_cast<const __half*>(Bp) + (size_t)n * r;
-#pragma unroll 2
-                for (int j = 0; j < r; j += 8) {
-                    float b[8];
-                    h8_to_f8(__ldg(reinterpret_cast<const uint4*>(B + j)), b);
-                    const float4 u = *reinterpret_cast<const float4*>(t + j), v = *reinterpret_cast<const float4*>(t + j + 4);
-                    d = fmaf(b[0], u.x, fmaf(b[1], u.y, fmaf(b[2], u.z, fmaf(b[3], u.w, d))));
-                    d = fmaf(b[4], v.x, fmaf(b[5], v.y, fmaf(b[6], v.z, fmaf(b[7], v.w, d))));
-                }
-            } else if (!a.f16 && (r & 3) == 0) {
-                const float* B = static_cast<const float*>(Bp) + (size_t)n * r;
-#pragma unroll 4
-                for (int j = 0; j < r; j += 4) {
-                    const float4 b = __ldg(reinterpret_cast<const float4*>(B + j)), u = *reinterpret_cast<const float4*>(t + j);
-                    d = fmaf(b.x, u.x, fmaf(b.y, u.y, fmaf(b.z, u.z, fmaf(b.w, u.w, d))));
-                }
-            } else {
-#pragma unroll 4
-                for (int j = 0; j < r; ++j) d = fmaf(lora_elem(Bp, (size_t)n * r + j, a.f16), t[j], d);
-            }
-            a.y[(size_t)m * a.N + n] = s + d;
+            a.y[(size_t)m * a.N + n] = s + lora_dot(Bp, (size_t)n * r, t, r, a.f16);
         }
     }
     if (nsplit > 1) cl.sync();   // no CTA leaves while another reads its sums
@@ -258,21 +303,20 @@ lora_rows_kernel(const __grid_constant__ LoraArgs a, const __grid_constant__ Lor
 
 template <bool W8, bool WIDE>
 static tvb_status launch_rows_kernel(const LoraArgs& a, bool dependent, cudaStream_t st) {
-    constexpr int kBlock = W8 ? 64 : 32, kMax = W8 ? 192 : kLrSlice;
+    const auto kernel = lora_rows_kernel<W8, WIDE>;
+    constexpr int kBlock = W8 ? 64 : 32, kMax = lr_slice(W8, WIDE);
     LoraRowsPlan plan;
     plan.tiles = (a.N + kLrCols - 1) / kLrCols;
-    // the fewest CTAs a cluster whose warps' slices hold K, slices as even as blocks of the load allow
-    const int nsplit = (a.K + kLrWarps * kMax - 1) / (kLrWarps * kMax);
-    const int per = (a.K + nsplit * kLrWarps - 1) / (nsplit * kLrWarps);
+    // CTAs a cluster: a power of two, which clusters pack best into the GPU, until the warps' slices hold K in one pass
+    int nsplit = 1;
+    while (nsplit < kLrMaxSplit && nsplit * kLrWarps * kMax < a.K) nsplit *= 2;
+    plan.passes = (a.K + nsplit * kLrWarps * kMax - 1) / (nsplit * kLrWarps * kMax);
+    const int per = (a.K + plan.passes * nsplit * kLrWarps - 1) / (plan.passes * nsplit * kLrWarps);
     plan.slice = (per + kBlock - 1) / kBlock * kBlock;
-    int groups = std::max(1, std::min(plan.tiles, num_sms() * (WIDE ? 1 : 2) / nsplit));
-    const int smem = ((plan.tiles + groups - 1) / groups * 256 + 2 * kLrWarps * 272) * 4;
-    static int set[kMaxDevices];
-    TVB_TRY(allow_smem(reinterpret_cast<const void*>(lora_rows_kernel<W8, WIDE>), smem, set));
+    constexpr int kWarpSums = 2 * kLrBatch * kLrWarps * kLrMaxRows * 17;
+
     cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3((unsigned)(groups * nsplit));
     cfg.blockDim = dim3(kLrThreads);
-    cfg.dynamicSmemBytes = (size_t)smem;
     cfg.stream = st;
     cudaLaunchAttribute attr[2];
     attr[0].id = cudaLaunchAttributeClusterDimension;
@@ -281,17 +325,30 @@ static tvb_status launch_rows_kernel(const LoraArgs& a, bool dependent, cudaStre
     attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
     attr[1].val.programmaticStreamSerializationAllowed = 1;
     cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    // clusters that fit the GPU at once: one more would be a second wave
+    static int resident[kMaxDevices][kLrMaxSplit + 1];
+    static int set[kMaxDevices];
+    constexpr int kSmem = 100 * 1024;
+    TVB_TRY(allow_smem(reinterpret_cast<const void*>(kernel), kSmem, set));
+    int dev = 0;
+    TVB_CUDA(cudaGetDevice(&dev));
+    if (!resident[dev][nsplit]) {
+        int n = 0;
+        cfg.gridDim = dim3((unsigned)nsplit);
+        cfg.dynamicSmemBytes = kSmem;
+        TVB_CUDA(cudaOccupancyMaxActiveClusters(&n, kernel, &cfg));
+        resident[dev][nsplit] = std::max(1, n);
+    }
+    // as many groups as are resident, or more where a group's sums would not fit
+    const int fit = (kSmem / 4 - kWarpSums) / 256;
+    const int groups = std::min(plan.tiles, std::max(resident[dev][nsplit], (plan.tiles + fit - 1) / fit));
+    plan.most = (plan.tiles + groups - 1) / groups;
+    cfg.gridDim = dim3((unsigned)(groups * nsplit));
+    cfg.dynamicSmemBytes = (size_t)(plan.most * 256 + kWarpSums) * 4;
     cfg.numAttrs = dependent ? 2 : 1;
-    TVB_CUDA(cudaLaunchKernelEx(&cfg, lora_rows_kernel<W8, WIDE>, a, plan));
+    TVB_CUDA(cudaLaunchKernelEx(&cfg, kernel, a, plan));
     return check_launch("lora_rows_kernel");
-}
-
-// Whether the few-rows kernel takes a call: its rows fit one operand and a
-// cluster's warps hold K.
-static bool lora_few_rows(const LoraArgs& a) {
-    const int most = kLrMaxSplit * kLrWarps * (a.w8 ? 192 : kLrSlice);
-    const int tiles = (a.N + kLrCols - 1) / kLrCols;
-    return a.M <= kLrMaxRows && a.K <= most && tiles <= 148 * 100;
 }
 
 // Thread per (row, output): t . B_a added to y.
@@ -351,10 +408,12 @@ extern "C" tvb_status tvb_matmul_lora(float* y, const float* x, int M, int K, co
     if (a.n) {
         TVB_TRY(ws.get((size_t)M * a.max_rank * 4));
         a.t = ws.at<float>();
-        lora_shrink_kernel<<<dim3((unsigned)M, (unsigned)((a.max_rank + 7) / 8)), 256, 0, st>>>(a);
+        const dim3 grid((unsigned)M, (unsigned)((a.max_rank + kLsRanks - 1) / kLsRanks));
+        if (a.f16) lora_shrink_kernel<true><<<grid, 256, 0, st>>>(a);
+        else lora_shrink_kernel<false><<<grid, 256, 0, st>>>(a);
         TVB_TRY(check_launch("lora_shrink_kernel"));
     }
-    if (lora_few_rows(a)) {
+    if (M <= kLrMaxRows) {
         const bool wide = M > 8, dep = a.n > 0;
         if (a.w8) return wide ? launch_rows_kernel<true, true>(a, dep, st) : launch_rows_kernel<true, false>(a, dep, st);
         return wide ? launch_rows_kernel<false, true>(a, dep, st) : launch_rows_kernel<false, false>(a, dep, st);
