@@ -351,18 +351,6 @@ static tvb_status launch_rows_kernel(const LoraArgs& a, bool dependent, cudaStre
     return check_launch("lora_rows_kernel");
 }
 
-// Thread per (row, output): t . B_a added to y.
-__global__ void __launch_bounds__(256) lora_expand_kernel(const __grid_constant__ LoraArgs a) {
-    const int m = blockIdx.y, n = blockIdx.x * 256 + threadIdx.x;
-    int rank;
-    const int ad = lora_of(a, m, &rank, false);
-    if (ad < 0 || n >= a.N) return;
-    const void* B = a.B[ad];
-    float s = 0.f;
-    for (int j = 0; j < rank; ++j) s = fmaf(a.t[(size_t)m * a.max_rank + j], lora_elem(B, (size_t)n * rank + j, a.f16), s);
-    a.y[(size_t)m * a.N + n] += s;
-}
-
 }  // namespace tvb
 
 extern "C" tvb_status tvb_matmul_lora(float* y, const float* x, int M, int K, const tvb_weight* w, int N,
@@ -404,6 +392,7 @@ extern "C" tvb_status tvb_matmul_lora(float* y, const float* x, int M, int K, co
     a.scale = table->scale;
     a.adapter = adapter;
     a.status = status;
+    if (M > kLrMaxRows) return lora_many_rows(a, st);
     Workspace ws(st);
     if (a.n) {
         TVB_TRY(ws.get((size_t)M * a.max_rank * 4));
@@ -413,13 +402,7 @@ extern "C" tvb_status tvb_matmul_lora(float* y, const float* x, int M, int K, co
         else lora_shrink_kernel<false><<<grid, 256, 0, st>>>(a);
         TVB_TRY(check_launch("lora_shrink_kernel"));
     }
-    if (M <= kLrMaxRows) {
-        const bool wide = M > 8, dep = a.n > 0;
-        if (a.w8) return wide ? launch_rows_kernel<true, true>(a, dep, st) : launch_rows_kernel<true, false>(a, dep, st);
-        return wide ? launch_rows_kernel<false, true>(a, dep, st) : launch_rows_kernel<false, false>(a, dep, st);
-    }
-    TVB_TRY(tvb_matmul(y, x, M, K, w, N, stream));
-    if (!a.n) return TVB_OK;
-    lora_expand_kernel<<<dim3((unsigned)((N + 255) / 256), (unsigned)M), 256, 0, st>>>(a);
-    return check_launch("lora_expand_kernel");
+    const bool wide = M > 8, dep = a.n > 0;
+    if (a.w8) return wide ? launch_rows_kernel<true, true>(a, dep, st) : launch_rows_kernel<true, false>(a, dep, st);
+    return wide ? launch_rows_kernel<false, true>(a, dep, st) : launch_rows_kernel<false, false>(a, dep, st);
 }

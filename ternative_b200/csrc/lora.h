@@ -49,4 +49,6 @@ __device__ __forceinline__ float lora_elem(const void* p, size_t i, bool f16) {
     return f16 ? __half2float(static_cast<const __half*>(p)[i]) : static_cast<const float*>(p)[i];
 }
 
+tvb_status lora_many_rows(LoraArgs a, cudaStream_t st);   // lora_gemm.cu
+
 }  // namespace tvb

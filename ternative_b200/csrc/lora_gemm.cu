@@ -1,0 +1,615 @@
+// A projection with an adapter for each row, for more rows than a decode batch
+// (tvb_matmul_lora; lora.cu has the few-rows kernels).
+//
+// x is split once into F16 hi + lo planes with a power-of-two factor a row
+// (pf_norm_split), so that F16 products are F32-faithful; the bound is the tensor
+// pipe at twice the FLOPs of the projection.
+//
+// lora_shrink_tile_kernel: t[m] = scale_a A_a x[m] for 16 rows a CTA.  x and A as
+// three bf16 planes (8 bits each, any magnitude), six products of mma.sync
+// m16n8k16; 16 warps cut K.  Small next to the projection (rank / N of it).
+// lora_gemm_kernel: 128 rows of x by 256 weight rows a tile, tcgen05 fed by TMA.
+// The tensor core truncates as it accumulates (about 2^-26 of the sum an MMA), so
+// four k-blocks (32 MMAs) are summed in TMEM and added to registers by the
+// epilogue warps while the next four go to the other half of TMEM.  After its
+// k-blocks a tile takes one more such product per adapter among its rows: t . B_a
+// as TF32 hi + lo planes (any magnitude, three products), added to that adapter's
+// rows alone, so one request's adapter never touches another's row, whatever it
+// holds.  Every CTA takes an equal run of the tiles' chunks; a tile that a cut
+// divides leaves F32 partial sums and lora_join_kernel adds them.
+#include <algorithm>
+
+#include "lora.h"
+#include "prefill.h"
+#include "tcgen05.cuh"
+
+namespace tvb {
+
+// ---- shrink -----------------------------------------------------------------------
+constexpr int kLtWarps = 16, kLtRows = 16, kLtRanks = 64;
+
+__device__ __forceinline__ void mma_bf16(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+    asm volatile(
+        "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+        : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+
+// (x, y) as three packed bf16 planes, each the rounded rest of the one before.
+__device__ __forceinline__ void bf16_planes(float x, float y, uint32_t (&p)[3]) {
+#pragma unroll
+    for (int i = 0; i < 3; ++i) {
+        asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(p[i]) : "f"(y), "f"(x));
+        x -= __uint_as_float(p[i] << 16);
+        y -= __uint_as_float(p[i] & 0xffff0000u);
+    }
+}
+
+// The next adapter after `prev` among ids[] (4 a lane, -1 none), or INT_MAX.
+__device__ __forceinline__ int next_adapter(const int (&ids)[4], int prev) {
+    int v = 0x7fffffff;
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+        if (ids[i] > prev) v = min(v, ids[i]);
+    return __reduce_min_sync(0xffffffffu, v);
+}
+
+template <bool F16>
+__device__ __forceinline__ float4 lora_load4(const void* p, size_t at) {
+    if constexpr (F16) {
+        const uint2 u = __ldg(reinterpret_cast<const uint2*>(static_cast<const __half*>(p) + at));
+        const float2 x = __half22float2(*reinterpret_cast<const __half2*>(&u.x)), y = __half22float2(*reinterpret_cast<const __half2*>(&u.y));
+        return make_float4(x.x, x.y, y.x, y.y);
+    } else {
+        return __ldg(reinterpret_cast<const float4*>(static_cast<const float*>(p) + at));
+    }
+}
+
+template <bool F16>
+__global__ void __launch_bounds__(32 * kLtWarps, 1) lora_shrink_tile_kernel(const __grid_constant__ LoraArgs a) {
+    extern __shared__ float lt_red[];   // [warp][16 rows][kLtRanks + 1]
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, q = lane & 3;
+    const int m0 = blockIdx.x * kLtRows;
+    int ids[4] = {-1, -1, -1, -1}, rank_of = 0;
+    if (lane < kLtRows && m0 + lane < a.M) ids[0] = lora_of(a, m0 + lane, &rank_of, warp == 0);
+    const int steps = ((a.K + 15) / 16 + kLtWarps - 1) / kLtWarps;   // of 16 k, a warp
+    const int s0 = warp * steps, s1 = min(s0 + steps, (a.K + 15) / 16);
+    for (int ad = next_adapter(ids, -1); ad != 0x7fffffff; ad = next_adapter(ids, ad)) {
+        const int rank = __ldg(a.rank + ad);
+        const void* A = a.A[ad];
+        for (int j0 = 0; j0 < rank; j0 += kLtRanks) {
+            const int nt = min(kLtRanks / 8, (rank - j0 + 7) / 8);
+            float acc[kLtRanks / 8][4] = {};
+#pragma unroll 1
+            for (int s = s0; s < s1; ++s) {
+                // k permuted so that a thread's fragments are 4 consecutive k
+                const int k = s * 16 + 4 * q;
+                const bool in = k < a.K;
+                uint32_t xa[3][4];
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                    const int m = m0 + g + 8 * h;
+                    const float4 x = in && m < a.M ? lora_load4<false>(a.x, (size_t)m * a.K + k) : make_float4(0.f, 0.f, 0.f, 0.f);
+                    uint32_t p[3], r[3];
+                    bf16_planes(x.x, x.y, p);
+                    bf16_planes(x.z, x.w, r);
+#pragma unroll
+                    for (int i = 0; i < 3; ++i) xa[i][h] = p[i], xa[i][2 + h] = r[i];
+                }
+#pragma unroll
+                for (int n = 0; n < kLtRanks / 8; ++n) {
+                    if (n >= nt) break;
+                    const int j = j0 + n * 8 + g;
+                    const float4 w = in && j < rank ? lora_load4<F16>(A, (size_t)j * a.K + k) : make_float4(0.f, 0.f, 0.f, 0.f);
+                    uint32_t p[3], r[3];
+                    bf16_planes(w.x, w.y, p);
+                    bf16_planes(w.z, w.w, r);
+                    // planes i + j <= 2: what is left out is below 2^-24
+                    mma_bf16(acc[n], xa[0], p[2], r[2]);
+                    mma_bf16(acc[n], xa[1], p[1], r[1]);
+                    mma_bf16(acc[n], xa[2], p[0], r[0]);
+                    mma_bf16(acc[n], xa[0], p[1], r[1]);
+                    mma_bf16(acc[n], xa[1], p[0], r[0]);
+                    mma_bf16(acc[n], xa[0], p[0], r[0]);
+                }
+            }
+            float* red = lt_red + warp * kLtRows * (kLtRanks + 1);
+#pragma unroll
+            for (int n = 0; n < kLtRanks / 8; ++n)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) red[(g + 8 * (e >> 1)) * (kLtRanks + 1) + n * 8 + 2 * q + (e & 1)] = acc[n][e];
+            __syncthreads();
+            const float scale = __ldg(a.scale + ad);
+            for (int i = threadIdx.x; i < kLtRows * kLtRanks; i += 32 * kLtWarps) {
+                const int m = i / kLtRanks, j = i % kLtRanks;
+                const bool mine = m0 + m < a.M && __ldg(a.adapter + m0 + m) == ad && j0 + j < rank;
+                float s = 0.f;
+#pragma unroll
+                for (int w = 0; w < kLtWarps; ++w) s += lt_red[(w * kLtRows + m) * (kLtRanks + 1) + j];
+                if (mine) a.t[(size_t)(m0 + m) * a.max_rank + j0 + j] = s * scale;
+            }
+            __syncthreads();
+        }
+    }
+}
+
+// ---- projection ---------------------------------------------------------------------
+constexpr int kLgRows = 128, kLgCols = 256, kLgStages = 3, kLgChunk = 4;   // k-blocks a chunk
+constexpr int kLgSoft = 8, kLgThreads = 384;
+constexpr int kLgExtra = 2;   // what starting and leaving a tile costs, in chunks
+constexpr int kLgPlane = kLgRows * 128, kLgStage = 2 * kLgPlane + kLgCols * 128;
+constexpr int kLgLora = 2 * (kLgRows + kLgCols) * 32;   // t hi, lo, B hi, lo of 8 rank indexes
+
+struct LgShared {
+    uint64_t full[kLgStages], empty[kLgStages];
+    uint64_t acc_full[2], acc_empty[2];
+    uint64_t l_full, l_empty, drained;
+    uint32_t tmem;
+    int abort;
+};
+constexpr int kLgSmem = kLgStages * kLgStage + kLgLora + (int)sizeof(LgShared) + 1024;
+
+struct LgMaps {
+    CUtensorMap xh, xl, w;
+};
+
+struct LgPlan {
+    int mt, tiles;      // tiles of rows, of both
+    int nk, chunks;     // k-blocks, chunks a tile
+    int ctas;
+    const int* row_exp;
+    float* part;        // [CTA][2][128][256]
+};
+
+struct LgPiece {
+    int m0, n0, c0, c1, slot, last_cta;
+};
+
+// The next piece from unit *u on: a tile's chunks [c0, c1).  A tile is kLgExtra +
+// chunks units; CTA c takes [T c / G, T (c + 1) / G) of them.
+__device__ __forceinline__ int64_t lg_begin(const LgPlan& p, int c) {
+    return (int64_t)p.tiles * (p.chunks + kLgExtra) * c / p.ctas;
+}
+__device__ __forceinline__ bool lg_next(const LgPlan& p, int64_t* u, int64_t end, LgPiece* out) {
+    const int per = p.chunks + kLgExtra;
+    while (*u < end) {
+        const int tile = (int)(*u / per), r = (int)(*u - (int64_t)tile * per);
+        const int e = (int)min((int64_t)per, r + (end - *u)), b = max(r, kLgExtra);
+        *u = (int64_t)tile * per + e;
+        if (b >= e) continue;
+        out->m0 = tile % p.mt * kLgRows;
+        out->n0 = tile / p.mt * kLgCols;
+        out->c0 = b - kLgExtra;
+        out->c1 = e - kLgExtra;
+        out->slot = out->c1 - out->c0 == p.chunks ? -1 : out->c0 > 0 ? 0 : 1;
+        out->last_cta = (int)((((int64_t)tile + 1) * per * p.ctas - 1) / ((int64_t)p.tiles * per));
+        return true;
+    }
+    return false;
+}
+
+__device__ __forceinline__ uint64_t sw32_desc(uint32_t saddr) {   // K-major, rows of 32 bytes, 8-row groups 256 apart
+    uint64_t d = (uint64_t)((saddr & 0x3FFFFu) >> 4);
+    d |= (uint64_t)1u << 16;
+    d |= (uint64_t)(256u >> 4) << 32;
+    d |= (uint64_t)1u << 46;
+    d |= (uint64_t)6u << 61;
+    return d;
+}
+__device__ __forceinline__ uint32_t sw32_offset(int row, int chunk) { return (uint32_t)(row * 32 + ((chunk ^ ((row >> 2) & 1)) * 16)); }
+
+__device__ __forceinline__ void tc_mma_tf32(uint32_t tmem_d, uint64_t adesc, uint64_t bdesc, uint32_t idesc, uint32_t accumulate) {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "setp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::tf32 [%0], %1, %2, %3, p;\n\t}" ::"r"(tmem_d),
+        "l"(adesc), "l"(bdesc), "r"(idesc), "r"(accumulate)
+        : "memory");
+}
+// kind::tf32: D F32, A and B TF32 (2), both K-major
+constexpr uint32_t umma_idesc_tf32(int M, int N) {
+    return (1u << 4) | (2u << 7) | (2u << 10) | ((uint32_t)(N >> 3) << 17) | ((uint32_t)(M >> 4) << 24);
+}
+
+__device__ __forceinline__ uint64_t lg_pack2(float x, float y) {
+    uint64_t r;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(x), "f"(y));
+    return r;
+}
+__device__ __forceinline__ float2 lg_unpack2(uint64_t v) {
+    float2 r;
+    asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(v));
+    return r;
+}
+__device__ __forceinline__ uint64_t lg_fma2(uint64_t a, uint64_t b, uint64_t c) {
+    uint64_t r;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+    return r;
+}
+__device__ __forceinline__ void lg_arrive(uint64_t* bar) {
+    asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_u32(bar)) : "memory");
+}
+
+// The adapters of rows [m0, m0 + 128): 4 rows a lane.
+__device__ __forceinline__ void lg_ids(const LoraArgs& a, int m0, int (&ids)[4]) {
+    const int lane = threadIdx.x & 31;
+    int r;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const int m = m0 + lane * 4 + i;
+        ids[i] = m < a.M ? lora_of(a, m, &r, false) : -1;
+        if (ids[i] >= 0 && r == 0) ids[i] = -1;
+    }
+}
+
+__global__ void __launch_bounds__(kLgThreads, 1)
+lora_gemm_kernel(const __grid_constant__ LgMaps maps, const __grid_constant__ LoraArgs a, const __grid_constant__ LgPlan plan) {
+    extern __shared__ unsigned char lg_raw[];
+    const uint32_t raw = smem_u32(lg_raw);
+    const uint32_t base = (raw + 1023u) & ~1023u;
+    unsigned char* smem = lg_raw + (base - raw);
+    LgShared& sh = *reinterpret_cast<LgShared*>(smem + kLgStages * kLgStage + kLgLora);
+    const uint32_t lora_s = base + kLgStages * kLgStage;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+
+    if (threadIdx.x == 0) {
+        for (int i = 0; i < kLgStages; ++i) {
+            mbar_init(sh.full + i, 1);
+            mbar_init(sh.empty + i, 1);
+        }
+        for (int i = 0; i < 2; ++i) {
+            mbar_init(sh.acc_full + i, 1);
+            mbar_init(sh.acc_empty + i, kLgSoft);
+        }
+        mbar_init(&sh.l_full, 2);
+        mbar_init(&sh.l_empty, 1);
+        mbar_init(&sh.drained, 1);
+        sh.abort = 0;
+        fence_barrier_init();
+    }
+    if (warp == 9) tmem_alloc(&sh.tmem, 512);
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem = sh.tmem;
+    volatile int* abort_flag = &sh.abort;
+    auto fail = [&]() {
+        *abort_flag = 1;
+        if (a.status) atomicOr(a.status, TVB_DEV_TIMEOUT);
+    };
+    pdl_wait();   // the planes and t come from the kernels before
+    int64_t u = lg_begin(plan, blockIdx.x);
+    const int64_t end = lg_begin(plan, blockIdx.x + 1);
+    LgPiece p;
+
+    // registers: 128 x (200 + 200 + 104) = 384 x 168, what the CTA was launched with
+    if (warp >= kLgSoft) {
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 104;");
+        if (warp == 8) {
+            // ---- TMA producer -----------------------------------------------------
+            if (lane == 0) {
+                prefetch_tmap(&maps.xh);
+                prefetch_tmap(&maps.xl);
+                prefetch_tmap(&maps.w);
+                int it = 0;
+                bool ok = true;
+                while (ok && lg_next(plan, &u, end, &p)) {
+                    for (int kb = p.c0 * kLgChunk; kb < min(plan.nk, p.c1 * kLgChunk); ++kb, ++it) {
+                        const int s = it % kLgStages;
+                        ok = mbar_wait_bounded(sh.empty + s, (uint32_t)((it / kLgStages + 1) & 1)) && !*abort_flag;
+                        if (!ok) break;
+                        const uint32_t st = base + s * kLgStage;
+                        mbar_expect_tx(sh.full + s, kLgStage);
+                        tma_load_2d(st, &maps.xh, kb * 64, p.m0, sh.full + s);
+                        tma_load_2d(st + kLgPlane, &maps.xl, kb * 64, p.m0, sh.full + s);
+                        tma_load_2d(st + 2 * kLgPlane, &maps.w, kb * 64, p.n0, sh.full + s);
+                    }
+                }
+                if (!ok) {
+                    fail();
+                    // no TMA write may outlive the CTA
+                    for (int i = max(0, it - kLgStages); i < it; ++i)
+                        mbar_wait_bounded(sh.full + i % kLgStages, (uint32_t)((i / kLgStages) & 1));
+                }
+            }
+        } else if (warp == 9) {
+            // ---- MMA issuer ----------------------------------------------------------
+            constexpr uint32_t idesc = umma_idesc_f16(kLgRows, kLgCols), idesc_l = umma_idesc_tf32(kLgRows, kLgCols);
+            int it = 0, chunk = 0, ls = 0;
+            bool ok = true;
+            while (ok && lg_next(plan, &u, end, &p)) {
+                if (lane == 0) {
+                    for (int c = p.c0; ok && c < p.c1; ++c, ++chunk) {
+                        const uint32_t d = tmem + (chunk & 1) * kLgCols;
+                        ok = chunk < 2 || mbar_wait_bounded(sh.acc_empty + (chunk & 1), (uint32_t)(((chunk - 2) >> 1) & 1));
+                        tc_fence_after();
+                        const int k1 = min(plan.nk, (c + 1) * kLgChunk);
+                        for (int kb = c * kLgChunk; ok && kb < k1; ++kb, ++it) {
+                            const int s = it % kLgStages;
+                            ok = mbar_wait_bounded(sh.full + s, (uint32_t)((it / kLgStages) & 1));
+                            if (!ok) break;
+                            tc_fence_after();
+                            const uint64_t x = sw128_desc(base + s * kLgStage), w = sw128_desc(base + s * kLgStage + 2 * kLgPlane);
+#pragma unroll
+                            for (int kk = 0; kk < 4; ++kk) {
+                                tc_mma(d, x + kk * 2, w + kk * 2, idesc, (kb != c * kLgChunk || kk) ? 1u : 0u);
+                                tc_mma(d, x + (kLgPlane >> 4) + kk * 2, w + kk * 2, idesc, 1u);
+                            }
+                            tc_commit(sh.empty + s);
+                        }
+                        if (ok) tc_commit(sh.acc_full + (chunk & 1));
+                    }
+                }
+                chunk = __shfl_sync(0xffffffffu, chunk, 0);
+                ok = __shfl_sync(0xffffffffu, (int)ok, 0) != 0;
+                if (ok && a.n && p.c0 == 0) {
+                    int ids[4];
+                    lg_ids(a, p.m0, ids);
+                    for (int ad = next_adapter(ids, -1); ok && ad != 0x7fffffff; ad = next_adapter(ids, ad), ++chunk) {
+                        const int steps = (__ldg(a.rank + ad) + 7) / 8;
+                        if (lane == 0) {
+                            const uint32_t d = tmem + (chunk & 1) * kLgCols;
+                            ok = chunk < 2 || mbar_wait_bounded(sh.acc_empty + (chunk & 1), (uint32_t)(((chunk - 2) >> 1) & 1));
+                            for (int s = 0; ok && s < steps; ++s) {
+                                ok = mbar_wait_bounded(&sh.l_full, (uint32_t)((ls + s) & 1));
+                                if (!ok) break;
+                                tc_fence_after();
+                                const uint64_t th = sw32_desc(lora_s), tl = th + (kLgRows * 32 >> 4);
+                                const uint64_t bh = th + (2 * kLgRows * 32 >> 4), bl = bh + (kLgCols * 32 >> 4);
+                                tc_mma_tf32(d, th, bh, idesc_l, s ? 1u : 0u);
+                                tc_mma_tf32(d, th, bl, idesc_l, 1u);
+                                tc_mma_tf32(d, tl, bh, idesc_l, 1u);
+                                tc_commit(&sh.l_empty);
+                            }
+                            if (ok) tc_commit(sh.acc_full + (chunk & 1));
+                        }
+                        ls += steps;
+                        ok = __shfl_sync(0xffffffffu, (int)ok, 0) != 0;
+                    }
+                }
+            }
+            if (lane == 0) {
+                if (!ok) fail();
+                tc_commit(&sh.drained);
+                mbar_wait_bounded(&sh.drained, 0u);
+            }
+            __syncwarp();
+        } else if (a.n) {
+            // ---- adapters: 8 rank indexes of t and B a step, as TF32 hi + lo ------------
+            const int tid = threadIdx.x - 320;   // 0 .. 63
+            int ls = 0;
+            bool ok = true;
+            while (ok && lg_next(plan, &u, end, &p)) {
+                if (p.c0 != 0) continue;
+                int ids[4];
+                lg_ids(a, p.m0, ids);
+                for (int ad = next_adapter(ids, -1); ok && ad != 0x7fffffff; ad = next_adapter(ids, ad)) {
+                    const int rank = __ldg(a.rank + ad);
+                    const void* B = a.B[ad];
+                    const bool vec = rank % 4 == 0;
+                    for (int j0 = 0; j0 < rank; j0 += 8, ++ls) {
+                        float4 v[6][2];
+#pragma unroll
+                        for (int i = 0; i < 6; ++i) {
+                            const int r = i * 64 + tid;   // rows 0-127: t, 128-383: B
+                            const int row = r < kLgRows ? p.m0 + r : p.n0 + r - kLgRows;
+                            const bool in = r < kLgRows ? row < a.M : row < a.N;
+#pragma unroll
+                            for (int h = 0; h < 2; ++h) {
+                                const int j = j0 + 4 * h;
+                                float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
+                                if (in && j < rank) {
+                                    if (r < kLgRows) {
+                                        x = *reinterpret_cast<const float4*>(a.t + (size_t)row * a.max_rank + j);
+                                    } else if (vec) {
+                                        x = a.f16 ? lora_load4<true>(B, (size_t)row * rank + j) : lora_load4<false>(B, (size_t)row * rank + j);
+                                    } else {
+                                        const size_t at = (size_t)row * rank + j;
+                                        x.x = lora_elem(B, at, a.f16);
+                                        if (j + 1 < rank) x.y = lora_elem(B, at + 1, a.f16);
+                                        if (j + 2 < rank) x.z = lora_elem(B, at + 2, a.f16);
+                                        if (j + 3 < rank) x.w = lora_elem(B, at + 3, a.f16);
+                                    }
+                                    if (r < kLgRows) {   // t ends with the rank
+                                        if (j + 1 >= rank) x.y = 0.f;
+                                        if (j + 2 >= rank) x.z = 0.f;
+                                        if (j + 3 >= rank) x.w = 0.f;
+                                    }
+                                }
+                                v[i][h] = x;
+                            }
+                        }
+                        ok = __all_sync(0xffffffffu, (ls == 0 || mbar_wait_bounded(&sh.l_empty, (uint32_t)((ls - 1) & 1))) && !*abort_flag);
+                        if (!ok) break;
+#pragma unroll
+                        for (int i = 0; i < 6; ++i) {
+                            const int r = i * 64 + tid;
+                            unsigned char* hi = smem + kLgStages * kLgStage + (r < kLgRows ? 0 : 2 * kLgRows * 32);
+                            const int rr = r < kLgRows ? r : r - kLgRows, lo = (r < kLgRows ? kLgRows : kLgCols) * 32;
+#pragma unroll
+                            for (int h = 0; h < 2; ++h) {
+                                const float f[4] = {v[i][h].x, v[i][h].y, v[i][h].z, v[i][h].w};
+                                uint32_t x[4], y[4];
+#pragma unroll
+                                for (int e = 0; e < 4; ++e) {
+                                    asm("cvt.rna.tf32.f32 %0, %1;" : "=r"(x[e]) : "f"(f[e]));
+                                    y[e] = __float_as_uint(f[e] - __uint_as_float(x[e]));
+                                }
+                                *reinterpret_cast<uint4*>(hi + sw32_offset(rr, h)) = make_uint4(x[0], x[1], x[2], x[3]);
+                                *reinterpret_cast<uint4*>(hi + lo + sw32_offset(rr, h)) = make_uint4(y[0], y[1], y[2], y[3]);
+                            }
+                        }
+                        fence_proxy_async_smem_cta();
+                        __syncwarp();
+                        if (lane == 0) lg_arrive(&sh.l_full);
+                    }
+                }
+            }
+            if (!ok && lane == 0) fail();
+        }
+    } else {
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 200;");
+        // ---- epilogue: two threads a row, 128 columns each, in registers ------------------
+        const int r = threadIdx.x & 127, half = warp >> 2;
+        const uint32_t lanes = tmem + ((uint32_t)(32 * (warp & 3)) << 16) + half * 128;
+        int chunk = 0;
+        bool ok = true;
+        while (ok && lg_next(plan, &u, end, &p)) {
+            const int m = p.m0 + r;
+            const bool live = m < a.M;
+            const float f = live ? ldexpf(1.0f, __ldg(plan.row_exp + m)) : 0.f;
+            uint64_t acc[64];
+#pragma unroll
+            for (int i = 0; i < 64; ++i) acc[i] = 0ull;
+            auto add = [&](uint64_t f2, bool mine) {
+                ok = __all_sync(0xffffffffu, mbar_wait_bounded(sh.acc_full + (chunk & 1), (uint32_t)((chunk >> 1) & 1)) && !*abort_flag);
+                if (!ok) return;
+                tc_fence_after();
+#pragma unroll
+                for (int c = 0; c < 4; ++c) {
+                    uint32_t v[32];
+                    tmem_ld32(lanes + (chunk & 1) * kLgCols + c * 32, v);
+                    tmem_wait_ld();
+                    if (mine) {
+#pragma unroll
+                        for (int i = 0; i < 16; ++i)
+                            acc[c * 16 + i] = lg_fma2(lg_pack2(__uint_as_float(v[2 * i]), __uint_as_float(v[2 * i + 1])), f2, acc[c * 16 + i]);
+                    }
+                }
+                tc_fence_before();
+                __syncwarp();
+                if (lane == 0) lg_arrive(sh.acc_empty + (chunk & 1));
+                ++chunk;
+            };
+            const uint64_t f2 = lg_pack2(f, f), one = lg_pack2(1.f, 1.f);
+#pragma unroll 1
+            for (int c = p.c0; ok && c < p.c1; ++c) add(f2, true);
+            const int n0 = p.n0 + half * 128;
+            if (a.w8 && ok) {   // INT8: the weight rows' scales
+#pragma unroll
+                for (int i = 0; i < 64; ++i) {
+                    const int n = n0 + 2 * i;
+                    const float s0 = a.row_scales ? (n < a.N ? __ldg(a.row_scales + n) : 0.f) : a.tscale;
+                    const float s1 = a.row_scales ? (n + 1 < a.N ? __ldg(a.row_scales + n + 1) : 0.f) : a.tscale;
+                    acc[i] = lg_fma2(acc[i], lg_pack2(s0, s1), 0ull);
+                }
+            }
+            if (ok && a.n && p.c0 == 0) {
+                int ids[4], rank;
+                lg_ids(a, p.m0, ids);
+                const int id = live ? lora_of(a, m, &rank, false) : -1;
+#pragma unroll 1
+                for (int ad = next_adapter(ids, -1); ok && ad != 0x7fffffff; ad = next_adapter(ids, ad)) add(one, ad == id);
+            }
+            if (!ok) break;
+            if (p.slot >= 0) {
+                float* to = plan.part + ((size_t)(blockIdx.x * 2 + p.slot) * kLgRows + r) * kLgCols + half * 128;
+#pragma unroll
+                for (int i = 0; i < 64; i += 2) {
+                    const float2 x = lg_unpack2(acc[i]), y = lg_unpack2(acc[i + 1]);
+                    *reinterpret_cast<float4*>(to + 2 * i) = make_float4(x.x, x.y, y.x, y.y);
+                }
+            } else if (live) {
+                float* to = a.y + (size_t)m * a.N + n0;
+                if (n0 + 128 <= a.N && a.N % 4 == 0) {
+#pragma unroll
+                    for (int i = 0; i < 64; i += 2) {
+                        const float2 x = lg_unpack2(acc[i]), y = lg_unpack2(acc[i + 1]);
+                        *reinterpret_cast<float4*>(to + 2 * i) = make_float4(x.x, x.y, y.x, y.y);
+                    }
+                } else {
+#pragma unroll
+                    for (int i = 0; i < 64; ++i) {
+                        const float2 x = lg_unpack2(acc[i]);
+                        if (n0 + 2 * i < a.N) to[2 * i] = x.x;
+                        if (n0 + 2 * i + 1 < a.N) to[2 * i + 1] = x.y;
+                    }
+                }
+            }
+        }
+        if (!ok) fail();
+    }
+    tc_fence_before();
+    __syncthreads();
+    if (warp == 9) {
+        tc_fence_after();
+        tmem_dealloc(tmem, 512);
+    }
+}
+
+// Adds the pieces of the tile that CTA blockIdx.x of lora_gemm_kernel began and
+// another ended, in order; 8 rows a CTA here.
+__global__ void __launch_bounds__(256) lora_join_kernel(const __grid_constant__ LoraArgs a, const __grid_constant__ LgPlan plan) {
+    pdl_wait();
+    const int c0 = blockIdx.x;
+    int64_t u = lg_begin(plan, c0);
+    const int64_t end = lg_begin(plan, c0 + 1);
+    LgPiece p;
+    p.slot = -1;
+    const int64_t per = plan.chunks + kLgExtra, start = (end - 1) / per * per;   // the run's last tile
+    if (end <= u || start < u - kLgExtra) return;
+    u = max(u, start);
+    if (!lg_next(plan, &u, end, &p) || p.slot != 1) return;
+    for (int r = blockIdx.y * 8 + (threadIdx.x >> 6); r < (int)blockIdx.y * 8 + 8; r += 4) {
+        const int m = p.m0 + r, col = (threadIdx.x & 63) * 4;
+        if (m >= a.M) return;
+        float4 s = make_float4(0.f, 0.f, 0.f, 0.f);
+        for (int c = c0; c <= p.last_cta; ++c) {
+            const float4 v = *reinterpret_cast<const float4*>(plan.part + ((size_t)(c * 2 + (c == c0)) * kLgRows + r) * kLgCols + col);
+            s = make_float4(s.x + v.x, s.y + v.y, s.z + v.z, s.w + v.w);
+        }
+        const float f[4] = {s.x, s.y, s.z, s.w};
+        float* to = a.y + (size_t)m * a.N + p.n0 + col;
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+            if (p.n0 + col + e < a.N) to[e] = f[e];
+    }
+}
+
+static size_t align256(size_t n) { return (n + 255) & ~(size_t)255; }
+
+tvb_status lora_many_rows(LoraArgs a, cudaStream_t st) {
+    TVB_REQUIRE(a.K <= 16384, "matmul_lora: K=%d with %d rows (at most 16384 above 16 rows)", a.K, a.M);
+    LgPlan plan = {};
+    plan.mt = (a.M + kLgRows - 1) / kLgRows;
+    plan.tiles = plan.mt * ((a.N + kLgCols - 1) / kLgCols);
+    plan.nk = (a.K + 63) / 64;
+    plan.chunks = (plan.nk + kLgChunk - 1) / kLgChunk;
+    // every SM, unless a run would be shorter than what a tile costs by itself
+    plan.ctas = (int)std::max<int64_t>(1, std::min<int64_t>(num_sms(), (int64_t)plan.tiles * (plan.chunks + kLgExtra) / (kLgExtra + 1)));
+    const size_t plane = align256((size_t)a.M * a.K * 2), wide = a.w8 ? align256((size_t)a.N * a.K * 2) : 0;
+    const size_t exps = align256((size_t)a.M * 4), ts = align256((size_t)a.M * a.max_rank * 4);
+    const size_t parts = (size_t)plan.ctas * 2 * kLgRows * kLgCols * 4;
+    Workspace ws(st);
+    TVB_TRY(ws.get(2 * plane + wide + exps + ts + parts));
+    uint16_t *xh = ws.at<uint16_t>(), *xl = ws.at<uint16_t>(plane), *w16 = ws.at<uint16_t>(2 * plane);
+    int* row_exp = ws.at<int>(2 * plane + wide);
+    a.t = ws.at<float>(2 * plane + wide + exps);
+    plan.row_exp = row_exp;
+    plan.part = ws.at<float>(2 * plane + wide + exps + ts);
+    const uint16_t* w = a.w8 ? w16 : static_cast<const uint16_t*>(a.w);
+    if (a.w8) TVB_TRY(pf_i8_to_f16(static_cast<const int8_t*>(a.w), (size_t)a.N * a.K, w16, st));
+    if (a.n) {
+        static int set[2][kMaxDevices];
+        constexpr int smem = kLtWarps * kLtRows * (kLtRanks + 1) * 4;
+        const auto kernel = a.f16 ? lora_shrink_tile_kernel<true> : lora_shrink_tile_kernel<false>;
+        TVB_TRY(allow_smem(reinterpret_cast<const void*>(kernel), smem, set[a.f16]));
+        kernel<<<(unsigned)((a.M + kLtRows - 1) / kLtRows), 32 * kLtWarps, smem, st>>>(a);
+        TVB_TRY(check_launch("lora_shrink_tile_kernel"));
+    }
+    TVB_TRY(pf_norm_split(a.x, nullptr, a.M, a.K, 0.f, xh, xl, row_exp, st));
+    LgMaps maps;
+    const uint64_t xd[2] = {(uint64_t)a.K, (uint64_t)a.M}, wd[2] = {(uint64_t)a.K, (uint64_t)a.N}, stride[1] = {(uint64_t)a.K * 2};
+    const uint32_t xb[2] = {64u, (uint32_t)kLgRows}, wb[2] = {64u, (uint32_t)kLgCols};
+    TVB_TRY(encode_f16_tiled(&maps.xh, xh, 2, xd, stride, xb));
+    TVB_TRY(encode_f16_tiled(&maps.xl, xl, 2, xd, stride, xb));
+    TVB_TRY(encode_f16_tiled(&maps.w, w, 2, wd, stride, wb));
+    static int set[kMaxDevices];
+    TVB_TRY(allow_smem(reinterpret_cast<const void*>(lora_gemm_kernel), kLgSmem, set));
+    lora_gemm_kernel<<<(unsigned)plan.ctas, kLgThreads, kLgSmem, st>>>(maps, a, plan);
+    TVB_TRY(check_launch("lora_gemm_kernel"));
+    TVB_CUDA(launch_maybe_pdl(lora_join_kernel, dim3((unsigned)plan.ctas, kLgRows / 8), dim3(256), 0, st, true, a, plan));
+    return check_launch("lora_join_kernel");
+}
+
+}  // namespace tvb
