@@ -6,8 +6,8 @@
 // pipe at twice the FLOPs of the projection.
 //
 // lora_shrink_tile_kernel: t[m] = scale_a A_a x[m] for 16 rows a CTA.  x and A as
-// three bf16 planes (8 bits each, any magnitude), six products of mma.sync
-// m16n8k16; 16 warps cut K.  Small next to the projection (rank / N of it).
+// TF32 hi + lo planes (any magnitude), three products of mma.sync m16n8k8; 16
+// warps cut K.  Small next to the projection (rank / N of it).
 // lora_gemm_kernel: 128 rows of x by 256 weight rows a tile, tcgen05 fed by TMA.
 // The tensor core truncates as it accumulates (about 2^-26 of the sum an MMA), so
 // four k-blocks (32 MMAs) are summed in TMEM and added to registers by the
@@ -28,21 +28,17 @@ namespace tvb {
 // ---- shrink -----------------------------------------------------------------------
 constexpr int kLtWarps = 16, kLtRows = 16, kLtRanks = 64;
 
-__device__ __forceinline__ void mma_bf16(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+__device__ __forceinline__ void mma_tf32(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
     asm volatile(
-        "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+        "mma.sync.aligned.m16n8k8.row.col.f32.tf32.tf32.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
         : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
         : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
 
-// (x, y) as three packed bf16 planes, each the rounded rest of the one before.
-__device__ __forceinline__ void bf16_planes(float x, float y, uint32_t (&p)[3]) {
-#pragma unroll
-    for (int i = 0; i < 3; ++i) {
-        asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(p[i]) : "f"(y), "f"(x));
-        x -= __uint_as_float(p[i] << 16);
-        y -= __uint_as_float(p[i] & 0xffff0000u);
-    }
+// x = hi + lo, hi rounded to TF32 (11 bits), lo the rest (the product takes its first 11 bits)
+__device__ __forceinline__ void tf32_planes(float x, uint32_t* hi, uint32_t* lo) {
+    asm("cvt.rna.tf32.f32 %0, %1;" : "=r"(*hi) : "f"(x));
+    *lo = __float_as_uint(x - __uint_as_float(*hi));
 }
 
 // The next adapter after `prev` among ids[] (4 a lane, -1 none), or INT_MAX.
@@ -80,37 +76,46 @@ __global__ void __launch_bounds__(32 * kLtWarps, 1) lora_shrink_tile_kernel(cons
         for (int j0 = 0; j0 < rank; j0 += kLtRanks) {
             const int nt = min(kLtRanks / 8, (rank - j0 + 7) / 8);
             float acc[kLtRanks / 8][4] = {};
+            // the loads of a step (16 k) ahead of its arithmetic; k permuted so that a thread's fragments are 4
+            // consecutive k
+            float4 x[2], w[kLtRanks / 8];
+            auto load_x = [&](int s, int h) {
+                const int k = s * 16 + 4 * q, m = m0 + g + 8 * h;
+                return s < s1 && k < a.K && m < a.M ? lora_load4<false>(a.x, (size_t)m * a.K + k) : make_float4(0.f, 0.f, 0.f, 0.f);
+            };
+            auto load_w = [&](int s, int n) {
+                const int k = s * 16 + 4 * q, j = j0 + n * 8 + g;
+                return s < s1 && k < a.K && j < rank ? lora_load4<F16>(A, (size_t)j * a.K + k) : make_float4(0.f, 0.f, 0.f, 0.f);
+            };
+            x[0] = load_x(s0, 0), x[1] = load_x(s0, 1);
+#pragma unroll
+            for (int n = 0; n < kLtRanks / 8; ++n)
+                if (n < nt) w[n] = load_w(s0, n);
 #pragma unroll 1
             for (int s = s0; s < s1; ++s) {
-                // k permuted so that a thread's fragments are 4 consecutive k
-                const int k = s * 16 + 4 * q;
-                const bool in = k < a.K;
-                uint32_t xa[3][4];
+                uint32_t xh[2][4], xl[2][4];   // [8 k][fragment]
 #pragma unroll
                 for (int h = 0; h < 2; ++h) {
-                    const int m = m0 + g + 8 * h;
-                    const float4 x = in && m < a.M ? lora_load4<false>(a.x, (size_t)m * a.K + k) : make_float4(0.f, 0.f, 0.f, 0.f);
-                    uint32_t p[3], r[3];
-                    bf16_planes(x.x, x.y, p);
-                    bf16_planes(x.z, x.w, r);
+                    const float v[4] = {x[h].x, x[h].y, x[h].z, x[h].w};
 #pragma unroll
-                    for (int i = 0; i < 3; ++i) xa[i][h] = p[i], xa[i][2 + h] = r[i];
+                    for (int e = 0; e < 4; ++e) tf32_planes(v[e], &xh[e >> 1][h + 2 * (e & 1)], &xl[e >> 1][h + 2 * (e & 1)]);
+                    x[h] = load_x(s + 1, h);
                 }
 #pragma unroll
                 for (int n = 0; n < kLtRanks / 8; ++n) {
-                    if (n >= nt) break;
-                    const int j = j0 + n * 8 + g;
-                    const float4 w = in && j < rank ? lora_load4<F16>(A, (size_t)j * a.K + k) : make_float4(0.f, 0.f, 0.f, 0.f);
-                    uint32_t p[3], r[3];
-                    bf16_planes(w.x, w.y, p);
-                    bf16_planes(w.z, w.w, r);
-                    // planes i + j <= 2: what is left out is below 2^-24
-                    mma_bf16(acc[n], xa[0], p[2], r[2]);
-                    mma_bf16(acc[n], xa[1], p[1], r[1]);
-                    mma_bf16(acc[n], xa[2], p[0], r[0]);
-                    mma_bf16(acc[n], xa[0], p[1], r[1]);
-                    mma_bf16(acc[n], xa[1], p[0], r[0]);
-                    mma_bf16(acc[n], xa[0], p[0], r[0]);
+                    if (n < nt) {
+                        const float v[4] = {w[n].x, w[n].y, w[n].z, w[n].w};
+                        uint32_t wh[4], wl[4];
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) tf32_planes(v[e], &wh[e], &wl[e]);
+                        w[n] = load_w(s + 1, n);
+#pragma unroll
+                        for (int i = 0; i < 2; ++i) {
+                            mma_tf32(acc[n], xl[i], wh[2 * i], wh[2 * i + 1]);
+                            mma_tf32(acc[n], xh[i], wl[2 * i], wl[2 * i + 1]);
+                            mma_tf32(acc[n], xh[i], wh[2 * i], wh[2 * i + 1]);
+                        }
+                    }
                 }
             }
             float* red = lt_red + warp * kLtRows * (kLtRanks + 1);
@@ -383,57 +388,63 @@ lora_gemm_kernel(const __grid_constant__ LgMaps maps, const __grid_constant__ Lo
                 if (p.c0 != 0) continue;
                 int ids[4];
                 lg_ids(a, p.m0, ids);
-                for (int ad = next_adapter(ids, -1); ok && ad != 0x7fffffff; ad = next_adapter(ids, ad)) {
-                    const int rank = __ldg(a.rank + ad);
-                    const void* B = a.B[ad];
-                    const bool vec = rank % 4 == 0;
-                    for (int j0 = 0; j0 < rank; j0 += 8, ++ls) {
+                // the tile's adapters, 32 at a time: lane i has the i-th's rank and factor
+                for (int ad = -1; ok && ad != 0x7fffffff;) {
+                    int mine = -1, count = 0;
+                    while (count < 32 && (ad = next_adapter(ids, ad)) != 0x7fffffff) {
+                        if (lane == count) mine = ad;
+                        ++count;
+                    }
+                    const int my_rank = mine >= 0 ? __ldg(a.rank + mine) : 0;
+                    const void* my_B = mine >= 0 ? a.B[mine] : nullptr;
+                    for (int c = 0, j0 = 0; c < count; ++ls) {
+                        const int rank = __shfl_sync(0xffffffffu, my_rank, c);
+                        const void* B = reinterpret_cast<const void*>(__shfl_sync(0xffffffffu, reinterpret_cast<uintptr_t>(my_B), c));
+                        // this thread's rows: two of t, four of B, 8 values each; nothing waits for a load before all
+                        // are under way
                         float4 v[6][2];
+                        const bool vec = rank % 4 == 0;
 #pragma unroll
                         for (int i = 0; i < 6; ++i) {
-                            const int r = i * 64 + tid;   // rows 0-127: t, 128-383: B
-                            const int row = r < kLgRows ? p.m0 + r : p.n0 + r - kLgRows;
-                            const bool in = r < kLgRows ? row < a.M : row < a.N;
+                            const int row = i < 2 ? p.m0 + i * 64 + tid : p.n0 + (i - 2) * 64 + tid;
+                            const bool in = i < 2 ? row < a.M : row < a.N;
 #pragma unroll
                             for (int h = 0; h < 2; ++h) {
                                 const int j = j0 + 4 * h;
-                                float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
-                                if (in && j < rank) {
-                                    if (r < kLgRows) {
-                                        x = *reinterpret_cast<const float4*>(a.t + (size_t)row * a.max_rank + j);
-                                    } else if (vec) {
-                                        x = a.f16 ? lora_load4<true>(B, (size_t)row * rank + j) : lora_load4<false>(B, (size_t)row * rank + j);
-                                    } else {
-                                        const size_t at = (size_t)row * rank + j;
-                                        x.x = lora_elem(B, at, a.f16);
-                                        if (j + 1 < rank) x.y = lora_elem(B, at + 1, a.f16);
-                                        if (j + 2 < rank) x.z = lora_elem(B, at + 2, a.f16);
-                                        if (j + 3 < rank) x.w = lora_elem(B, at + 3, a.f16);
-                                    }
-                                    if (r < kLgRows) {   // t ends with the rank
-                                        if (j + 1 >= rank) x.y = 0.f;
-                                        if (j + 2 >= rank) x.z = 0.f;
-                                        if (j + 3 >= rank) x.w = 0.f;
-                                    }
+                                v[i][h] = make_float4(0.f, 0.f, 0.f, 0.f);
+                                if (i < 2) {
+                                    if (in && j < rank) v[i][h] = *reinterpret_cast<const float4*>(a.t + (size_t)row * a.max_rank + j);
+                                } else if (vec) {
+                                    if (in && j < rank)
+                                        v[i][h] = a.f16 ? lora_load4<true>(B, (size_t)row * rank + j) : lora_load4<false>(B, (size_t)row * rank + j);
                                 }
-                                v[i][h] = x;
+                            }
+                        }
+                        if (!vec) {
+#pragma unroll
+                            for (int i = 2; i < 6; ++i) {
+                                const int row = p.n0 + (i - 2) * 64 + tid;
+                                float f[8];
+#pragma unroll
+                                for (int e = 0; e < 8; ++e)
+                                    f[e] = row < a.N && j0 + e < rank ? lora_elem(B, (size_t)row * rank + j0 + e, a.f16) : 0.f;
+                                v[i][0] = make_float4(f[0], f[1], f[2], f[3]);
+                                v[i][1] = make_float4(f[4], f[5], f[6], f[7]);
                             }
                         }
                         ok = __all_sync(0xffffffffu, (ls == 0 || mbar_wait_bounded(&sh.l_empty, (uint32_t)((ls - 1) & 1))) && !*abort_flag);
                         if (!ok) break;
 #pragma unroll
                         for (int i = 0; i < 6; ++i) {
-                            const int r = i * 64 + tid;
-                            unsigned char* hi = smem + kLgStages * kLgStage + (r < kLgRows ? 0 : 2 * kLgRows * 32);
-                            const int rr = r < kLgRows ? r : r - kLgRows, lo = (r < kLgRows ? kLgRows : kLgCols) * 32;
+                            unsigned char* hi = smem + kLgStages * kLgStage + (i < 2 ? 0 : 2 * kLgRows * 32);
+                            const int rr = (i < 2 ? i : i - 2) * 64 + tid, lo = (i < 2 ? kLgRows : kLgCols) * 32;
 #pragma unroll
                             for (int h = 0; h < 2; ++h) {
                                 const float f[4] = {v[i][h].x, v[i][h].y, v[i][h].z, v[i][h].w};
                                 uint32_t x[4], y[4];
 #pragma unroll
-                                for (int e = 0; e < 4; ++e) {
-                                    asm("cvt.rna.tf32.f32 %0, %1;" : "=r"(x[e]) : "f"(f[e]));
-                                    y[e] = __float_as_uint(f[e] - __uint_as_float(x[e]));
+                                for (int e = 0; e < 4; ++e) {   // t ends with the rank
+                                    tf32_planes(i < 2 && j0 + 4 * h + e >= rank ? 0.f : f[e], &x[e], &y[e]);
                                 }
                                 *reinterpret_cast<uint4*>(hi + sw32_offset(rr, h)) = make_uint4(x[0], x[1], x[2], x[3]);
                                 *reinterpret_cast<uint4*>(hi + lo + sw32_offset(rr, h)) = make_uint4(y[0], y[1], y[2], y[3]);
@@ -442,6 +453,8 @@ lora_gemm_kernel(const __grid_constant__ LgMaps maps, const __grid_constant__ Lo
                         fence_proxy_async_smem_cta();
                         __syncwarp();
                         if (lane == 0) lg_arrive(&sh.l_full);
+                        j0 += 8;
+                        if (j0 >= rank) j0 = 0, ++c;
                     }
                 }
             }
