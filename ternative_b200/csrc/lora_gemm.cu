@@ -6,8 +6,8 @@
 // pipe at twice the FLOPs of the projection.
 //
 // lora_shrink_tile_kernel: t[m] = scale_a A_a x[m] for 16 rows a CTA.  x and A as
-// TF32 hi + lo planes (any magnitude), three products of mma.sync m16n8k8; 16
-// warps cut K.  Small next to the projection (rank / N of it).
+// TF32 hi + lo planes (any magnitude), three products of mma.sync m16n8k8; 8
+// warps, and the CTAs of a cluster, cut K.  Small next to the projection (rank / N of it).
 // lora_gemm_kernel: 128 rows of x by 256 weight rows a tile, tcgen05 fed by TMA.
 // The tensor core truncates as it accumulates (about 2^-26 of the sum an MMA), so
 // four k-blocks (32 MMAs) are summed in TMEM and added to registers by the
@@ -18,15 +18,18 @@
 // holds.  Every CTA takes an equal run of the tiles' chunks; a tile that a cut
 // divides leaves F32 partial sums and lora_join_kernel adds them.
 #include <algorithm>
+#include <cooperative_groups.h>
 
 #include "lora.h"
 #include "prefill.h"
 #include "tcgen05.cuh"
 
+namespace cg = cooperative_groups;
+
 namespace tvb {
 
 // ---- shrink -----------------------------------------------------------------------
-constexpr int kLtWarps = 16, kLtRows = 16, kLtRanks = 64;
+constexpr int kLtWarps = 8, kLtRows = 16, kLtRanks = 64;
 
 __device__ __forceinline__ void mma_tf32(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
     asm volatile(
@@ -62,19 +65,23 @@ __device__ __forceinline__ float4 lora_load4(const void* p, size_t at) {
 }
 
 template <bool F16>
-__global__ void __launch_bounds__(32 * kLtWarps, 1) lora_shrink_tile_kernel(const __grid_constant__ LoraArgs a) {
+__global__ void __launch_bounds__(32 * kLtWarps, 2) lora_shrink_tile_kernel(const __grid_constant__ LoraArgs a) {
     extern __shared__ float lt_red[];   // [warp][16 rows][kLtRanks + 1]
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, q = lane & 3;
-    const int m0 = blockIdx.x * kLtRows;
+    cg::cluster_group cl = cg::this_cluster();   // its CTAs cut K
+    const int rank = (int)cl.block_rank(), nsplit = (int)cl.num_blocks();
+    const int m0 = blockIdx.y * kLtRows;
     int ids[4] = {-1, -1, -1, -1}, rank_of = 0;
-    if (lane < kLtRows && m0 + lane < a.M) ids[0] = lora_of(a, m0 + lane, &rank_of, warp == 0);
-    const int steps = ((a.K + 15) / 16 + kLtWarps - 1) / kLtWarps;   // of 16 k, a warp
-    const int s0 = warp * steps, s1 = min(s0 + steps, (a.K + 15) / 16);
+    if (lane < kLtRows && m0 + lane < a.M) ids[0] = lora_of(a, m0 + lane, &rank_of, warp == 0 && rank == 0);
+    if (rank_of == 0) ids[0] = -1;
+    const int parts = kLtWarps * nsplit, part = rank * kLtWarps + warp;
+    const int steps = ((a.K + 15) / 16 + parts - 1) / parts;   // of 16 k, a warp
+    const int s0 = part * steps, s1 = min(s0 + steps, (a.K + 15) / 16);
     for (int ad = next_adapter(ids, -1); ad != 0x7fffffff; ad = next_adapter(ids, ad)) {
-        const int rank = __ldg(a.rank + ad);
+        const int r = __ldg(a.rank + ad);
         const void* A = a.A[ad];
-        for (int j0 = 0; j0 < rank; j0 += kLtRanks) {
-            const int nt = min(kLtRanks / 8, (rank - j0 + 7) / 8);
+        for (int j0 = 0; j0 < r; j0 += kLtRanks) {
+            const int nt = min(kLtRanks / 8, (r - j0 + 7) / 8);
             float acc[kLtRanks / 8][4] = {};
             // the loads of a step (16 k) ahead of its arithmetic; k permuted so that a thread's fragments are 4
             // consecutive k
@@ -85,7 +92,7 @@ __global__ void __launch_bounds__(32 * kLtWarps, 1) lora_shrink_tile_kernel(cons
             };
             auto load_w = [&](int s, int n) {
                 const int k = s * 16 + 4 * q, j = j0 + n * 8 + g;
-                return s < s1 && k < a.K && j < rank ? lora_load4<F16>(A, (size_t)j * a.K + k) : make_float4(0.f, 0.f, 0.f, 0.f);
+                return s < s1 && k < a.K && j < r ? lora_load4<F16>(A, (size_t)j * a.K + k) : make_float4(0.f, 0.f, 0.f, 0.f);
             };
             x[0] = load_x(s0, 0), x[1] = load_x(s0, 1);
 #pragma unroll
@@ -123,17 +130,24 @@ __global__ void __launch_bounds__(32 * kLtWarps, 1) lora_shrink_tile_kernel(cons
             for (int n = 0; n < kLtRanks / 8; ++n)
 #pragma unroll
                 for (int e = 0; e < 4; ++e) red[(g + 8 * (e >> 1)) * (kLtRanks + 1) + n * 8 + 2 * q + (e & 1)] = acc[n][e];
-            __syncthreads();
+            if (nsplit > 1) cl.sync();
+            else __syncthreads();
+            // the cluster's CTAs share the rows; sums in the order of K
             const float scale = __ldg(a.scale + ad);
-            for (int i = threadIdx.x; i < kLtRows * kLtRanks; i += 32 * kLtWarps) {
+            for (int i = rank * 32 * kLtWarps + threadIdx.x; i < kLtRows * kLtRanks; i += nsplit * 32 * kLtWarps) {
                 const int m = i / kLtRanks, j = i % kLtRanks;
-                const bool mine = m0 + m < a.M && __ldg(a.adapter + m0 + m) == ad && j0 + j < rank;
+                const bool mine = m0 + m < a.M && __ldg(a.adapter + m0 + m) == ad && j0 + j < r;
+                if (!mine) continue;
                 float s = 0.f;
+                for (int p = 0; p < nsplit; ++p) {
+                    const float* from = cl.map_shared_rank(lt_red, p);
 #pragma unroll
-                for (int w = 0; w < kLtWarps; ++w) s += lt_red[(w * kLtRows + m) * (kLtRanks + 1) + j];
-                if (mine) a.t[(size_t)(m0 + m) * a.max_rank + j0 + j] = s * scale;
+                    for (int w = 0; w < kLtWarps; ++w) s += from[(w * kLtRows + m) * (kLtRanks + 1) + j];
+                }
+                a.t[(size_t)(m0 + m) * a.max_rank + j0 + j] = s * scale;
             }
-            __syncthreads();
+            if (nsplit > 1) cl.sync();
+            else __syncthreads();
         }
     }
 }
@@ -607,7 +621,21 @@ tvb_status lora_many_rows(LoraArgs a, cudaStream_t st) {
         constexpr int smem = kLtWarps * kLtRows * (kLtRanks + 1) * 4;
         const auto kernel = a.f16 ? lora_shrink_tile_kernel<true> : lora_shrink_tile_kernel<false>;
         TVB_TRY(allow_smem(reinterpret_cast<const void*>(kernel), smem, set[a.f16]));
-        kernel<<<(unsigned)((a.M + kLtRows - 1) / kLtRows), 32 * kLtWarps, smem, st>>>(a);
+        const int rows = (a.M + kLtRows - 1) / kLtRows;
+        int nsplit = 1;   // CTAs that cut K: while two an SM hold them all
+        while (nsplit < 8 && rows * nsplit * 2 <= 2 * num_sms()) nsplit *= 2;
+        cudaLaunchConfig_t cfg = {};
+        cfg.gridDim = dim3((unsigned)nsplit, (unsigned)rows);
+        cfg.blockDim = dim3(32 * kLtWarps);
+        cfg.dynamicSmemBytes = smem;
+        cfg.stream = st;
+        cudaLaunchAttribute attr[1];
+        attr[0].id = cudaLaunchAttributeClusterDimension;
+        attr[0].val.clusterDim.x = (unsigned)nsplit;
+        attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+        cfg.attrs = attr;
+        cfg.numAttrs = 1;
+        TVB_CUDA(cudaLaunchKernelEx(&cfg, kernel, a));
         TVB_TRY(check_launch("lora_shrink_tile_kernel"));
     }
     TVB_TRY(pf_norm_split(a.x, nullptr, a.M, a.K, 0.f, xh, xl, row_exp, st));
