@@ -172,11 +172,10 @@ _SIGS = {
     "tvb_gguf_read": [_P, C.c_char_p, _P, C.c_uint64],
     "tvb_gguf_close": [_P],
     "tvb_decode_batch": [_P, _P, _P, _I, _P, _P],
-    "tvb_rope_append_paged": [_P, _I, _P, _I, _P, _I, _P, _I, C.POINTER(KvPages), C.POINTER(PagedBatchDesc),
-                              C.POINTER(RopeDesc), _I, _I, _I, _P, _P],
-    "tvb_attention_paged": [_P, _I, _P, _P, _I, C.POINTER(KvPages), C.POINTER(PagedBatchDesc), _I, _I, _I, _F, _I,
-                            _P, _P],
-    "tvb_matmul_lora": [_P, _P, _I, _I, C.POINTER(Weight), _I, C.POINTER(LoraTableDesc), _P, _P, _P],
+    # descriptors by address: KvPages, PagedBatchDesc, RopeDesc, LoraTableDesc
+    "tvb_rope_append_paged": [_P, _I, _P, _I, _P, _I, _P, _I, _P, _P, _P, _I, _I, _I, _P, _P],
+    "tvb_attention_paged": [_P, _I, _P, _P, _I, _P, _P, _I, _I, _I, _F, _I, _P, _P],
+    "tvb_matmul_lora": [_P, _P, _I, _I, C.POINTER(Weight), _I, _P, _P, _P, _P],
     "tvb_tp_init": [_P, _I, _I, C.POINTER(C.c_void_p)],
     "tvb_tp_set_peers": [_P, C.POINTER(C.c_void_p)],
     "tvb_ipc_export": [_P, C.POINTER(IpcHandle)],

@@ -88,15 +88,27 @@ def _tensor(x, name: str, dtype: str, ndim: int):
     return x
 
 
-def _heads(x, name: str, rows: int, heads: int, head_dim: int) -> int:
-    """Leading dimension of a token buffer: [rows][>= heads * head_dim] or
-    [rows][heads][head_dim], rows any distance apart."""
-    _tensor(x, name, "float32", x.dim() if x.dim() in (2, 3) else 2)
-    if x.dim() == 3 and (tuple(x.shape[1:]) != (heads, head_dim) or (heads > 1 and x.stride(1) != head_dim)):
-        raise ValueError(f"{name}: shape {tuple(x.shape)}, strides {x.stride()} for {heads} heads of {head_dim}")
-    if x.shape[0] < rows or (x.dim() == 2 and x.shape[1] < heads * head_dim):
-        raise ValueError(f"{name}: shape {tuple(x.shape)} for {rows} rows of {heads} heads of {head_dim}")
-    return x.stride(0) if x.shape[0] > 1 else heads * head_dim
+def _rows(x, name: str, rows: int, heads: int, head_dim: int, torch, device: int) -> int:
+    """Leading dimension of a float32 token buffer on the current device:
+    [rows][>= heads * head_dim] or [rows][heads][head_dim], rows any distance
+    apart.  (On the path of every decode step: one read of each property.)"""
+    shape, stride = x.shape, x.stride()
+    if x.dtype is torch.float32 and x.get_device() == device and shape[0] >= rows:
+        if len(shape) == 3:
+            if shape[1] == heads and shape[2] == head_dim and stride[2] == 1 and (stride[1] == head_dim or heads == 1):
+                return stride[0] if shape[0] > 1 else heads * head_dim
+        elif len(shape) == 2 and shape[1] >= heads * head_dim and stride[1] == 1:
+            return stride[0] if shape[0] > 1 else heads * head_dim
+    raise ValueError(f"{name}: {x.dtype} on {x.device}, shape {tuple(shape)}, strides {stride}; want float32 on the current "
+                     f"CUDA device, {rows} rows of {heads} heads of {head_dim}")
+
+
+def _flat(x, name: str, dtype, n: int, device: int) -> int:
+    """Address of n contiguous values of a type on the current device."""
+    if x.dtype is not dtype or x.get_device() != device or x.numel() < n or not x.is_contiguous():
+        raise ValueError(f"{name}: {x.dtype} on {x.device}, shape {tuple(x.shape)}; want {n} contiguous {dtype} values on the "
+                         f"current CUDA device")
+    return x.data_ptr()
 
 
 class PagedCache:
@@ -117,6 +129,7 @@ class PagedCache:
         ps, rs, hs, _ = k.stride()
         self.desc = KvPages(k.data_ptr(), v.data_ptr(), TVB_F32 if k.dtype == torch.float32 else TVB_F16, n_pages,
                             page_size, ps, rs, hs)
+        self.address = C.addressof(self.desc)
 
 
 class PagedBatch:
@@ -135,6 +148,7 @@ class PagedBatch:
         self.n_tokens = n_tokens
         self.desc = PagedBatchDesc(n, n_tokens, max_new, max_kv, cu_tokens.data_ptr(), kv_len.data_ptr(),
                                    block_table.data_ptr(), block_table.stride(0) if n > 1 else block_table.shape[1])
+        self.address = C.addressof(self.desc)
 
 
 class RopeConfig:
@@ -149,6 +163,7 @@ class RopeConfig:
             raise ValueError(f"pairs {pairs!r} (of {kinds}), scaling {scaling!r} (of {scalings})")
         self.desc = RopeDesc(rot_dim, kinds.index(pairs), scalings.index(scaling), theta, factor, original_len,
                              low_turns, high_turns, fast_turns, slow_turns)
+        self.address = C.addressof(self.desc)
 
 
 class LoraTable:
@@ -181,6 +196,7 @@ class LoraTable:
         self.tensors = (list(A), list(B), rank, scale, ptrs)   # kept alive with the descriptor
         self.desc = LoraTableDesc(len(A), max_rank, TVB_F32 if dtype == torch.float32 else TVB_F16,
                                   ptrs[0].data_ptr(), ptrs[1].data_ptr(), rank.data_ptr(), scale.data_ptr())
+        self.address = C.addressof(self.desc)
 
 
 class CUDABackend:
@@ -322,42 +338,47 @@ class CUDABackend:
         """Rotary positions of the new tokens and their append to the cache
         (tvb_rope_append_paged).  Token buffers are float32 tensors [rows][heads *
         head_dim] or [rows][heads][head_dim]; rows may be a slice of a wider buffer."""
-        if (cache.n_kv_heads, cache.head_dim) != (n_kv_heads, head_dim):
+        import torch
+        if cache.n_kv_heads != n_kv_heads or cache.head_dim != head_dim:
             raise ValueError(f"a cache of {cache.n_kv_heads} heads of {cache.head_dim}")
-        T = batch.n_tokens
-        ld = [_heads(x, name, T, h, head_dim) for x, name, h in
-              ((d_q_out, "q_out", n_heads), (d_q, "q", n_heads), (d_k, "k", n_kv_heads), (d_v, "v", n_kv_heads))]
-        call("tvb_rope_append_paged", d_q_out.data_ptr(), ld[0], d_q.data_ptr(), ld[1], d_k.data_ptr(), ld[2],
-             d_v.data_ptr(), ld[3], cache.desc, batch.desc, rope.desc, n_heads, n_kv_heads, head_dim, _ptr(status),
-             self.stream if stream is None else stream)
+        T, dev = batch.n_tokens, torch.cuda.current_device()
+        _lib.check(self.lib.tvb_rope_append_paged(
+            d_q_out.data_ptr(), _rows(d_q_out, "q_out", T, n_heads, head_dim, torch, dev),
+            d_q.data_ptr(), _rows(d_q, "q", T, n_heads, head_dim, torch, dev),
+            d_k.data_ptr(), _rows(d_k, "k", T, n_kv_heads, head_dim, torch, dev),
+            d_v.data_ptr(), _rows(d_v, "v", T, n_kv_heads, head_dim, torch, dev),
+            cache.address, batch.address, rope.address, n_heads, n_kv_heads, head_dim, _ptr(status),
+            self.stream if stream is None else stream), "tvb_rope_append_paged")
 
     def attention_paged_d(self, d_out, d_q, cache: PagedCache, batch: PagedBatch, n_heads, n_kv_heads, head_dim, scale,
                           window=0, lse=None, status=None, stream=None):
         """Causal attention of the new tokens over the cache (tvb_attention_paged),
         window keys back at most when window > 0; lse: float32 [rows][n_heads]."""
-        if (cache.n_kv_heads, cache.head_dim) != (n_kv_heads, head_dim):
+        import torch
+        if cache.n_kv_heads != n_kv_heads or cache.head_dim != head_dim:
             raise ValueError(f"a cache of {cache.n_kv_heads} heads of {cache.head_dim}")
-        T = batch.n_tokens
-        ldo, ldq = _heads(d_out, "out", T, n_heads, head_dim), _heads(d_q, "q", T, n_heads, head_dim)
-        if lse is not None:
-            _tensor(lse, "lse", "float32", 2)
-            if lse.shape[0] < T or lse.shape[1] != n_heads or not lse.is_contiguous():
-                raise ValueError(f"lse: shape {tuple(lse.shape)} for {T} rows of {n_heads} heads")
-        call("tvb_attention_paged", d_out.data_ptr(), ldo, _ptr(lse), d_q.data_ptr(), ldq, cache.desc, batch.desc,
-             n_heads, n_kv_heads, head_dim, scale, window, _ptr(status), self.stream if stream is None else stream)
+        T, dev = batch.n_tokens, torch.cuda.current_device()
+        if lse is not None and lse.shape[-1] != n_heads:
+            raise ValueError(f"lse: shape {tuple(lse.shape)} for {n_heads} heads")
+        _lib.check(self.lib.tvb_attention_paged(
+            d_out.data_ptr(), _rows(d_out, "out", T, n_heads, head_dim, torch, dev),
+            None if lse is None else _flat(lse, "lse", torch.float32, T * n_heads, dev),
+            d_q.data_ptr(), _rows(d_q, "q", T, n_heads, head_dim, torch, dev),
+            cache.address, batch.address, n_heads, n_kv_heads, head_dim, scale, window, _ptr(status),
+            self.stream if stream is None else stream), "tvb_attention_paged")
 
     def matmul_lora_d(self, d_y, d_x, M, K, weight: DeviceWeight, N, table: LoraTable, d_adapter, status=None,
                       stream=None):
         """y[m] = W x[m] + scale_a B_a A_a x[m], a = adapter[m] (int32, -1: none)
         (tvb_matmul_lora)."""
-        for x, name, dtype, n in ((d_y, "y", "float32", M * N), (d_x, "x", "float32", M * K), (d_adapter, "adapter", "int32", M)):
-            _tensor(x, name, dtype, x.dim())
-            if x.numel() < n or not x.is_contiguous():
-                raise ValueError(f"{name}: want {n} contiguous values, got shape {tuple(x.shape)}")
-        if table.K is not None and (table.K, table.N) != (K, N):
+        import torch
+        dev = torch.cuda.current_device()
+        if table.K is not None and (table.K != K or table.N != N):
             raise ValueError(f"adapters of a projection {table.K} -> {table.N}, not {K} -> {N}")
-        call("tvb_matmul_lora", d_y.data_ptr(), d_x.data_ptr(), M, K, C.byref(weight.to_c()), N, table.desc,
-             d_adapter.data_ptr(), _ptr(status), self.stream if stream is None else stream)
+        _lib.check(self.lib.tvb_matmul_lora(
+            _flat(d_y, "y", torch.float32, M * N, dev), _flat(d_x, "x", torch.float32, M * K, dev), M, K,
+            C.byref(weight.to_c()), N, table.address, _flat(d_adapter, "adapter", torch.int32, M, dev), _ptr(status),
+            self.stream if stream is None else stream), "tvb_matmul_lora")
 
     # ---- load-time merge (replaces apply_lora, src/model.cpp:205-258) ----------
     def apply_lora_i2s(self, i2s, scale, K, N, lora_a, lora_b, alpha, out_dtype, dst,

@@ -7,7 +7,7 @@
 // 2^(m_old - m_new) when it grows.
 //
 // paged_rows_kernel: a CTA takes its run of tiles (attn_schedule: RB query rows of
-// one KV head of one sequence against 64 keys a tile); per piece its 8 warps take
+// one KV head of one sequence against 8 keys a warp and tile); per piece its warps take
 // batches of 8 keys in turn and merge at the end.  K and V rows pass
 // through a ring of cp.async stages private to each warp, so no warp waits for
 // another while it streams; each lane owns head_dim / 32 dimensions.  The RB x 8
@@ -19,9 +19,7 @@
 
 namespace tvb {
 
-constexpr int kPrWarps = 8, kPrThreads = 32 * kPrWarps;
 constexpr int kPrKeys = 8;   // keys a batch
-constexpr int kPrTile = kPrKeys * kPrWarps;   // keys a tile
 constexpr int kPrExtra = 1;   // what starting and leaving a block costs, in tiles
 constexpr int kTensorRows = 32;   // rows of a KV head from which F16 caches take the tensor cores
 
@@ -39,8 +37,11 @@ template <typename T, int HD>
 struct PrStage {
     static constexpr int kRow = HD * (int)sizeof(T);     // bytes of a key
     static constexpr int kBytes = 2 * kPrKeys * kRow;    // K rows, then V rows
-    static constexpr int kStages = sizeof(T) == 2 ? 4 : 3;
-    static constexpr int kSmem = kPrWarps * kStages * kBytes;
+    // as many warps as leave each a few stages of its own in shared memory: the loads in flight hide the latency
+    static constexpr int kWarps = sizeof(T) == 2 ? 16 : 12, kThreads = 32 * kWarps;
+    static constexpr int kStages = 2;
+    static constexpr int kTile = kPrKeys * kWarps;       // keys a tile
+    static constexpr int kSmem = kWarps * kStages * kBytes;
 };
 
 // Sum over the lanes of v[0 .. NV): lane l returns the sum of v[l / (32 / NV)].
@@ -67,7 +68,34 @@ __device__ __forceinline__ float pr_reduce(float (&v)[NV], int lane) {
 
 template <typename T, int HD, int RB>
 __host__ __device__ constexpr int rows_smem() {
-    return PrStage<T, HD>::kSmem > kPrWarps * RB * (HD + 2) * 4 ? PrStage<T, HD>::kSmem : kPrWarps * RB * (HD + 2) * 4;
+    using St = PrStage<T, HD>;
+    return St::kSmem > St::kWarps * RB * (HD + 2) * 4 ? St::kSmem : St::kWarps * RB * (HD + 2) * 4;
+}
+
+// Joins the warps' sums of a piece: [warp][row][HD + 2], maximum and sum last.
+template <int HD, int RB, int WARPS>
+__device__ __forceinline__ void merge_warps(const PagedAttnArgs& a, const AttnPiece& pc, const float* red) {
+    constexpr int ND = HD / 32, kW = HD + 2;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    for (int r = warp; r < pc.rows; r += WARPS) {
+        float M = -INFINITY;
+#pragma unroll
+        for (int w = 0; w < WARPS; ++w) M = fmaxf(M, red[(w * RB + r) * kW + HD]);
+        float L = 0.f, o[ND];
+#pragma unroll
+        for (int d = 0; d < ND; ++d) o[d] = 0.f;
+#pragma unroll
+        for (int w = 0; w < WARPS; ++w) {
+            const float* x = red + (w * RB + r) * kW;
+            const float c = x[HD] == -INFINITY ? 0.f : exp2f(x[HD] - M);
+            if (c != 0.f) {
+                L = fmaf(x[HD + 1], c, L);
+#pragma unroll
+                for (int d = 0; d < ND; ++d) o[d] = fmaf(x[lane * ND + d], c, o[d]);
+            }
+        }
+        attn_row_store<RB, HD, ND>(a, pc, r, L, M, o);
+    }
 }
 
 // One piece; whole CTA.
@@ -135,8 +163,8 @@ __device__ __forceinline__ void rows_piece(const PagedAttnArgs& a, const AttnPie
         return have;
     };
 
-    // batches warp, warp + 8, ... of the keys from k0 on
-    const int step = kPrWarps * kPrKeys;
+    // batches warp, warp + kWarps, ... of the keys from k0 on
+    const int step = St::kTile;
     int t = k0 + warp * kPrKeys, tn = t;
     unsigned have = 0u;
     for (int i = 0; i < St::kStages - 1; ++i, tn += step) {
@@ -238,45 +266,307 @@ __device__ __forceinline__ void rows_piece(const PagedAttnArgs& a, const AttnPie
 #pragma unroll
         for (int d = 0; d < ND; ++d) red[(warp * RB + r) * kW + lane * ND + d] = acc[r][d];
     __syncthreads();
-    for (int r = warp; r < rows; r += kPrWarps) {
-        float M = -INFINITY;
-#pragma unroll
-        for (int w = 0; w < kPrWarps; ++w) M = fmaxf(M, red[(w * RB + r) * kW + HD]);
-        float L = 0.f, o[ND];
-#pragma unroll
-        for (int d = 0; d < ND; ++d) o[d] = 0.f;
-#pragma unroll
-        for (int w = 0; w < kPrWarps; ++w) {
-            const float* x = red + (w * RB + r) * kW;
-            const float c = x[HD] == -INFINITY ? 0.f : exp2f(x[HD] - M);
-            if (c != 0.f) {
-                L = fmaf(x[HD + 1], c, L);
-#pragma unroll
-                for (int d = 0; d < ND; ++d) o[d] = fmaf(x[lane * ND + d], c, o[d]);
-            }
-        }
-        attn_row_store<RB, HD, ND>(a, pc, r, L, M, o);
-    }
+    merge_warps<HD, RB, St::kWarps>(a, pc, red);
 }
 
-template <typename T, int HD, int RB>
-__global__ void __launch_bounds__(kPrThreads) paged_rows_kernel(const __grid_constant__ PagedAttnArgs a) {
-    extern __shared__ __align__(128) unsigned char pr_smem_raw[];
-    __shared__ AttnRun run;
-    __shared__ AttnPiece pieces[kPrWarps];
-    if (!a.balanced) {
-        AttnPiece p;
-        if (attn_block<RB, kPrTile, kPrThreads>(a, 1, &p)) rows_piece<T, HD, RB>(a, p, pr_smem_raw);
+// ---- three to sixteen rows over an F16 cache: mma.sync ------------------------------
+// The rows are the 16-row operand of mma.sync m16n8k16 (a memory-bound product: the
+// legacy tensor path keeps up with memory where the FP32 pipe does not, 55 against
+// 52 us for 32 sequences).  q and p are split into F16 hi + lo planes, K and V rows
+// come from shared memory by ldmatrix.  Every 16 keys make a fresh product that is
+// added to F32 registers, so the tensor core's truncation does not add up.
+template <int HD, int RB>
+struct PmStage {
+    static constexpr int kKeys = 16, kRow = HD * 2;
+    static constexpr int kBytes = 2 * kKeys * kRow;   // K rows, then V rows, 16-byte chunk c of a row at c ^ (row % 8)
+    static constexpr int kWarps = RB == 16 ? 8 : 12, kThreads = 32 * kWarps;   // (registers of 16 rows' queries)
+    static constexpr int kStages = RB == 16 ? 3 : 2;
+    static constexpr int kTile = kKeys * kWarps;
+    static constexpr int kRing = kWarps * kStages * kBytes, kRed = kWarps * RB * (HD + 2) * 4;
+    static constexpr int kSmem = kRing > kRed ? kRing : kRed;
+};
+
+__device__ __forceinline__ void ldsm4(uint32_t (&r)[4], uint32_t addr) {
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0, %1, %2, %3}, [%4];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+                 : "r"(addr));
+}
+__device__ __forceinline__ void ldsm4_trans(uint32_t (&r)[4], uint32_t addr) {
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0, %1, %2, %3}, [%4];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+                 : "r"(addr));
+}
+__device__ __forceinline__ void pm_mma(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+    asm volatile(
+        "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+        : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ void pm_split(float x, float y, uint32_t* hi, uint32_t* lo) {
+    const __half2 h = __floats2half2_rn(x, y);
+    const float2 f = __half22float2(h);
+    const __half2 l = __floats2half2_rn(x - f.x, y - f.y);
+    *hi = *reinterpret_cast<const uint32_t*>(&h);
+    *lo = *reinterpret_cast<const uint32_t*>(&l);
+}
+
+// One piece; whole CTA.  `odd` (shared): a value that some row does not see is not finite.
+template <int HD, int RB>
+__device__ __forceinline__ void mma_piece(const PagedAttnArgs& a, const AttnPiece& pc, unsigned char* smem, int* odd) {
+    using St = PmStage<HD, RB>;
+    constexpr int kHalves = RB / 8;   // 8 rows each
+    constexpr int kSteps = HD / 16;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, q = lane & 3;
+    const int rows = pc.rows, kvh = pc.kvh, k0 = max(pc.k0, pc.first), k1 = pc.k1;
+    const int p_first = pc.pos0 + (int)a.gdiv.div((uint32_t)pc.row);
+    const int p_last = pc.pos0 + (int)a.gdiv.div((uint32_t)(pc.row + rows - 1));
+    if (threadIdx.x == 0) *odd = 0;
+    __syncthreads();
+
+    unsigned char* ring = smem + warp * St::kStages * St::kBytes;
+    const unsigned char* kb = a.kv.k + (int64_t)kvh * a.kv.head_stride;
+    const unsigned char* vb = a.kv.v + (int64_t)kvh * a.kv.head_stride;
+    const int* table = a.s.table + (size_t)pc.b * a.s.table_ld;
+    bool bad = false;
+    auto request = [&](int t, int st) -> unsigned {
+        int64_t off = -1;
+        if (lane < St::kKeys && t + lane >= k0 && t + lane < k1) {
+            off = paged_offset(a.kv, table, t + lane);
+            bad |= off < 0;
+        }
+        const unsigned have = __ballot_sync(0xffffffffu, off >= 0) & 0xffffu;
+        constexpr int kLanes = St::kRow / 16, kRows = 32 / kLanes;   // lanes a row, rows a pass
+        const uint32_t dst = pr_smem(ring + st * St::kBytes);
+        const int c = lane % kLanes;
+#pragma unroll
+        for (int j = 0; j < St::kKeys / kRows; ++j) {
+            const int key = j * kRows + lane / kLanes;
+            const int64_t o = __shfl_sync(0xffffffffu, off, key);
+            const int64_t at = (o >= 0 ? o : 0) + c * 16;
+            const uint32_t to = dst + key * St::kRow + ((c ^ (key & 7)) * 16);
+            cp_async16(to, kb + at, o >= 0);
+            cp_async16(to + St::kKeys * St::kRow, vb + at, o >= 0);
+        }
+        return have;
+    };
+    const int step = St::kTile;
+    int t = k0 + warp * St::kKeys, tn = t;
+    uint64_t have = 0;   // keys of the stages in order, 16 bits each
+#pragma unroll
+    for (int i = 0; i < St::kStages - 1; ++i, tn += step) {
+        have |= (uint64_t)(tn < k1 ? request(tn, i) : 0u) << (16 * i);
+        cp_async_commit();
+    }
+
+    // queries of rows g (and g + 8) as operand fragments, scale log2 e and a power of two a row taken out
+    uint32_t qh[kSteps][2 * kHalves], ql[kSteps][2 * kHalves];
+    float f[2] = {1.f, 1.f}, m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
+    int pos[2] = {-1, -1};
+#pragma unroll
+    for (int h = 0; h < kHalves; ++h) {
+        const int r = g + 8 * h, row = pc.row + min(r, rows - 1), n = (int)a.gdiv.div((uint32_t)row);
+        if (r < rows) pos[h] = pc.pos0 + n;
+        const float* src = a.q + (size_t)(pc.tok0 + n) * a.ldq + (kvh * a.group + row - n * a.group) * HD + 2 * q;
+        float2 x[kSteps][2];
+        float mx = 0.f;
+#pragma unroll
+        for (int s = 0; s < kSteps; ++s)
+#pragma unroll
+            for (int p = 0; p < 2; ++p) {
+                float2 v = __ldg(reinterpret_cast<const float2*>(src + 16 * s + 8 * p));
+                v.x *= a.scale2, v.y *= a.scale2;
+                x[s][p] = v;
+                mx = fmaxf(mx, fmaxf(fabsf(v.x), fabsf(v.y)));
+            }
+        mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
+        mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
+        int e = 0;
+        if (mx > 0.f && mx < INFINITY) e = max(-100, min(100, (int)((__float_as_uint(mx) >> 23) & 255) - 127 - 13));
+        f[h] = __uint_as_float((uint32_t)(127 + e) << 23);
+        const float inv = __uint_as_float((uint32_t)(127 - e) << 23);
+#pragma unroll
+        for (int s = 0; s < kSteps; ++s)
+#pragma unroll
+            for (int p = 0; p < 2; ++p)
+                pm_split(x[s][p].x * inv, x[s][p].y * inv, &qh[s][p * kHalves + h], &ql[s][p * kHalves + h]);
+    }
+    float o[HD / 8][2 * kHalves];
+#pragma unroll
+    for (int n = 0; n < HD / 8; ++n)
+#pragma unroll
+        for (int e = 0; e < 2 * kHalves; ++e) o[n][e] = 0.f;
+
+    const int mi = lane >> 3, r8 = lane & 7;
+    int st = 0;
+#pragma unroll 1
+    while (t < k1) {
+        const int ns = st == 0 ? St::kStages - 1 : st - 1;
+        __syncwarp();   // every lane is done with the stage that is filled now
+        have |= (uint64_t)(tn < k1 ? request(tn, ns) : 0u) << (16 * (St::kStages - 1));
+        cp_async_commit();
+        tn += step;
+        cp_async_wait<St::kStages - 1>();
+        __syncwarp();
+        const uint32_t stage = pr_smem(ring + st * St::kBytes), vstage = stage + St::kKeys * St::kRow;
+        const unsigned hv = (unsigned)have & 0xffffu;
+        have >>= 16;
+        const unsigned char* vrows = ring + st * St::kBytes + St::kKeys * St::kRow;
+        st = st == St::kStages - 1 ? 0 : st + 1;
+
+        float s[2][4] = {};   // 8 keys each
+#pragma unroll
+        for (int kk = 0; kk < kSteps; ++kk) {
+            uint32_t k[4];
+            const int row = (mi >> 1) * 8 + r8, c = kk * 2 + (mi & 1);
+            ldsm4(k, stage + row * St::kRow + ((c ^ (row & 7)) * 16));
+            const uint32_t h0 = qh[kk][0], h1 = kHalves == 2 ? qh[kk][1] : 0u, h2 = qh[kk][kHalves], h3 = kHalves == 2 ? qh[kk][3 & (2 * kHalves - 1)] : 0u;
+            const uint32_t l0 = ql[kk][0], l1 = kHalves == 2 ? ql[kk][1] : 0u, l2 = ql[kk][kHalves], l3 = kHalves == 2 ? ql[kk][3 & (2 * kHalves - 1)] : 0u;
+            pm_mma(s[0], l0, l1, l2, l3, k[0], k[1]);
+            pm_mma(s[1], l0, l1, l2, l3, k[2], k[3]);
+            pm_mma(s[0], h0, h1, h2, h3, k[0], k[1]);
+            pm_mma(s[1], h0, h1, h2, h3, k[2], k[3]);
+        }
+        const bool whole = hv == 0xffffu && t + St::kKeys - 1 <= p_first && (!a.window || t > p_last - a.window);
+        uint32_t ph[2][2] = {}, pl[2][2] = {};   // [8 keys][rows g, g + 8]
+        float corr[2] = {1.f, 1.f};
+#pragma unroll
+        for (int h = 0; h < kHalves; ++h) {
+            float v[4] = {s[0][2 * h] * f[h], s[0][2 * h + 1] * f[h], s[1][2 * h] * f[h], s[1][2 * h + 1] * f[h]};
+            if (!whole) {
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const int k = (i >> 1) * 8 + 2 * q + (i & 1), kt = t + k;
+                    if (!((hv >> k) & 1u) || kt > pos[h] || (a.window && kt <= pos[h] - a.window)) v[i] = -INFINITY;
+                }
+            }
+            float mx = fmaxf(fmaxf(v[0], v[1]), fmaxf(v[2], v[3]));
+            mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
+            mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
+            const float mn = fmaxf(m[h], mx);
+            corr[h] = m[h] == mn ? 1.f : exp2f(m[h] - mn);
+            m[h] = mn;
+            const float ref = mn == -INFINITY ? 0.f : mn;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) v[i] = exp2f(v[i] - ref);
+            l[h] = l[h] * corr[h] + ((v[0] + v[1]) + (v[2] + v[3]));
+            pm_split(v[0], v[1], &ph[0][h], &pl[0][h]);
+            pm_split(v[2], v[3], &ph[1][h], &pl[1][h]);
+        }
+        if (!whole) {   // zero times a value that is not finite: leave the piece to the rows' own pace
+            uint32_t nonfinite = 0;
+            for (int i = lane; i < St::kKeys * St::kRow / 4; i += 32) {
+                const uint32_t v = reinterpret_cast<const uint32_t*>(vrows)[i];
+                nonfinite |= (uint32_t)((v & 0x7C00u) == 0x7C00u) | (uint32_t)((v & 0x7C000000u) == 0x7C000000u);
+            }
+            if (nonfinite) *reinterpret_cast<volatile int*>(odd) = 1;
+        }
+#pragma unroll
+        for (int n = 0; n < HD / 16; ++n) {
+            uint32_t v[4];
+            const int row = (mi & 1) * 8 + r8, c = n * 2 + (mi >> 1);
+            ldsm4_trans(v, vstage + row * St::kRow + ((c ^ (row & 7)) * 16));
+            float d[2][4] = {};
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+                pm_mma(d[i], pl[0][0], pl[0][1], pl[1][0], pl[1][1], v[2 * i], v[2 * i + 1]);
+                pm_mma(d[i], ph[0][0], ph[0][1], ph[1][0], ph[1][1], v[2 * i], v[2 * i + 1]);
+#pragma unroll
+                for (int e = 0; e < 2 * kHalves; ++e) o[2 * n + i][e] = fmaf(o[2 * n + i][e], corr[e >> 1], d[i][e]);
+            }
+        }
+        t += step;
+    }
+    cp_async_wait<0>();
+    if (bad) report_bad(a.status);
+    __syncthreads();
+    if (*odd) {
+        for (int r = warp; r < rows; r += St::kWarps) attn_row_slow<__half, RB, HD>(a, pc, r);
         return;
     }
-    AttnSchedule& sched = *reinterpret_cast<AttnSchedule*>(pr_smem_raw + rows_smem<T, HD, RB>());
-    const int per_head = attn_schedule<RB, kPrTile, kPrExtra, kPrThreads>(a, sched, 1);
+    float* red = reinterpret_cast<float*>(smem);
+    constexpr int kW = HD + 2;
+#pragma unroll
+    for (int h = 0; h < kHalves; ++h) {
+        l[h] += __shfl_xor_sync(0xffffffffu, l[h], 1);
+        l[h] += __shfl_xor_sync(0xffffffffu, l[h], 2);
+        float* w = red + (warp * RB + g + 8 * h) * kW;
+#pragma unroll
+        for (int n = 0; n < HD / 8; ++n) *reinterpret_cast<float2*>(w + n * 8 + 2 * q) = make_float2(o[n][2 * h], o[n][2 * h + 1]);
+        if (q == 0) *reinterpret_cast<float2*>(w + HD) = make_float2(m[h], l[h]);
+    }
+    __syncthreads();
+    merge_warps<HD, RB, St::kWarps>(a, pc, red);
+}
+
+template <int HD, int RB>
+__global__ void __launch_bounds__(PmStage<HD, RB>::kThreads, 1) paged_mma_kernel(const __grid_constant__ PagedAttnArgs a) {
+    using St = PmStage<HD, RB>;
+    extern __shared__ __align__(128) unsigned char pr_smem_raw[];
+    __shared__ AttnRun run;
+    __shared__ AttnPiece pieces[St::kWarps];
+    __shared__ int odd;
+    if (!a.balanced) {
+        AttnPiece p;
+        if (attn_block<RB, St::kTile, St::kThreads>(a, 1, &p)) mma_piece<HD, RB>(a, p, pr_smem_raw, &odd);
+        return;
+    }
+    AttnSchedule& sched = *reinterpret_cast<AttnSchedule*>(pr_smem_raw + St::kSmem);
+    const int per_head = attn_schedule<RB, St::kTile, kPrExtra, St::kThreads>(a, sched, 1);
     if (threadIdx.x == 0) run = attn_run(a, per_head);
     __syncthreads();
     pdl_launch_dependents();
     bool begun = false;
     const AttnPiece& p = pieces[threadIdx.x >> 5];
-    for (int at = run.u; (at = attn_next<RB, kPrTile, kPrExtra>(a, sched, run, at, 1, &pieces[threadIdx.x >> 5])) != 0;) {
+    for (int at = run.u; (at = attn_next<RB, St::kTile, kPrExtra>(a, sched, run, at, 1, &pieces[threadIdx.x >> 5])) != 0;) {
+        mma_piece<HD, RB>(a, p, pr_smem_raw, &odd);
+        __syncthreads();
+        if (p.slot == 1) {
+            begun = true;
+            if (threadIdx.x == 0) attn_header(a, &p);
+        }
+    }
+    if (!begun && threadIdx.x == 0) attn_header(a, nullptr);
+}
+
+template <int HD, int RB>
+static tvb_status launch_mma(PagedAttnArgs a, cudaStream_t st) {
+    using St = PmStage<HD, RB>;
+    static int set[kMaxDevices];
+    constexpr int smem = St::kSmem + (int)sizeof(AttnSchedule);
+    TVB_TRY(allow_smem(reinterpret_cast<const void*>(paged_mma_kernel<HD, RB>), smem, set));
+    a.min_units = 1 + kPrExtra;
+    Workspace ws(st);
+    dim3 grid;
+    if (a.balanced) {
+        grid = dim3((unsigned)num_sms());
+        TVB_TRY((attn_workspace<RB, HD>(&a, (int)grid.x, &ws)));
+    } else {
+        grid = dim3((unsigned)(((int64_t)a.s.n_tokens * a.group) / RB + a.s.n_seqs), (unsigned)a.nkv);
+    }
+    paged_mma_kernel<HD, RB><<<grid, St::kThreads, smem, st>>>(a);
+    TVB_TRY(check_launch("paged_mma_kernel"));
+    return launch_merge<RB, HD>(a, (int)grid.x, st);
+}
+
+template <typename T, int HD, int RB>
+__global__ void __launch_bounds__(PrStage<T, HD>::kThreads, 1) paged_rows_kernel(const __grid_constant__ PagedAttnArgs a) {
+    extern __shared__ __align__(128) unsigned char pr_smem_raw[];
+    __shared__ AttnRun run;
+    using St = PrStage<T, HD>;
+    __shared__ AttnPiece pieces[St::kWarps];
+    if (!a.balanced) {
+        AttnPiece p;
+        if (attn_block<RB, St::kTile, St::kThreads>(a, 1, &p)) rows_piece<T, HD, RB>(a, p, pr_smem_raw);
+        return;
+    }
+    AttnSchedule& sched = *reinterpret_cast<AttnSchedule*>(pr_smem_raw + rows_smem<T, HD, RB>());
+    const int per_head = attn_schedule<RB, St::kTile, kPrExtra, St::kThreads>(a, sched, 1);
+    if (threadIdx.x == 0) run = attn_run(a, per_head);
+    __syncthreads();
+    pdl_launch_dependents();
+    bool begun = false;
+    const AttnPiece& p = pieces[threadIdx.x >> 5];
+    for (int at = run.u; (at = attn_next<RB, St::kTile, kPrExtra>(a, sched, run, at, 1, &pieces[threadIdx.x >> 5])) != 0;) {
         rows_piece<T, HD, RB>(a, p, pr_smem_raw);
         __syncthreads();
         if (p.slot == 1) {
@@ -290,6 +580,7 @@ __global__ void __launch_bounds__(kPrThreads) paged_rows_kernel(const __grid_con
 template <typename T, int HD, int RB>
 static tvb_status launch_rows(PagedAttnArgs a, cudaStream_t st) {
     static int set[kMaxDevices];
+    using St = PrStage<T, HD>;
     constexpr int smem = rows_smem<T, HD, RB>() + (int)sizeof(AttnSchedule);
     TVB_TRY(allow_smem(reinterpret_cast<const void*>(paged_rows_kernel<T, HD, RB>), smem, set));
     a.min_units = 1 + kPrExtra;
@@ -301,7 +592,7 @@ static tvb_status launch_rows(PagedAttnArgs a, cudaStream_t st) {
     } else {
         grid = dim3((unsigned)(((int64_t)a.s.n_tokens * a.group) / RB + a.s.n_seqs), (unsigned)a.nkv);
     }
-    paged_rows_kernel<T, HD, RB><<<grid, kPrThreads, smem, st>>>(a);
+    paged_rows_kernel<T, HD, RB><<<grid, St::kThreads, smem, st>>>(a);
     TVB_TRY(check_launch("paged_rows_kernel"));
     return launch_merge<RB, HD>(a, (int)grid.x, st);
 }
@@ -310,6 +601,7 @@ template <typename T, int HD>
 static tvb_status launch_rows_rb(const PagedAttnArgs& a, int rows, cudaStream_t st) {
     if (rows <= 1) return launch_rows<T, HD, 1>(a, st);
     if (rows <= 2) return launch_rows<T, HD, 2>(a, st);
+    if constexpr (sizeof(T) == 2) return rows <= 8 ? launch_mma<HD, 8>(a, st) : launch_mma<HD, 16>(a, st);
     if (rows <= 4) return launch_rows<T, HD, 4>(a, st);
     return launch_rows<T, HD, 8>(a, st);
 }

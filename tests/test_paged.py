@@ -40,15 +40,16 @@ def rope(**kw):
 
 def attention(lib, kv=None, bt=None, **kw):
     a = dict(out=P, ldo=512, lse=None, q=P, ldq=512, nh=4, nkv=2, hd=128, scale=0.1, window=0) | kw
-    st = lib.tvb_attention_paged(a["out"], a["ldo"], a["lse"], a["q"], a["ldq"], kv or cache(), bt or batch(), a["nh"],
-                                 a["nkv"], a["hd"], a["scale"], a["window"], None, None)
+    st = lib.tvb_attention_paged(a["out"], a["ldo"], a["lse"], a["q"], a["ldq"], C.byref(kv or cache()),
+                                 C.byref(bt or batch()), a["nh"], a["nkv"], a["hd"], a["scale"], a["window"], None, None)
     return st, lib.tvb_last_error()
 
 
 def append(lib, kv=None, bt=None, rp=None, **kw):
     a = dict(qo=P, ldqo=512, q=P, ldq=512, k=P, ldk=256, v=P, ldv=256, nh=4, nkv=2, hd=128) | kw
-    st = lib.tvb_rope_append_paged(a["qo"], a["ldqo"], a["q"], a["ldq"], a["k"], a["ldk"], a["v"], a["ldv"], kv or cache(),
-                                   bt or batch(), rp or rope(), a["nh"], a["nkv"], a["hd"], None, None)
+    st = lib.tvb_rope_append_paged(a["qo"], a["ldqo"], a["q"], a["ldq"], a["k"], a["ldk"], a["v"], a["ldv"],
+                                   C.byref(kv or cache()), C.byref(bt or batch()), C.byref(rp or rope()), a["nh"], a["nkv"],
+                                   a["hd"], None, None)
     return st, lib.tvb_last_error()
 
 
@@ -108,7 +109,8 @@ def lora(lib, t=None, w=None, **kw):
     a = dict(y=P, x=P, M=2, K=256, N=64, adapter=P) | kw
     table = desc(LoraTableDesc, **(dict(n=1, max_rank=16, dtype=0, A=P, B=P, rank=P, scale=P) | (t or {})))
     weight = desc(Weight, **(dict(w=P, dtype=1) | (w or {})))
-    st = lib.tvb_matmul_lora(a["y"], a["x"], a["M"], a["K"], C.byref(weight), a["N"], table, a["adapter"], None, None)
+    st = lib.tvb_matmul_lora(a["y"], a["x"], a["M"], a["K"], C.byref(weight), a["N"], C.byref(table), a["adapter"],
+                             None, None)
     return st, lib.tvb_last_error()
 
 
