@@ -37,9 +37,10 @@ template <typename T, int HD>
 struct PrStage {
     static constexpr int kRow = HD * (int)sizeof(T);     // bytes of a key
     static constexpr int kBytes = 2 * kPrKeys * kRow;    // K rows, then V rows
-    // as many warps as leave each a few stages of its own in shared memory: the loads in flight hide the latency
-    static constexpr int kWarps = sizeof(T) == 2 ? 16 : 12, kThreads = 32 * kWarps;
-    static constexpr int kStages = 2;
+    // two CTAs an SM, so that one streams while the other starts or ends a piece; as many warps as leave each a
+    // few stages of its own in shared memory
+    static constexpr int kWarps = sizeof(T) == 2 ? 8 : 6, kThreads = 32 * kWarps;
+    static constexpr int kStages = sizeof(T) == 2 ? 3 : 2;
     static constexpr int kTile = kPrKeys * kWarps;       // keys a tile
     static constexpr int kSmem = kWarps * kStages * kBytes;
 };
@@ -279,7 +280,7 @@ template <int HD, int RB>
 struct PmStage {
     static constexpr int kKeys = 16, kRow = HD * 2;
     static constexpr int kBytes = 2 * kKeys * kRow;   // K rows, then V rows, 16-byte chunk c of a row at c ^ (row % 8)
-    static constexpr int kWarps = RB == 16 ? 8 : 12, kThreads = 32 * kWarps;   // (registers of 16 rows' queries)
+    static constexpr int kWarps = RB == 16 ? 4 : 6, kThreads = 32 * kWarps;   // (registers of 16 rows' queries)
     static constexpr int kStages = RB == 16 ? 3 : 2;
     static constexpr int kTile = kKeys * kWarps;
     static constexpr int kRing = kWarps * kStages * kBytes, kRed = kWarps * RB * (HD + 2) * 4;
@@ -499,7 +500,7 @@ __device__ __forceinline__ void mma_piece(const PagedAttnArgs& a, const AttnPiec
 }
 
 template <int HD, int RB>
-__global__ void __launch_bounds__(PmStage<HD, RB>::kThreads, 1) paged_mma_kernel(const __grid_constant__ PagedAttnArgs a) {
+__global__ void __launch_bounds__(PmStage<HD, RB>::kThreads, 2) paged_mma_kernel(const __grid_constant__ PagedAttnArgs a) {
     using St = PmStage<HD, RB>;
     extern __shared__ __align__(128) unsigned char pr_smem_raw[];
     __shared__ AttnRun run;
@@ -538,7 +539,7 @@ static tvb_status launch_mma(PagedAttnArgs a, cudaStream_t st) {
     Workspace ws(st);
     dim3 grid;
     if (a.balanced) {
-        grid = dim3((unsigned)num_sms());
+        grid = dim3(2u * (unsigned)num_sms());
         TVB_TRY((attn_workspace<RB, HD>(&a, (int)grid.x, &ws)));
     } else {
         grid = dim3((unsigned)(((int64_t)a.s.n_tokens * a.group) / RB + a.s.n_seqs), (unsigned)a.nkv);
@@ -549,7 +550,7 @@ static tvb_status launch_mma(PagedAttnArgs a, cudaStream_t st) {
 }
 
 template <typename T, int HD, int RB>
-__global__ void __launch_bounds__(PrStage<T, HD>::kThreads, 1) paged_rows_kernel(const __grid_constant__ PagedAttnArgs a) {
+__global__ void __launch_bounds__(PrStage<T, HD>::kThreads, 2) paged_rows_kernel(const __grid_constant__ PagedAttnArgs a) {
     extern __shared__ __align__(128) unsigned char pr_smem_raw[];
     __shared__ AttnRun run;
     using St = PrStage<T, HD>;
@@ -587,7 +588,7 @@ static tvb_status launch_rows(PagedAttnArgs a, cudaStream_t st) {
     Workspace ws(st);
     dim3 grid;
     if (a.balanced) {
-        grid = dim3((unsigned)num_sms());
+        grid = dim3(2u * (unsigned)num_sms());
         TVB_TRY((attn_workspace<RB, HD>(&a, (int)grid.x, &ws)));
     } else {
         grid = dim3((unsigned)(((int64_t)a.s.n_tokens * a.group) / RB + a.s.n_seqs), (unsigned)a.nkv);
@@ -602,8 +603,7 @@ static tvb_status launch_rows_rb(const PagedAttnArgs& a, int rows, cudaStream_t 
     if (rows <= 1) return launch_rows<T, HD, 1>(a, st);
     if (rows <= 2) return launch_rows<T, HD, 2>(a, st);
     if constexpr (sizeof(T) == 2) return rows <= 8 ? launch_mma<HD, 8>(a, st) : launch_mma<HD, 16>(a, st);
-    if (rows <= 4) return launch_rows<T, HD, 4>(a, st);
-    return launch_rows<T, HD, 8>(a, st);
+    else return rows <= 4 ? launch_rows<T, HD, 4>(a, st) : launch_rows<T, HD, 8>(a, st);
 }
 
 }  // namespace tvb

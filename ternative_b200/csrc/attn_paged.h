@@ -25,7 +25,7 @@ struct PagedAttnArgs {
     PagedSeqs s;
 };
 
-constexpr int kAttnSeqs = 1024;   // sequences that a balanced grid keeps in shared memory
+constexpr int kAttnSeqs = 512;   // sequences that a balanced grid keeps in shared memory
 
 // The work: row blocks (RB rows -- new token x query head of the group -- of one
 // KV head of one sequence) with the tiles of TK keys that some row of the block
