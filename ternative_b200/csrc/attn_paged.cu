@@ -21,7 +21,7 @@ namespace tvb {
 
 constexpr int kPrKeys = 8;   // keys a batch
 constexpr int kPrExtra = 1;   // what starting and leaving a block costs, in tiles
-constexpr int kTensorRows = 32;   // rows of a KV head from which F16 caches take the tensor cores
+constexpr int kTensorRows = 32;   // rows of a KV head from which chunks take the tensor cores
 
 __device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, bool valid) {
     asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(valid ? 16 : 0) : "memory");
@@ -641,10 +641,10 @@ extern "C" tvb_status tvb_attention_paged(float* out, int ldo, float* lse, const
     const int64_t rows64 = (int64_t)std::min(a.s.max_new, a.s.n_tokens) * a.group;
     const int rows = (int)std::min<int64_t>(rows64, 1 << 20);
     const bool f16 = kv->dtype == TVB_F16;
-    const bool tensor = f16 && rows >= kTensorRows;
+    const bool tensor = rows >= kTensorRows;
     a.balanced = a.s.n_seqs <= kAttnSeqs;   // more sequences than that fill the SMs block by block
     if (tensor) {
-        TVB_TRY(paged_attn_chunk_f16(a, hd, st));
+        TVB_TRY(paged_attn_chunk(a, hd, f16, st));
     } else if (hd == 128) {
         TVB_TRY((f16 ? launch_rows_rb<__half, 128>(a, rows, st) : launch_rows_rb<float, 128>(a, rows, st)));
     } else {

@@ -373,6 +373,6 @@ tvb_status attn_workspace(PagedAttnArgs* a, int ctas, Workspace* ws) {
     return TVB_OK;
 }
 
-tvb_status paged_attn_chunk_f16(const PagedAttnArgs& a, int hd, cudaStream_t st);   // attn_paged_tc.cu
+tvb_status paged_attn_chunk(const PagedAttnArgs& a, int hd, bool f16, cudaStream_t st);   // attn_paged_tc.cu
 
 }  // namespace tvb

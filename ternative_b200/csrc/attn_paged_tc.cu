@@ -30,18 +30,36 @@
 
 namespace tvb {
 
-constexpr int kPcRows = 128, kPcKeys = 128, kPcSlots = 4;
-// Warps 0-7 softmax, 8-9 loaders, 10 pieces, 11 MMA.
-constexpr int kPcSoft = 8, kPcLoaders = 2, kPcPieceWarp = kPcSoft + kPcLoaders, kPcMmaWarp = kPcPieceWarp + 1;
-constexpr int kPcThreads = 32 * (kPcMmaWarp + 1);
+constexpr int kPcRows = 128, kPcSoft = 8, kPcTeams = 2, kPcMaxSlots = 4;
 constexpr int kPcExtra = 3;   // what starting and leaving a block costs, in tiles
+
+// What depends on the cache's type.
+template <typename T>
+struct PcType;
+template <>
+struct PcType<__half> {   // q and p in F16 hi + lo, K and V as they are
+    static constexpr int kQPlanes = 2, kPlanes = 1, kKeys = 128, kSlots = 4;
+    static constexpr int kTeam = 1;            // warps that load an item together
+    static constexpr int kSoftRegs = 200, kAuxRegs = 104, kThreads = 384;
+};
+template <>
+struct PcType<float> {    // everything in three bf16 planes
+    static constexpr int kQPlanes = 3, kPlanes = 3, kKeys = 64, kSlots = 2;
+    static constexpr int kTeam = 3;
+    static constexpr int kSoftRegs = 176, kAuxRegs = 80, kThreads = 512;
+};
+// Warps 0-7 softmax, then the loaders' teams, the pieces' warp, the MMA's.
+template <typename T>
+constexpr int pc_piece_warp() {
+    return kPcSoft + kPcTeams * PcType<T>::kTeam;
+}
 
 // Barriers and flags of a CTA.
 struct PcShared {
-    uint64_t full[kPcSlots], empty[kPcSlots];
+    uint64_t full[kPcMaxSlots], empty[kPcMaxSlots];
     uint64_t s_full[2], p_full[2], o_full[2], o_read[2];
     uint64_t q_full, drained;
-    uint64_t fix[kPcLoaders];   // a V tile that its loader looks over
+    uint64_t fix[kPcTeams];   // a V tile that its loader looks over
     uint32_t tmem;
     int abort;
     int slow, slow_done;        // warps that compute rows key by key now; how many have done so
@@ -55,13 +73,15 @@ struct PcShared {
     float sum[2][2][128];       // a row's sum and maximum in each group, at the end of a piece
 };
 
-template <int HD>
+template <typename T, int HD>
 struct PcSmem {
-    static constexpr int kAtom = 128 * 128;               // 128 rows x 64 dims of F16
-    static constexpr int kPlane = kAtom * (HD / 64);      // Q plane, K or V tile
+    using Ty = PcType<T>;
+    static constexpr int kQAtom = kPcRows * 128, kAtom = Ty::kKeys * 128;       // rows x 64 dims of 16 bits
+    static constexpr int kQPlane = kQAtom * (HD / 64), kPlane = kAtom * (HD / 64);
     static constexpr int kQ = 0;
-    static constexpr int kSlots = 2 * kPlane;
-    static constexpr int kShared = kSlots + kPcSlots * kPlane;
+    static constexpr int kSlots = Ty::kQPlanes * kQPlane;
+    static constexpr int kSlot = Ty::kPlanes * kPlane;                          // a tile of K or V
+    static constexpr int kShared = kSlots + Ty::kSlots * kSlot;
     static constexpr int kSched = kShared + (int)((sizeof(PcShared) + 127) / 128 * 128);
     static constexpr int kBytes = kSched + (int)sizeof(AttnSchedule) + 1024;   // alignment
 };
@@ -103,6 +123,11 @@ __device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t (&r)[16
         "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]),
         "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
         : "memory");
+}
+__device__ __forceinline__ void tmem_st8(uint32_t taddr, const uint32_t (&r)[8]) {
+    asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"r"(taddr), "r"(r[0]),
+                 "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7])
+                 : "memory");
 }
 __device__ __forceinline__ void tmem_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 
@@ -146,6 +171,18 @@ __device__ __forceinline__ void tma_load_4d(uint32_t dst, const CUtensorMap* map
         : "memory");
 }
 
+// (x, y) as three packed bf16 planes, each the rounded rest of the one before: 24
+// bits, at any magnitude.
+__device__ __forceinline__ void bf16_planes(float x, float y, uint32_t* p0, uint32_t* p1, uint32_t* p2) {
+    asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(*p0) : "f"(y), "f"(x));
+    x -= __uint_as_float(*p0 << 16);
+    y -= __uint_as_float(*p0 & 0xffff0000u);
+    asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(*p1) : "f"(y), "f"(x));
+    x -= __uint_as_float(*p1 << 16);
+    y -= __uint_as_float(*p1 & 0xffff0000u);
+    asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(*p2) : "f"(y), "f"(x));
+}
+
 // K and V pools as [page][row][head][dim], boxes of `box` rows of one head and 64
 // dimensions; box 0: no maps (cp.async).
 struct PcMaps {
@@ -156,11 +193,18 @@ __device__ __forceinline__ void pc_cp_async16(uint32_t dst, const void* src, boo
     asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(valid ? 16 : 0) : "memory");
 }
 
-template <int HD>
-__global__ void __launch_bounds__(kPcThreads, 1)
+template <typename T, int HD>
+__global__ void __launch_bounds__(PcType<T>::kThreads, 1)
 paged_chunk_kernel(const __grid_constant__ PcMaps maps, const __grid_constant__ PagedAttnArgs a, int box) {
-    using Sm = PcSmem<HD>;
-    constexpr int kO = 2 * kPcKeys;   // TMEM: two S/P buffers in columns [0, 256), two O buffers behind
+    using Ty = PcType<T>;
+    using Sm = PcSmem<T, HD>;
+    constexpr bool kF32 = sizeof(T) == 4;
+    constexpr int kPcKeys = Ty::kKeys, kPcSlots = Ty::kSlots, kPcThreads = Ty::kThreads;
+    constexpr int kPcPieceWarp = pc_piece_warp<T>(), kPcMmaWarp = kPcPieceWarp + 1;
+    static_assert(kPcThreads == 32 * (kPcMmaWarp + 1), "warps");
+    // TMEM: two buffers of a tile's scores and, in their place, probabilities (8 columns a plane and 16 keys); two of O
+    constexpr int kPStep = 8 * Ty::kQPlanes, kSBuf = kF32 ? kPcKeys / 16 * kPStep : kPcKeys, kO = 2 * kSBuf;
+    static_assert(kO + 2 * HD <= 512 && kSBuf >= kPcKeys && kSBuf >= kPcKeys / 16 * kPStep, "TMEM");
     extern __shared__ unsigned char pc_smem_raw[];
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const uint32_t raw = smem_u32(pc_smem_raw);
@@ -187,7 +231,7 @@ paged_chunk_kernel(const __grid_constant__ PcMaps maps, const __grid_constant__ 
     }
     if (threadIdx.x == 0) {
         for (int i = 0; i < kPcSlots; ++i) {
-            mbar_init(sh.full + i, 1);
+            mbar_init(sh.full + i, Ty::kTeam);
             mbar_init(sh.empty + i, 1);
         }
         for (int i = 0; i < 2; ++i) {
@@ -198,11 +242,11 @@ paged_chunk_kernel(const __grid_constant__ PcMaps maps, const __grid_constant__ 
         }
         for (int i = 0; i < 4; ++i) {
             mbar_init(sh.piece_full + i, 1);
-            mbar_init(sh.piece_empty + i, kPcSoft + kPcLoaders + 1);
+            mbar_init(sh.piece_empty + i, kPcSoft + kPcTeams * Ty::kTeam + 1);
         }
         mbar_init(&sh.q_full, kPcSoft);
         mbar_init(&sh.drained, 1);
-        for (int i = 0; i < kPcLoaders; ++i) mbar_init(sh.fix + i, 1);
+        for (int i = 0; i < kPcTeams; ++i) mbar_init(sh.fix + i, 1);
         sh.abort = 0;
         sh.slow = sh.slow_done = 0;
         for (int i = 0; i < 4; ++i) sh.gone[i] = 0;
@@ -242,12 +286,14 @@ paged_chunk_kernel(const __grid_constant__ PcMaps maps, const __grid_constant__ 
         if (lane == 0) mbar_arrive(sh.piece_empty + (i & 3));
     };
 
-    // the softmax warps' registers: 128 x (200 + 200 + 104) = 384 x 168, what the CTA was launched with
+    // registers to the softmax warps: 128 x (200 + 200 + 104) = 384 x 168, 256 x (176 + 80) = 512 x 128, what the CTA was
+    // launched with
+    static_assert(256 * Ty::kSoftRegs + (kPcThreads - 256) * Ty::kAuxRegs <= kPcThreads * (kF32 ? 128 : 168), "registers");
     if (warp >= kPcSoft) {
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 104;");
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(Ty::kAuxRegs));
     if (warp < kPcPieceWarp) {
         // ---- loaders ---------------------------------------------------------------
-        const int w = warp - kPcSoft;
+        const int w = (warp - kPcSoft) / Ty::kTeam;   // team
         constexpr int kLanes = HD / 8;          // 16-byte chunks, lanes a row (cp.async)
         constexpr int kPass = 32 / kLanes;      // rows a warp instruction
         const int c = lane % kLanes;
@@ -267,9 +313,9 @@ paged_chunk_kernel(const __grid_constant__ PcMaps maps, const __grid_constant__ 
             const int p_last = p.pos0 + (int)a.gdiv.div((uint32_t)(p.row + p.rows - 1));
             for (int i = 0; i < nitems; ++i) {
                 const int gi = item0 + i;
-                if (gi % kPcLoaders != w) continue;
+                if (gi % kPcTeams != w) continue;
                 const int sl = gi % kPcSlots;
-                const uint32_t slot = base + Sm::kSlots + sl * Sm::kPlane;
+                const uint32_t slot = base + Sm::kSlots + sl * Sm::kSlot;
                 const bool is_k = i != nitems - 1 && (i == 0 || (i & 1));
                 const int tile = i == 0 ? 0 : is_k ? (i + 1) >> 1 : i == nitems - 1 ? nt - 1 : (i >> 1) - 1;
                 const bool free_slot = landed(sh.empty + sl, gi / kPcSlots + 1);
@@ -283,6 +329,50 @@ paged_chunk_kernel(const __grid_constant__ PcMaps maps, const __grid_constant__ 
                 const bool look = !is_k && (t1 - t0 < kPcKeys || t1 - 1 > p_first || t0 < p.first ||
                                             (a.window && t0 <= p_last - a.window));
                 bool bad = false;
+                if constexpr (kF32) {
+                    // this warp's rows of the tile, every third: loads of eight rows (pairs of rows, HD 64) before their
+                    // planes.  Values that are not finite have none: their piece goes key by key
+                    constexpr int kRowLanes = HD / 4, kPer = 32 / kRowLanes, kMine = (kPcKeys + Ty::kTeam - 1) / Ty::kTeam;
+                    const int first = (warp - kPcSoft) % Ty::kTeam, sub = lane / kRowLanes, d = lane % kRowLanes * 4;
+                    int64_t off = -1;
+                    const int my = first + lane * Ty::kTeam;
+                    if (lane < kMine && my < kPcKeys && t0 + my < p.k1) {
+                        off = paged_offset(a.kv, table, t0 + my);
+                        bad = off < 0;
+                    }
+                    const unsigned char* src = (is_k ? a.kv.k : a.kv.v) + (int64_t)p.kvh * a.kv.head_stride + d * 4;
+                    unsigned char* dst = smem + Sm::kSlots + sl * Sm::kSlot + (d >> 6) * Sm::kAtom + (d & 4) * 2;
+                    bool odd = false;
+#pragma unroll 1
+                    for (int r0 = 0; r0 < kMine; r0 += 8 * kPer) {
+                        float4 x[8];
+#pragma unroll
+                        for (int i = 0; i < 8; ++i) {
+                            const int64_t o = __shfl_sync(0xffffffffu, off, min(r0 + i * kPer + sub, 31));
+                            x[i] = o >= 0 ? *reinterpret_cast<const float4*>(src + o) : make_float4(0.f, 0.f, 0.f, 0.f);
+                        }
+#pragma unroll
+                        for (int i = 0; i < 8; ++i) {
+                            const int row = first + (r0 + i * kPer + sub) * Ty::kTeam;
+                            uint2 u[3];
+                            bf16_planes(x[i].x, x[i].y, &u[0].x, &u[1].x, &u[2].x);
+                            bf16_planes(x[i].z, x[i].w, &u[0].y, &u[1].y, &u[2].y);
+                            const float big = fmaxf(fmaxf(fabsf(x[i].x), fabsf(x[i].y)), fmaxf(fabsf(x[i].z), fabsf(x[i].w)));
+                            odd |= !(big < 3.3e38f) || x[i].x + x[i].y + x[i].z + x[i].w != x[i].x + x[i].y + x[i].z + x[i].w;
+                            if (row < kPcKeys) {
+#pragma unroll
+                                for (int pl = 0; pl < 3; ++pl)
+                                    *reinterpret_cast<uint2*>(dst + pl * Sm::kPlane + sw128_offset(row, (d >> 3) & 7)) = u[pl];
+                            }
+                        }
+                    }
+                    if (bad || odd) *reinterpret_cast<volatile int*>(&sh.poison[pi & 7]) = pi + 1;
+                    if (bad) report_bad(a.status);
+                    fence_proxy_async_smem_cta();
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(sh.full + sl);
+                    continue;
+                }
                 if (box) {
                     // one box a lane: `box` rows x 64 dimensions
                     const int per = kPcKeys / box, n = per * (HD / 64), row = (lane % per) * box, at = lane / per;
@@ -345,7 +435,7 @@ paged_chunk_kernel(const __grid_constant__ PcMaps maps, const __grid_constant__ 
                     uint32_t nonfinite = 0;
                     for (int j = lane; j < Sm::kPlane / 16; j += 32) {
                         const int key = (j * 16 % Sm::kAtom) / 128;
-                        uint4* at = reinterpret_cast<uint4*>(smem + Sm::kSlots + sl * Sm::kPlane + j * 16);
+                        uint4* at = reinterpret_cast<uint4*>(smem + Sm::kSlots + sl * Sm::kSlot + j * 16);
                         if (t0 + key >= p.k1) {
                             *at = make_uint4(0u, 0u, 0u, 0u);
                         } else {
@@ -367,7 +457,7 @@ paged_chunk_kernel(const __grid_constant__ PcMaps maps, const __grid_constant__ 
         }
         asm volatile("cp.async.wait_all;" ::: "memory");
         if (box && *abort_flag) {   // no TMA write may outlive the CTA: the last two items cover every slot still in flight
-            for (int i = max(w, issued - kPcLoaders); i <= issued; i += kPcLoaders)
+            for (int i = max(w, issued - kPcTeams); i <= issued; i += kPcTeams)
                 mbar_wait_bounded(sh.full + i % kPcSlots, (uint32_t)((i / kPcSlots) & 1));
         }
     } else if (warp == kPcPieceWarp) {
@@ -390,8 +480,9 @@ paged_chunk_kernel(const __grid_constant__ PcMaps maps, const __grid_constant__ 
         }
     } else {
         // ---- MMA issuer --------------------------------------------------------------
-        constexpr uint32_t idesc_s = umma_idesc_f16(kPcRows, kPcKeys);
-        constexpr uint32_t idesc_o = umma_idesc_f16(kPcRows, HD) | (1u << 16);   // B is MN-major
+        constexpr uint32_t kBf16 = kF32 ? (1u << 7) | (1u << 10) : 0u;                   // operands' type
+        constexpr uint32_t idesc_s = umma_idesc_f16(kPcRows, kPcKeys) | kBf16;
+        constexpr uint32_t idesc_o = umma_idesc_f16(kPcRows, HD) | (1u << 16) | kBf16;   // B is MN-major
         int item = 0, tile = 0;   // over all pieces
         bool ok = true;
         for (int pi = 0; ok && next(pi); ++pi) {
@@ -399,16 +490,29 @@ paged_chunk_kernel(const __grid_constant__ PcMaps maps, const __grid_constant__ 
             if (lane == 0) {
                 auto ready = [&]() { return landed(sh.full + item % kPcSlots, item / kPcSlots); };
                 auto mma_s = [&](int j) {   // tile j (of all) takes the buffer of P(j - 2)
-                    const uint32_t d = tmem + (j & 1) * kPcKeys;
-                    const uint64_t qd = sw128_desc(base + Sm::kQ), kd = sw128_desc(base + Sm::kSlots + (item % kPcSlots) * Sm::kPlane);
+                    const uint32_t d = tmem + (j & 1) * kSBuf;
+                    const uint64_t qd = sw128_desc(base + Sm::kQ), kd = sw128_desc(base + Sm::kSlots + (item % kPcSlots) * Sm::kSlot);
                     tc_fence_after();
+                    // products of plane x of q and plane y of K, the small ones of all steps before the large: the sum is
+                    // small while most are added.  Addresses in a descriptor count 16 bytes
+                    auto product = [&](int x, int y, bool begin) {
 #pragma unroll
-                    for (int kk = 0; kk < HD / 16; ++kk) {   // addresses in a descriptor count 16 bytes
-                        constexpr uint64_t kLo = Sm::kPlane >> 4;
-                        const uint64_t o = (kk >> 2) * (Sm::kAtom >> 4) + (kk & 3) * 2;
-                        tc_mma(d, qd + o, kd + o, idesc_s, kk ? 1u : 0u);
-                        tc_mma(d, qd + (o + kLo), kd + o, idesc_s, 1u);
+                        for (int kk = 0; kk < HD / 16; ++kk) {
+                            const uint64_t qo = (kk >> 2) * (Sm::kQAtom >> 4) + (kk & 3) * 2 + x * (Sm::kQPlane >> 4);
+                            const uint64_t ko = (kk >> 2) * (Sm::kAtom >> 4) + (kk & 3) * 2 + y * (Sm::kPlane >> 4);
+                            tc_mma(d, qd + qo, kd + ko, idesc_s, begin && kk == 0 ? 0u : 1u);
+                        }
+                    };
+                    if constexpr (kF32) {
+                        product(0, 2, true);
+                        product(1, 1, false);
+                        product(2, 0, false);
+                        product(0, 1, false);
+                        product(1, 0, false);
+                    } else {
+                        product(1, 0, true);
                     }
+                    product(0, 0, false);
                     tc_commit(sh.s_full + (j & 1));
                     tc_commit(sh.empty + item % kPcSlots);
                     ++item;
@@ -423,13 +527,24 @@ paged_chunk_kernel(const __grid_constant__ PcMaps maps, const __grid_constant__ 
                     ok = ready() && (j < 2 || landed(sh.o_read + (j & 1), (j - 2) >> 1)) && landed(sh.p_full + (j & 1), j >> 1);
                     if (!ok) break;
                     tc_fence_after();
-                    const uint64_t vd = sw128_mn_desc(base + Sm::kSlots + (item % kPcSlots) * Sm::kPlane, Sm::kAtom);
-                    const uint32_t pt = tmem + (j & 1) * kPcKeys, ot = tmem + kO + (j & 1) * HD;
+                    const uint64_t vd = sw128_mn_desc(base + Sm::kSlots + (item % kPcSlots) * Sm::kSlot, Sm::kAtom);
+                    const uint32_t pt = tmem + (j & 1) * kSBuf, ot = tmem + kO + (j & 1) * HD;
+                    auto product = [&](int x, int y, bool begin) {
 #pragma unroll
-                    for (int kk = 0; kk < kPcKeys / 16; ++kk) {
-                        tc_mma_ts(ot, pt + kk * 16, vd + kk * (2048 >> 4), idesc_o, kk ? 1u : 0u);
-                        tc_mma_ts(ot, pt + kk * 16 + 8, vd + kk * (2048 >> 4), idesc_o, 1u);
+                        for (int kk = 0; kk < kPcKeys / 16; ++kk)
+                            tc_mma_ts(ot, pt + kk * kPStep + 8 * x, vd + kk * (2048 >> 4) + y * (Sm::kPlane >> 4), idesc_o,
+                                      begin && kk == 0 ? 0u : 1u);
+                    };
+                    if constexpr (kF32) {
+                        product(0, 2, true);
+                        product(1, 1, false);
+                        product(2, 0, false);
+                        product(0, 1, false);
+                        product(1, 0, false);
+                    } else {
+                        product(1, 0, true);
                     }
+                    product(0, 0, false);
                     tc_commit(sh.o_full + (j & 1));
                     tc_commit(sh.empty + item % kPcSlots);
                     ++item;
@@ -451,7 +566,7 @@ paged_chunk_kernel(const __grid_constant__ PcMaps maps, const __grid_constant__ 
         __syncwarp();
     }
     } else {
-        asm volatile("setmaxnreg.inc.sync.aligned.u32 200;");
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(Ty::kSoftRegs));
         // ---- softmax: thread = row; group `half` takes the tiles of its parity, and half of the dimensions ----
         constexpr int kD = HD / 2;   // dimensions of this thread
         const int r = threadIdx.x & 127, half = warp >> 2;
@@ -493,29 +608,38 @@ paged_chunk_kernel(const __grid_constant__ PcMaps maps, const __grid_constant__ 
                 for (int k = 0; k < kLoads; ++k) {
                     const int qr = warp * 16 + k * kPer + sub;
                     const float4 y = make_float4(x[k].x * a.scale2, x[k].y * a.scale2, x[k].z * a.scale2, x[k].w * a.scale2);
-                    // the largest magnitude by its bits, infinities and NaN apart
-                    uint32_t mx = max(max(__float_as_uint(fabsf(y.x)), __float_as_uint(fabsf(y.y))),
-                                      max(__float_as_uint(fabsf(y.z)), __float_as_uint(fabsf(y.w))));
-                    if constexpr (HD == 128) {
-                        mx = __reduce_max_sync(0xffffffffu, mx);
+                    int e = 0;
+                    unsigned char* dst = smem + Sm::kQ + (d >> 6) * Sm::kQAtom + sw128_offset(qr, (d >> 3) & 7) + (d & 4) * 2;
+                    if constexpr (kF32) {
+                        uint2 u[3];
+                        bf16_planes(y.x, y.y, &u[0].x, &u[1].x, &u[2].x);
+                        bf16_planes(y.z, y.w, &u[0].y, &u[1].y, &u[2].y);
+#pragma unroll
+                        for (int pl = 0; pl < 3; ++pl) *reinterpret_cast<uint2*>(dst + pl * Sm::kQPlane) = u[pl];
                     } else {
+                        // the largest magnitude by its bits, infinities and NaN apart
+                        uint32_t mx = max(max(__float_as_uint(fabsf(y.x)), __float_as_uint(fabsf(y.y))),
+                                          max(__float_as_uint(fabsf(y.z)), __float_as_uint(fabsf(y.w))));
+                        if constexpr (HD == 128) {
+                            mx = __reduce_max_sync(0xffffffffu, mx);
+                        } else {
 #pragma unroll
-                        for (int o = 8; o > 0; o >>= 1) mx = max(mx, __shfl_xor_sync(0xffffffffu, mx, o));
-                    }
-                    // 2^e with the largest / 2^e in [2^13, 2^14): both planes of every value that matters are normal F16
-                    const int e = mx > 0u && mx < 0x7f800000u ? max(-100, min(100, (int)(mx >> 23) - 127 - 13)) : 0;
-                    const float g = __uint_as_float((uint32_t)(127 - e) << 23);
-                    const float v[4] = {y.x * g, y.y * g, y.z * g, y.w * g};
-                    __half2 hi[2], lo[2];
+                            for (int o = 8; o > 0; o >>= 1) mx = max(mx, __shfl_xor_sync(0xffffffffu, mx, o));
+                        }
+                        // 2^e with the largest / 2^e in [2^13, 2^14): both planes of every value that matters are normal F16
+                        if (mx > 0u && mx < 0x7f800000u) e = max(-100, min(100, (int)(mx >> 23) - 127 - 13));
+                        const float g = __uint_as_float((uint32_t)(127 - e) << 23);
+                        const float v[4] = {y.x * g, y.y * g, y.z * g, y.w * g};
+                        __half2 hi[2], lo[2];
 #pragma unroll
-                    for (int i = 0; i < 2; ++i) {
-                        hi[i] = __floats2half2_rn(v[2 * i], v[2 * i + 1]);
-                        const float2 h = __half22float2(hi[i]);
-                        lo[i] = __floats2half2_rn(v[2 * i] - h.x, v[2 * i + 1] - h.y);
+                        for (int i = 0; i < 2; ++i) {
+                            hi[i] = __floats2half2_rn(v[2 * i], v[2 * i + 1]);
+                            const float2 h = __half22float2(hi[i]);
+                            lo[i] = __floats2half2_rn(v[2 * i] - h.x, v[2 * i + 1] - h.y);
+                        }
+                        *reinterpret_cast<uint2*>(dst) = *reinterpret_cast<const uint2*>(hi);
+                        *reinterpret_cast<uint2*>(dst + Sm::kQPlane) = *reinterpret_cast<const uint2*>(lo);
                     }
-                    unsigned char* dst = smem + Sm::kQ + (d >> 6) * Sm::kAtom + sw128_offset(qr, (d >> 3) & 7) + (d & 4) * 2;
-                    *reinterpret_cast<uint2*>(dst) = *reinterpret_cast<const uint2*>(hi);
-                    *reinterpret_cast<uint2*>(dst + Sm::kPlane) = *reinterpret_cast<const uint2*>(lo);
                     if (d == 0) sh.f[qr] = __uint_as_float((uint32_t)(127 + e) << 23);
                 }
                 fence_proxy_async_smem_cta();
@@ -560,7 +684,7 @@ paged_chunk_kernel(const __grid_constant__ PcMaps maps, const __grid_constant__ 
                 if (!ok) break;
                 const float f = sh.f[r];   // written before the row's scores were
                 tc_fence_after();
-                const uint32_t sb = lanes + (j & 1) * kPcKeys;
+                const uint32_t sb = lanes + (j & 1) * kSBuf;
                 const int t0 = p.k0 + (j - tile) * kPcKeys, t1 = min(t0 + kPcKeys, p.k1);
                 const bool edge = t1 - t0 < kPcKeys || t0 < p.first || t1 - 1 > p_first || (a.window && t0 <= p_last - a.window);
                 // keys [first, last] of the tile are the row's: bits of the 32 (or 16) from key c on
@@ -570,60 +694,100 @@ paged_chunk_kernel(const __grid_constant__ PcMaps maps, const __grid_constant__ 
                     return hi < lo ? 0u : (0xffffffffu >> (31 - hi)) & (0xffffffffu << lo);
                 };
                 float m4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-                // loops rolled on purpose: what the three roles run between tiles fits the instruction cache
-#pragma unroll 1
-                for (int c = 0; c < kPcKeys; c += 32) {
-                    uint32_t s[32];
-                    tmem_ld32(sb + c, s);
-                    tmem_wait_ld();
-                    if (edge) {
-                        const uint32_t mk = seen(c);
-#pragma unroll
-                        for (int k = 0; k < 32; ++k)
-                            if (!(mk & (1u << k))) s[k] = 0xff800000u;   // -infinity
-                    }
-#pragma unroll
-                    for (int k = 0; k < 32; ++k) m4[k & 3] = fmaxf(m4[k & 3], __uint_as_float(s[k]));
-                }
-                const float mn = fmaxf(m, fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3])) * f);
-                const float corr = m == mn ? 1.f : ex2(m - mn);
-                const float mref = mn == -INFINITY ? 0.f : mn;
-                const uint64_t f2 = pack2(f, f), m2 = pack2(-mref, -mref);
-                const uint64_t minus1 = pack2(-1.f, -1.f);
+                float mn, corr, mref;
+                auto maximum = [&]() {
+                    mn = fmaxf(m, fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3])) * f);
+                    corr = m == mn ? 1.f : ex2(m - mn);
+                    mref = mn == -INFINITY ? 0.f : mn;
+                };
                 uint64_t sum[2] = {0ull, 0ull};
-#pragma unroll 1
-                for (int c = 0; c < kPcKeys; c += 16) {   // 16 keys: 8 columns of hi, 8 of lo, in place of their scores
-                    uint32_t zc[16];
-                    tmem_ld16(sb + c, zc);
+                if constexpr (kF32) {
+                    // the whole tile in registers: the planes of p take more columns than its scores
+                    uint32_t s[kPcKeys];
+#pragma unroll
+                    for (int c = 0; c < kPcKeys; c += 32) tmem_ld32(sb + c, *reinterpret_cast<uint32_t(*)[32]>(s + c));
                     tmem_wait_ld();
                     if (edge) {
-                        const uint32_t mk = seen(c);
 #pragma unroll
-                        for (int k = 0; k < 16; ++k)
-                            if (!(mk & (1u << k))) zc[k] = 0xff800000u;
-                    }
-                    uint64_t x[8];
-                    uint32_t pl[16];
+                        for (int c = 0; c < kPcKeys; c += 32) {
+                            const uint32_t mk = seen(c);
 #pragma unroll
-                    for (int k = 0; k < 8; ++k)
-                        x[k] = fma2(pack2(__uint_as_float(zc[2 * k]), __uint_as_float(zc[2 * k + 1])), f2, m2);
-#pragma unroll
-                    for (int k = 0; k < 8; ++k) {
-                        const float2 y = unpack2(x[k]);
-                        x[k] = pack2(ex2(y.x), ex2(y.y));
+                            for (int k = 0; k < 32; ++k)
+                                if (!(mk & (1u << k))) s[c + k] = 0xff800000u;   // -infinity
+                        }
                     }
 #pragma unroll
-                    for (int k = 0; k < 8; ++k) sum[k & 1] = add2(sum[k & 1], x[k]);
-                    // hi: the upper 11 bits as they are; lo: the rest, rounded to F16
+                    for (int k = 0; k < kPcKeys; ++k) m4[k & 3] = fmaxf(m4[k & 3], __uint_as_float(s[k]));
+                    maximum();
+                    const uint64_t m2 = pack2(-mref, -mref);
 #pragma unroll
-                    for (int k = 0; k < 8; ++k) {
-                        const uint64_t h = x[k] & 0xffffe000ffffe000ull;
-                        const float2 y = unpack2(h), w = unpack2(fma2(h, minus1, x[k]));
-                        const __half2 hi = __floats2half2_rn(y.x, y.y), lo = __floats2half2_rn(w.x, w.y);
-                        pl[k] = *reinterpret_cast<const uint32_t*>(&hi);
-                        pl[8 + k] = *reinterpret_cast<const uint32_t*>(&lo);
+                    for (int c = 0; c < kPcKeys; c += 16) {   // 16 keys: 8 columns a plane
+                        uint32_t p0[8], p1[8], p2[8];
+#pragma unroll
+                        for (int k = 0; k < 8; ++k) {
+                            const float2 z = unpack2(add2(pack2(__uint_as_float(s[c + 2 * k]), __uint_as_float(s[c + 2 * k + 1])), m2));
+                            const float x = ex2(z.x), y = ex2(z.y);
+                            sum[k & 1] = add2(sum[k & 1], pack2(x, y));
+                            bf16_planes(x, y, &p0[k], &p1[k], &p2[k]);
+                        }
+                        const uint32_t to = sb + c / 16 * kPStep;
+                        tmem_st8(to, p0);
+                        tmem_st8(to + 8, p1);
+                        tmem_st8(to + 16, p2);
                     }
-                    tmem_st16(sb + c, pl);
+                } else {
+                    // loops rolled on purpose: what the three roles run between tiles fits the instruction cache
+#pragma unroll 1
+                    for (int c = 0; c < kPcKeys; c += 32) {
+                        uint32_t s[32];
+                        tmem_ld32(sb + c, s);
+                        tmem_wait_ld();
+                        if (edge) {
+                            const uint32_t mk = seen(c);
+#pragma unroll
+                            for (int k = 0; k < 32; ++k)
+                                if (!(mk & (1u << k))) s[k] = 0xff800000u;   // -infinity
+                        }
+#pragma unroll
+                        for (int k = 0; k < 32; ++k) m4[k & 3] = fmaxf(m4[k & 3], __uint_as_float(s[k]));
+                    }
+                    maximum();
+                    const uint64_t f2 = pack2(f, f), m2 = pack2(-mref, -mref);
+                    const uint64_t minus1 = pack2(-1.f, -1.f);
+#pragma unroll 1
+                    for (int c = 0; c < kPcKeys; c += 16) {   // 16 keys: 8 columns of hi, 8 of lo, in place of their scores
+                        uint32_t zc[16];
+                        tmem_ld16(sb + c, zc);
+                        tmem_wait_ld();
+                        if (edge) {
+                            const uint32_t mk = seen(c);
+#pragma unroll
+                            for (int k = 0; k < 16; ++k)
+                                if (!(mk & (1u << k))) zc[k] = 0xff800000u;
+                        }
+                        uint64_t x[8];
+                        uint32_t pl[16];
+#pragma unroll
+                        for (int k = 0; k < 8; ++k)
+                            x[k] = fma2(pack2(__uint_as_float(zc[2 * k]), __uint_as_float(zc[2 * k + 1])), f2, m2);
+#pragma unroll
+                        for (int k = 0; k < 8; ++k) {
+                            const float2 y = unpack2(x[k]);
+                            x[k] = pack2(ex2(y.x), ex2(y.y));
+                        }
+#pragma unroll
+                        for (int k = 0; k < 8; ++k) sum[k & 1] = add2(sum[k & 1], x[k]);
+                        // hi: the upper 11 bits as they are; lo: the rest, rounded to F16
+#pragma unroll
+                        for (int k = 0; k < 8; ++k) {
+                            const uint64_t h = x[k] & 0xffffe000ffffe000ull;
+                            const float2 y = unpack2(h), w = unpack2(fma2(h, minus1, x[k]));
+                            const __half2 hi = __floats2half2_rn(y.x, y.y), lo = __floats2half2_rn(w.x, w.y);
+                            pl[k] = *reinterpret_cast<const uint32_t*>(&hi);
+                            pl[8 + k] = *reinterpret_cast<const uint32_t*>(&lo);
+                        }
+                        tmem_st16(sb + c, pl);
+                    }
                 }
                 sh.m[j & 3][r] = mn;
                 tmem_wait_st();
@@ -683,7 +847,7 @@ paged_chunk_kernel(const __grid_constant__ PcMaps maps, const __grid_constant__ 
             }
             if (ok && poisoned) {
                 if (lane == 0) atomicAdd(&sh.slow, 1);
-                for (int k = warp; k < p.rows; k += kPcSoft) attn_row_slow<__half, kPcRows, HD>(a, p, k);
+                for (int k = warp; k < p.rows; k += kPcSoft) attn_row_slow<T, kPcRows, HD>(a, p, k);
                 if (lane == 0) {
                     atomicAdd(&sh.slow_done, 1);
                     atomicSub(&sh.slow, 1);
@@ -716,15 +880,20 @@ static bool pool_map(CUtensorMap* m, const void* p, const PagedKV& kv, int nkv, 
     return encode_f16_tiled(m, p, 4, dims, strides, b) == TVB_OK;
 }
 
-template <int HD>
+template <typename T, int HD>
 static tvb_status launch_chunk(PagedAttnArgs a, cudaStream_t st) {
+    using Ty = PcType<T>;
     static int set[kMaxDevices];
-    TVB_TRY(allow_smem(reinterpret_cast<const void*>(paged_chunk_kernel<HD>), PcSmem<HD>::kBytes, set));
-    // boxes: the largest power of two that divides a page, up to a tile; pages that leave less than 8 rows go by cp.async
-    int box = 1;
-    while (box < kPcKeys && a.kv.page.d % (2u * box) == 0) box *= 2;
-    PcMaps maps;
-    if (box < 8 || !pool_map(&maps.k, a.kv.k, a.kv, a.nkv, HD, box) || !pool_map(&maps.v, a.kv.v, a.kv, a.nkv, HD, box)) box = 0;
+    constexpr int smem = PcSmem<T, HD>::kBytes;
+    TVB_TRY(allow_smem(reinterpret_cast<const void*>(paged_chunk_kernel<T, HD>), smem, set));
+    PcMaps maps = {};
+    int box = 0;
+    if constexpr (sizeof(T) == 2) {
+        // boxes: the largest power of two that divides a page, up to a tile; pages that leave less than 8 rows go by cp.async
+        box = 1;
+        while (box < Ty::kKeys && a.kv.page.d % (2u * box) == 0) box *= 2;
+        if (box < 8 || !pool_map(&maps.k, a.kv.k, a.kv, a.nkv, HD, box) || !pool_map(&maps.v, a.kv.v, a.kv, a.nkv, HD, box)) box = 0;
+    }
     // a piece of two tiles still pays for its start (the block's queries) and its partial sums
     a.min_units = 2 + kPcExtra;
     Workspace ws(st);
@@ -735,13 +904,14 @@ static tvb_status launch_chunk(PagedAttnArgs a, cudaStream_t st) {
     } else {
         grid = dim3((unsigned)(((int64_t)a.s.n_tokens * a.group) / kPcRows + a.s.n_seqs), (unsigned)a.nkv);
     }
-    paged_chunk_kernel<HD><<<grid, kPcThreads, PcSmem<HD>::kBytes, st>>>(maps, a, box);
+    paged_chunk_kernel<T, HD><<<grid, Ty::kThreads, smem, st>>>(maps, a, box);
     TVB_TRY(check_launch("paged_chunk_kernel"));
     return launch_merge<kPcRows, HD>(a, (int)grid.x, st);
 }
 
-tvb_status paged_attn_chunk_f16(const PagedAttnArgs& a, int hd, cudaStream_t st) {
-    return hd == 128 ? launch_chunk<128>(a, st) : launch_chunk<64>(a, st);
+tvb_status paged_attn_chunk(const PagedAttnArgs& a, int hd, bool f16, cudaStream_t st) {
+    if (f16) return hd == 128 ? launch_chunk<__half, 128>(a, st) : launch_chunk<__half, 64>(a, st);
+    return hd == 128 ? launch_chunk<float, 128>(a, st) : launch_chunk<float, 64>(a, st);
 }
 
 }  // namespace tvb
