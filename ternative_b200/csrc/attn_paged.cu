@@ -21,7 +21,15 @@ namespace tvb {
 
 constexpr int kPrKeys = 8;   // keys a batch
 constexpr int kPrExtra = 1;   // what starting and leaving a block costs, in tiles
-constexpr int kTensorRows = 32;   // rows of a KV head from which chunks take the tensor cores
+// Rows of a KV head from which a call takes the tensor cores (paged_chunk_kernel):
+// below, its 128-row tiles are too empty.  Measured with 20/5 heads, 8 sequences of
+// 3000 keys: F16 24 rows 32 against 31 us, 48 rows 29 against 32; F32 32 rows 110
+// against 79 us, 64 rows 63 against 79.
+constexpr int kTensorRows16 = 32, kTensorRows32 = 64;
+// Keys up to which a CTA takes whole blocks: sharing tiles evenly costs a second
+// launch.  One token of one sequence, 130 keys 6.7 against 10.4 us, 400 keys 13.2
+// against 11.3.
+constexpr int kWholeKeys = 256;
 
 __device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, bool valid) {
     asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(valid ? 16 : 0) : "memory");
@@ -641,8 +649,9 @@ extern "C" tvb_status tvb_attention_paged(float* out, int ldo, float* lse, const
     const int64_t rows64 = (int64_t)std::min(a.s.max_new, a.s.n_tokens) * a.group;
     const int rows = (int)std::min<int64_t>(rows64, 1 << 20);
     const bool f16 = kv->dtype == TVB_F16;
-    const bool tensor = rows >= kTensorRows;
-    a.balanced = a.s.n_seqs <= kAttnSeqs;   // more sequences than that fill the SMs block by block
+    const bool tensor = rows >= (f16 ? kTensorRows16 : kTensorRows32);
+    const int64_t span = window ? std::min<int64_t>(a.s.max_kv, (int64_t)window + a.s.max_new) : a.s.max_kv;
+    a.balanced = a.s.n_seqs <= kAttnSeqs && span > kWholeKeys;   // more sequences fill the SMs block by block
     if (tensor) {
         TVB_TRY(paged_attn_chunk(a, hd, f16, st));
     } else if (hd == 128) {

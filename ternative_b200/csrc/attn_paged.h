@@ -217,14 +217,18 @@ __device__ __forceinline__ bool attn_block(const PagedAttnArgs& a, int align, At
 }
 
 // Partial (CTA, slot) of RB rows: HD weighted values of each, then each row's sum
-// and maximum.
+// and maximum; partials start at multiples of 16 bytes.
+template <int RB, int HD>
+__host__ __device__ constexpr int attn_part_floats() {
+    return (RB * (HD + 2) + 3) / 4 * 4;
+}
 template <int RB, int HD>
 __device__ __forceinline__ float* attn_part(const PagedAttnArgs& a, int cta, int slot, int r) {
-    return a.part + ((size_t)cta * 2 + slot) * RB * (HD + 2) + (size_t)r * HD;
+    return a.part + ((size_t)cta * 2 + slot) * attn_part_floats<RB, HD>() + (size_t)r * HD;
 }
 template <int RB, int HD>
 __device__ __forceinline__ float* attn_part_sum(const PagedAttnArgs& a, int cta, int slot, int r) {
-    return a.part + (((size_t)cta * 2 + slot) * (HD + 2) + HD) * RB + 2 * r;
+    return a.part + ((size_t)cta * 2 + slot) * attn_part_floats<RB, HD>() + RB * HD + 2 * r;
 }
 
 // Tells paged_merge_kernel about the cut block that this CTA begins (one thread).
@@ -273,14 +277,14 @@ __device__ __forceinline__ void attn_row_store(const PagedAttnArgs& a, const Att
         float* pp = attn_part<RB, HD>(a, blockIdx.x, p.slot, r);
         if (lane == 0) *reinterpret_cast<float2*>(attn_part_sum<RB, HD>(a, blockIdx.x, p.slot, r)) = make_float2(l, m);
 #pragma unroll
-        for (int d = 0; d < ND; ++d) pp[lane * ND + d] = o[d];
+        for (int d = 0; d < ND; d += 2) *reinterpret_cast<float2*>(pp + lane * ND + d) = make_float2(o[d], o[d + 1]);
     } else {
         const int t = (int)a.gdiv.div((uint32_t)(p.row + r)), tok = p.tok0 + t;
         const int head = p.kvh * a.group + p.row + r - t * a.group;
         const float inv = attn_inv(l);
         float* po = a.out + (size_t)tok * a.ldo + head * HD + lane * ND;
 #pragma unroll
-        for (int d = 0; d < ND; ++d) po[d] = o[d] * inv;
+        for (int d = 0; d < ND; d += 2) *reinterpret_cast<float2*>(po + d) = make_float2(o[d] * inv, o[d + 1] * inv);
         if (a.lse && lane == 0) a.lse[(size_t)tok * a.nh + head] = attn_lse(l, m);
     }
 }
@@ -342,14 +346,21 @@ __global__ void __launch_bounds__(256) paged_merge_kernel(const __grid_constant_
         float L = 0.f, o[ND];
 #pragma unroll
         for (int d = 0; d < ND; ++d) o[d] = 0.f;
-        for (int c = c0; c <= last; ++c) {
-            const float* x = attn_part<RB, HD>(a, c, c == c0, r);
-            const float2 lm = *reinterpret_cast<const float2*>(attn_part_sum<RB, HD>(a, c, c == c0, r));
-            const float w = lm.y == -INFINITY ? 0.f : exp2f(lm.y - M);
-            if (w != 0.f) {
-                L = fmaf(lm.x, w, L);
+        for (int b = c0; b <= last; b += 32) {
+            // lane i: weight of piece b + i; then the pieces' values, several loads at once
+            const int c = b + lane;
+            float2 lm = make_float2(0.f, -INFINITY);
+            if (c <= last) lm = *reinterpret_cast<const float2*>(attn_part_sum<RB, HD>(a, c, c == c0, r));
+            const float w = lm.y == -INFINITY ? (lm.x == 0.f ? 0.f : 1.f) : exp2f(lm.y - M);   // no maximum but a sum: NaN
+            L += warp_sum(w == 0.f ? 0.f : lm.x * w);
+            const int n = min(32, last - b + 1);
+#pragma unroll 8
+            for (int k = 0; k < n; ++k) {
+                const float wk = __shfl_sync(0xffffffffu, w, k);
+                float x[ND];
+                pr_load<float, ND>(reinterpret_cast<const unsigned char*>(attn_part<RB, HD>(a, b + k, b + k == c0, r) + lane * ND), x);
 #pragma unroll
-                for (int d = 0; d < ND; ++d) o[d] = fmaf(x[lane * ND + d], w, o[d]);
+                for (int d = 0; d < ND; ++d) o[d] = wk != 0.f ? fmaf(x[d], wk, o[d]) : o[d];
             }
         }
         attn_row_store<RB, HD, ND>(a, p, r, L, M, o);
@@ -366,7 +377,7 @@ tvb_status launch_merge(const PagedAttnArgs& a, int ctas, cudaStream_t st) {
 // Workspace of a balanced grid.
 template <int RB, int HD>
 tvb_status attn_workspace(PagedAttnArgs* a, int ctas, Workspace* ws) {
-    const size_t part = (size_t)ctas * 2 * RB * (HD + 2) * 4;
+    const size_t part = (size_t)ctas * 2 * attn_part_floats<RB, HD>() * 4;
     TVB_TRY(ws->get(part + (size_t)ctas * 32));
     a->part = ws->at<float>();
     a->header = ws->at<int>(part);
