@@ -526,7 +526,7 @@ __global__ void __launch_bounds__(PmStage<HD, RB>::kThreads, 2) paged_mma_kernel
     pdl_launch_dependents();
     bool begun = false;
     const AttnPiece& p = pieces[threadIdx.x >> 5];
-    for (int at = run.u; (at = attn_next<RB, St::kTile, kPrExtra>(a, sched, run, at, 1, &pieces[threadIdx.x >> 5])) != 0;) {
+    for (int64_t at = run.u; (at = attn_next<RB, St::kTile, kPrExtra>(a, sched, run, at, 1, &pieces[threadIdx.x >> 5])) != 0;) {
         mma_piece<HD, RB>(a, p, pr_smem_raw, &odd);
         __syncthreads();
         if (p.slot == 1) {
@@ -575,7 +575,7 @@ __global__ void __launch_bounds__(PrStage<T, HD>::kThreads, 2) paged_rows_kernel
     pdl_launch_dependents();
     bool begun = false;
     const AttnPiece& p = pieces[threadIdx.x >> 5];
-    for (int at = run.u; (at = attn_next<RB, St::kTile, kPrExtra>(a, sched, run, at, 1, &pieces[threadIdx.x >> 5])) != 0;) {
+    for (int64_t at = run.u; (at = attn_next<RB, St::kTile, kPrExtra>(a, sched, run, at, 1, &pieces[threadIdx.x >> 5])) != 0;) {
         rows_piece<T, HD, RB>(a, p, pr_smem_raw);
         __syncthreads();
         if (p.slot == 1) {
@@ -651,7 +651,9 @@ extern "C" tvb_status tvb_attention_paged(float* out, int ldo, float* lse, const
     const bool f16 = kv->dtype == TVB_F16;
     const bool tensor = rows >= (f16 ? kTensorRows16 : kTensorRows32);
     const int64_t span = window ? std::min<int64_t>(a.s.max_kv, (int64_t)window + a.s.max_new) : a.s.max_kv;
-    a.balanced = a.s.n_seqs <= kAttnSeqs && span > kWholeKeys;   // more sequences fill the SMs block by block
+    // many sequences or row blocks fill the SMs evenly enough block by block
+    const int64_t blocks = ((int64_t)a.s.n_tokens * a.group / (tensor ? 128 : 8) + a.s.n_seqs) * nkv;
+    a.balanced = a.s.n_seqs <= kAttnSeqs && span > kWholeKeys && blocks <= 64 * num_sms();
     if (tensor) {
         TVB_TRY(paged_attn_chunk(a, hd, f16, st));
     } else if (hd == 128) {

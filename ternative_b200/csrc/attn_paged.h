@@ -105,9 +105,8 @@ __device__ __forceinline__ int attn_schedule(const PagedAttnArgs& a, AttnSchedul
 
 // A CTA's run of units.
 struct AttnRun {
-    int64_t total;
+    int64_t total, u, end;
     int per_head, ctas;
-    int u, end;
 };
 
 __device__ __forceinline__ AttnRun attn_run(const PagedAttnArgs& a, int per_head) {
@@ -115,8 +114,8 @@ __device__ __forceinline__ AttnRun attn_run(const PagedAttnArgs& a, int per_head
     r.per_head = per_head;
     r.total = (int64_t)per_head * a.nkv;
     r.ctas = (int)min((int64_t)gridDim.x, max((int64_t)1, r.total / a.min_units));
-    r.u = (int)(r.total * min((int)blockIdx.x, r.ctas) / r.ctas);
-    r.end = (int)(r.total * min((int)blockIdx.x + 1, r.ctas) / r.ctas);
+    r.u = r.total * min((int)blockIdx.x, r.ctas) / r.ctas;
+    r.end = r.total * min((int)blockIdx.x + 1, r.ctas) / r.ctas;
     return r;
 }
 
@@ -124,14 +123,14 @@ __device__ __forceinline__ AttnRun attn_run(const PagedAttnArgs& a, int per_head
 // of this warp); returns the unit after it, 0 when the run has no more.  Not
 // inlined, for the instruction cache's sake.
 template <int RB, int TK, int EX>
-__device__ __noinline__ int attn_next(const PagedAttnArgs& a, const AttnSchedule& s, const AttnRun& r, int u, int align,
-                                      AttnPiece* out) {
+__device__ __noinline__ int64_t attn_next(const PagedAttnArgs& a, const AttnSchedule& s, const AttnRun& r, int64_t u,
+                                          int align, AttnPiece* out) {
     const int lane = threadIdx.x & 31;
     AttnPiece p;
 again:
     if (u >= r.end) return 0;
-    p.kvh = u / r.per_head;
-    int t = u - p.kvh * r.per_head;
+    p.kvh = (int)(u / r.per_head);
+    int t = (int)(u - (int64_t)p.kvh * r.per_head);
     int lo = 0, hi = a.s.n_seqs - 1;   // the last sequence that starts at or before t
     while (lo < hi) {
         const int mid = (lo + hi + 1) >> 1;
@@ -165,8 +164,8 @@ again:
         t -= __shfl_sync(0xffffffffu, sum, 31);
     }
     // t: unit of the block, `tiles` of them; the tiles are those from EX on
-    const int begin = max(t, EX), end = min(tiles, t + r.end - u);
-    const int first_unit = u - t;
+    const int begin = max(t, EX), end = (int)min((int64_t)tiles, t + r.end - u);
+    const int64_t first_unit = u - t;
     u = first_unit + end;
     if (begin >= end) goto again;   // the run ends, or begins, before the block's first tile
     attn_tiles<RB, TK>(a, n, p.pos0, i0, align, &p.first, &p.k0, &p.k1);
@@ -174,7 +173,7 @@ again:
     p.rows = min(RB, n * a.group - p.row);
     p.tiles = end - begin;
     p.slot = p.tiles == tiles - EX ? -1 : begin > EX ? 0 : 1;
-    p.last_cta = (int)(((int64_t)(first_unit + tiles) * r.ctas - 1) / r.total);
+    p.last_cta = (int)(((first_unit + tiles) * r.ctas - 1) / r.total);
     p.k0 += (begin - EX) * TK;
     p.k1 = min(p.k1, p.k0 + p.tiles * TK);
     __syncwarp();

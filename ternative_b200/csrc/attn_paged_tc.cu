@@ -1,16 +1,19 @@
-// Attention of chunks of new tokens over an F16 paged cache on the tensor cores
+// Attention of chunks of new tokens over the paged cache on the tensor cores
 // (tvb_attention_paged; attn_paged.cu has the formula).
 //
 // paged_chunk_kernel: one CTA an SM takes its run of tiles (attn_schedule):
 // blocks of 128 query rows (new token x query head of the group) of one KV head
-// of one sequence against tiles of 128 keys.  Products in F32 accuracy from F16
-// operands: q (times scale log2 e, with a power-of-two exponent a row) and p are
-// split into F16 hi + lo planes, K and V are F16 as they are, so every product
-// takes two MMAs and the bound is the tensor pipe at twice the algorithmic FLOPs.
+// of one sequence against tiles of 128 keys (64, F32).  Products in F32 accuracy:
+// over an F16 cache q (times scale log2 e, with a power-of-two exponent a row) and
+// p are split into F16 hi + lo planes, K and V are F16 as they are, so every
+// product takes two MMAs and the bound is the tensor pipe at twice the algorithmic
+// FLOPs; over an F32 cache q, K, p and V are split into three bf16 planes (24 bits
+// at any magnitude) and a product takes six MMAs.
 //
 //   loader warps (a slot of shared memory at a time each): K or V by TMA, a box of
 //     rows a lane, page by page (pages that no box of 8 rows divides: by 16-byte
-//     cp.async); in V rows behind the last key become zeros
+//     cp.async); in V rows behind the last key become zeros.  F32: three warps a
+//     slot, loads to registers, planes to the swizzled tile
 //   MMA warp: S = Q K^T (K-major operands) into one of two TMEM buffers, then O =
 //     P V with P from TMEM and V as the MN-major operand it is in memory (no
 //     transpose): PV(j), S(j + 2), PV(j + 1), S(j + 3), ...
@@ -19,7 +22,10 @@
 //     in TMEM), so that one group's exponentials run under the other's MMAs.  Both
 //     add every tile's O, half of the dimensions each, to registers with the
 //     rescaling; a fresh product per tile also keeps the tensor core's truncating
-//     sums short (16 MMAs: 3e-7; a sum over 6000 keys in TMEM would lose 1.4e-5)
+//     sums short (16 MMAs: 3e-7; a sum over 6000 keys in TMEM would lose 1.4e-5).
+//     Registers move to these warps (setmaxnreg), and what the roles run between
+//     tiles stays in rolled loops: unrolled, instruction fetch took half the time
+//   a warp works out the pieces ahead of the others
 //
 // A masked probability is zero but 0 x inf is not: a loader that finds a
 // non-finite value in a V tile that some row does not see whole, or a page that
@@ -462,7 +468,8 @@ paged_chunk_kernel(const __grid_constant__ PcMaps maps, const __grid_constant__ 
         }
     } else if (warp == kPcPieceWarp) {
         // ---- the pieces, ahead of the others ------------------------------------------
-        for (int pi = 0, at = a.balanced ? sh.run.u : 0;; ++pi) {
+        int64_t at = a.balanced ? sh.run.u : 0;
+        for (int pi = 0;; ++pi) {
             if (pi >= 4 && !__all_sync(0xffffffffu, landed(sh.piece_empty + (pi & 3), (pi >> 2) - 1))) break;
             AttnPiece* out = sh.piece + (pi & 3);
             int n = 0;

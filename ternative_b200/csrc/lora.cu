@@ -28,10 +28,12 @@ namespace cg = cooperative_groups;
 namespace tvb {
 
 constexpr int kLrWarps = 8, kLrThreads = 32 * kLrWarps;
-constexpr int kLrCols = 16;        // weight rows a tile
 // Largest K slice of a warp: what two CTAs an SM (one, when WIDE) have registers for.
-__host__ __device__ constexpr int lr_slice(bool w8, bool wide) { return !wide ? 128 : w8 ? 192 : 160; }
-constexpr int kLrBatch = 4;        // tiles between two barriers of the CTA
+__host__ __device__ constexpr int lr_slice(bool w8, bool wide) { return w8 || !wide ? 128 : 160; }
+// Weight rows a tile: what keeps enough loads under way (a warp's slice of an INT8
+// row is half as many bytes).
+__host__ __device__ constexpr int lr_cols(bool w8) { return w8 ? 32 : 16; }
+__host__ __device__ constexpr int lr_batch(bool w8) { return w8 ? 2 : 4; }   // tiles between two barriers of the CTA
 constexpr int kLrMaxSplit = 8;     // CTAs of a cluster
 constexpr int kLrMaxRows = 16;
 
@@ -148,14 +150,16 @@ lora_rows_kernel(const __grid_constant__ LoraArgs a, const __grid_constant__ Lor
     constexpr int kBlocks = lr_slice(W8, WIDE) / kBlock;     // loads a weight row
     constexpr int kSteps = E / 4;                      // MMA steps a load
     constexpr int kHalves = WIDE ? 2 : 1;
-    constexpr int kRed = kLrMaxRows * 17;              // a warp's sums of a tile
-    extern __shared__ __align__(16) float lr_smem[];   // [tile][16 rows][16 weight rows], then the warps' sums
+    constexpr int kCols = lr_cols(W8), kGroups = kCols / 8, kBatch = lr_batch(W8), kRows = 8 * kHalves;
+    constexpr int kRed = kRows * (kCols + 1);          // a warp's sums of a tile
+    constexpr int kOut = kRows * kCols;
+    extern __shared__ __align__(16) float lr_smem[];   // [tile][rows][weight rows], then the warps' sums
     cg::cluster_group cl = cg::this_cluster();
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, q = lane & 3;
     const int rank = (int)cl.block_rank(), nsplit = (int)cl.num_blocks();
     const int group = (int)(blockIdx.x / nsplit), groups = (int)(gridDim.x / nsplit);
     const int my_tiles = plan.tiles > group ? (plan.tiles - group + groups - 1) / groups : 0;
-    float* warps = lr_smem + plan.most * 256;          // [2][kLrBatch tiles][8 warps][16][16 + 1]
+    float* warps = lr_smem + plan.most * kOut;         // [2][kBatch tiles][8 warps][rows][weight rows + 1]
     const int64_t row_bytes = (int64_t)a.K * (W8 ? 1 : 2);
     int batch = 0;
 
@@ -166,21 +170,21 @@ lora_rows_kernel(const __grid_constant__ LoraArgs a, const __grid_constant__ Lor
 #pragma unroll
         for (int i = 0; i < kBlocks; ++i) in_k |= (unsigned)(i * kBlock < plan.slice && k0 + i * kBlock < a.K) << i;
 
-        // this warp's weights of 16 rows: 16 bytes of row g and of row g + 8 a load
-        uint4 w[2][kBlocks];
-        int n = group * kLrCols + g;
+        // this warp's weights of the tile's rows: 16 bytes of row g of each 8 a load
+        uint4 w[kGroups][kBlocks];
+        int n = group * kCols + g;
         const unsigned char* wp = static_cast<const unsigned char*>(a.w) + n * row_bytes + (int64_t)k0 * (W8 ? 1 : 2);
         auto request = [&]() {
 #pragma unroll
-            for (int h = 0; h < 2; ++h) {
+            for (int h = 0; h < kGroups; ++h) {
                 const bool row = n + 8 * h < a.N;
                 const unsigned char* p = wp + 8 * h * row_bytes;
 #pragma unroll
                 for (int i = 0; i < kBlocks; ++i)
                     w[h][i] = row && ((in_k >> i) & 1u) ? ld_stream16(p + i * 64) : make_uint4(0u, 0u, 0u, 0u);
             }
-            n += groups * kLrCols;
-            wp += groups * kLrCols * row_bytes;
+            n += groups * kCols;
+            wp += groups * kCols * row_bytes;
         };
         if (my_tiles) request();
 
@@ -224,16 +228,16 @@ lora_rows_kernel(const __grid_constant__ LoraArgs a, const __grid_constant__ Lor
                     }
         }
 
-        // kLrBatch tiles between barriers: the warps run apart as far as that
+        // kBatch tiles between barriers: the warps run apart as far as that
 #pragma unroll 1
-        for (int it = 0; it < my_tiles; it += kLrBatch, ++batch) {
-            float* half = warps + (batch & 1) * (kLrBatch * kLrWarps * kRed);
-            const int nb = min(kLrBatch, my_tiles - it);
+        for (int it = 0; it < my_tiles; it += kBatch, ++batch) {
+            float* half = warps + (batch & 1) * (kBatch * kLrWarps * kRed);
+            const int nb = min(kBatch, my_tiles - it);
 #pragma unroll 1
             for (int b = 0; b < nb; ++b) {
-                float hi[2][4] = {}, lo[2][4] = {};   // sums of the two planes apart: shorter chains
+                float hi[kGroups][4] = {}, lo[kGroups][4] = {};   // sums of the two planes apart: shorter chains
 #pragma unroll
-                for (int h = 0; h < 2; ++h)
+                for (int h = 0; h < kGroups; ++h)
 #pragma unroll
                     for (int i = 0; i < kBlocks; ++i) {
                         const uint32_t ww[4] = {w[h][i].x, w[h][i].y, w[h][i].z, w[h][i].w};
@@ -258,22 +262,20 @@ lora_rows_kernel(const __grid_constant__ LoraArgs a, const __grid_constant__ Lor
                 // D: rows g, g + 8; weight rows 2q, 2q + 1 of each 8
                 float* red = half + (b * kLrWarps + warp) * kRed;
 #pragma unroll
-                for (int h = 0; h < 2; ++h)
+                for (int h = 0; h < kGroups; ++h)
 #pragma unroll
                     for (int e = 0; e < 4; ++e)
-                        if (WIDE || e < 2) red[(g + 8 * (e >> 1)) * 17 + h * 8 + 2 * q + (e & 1)] = (hi[h][e] + lo[h][e]) * f[e >> 1];
+                        if (WIDE || e < 2) red[(g + 8 * (e >> 1)) * (kCols + 1) + h * 8 + 2 * q + (e & 1)] = (hi[h][e] + lo[h][e]) * f[e >> 1];
             }
             __syncthreads();
-            if (WIDE || threadIdx.x < 128) {
-                const int at = (threadIdx.x >> 4) * 17 + (threadIdx.x & 15);
-                for (int b = 0; b < nb; ++b) {
-                    const float* r = half + b * kLrWarps * kRed + at;
-                    float s = r[0];
+            for (int i = threadIdx.x; i < nb * kOut; i += kLrThreads) {
+                const int b = i / kOut, at = i % kOut / kCols * (kCols + 1) + i % kCols;
+                const float* r = half + b * kLrWarps * kRed + at;
+                float s = r[0];
 #pragma unroll
-                    for (int v = 1; v < kLrWarps; ++v) s += r[v * kRed];
-                    float* sum = lr_smem + (it + b) * 256 + threadIdx.x;
-                    *sum = pass ? *sum + s : s;
-                }
+                for (int v = 1; v < kLrWarps; ++v) s += r[v * kRed];
+                float* sum = lr_smem + it * kOut + i;
+                *sum = pass ? *sum + s : s;
             }
         }
     }
@@ -282,18 +284,21 @@ lora_rows_kernel(const __grid_constant__ LoraArgs a, const __grid_constant__ Lor
     if (a.n) pdl_wait();   // t of the shrink kernel
 
     // epilogue: the cluster's CTAs share its tiles; partial sums in rank order
-    const int m = threadIdx.x >> 4, c = threadIdx.x & 15;
-    if (m < a.M) {
+    // a thread keeps its row: kLrThreads / kCols rows a step
+    constexpr int kStep = kLrThreads / kCols;
+#pragma unroll 1
+    for (int m = threadIdx.x / kCols; m < min(a.M, kRows); m += kStep) {
+        const int c = threadIdx.x % kCols;
         int r;
         const int ad = lora_of(a, m, &r, false);
         const float* t = a.t + (size_t)m * a.max_rank;
         const void* Bp = ad >= 0 ? a.B[ad] : nullptr;
 #pragma unroll 1
         for (int it = rank; it < my_tiles; it += nsplit) {
-            const int n = (group + it * groups) * kLrCols + c;
+            const int n = (group + it * groups) * kCols + c;
             if (n >= a.N) continue;
             float s = 0.f;
-            for (int p = 0; p < nsplit; ++p) s += *(cl.map_shared_rank(lr_smem, p) + it * 256 + threadIdx.x);
+            for (int p = 0; p < nsplit; ++p) s += *(cl.map_shared_rank(lr_smem, p) + it * kOut + m * kCols + c);
             s *= a.row_scales ? __ldg(a.row_scales + n) : a.tscale;
             a.y[(size_t)m * a.N + n] = s + lora_dot(Bp, (size_t)n * r, t, r, a.f16);
         }
@@ -306,14 +311,15 @@ static tvb_status launch_rows_kernel(const LoraArgs& a, bool dependent, cudaStre
     const auto kernel = lora_rows_kernel<W8, WIDE>;
     constexpr int kBlock = W8 ? 64 : 32, kMax = lr_slice(W8, WIDE);
     LoraRowsPlan plan;
-    plan.tiles = (a.N + kLrCols - 1) / kLrCols;
+    constexpr int kCols = lr_cols(W8), kOut = kCols * (WIDE ? 16 : 8);
+    plan.tiles = (a.N + kCols - 1) / kCols;
     // CTAs a cluster: a power of two, which clusters pack best into the GPU, until the warps' slices hold K in one pass
     int nsplit = 1;
     while (nsplit < kLrMaxSplit && nsplit * kLrWarps * kMax < a.K) nsplit *= 2;
     plan.passes = (a.K + nsplit * kLrWarps * kMax - 1) / (nsplit * kLrWarps * kMax);
     const int per = (a.K + plan.passes * nsplit * kLrWarps - 1) / (plan.passes * nsplit * kLrWarps);
     plan.slice = (per + kBlock - 1) / kBlock * kBlock;
-    constexpr int kWarpSums = 2 * kLrBatch * kLrWarps * kLrMaxRows * 17;
+    constexpr int kWarpSums = 2 * lr_batch(W8) * kLrWarps * (kOut / kCols) * (kCols + 1);
 
     cudaLaunchConfig_t cfg = {};
     cfg.blockDim = dim3(kLrThreads);
@@ -341,11 +347,11 @@ static tvb_status launch_rows_kernel(const LoraArgs& a, bool dependent, cudaStre
         resident[dev][nsplit] = std::max(1, n);
     }
     // as many groups as are resident, or more where a group's sums would not fit
-    const int fit = (kSmem / 4 - kWarpSums) / 256;
+    const int fit = (kSmem / 4 - kWarpSums) / kOut;
     const int groups = std::min(plan.tiles, std::max(resident[dev][nsplit], (plan.tiles + fit - 1) / fit));
     plan.most = (plan.tiles + groups - 1) / groups;
     cfg.gridDim = dim3((unsigned)(groups * nsplit));
-    cfg.dynamicSmemBytes = (size_t)(plan.most * 256 + kWarpSums) * 4;
+    cfg.dynamicSmemBytes = (size_t)(plan.most * kOut + kWarpSums) * 4;
     cfg.numAttrs = dependent ? 2 : 1;
     TVB_CUDA(cudaLaunchKernelEx(&cfg, kernel, a, plan));
     return check_launch("lora_rows_kernel");

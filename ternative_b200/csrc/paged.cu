@@ -46,6 +46,14 @@ tvb_status paged_batch_arg(const char* who, const tvb_paged_batch* b, const tvb_
     return TVB_OK;
 }
 
+// One-time set-up may come while the caller captures a stream, where it would end
+// the capture; it touches no stream.
+struct OutsideCapture {
+    cudaStreamCaptureMode mode = cudaStreamCaptureModeRelaxed;
+    OutsideCapture() { cudaThreadExchangeStreamCaptureMode(&mode); }
+    ~OutsideCapture() { cudaThreadExchangeStreamCaptureMode(&mode); }
+};
+
 static std::mutex g_pool_mutex;
 static cudaMemPool_t g_pools[kMaxDevices];
 
@@ -56,6 +64,7 @@ tvb_status Workspace::get(size_t bytes) {
     {
         std::lock_guard<std::mutex> lock(g_pool_mutex);
         if (!g_pools[dev]) {
+            OutsideCapture outside;
             cudaMemPoolProps props = {};
             props.allocType = cudaMemAllocationTypePinned;
             props.location.type = cudaMemLocationTypeDevice;
@@ -83,6 +92,7 @@ tvb_status allow_smem(const void* kernel, int bytes, int (&set)[kMaxDevices]) {
     TVB_REQUIRE(dev >= 0 && dev < kMaxDevices, "device %d", dev);
     std::lock_guard<std::mutex> lock(g_smem_mutex);
     if (bytes > set[dev]) {
+        OutsideCapture outside;
         TVB_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes));
         set[dev] = bytes;
     }
