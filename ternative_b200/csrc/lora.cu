@@ -1,13 +1,18 @@
 // Adapters of many requests beside a shared projection (tvb_matmul_lora):
 //   y[m] = W x[m] + scale_a B_a (A_a x[m]),  a = adapter[m]
 //
-// Up to 16 rows (a decode batch) the call is bound by the bytes of W and of the
-// adapters in use, each read once:
+// Up to 64 rows (a decode batch) the call is bound by the bytes of W and of the
+// adapters in use, and by how fast weights reach the warps from L2:
 //
 // lora_shrink_kernel: t[m] = scale_a A_a x[m], a warp a (row, rank index).
-// lora_rows_kernel: W streamed once for all rows through mma.sync m16n8k16 (rows
+// lora_rows_kernel: W streamed once for 16 rows through mma.sync m16n8k16 (rows
 // of x are the 16-row operand, 8 weight rows the other; a memory-bound product
-// that needs no more than the legacy tensor path).  x is split into F16 hi + lo
+// that needs no more than the legacy tensor path).  More rows are blocks of 16 that
+// share the GPU and walk the weights together, so that HBM gives them once and L2
+// the other times.  2560 -> 6912 with 8 adapters among 16, 64, 96 rows: 18.7, 42,
+// 57 us; the many-rows kernels take 80, 83, 84 us of rows mixed so (50 of them for
+// what adapters cost there, less where a chunk's rows share one) and 29, 31, 31 us
+// without adapters against 13.7, 34, 47: hence 64.  x is split into F16 hi + lo
 // planes with a power-of-two factor a row, so products are F32-faithful; each
 // warp keeps its K slice of x in registers for the whole kernel and weights come
 // straight from global memory in the operand's layout: with k permuted so that a
@@ -35,7 +40,8 @@ __host__ __device__ constexpr int lr_slice(bool w8, bool wide) { return w8 || !w
 __host__ __device__ constexpr int lr_cols(bool w8) { return w8 ? 32 : 16; }
 __host__ __device__ constexpr int lr_batch(bool w8) { return w8 ? 2 : 4; }   // tiles between two barriers of the CTA
 constexpr int kLrMaxSplit = 8;     // CTAs of a cluster
-constexpr int kLrMaxRows = 16;
+constexpr int kLrRows = 16;        // rows of x a CTA
+constexpr int kLrMaxRows = 64;
 
 // A CTA takes 4 rank indexes of a row; its 8 warps cut K (8 k a lane), so that all
 // loads of a short K are in flight at once.
@@ -150,7 +156,7 @@ lora_rows_kernel(const __grid_constant__ LoraArgs a, const __grid_constant__ Lor
     constexpr int kBlocks = lr_slice(W8, WIDE) / kBlock;     // loads a weight row
     constexpr int kSteps = E / 4;                      // MMA steps a load
     constexpr int kHalves = WIDE ? 2 : 1;
-    constexpr int kCols = lr_cols(W8), kGroups = kCols / 8, kBatch = lr_batch(W8), kRows = 8 * kHalves;
+    constexpr int kCols = lr_cols(W8), kGroups = kCols / 8, kBatch = lr_batch(W8), kRows = kLrRows / 2 * kHalves;
     constexpr int kRed = kRows * (kCols + 1);          // a warp's sums of a tile
     constexpr int kOut = kRows * kCols;
     extern __shared__ __align__(16) float lr_smem[];   // [tile][rows][weight rows], then the warps' sums
@@ -158,6 +164,7 @@ lora_rows_kernel(const __grid_constant__ LoraArgs a, const __grid_constant__ Lor
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, q = lane & 3;
     const int rank = (int)cl.block_rank(), nsplit = (int)cl.num_blocks();
     const int group = (int)(blockIdx.x / nsplit), groups = (int)(gridDim.x / nsplit);
+    const int mb = blockIdx.y * kLrRows, M = min(a.M - mb, kLrRows);   // this CTA's rows
     const int my_tiles = plan.tiles > group ? (plan.tiles - group + groups - 1) / groups : 0;
     float* warps = lr_smem + plan.most * kOut;         // [2][kBatch tiles][8 warps][rows][weight rows + 1]
     const int64_t row_bytes = (int64_t)a.K * (W8 ? 1 : 2);
@@ -198,10 +205,10 @@ lora_rows_kernel(const __grid_constant__ LoraArgs a, const __grid_constant__ Lor
             float mx = 0.f;
 #pragma unroll
             for (int i = 0; i < kBlocks; ++i) {
-                const bool in = m < a.M && ((in_k >> i) & 1u);
+                const bool in = m < M && ((in_k >> i) & 1u);
 #pragma unroll
                 for (int e = 0; e < E; e += 4) {
-                    const float4 x = in ? __ldg(reinterpret_cast<const float4*>(a.x + (size_t)m * a.K + k0 + i * kBlock + e))
+                    const float4 x = in ? __ldg(reinterpret_cast<const float4*>(a.x + (size_t)(mb + m) * a.K + k0 + i * kBlock + e))
                                         : make_float4(0.f, 0.f, 0.f, 0.f);
                     v[i][e] = x.x, v[i][e + 1] = x.y, v[i][e + 2] = x.z, v[i][e + 3] = x.w;
                     mx = fmaxf(mx, fmaxf(fmaxf(fabsf(x.x), fabsf(x.y)), fmaxf(fabsf(x.z), fabsf(x.w))));
@@ -287,11 +294,11 @@ lora_rows_kernel(const __grid_constant__ LoraArgs a, const __grid_constant__ Lor
     // a thread keeps its row: kLrThreads / kCols rows a step
     constexpr int kStep = kLrThreads / kCols;
 #pragma unroll 1
-    for (int m = threadIdx.x / kCols; m < min(a.M, kRows); m += kStep) {
+    for (int m = threadIdx.x / kCols; m < M; m += kStep) {
         const int c = threadIdx.x % kCols;
         int r;
-        const int ad = lora_of(a, m, &r, false);
-        const float* t = a.t + (size_t)m * a.max_rank;
+        const int ad = lora_of(a, mb + m, &r, false);
+        const float* t = a.t + (size_t)(mb + m) * a.max_rank;
         const void* Bp = ad >= 0 ? a.B[ad] : nullptr;
 #pragma unroll 1
         for (int it = rank; it < my_tiles; it += nsplit) {
@@ -300,7 +307,7 @@ lora_rows_kernel(const __grid_constant__ LoraArgs a, const __grid_constant__ Lor
             float s = 0.f;
             for (int p = 0; p < nsplit; ++p) s += *(cl.map_shared_rank(lr_smem, p) + it * kOut + m * kCols + c);
             s *= a.row_scales ? __ldg(a.row_scales + n) : a.tscale;
-            a.y[(size_t)m * a.N + n] = s + lora_dot(Bp, (size_t)n * r, t, r, a.f16);
+            a.y[(size_t)(mb + m) * a.N + n] = s + lora_dot(Bp, (size_t)n * r, t, r, a.f16);
         }
     }
     if (nsplit > 1) cl.sync();   // no CTA leaves while another reads its sums
@@ -335,7 +342,7 @@ static tvb_status launch_rows_kernel(const LoraArgs& a, bool dependent, cudaStre
     // clusters that fit the GPU at once: one more would be a second wave
     static int resident[kMaxDevices][kLrMaxSplit + 1];
     static int set[kMaxDevices];
-    constexpr int kSmem = 100 * 1024;
+    constexpr int kSmem = (WIDE ? 200 : 100) * 1024;   // one CTA an SM, or two
     TVB_TRY(allow_smem(reinterpret_cast<const void*>(kernel), kSmem, set));
     int dev = 0;
     TVB_CUDA(cudaGetDevice(&dev));
@@ -348,9 +355,10 @@ static tvb_status launch_rows_kernel(const LoraArgs& a, bool dependent, cudaStre
     }
     // as many groups as are resident, or more where a group's sums would not fit
     const int fit = (kSmem / 4 - kWarpSums) / kOut;
-    const int groups = std::min(plan.tiles, std::max(resident[dev][nsplit], (plan.tiles + fit - 1) / fit));
+    const int blocks = (a.M + kLrRows - 1) / kLrRows;
+    const int groups = std::min(plan.tiles, std::max(std::max(1, resident[dev][nsplit] / blocks), (plan.tiles + fit - 1) / fit));
     plan.most = (plan.tiles + groups - 1) / groups;
-    cfg.gridDim = dim3((unsigned)(groups * nsplit));
+    cfg.gridDim = dim3((unsigned)(groups * nsplit), (unsigned)blocks);
     cfg.dynamicSmemBytes = (size_t)(plan.most * kOut + kWarpSums) * 4;
     cfg.numAttrs = dependent ? 2 : 1;
     TVB_CUDA(cudaLaunchKernelEx(&cfg, kernel, a, plan));

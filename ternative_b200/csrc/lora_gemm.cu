@@ -538,7 +538,7 @@ lora_gemm_kernel(const __grid_constant__ LgMaps maps, const __grid_constant__ Lo
                 }
             } else if (live) {
                 float* to = a.y + (size_t)m * a.N + n0;
-                if (n0 + 128 <= a.N && a.N % 4 == 0) {
+                if (n0 + 128 <= a.N && a.N % 4 == 0 && (reinterpret_cast<uintptr_t>(a.y) & 15) == 0) {
 #pragma unroll
                     for (int i = 0; i < 64; i += 2) {
                         const float2 x = lg_unpack2(acc[i]), y = lg_unpack2(acc[i + 1]);
@@ -596,7 +596,7 @@ __global__ void __launch_bounds__(256) lora_join_kernel(const __grid_constant__ 
 static size_t align256(size_t n) { return (n + 255) & ~(size_t)255; }
 
 tvb_status lora_many_rows(LoraArgs a, cudaStream_t st) {
-    TVB_REQUIRE(a.K <= 16384, "matmul_lora: K=%d with %d rows (at most 16384 above 16 rows)", a.K, a.M);
+    TVB_REQUIRE(a.K <= 16384, "matmul_lora: K=%d with %d rows (at most 16384 above 64 rows)", a.K, a.M);
     LgPlan plan = {};
     plan.mt = (a.M + kLgRows - 1) / kLgRows;
     plan.tiles = plan.mt * ((a.N + kLgCols - 1) / kLgCols);

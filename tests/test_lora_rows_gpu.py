@@ -213,3 +213,117 @@ def test_a_layers_serving_step(be, new, kv):
     want, _ = o(out.reshape(T, -1), ids)
     # four operators of relative error below 4e-6 each (and a softmax that passes its inputs' on): 2e-5
     assert float((z - want).norm() / want.norm()) < 2e-5
+
+
+# Around the rows where the kernels change over, and several blocks of rows at once.
+MORE = [
+    (63, 1008, 333, "i8tensor", [16, 3], F32),
+    (64, 2560, 2560, "f16", [16] * 8, F32),
+    (65, 640, 1025, "i8row", [8, 8, 8, 8], F16),
+    (70, 512, 130, "f16", [12, 64], F32),
+    (100, 264, 700, "f16", [200, 7, 1], F16),
+    (33, 6912, 2560, "i8row", [64, 8], F32),
+    (3, 14336, 96, "f16", [16, 4], F32),
+    (16, 14336, 64, "i8row", [8], F32),
+    (49, 20000, 40, "f16", [4, 9], F32),
+    (1500, 128, 520, "f16", [16, 1], F16),
+]
+
+
+@pytest.mark.parametrize("case", MORE, ids=lambda c: f"{c[0]}x{c[1]}x{c[2]}-{c[3]}-r{c[4][0]}x{len(c[4])}")
+@pytest.mark.parametrize("order", ["mixed", "runs"])
+def test_matmul_lora_rows_in_blocks(be, case, order):
+    test_matmul_lora(be, case, order)
+
+
+def test_many_rows_of_any_magnitude(be):
+    test_rows_of_any_magnitude(be, 100)
+
+
+def test_many_rows_ids_out_of_range_and_no_adapters(be):
+    test_ids_out_of_range_and_no_adapters(be, 80)
+
+
+@pytest.mark.parametrize("M", [40, 90])
+def test_one_bad_row_of_many(be, M):
+    test_a_row_that_is_not_finite_stays_alone(be, M)
+
+
+@pytest.mark.parametrize("M", [2, 16, 40, 200])
+@pytest.mark.parametrize("bad", [math.nan, math.inf])
+def test_an_adapter_that_is_not_finite_stays_alone(be, M, bad):
+    """A request's broken adapter spoils its own rows and no other's."""
+    p = Projection(256, 300, "f16", [16, 8, 4], F32, seed=5)
+    x = torch.randn(M, 256, generator=torch.Generator().manual_seed(M)).cuda()
+    ids = (torch.arange(M) % 4 - 1).to(torch.int32)
+    from ternative_b200 import LoraTable
+    want = project(be, p, x, ids.cuda()).cpu()
+    for which in ("A", "B"):
+        A, B = [a.clone().cuda() for a in p.A], [b.clone().cuda() for b in p.B]
+        (A if which == "A" else B)[0].fill_(bad)
+        keep = p.table
+        p.table = LoraTable(A, B, torch.tensor(p.ranks, dtype=torch.int32).cuda(), p.scale.cuda(), max_rank=16)
+        y = project(be, p, x, ids.cuda()).cpu()
+        p.table = keep
+        assert torch.equal(y[ids != 0], want[ids != 0])
+        assert not torch.isfinite(y[ids == 0]).any()
+
+
+@pytest.mark.parametrize("M", [3, 30, 90])
+def test_output_at_any_address(be, M):
+    p = Projection(256, 512, "f16", [8], F32, seed=6)
+    x = torch.randn(M, 256, device="cuda")
+    ids = torch.zeros(M, dtype=torch.int32, device="cuda")
+    want = project(be, p, x, ids)
+    buf = torch.full((M * 512 + 8,), 7.0, device="cuda")
+    y = buf[1:1 + M * 512].view(M, 512)
+    be.matmul_lora_d(y, x, M, 256, p.weight, 512, p.table, ids)
+    torch.cuda.synchronize()
+    assert torch.equal(y, want) and float(buf[0]) == 7.0 and (buf[1 + M * 512:] == 7.0).all()
+
+
+@pytest.mark.parametrize("M", [4, 40, 100])
+def test_an_adapter_of_misaligned_rows_is_reported(be, M):
+    """Pointers that the kernels could not load from are reported and left out."""
+    from ternative_b200 import LoraTable
+    p = Projection(256, 64, "f16", [8, 8], F32, seed=7)
+    x = torch.randn(M, 256, device="cuda")
+    ids = torch.arange(M) % 2
+    odd = torch.zeros(8 * 256 + 1, device="cuda")
+    p.table = LoraTable([p.A[0].cuda(), odd[1:].view(8, 256)], [b.cuda() for b in p.B],
+                        torch.tensor(p.ranks, dtype=torch.int32).cuda(), p.scale.cuda(), max_rank=8)
+    st = torch.zeros(1, dtype=torch.int32, device="cuda")
+    y = project(be, p, x, ids.to(torch.int32).cuda(), st).cpu().double()
+    assert int(st.item()) == 2
+    ref, tol = p(x.cpu(), torch.where(ids == 1, -1, ids))
+    assert ((y - ref).abs() <= tol).all()
+
+
+@pytest.mark.parametrize("M", [2, 100])
+def test_first_call_inside_a_capture(M):
+    """No call before the capture: one-time set-up comes inside it, in a process of its own."""
+    import os
+    import subprocess
+    import sys
+    code = f"""
+import torch
+from ternative_b200 import CUDABackend, DeviceWeight, LoraTable, TVB_F16
+be = CUDABackend()
+w = torch.randn(200, 256, device='cuda').half()
+x = torch.randn({M}, 256, device='cuda')
+A, B = [torch.randn(8, 256, device='cuda')], [torch.randn(200, 8, device='cuda')]
+tab = LoraTable(A, B, torch.full((1,), 8, dtype=torch.int32, device='cuda'), torch.ones(1, device='cuda'), 8)
+ids = torch.zeros({M}, dtype=torch.int32, device='cuda')
+y = torch.empty({M}, 200, device='cuda')
+s, g = torch.cuda.Stream(), torch.cuda.CUDAGraph()
+torch.cuda.synchronize()
+with torch.cuda.graph(g, stream=s):
+    be.matmul_lora_d(y, x, {M}, 256, DeviceWeight(w.data_ptr(), TVB_F16), 200, tab, ids,
+                     stream=torch.cuda.current_stream().cuda_stream)
+g.replay()
+torch.cuda.synchronize()
+ref = x.double() @ w.double().T + (x.double() @ A[0].double().T) @ B[0].double().T
+assert float((y - ref).norm() / ref.norm()) < 4e-6
+"""
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    subprocess.run([sys.executable, "-c", code], check=True, cwd=root, timeout=300)
