@@ -37,7 +37,7 @@ def build(reference: bool = True) -> None:
     """Compile the restatement (and, where the reference sources exist, the
     reference harness) with oracle/Makefile."""
     targets = ["libtvoracle.so"]
-    if reference and os.path.isdir(REFERENCE_SRC):
+    if reference and os.path.isfile(os.path.join(REFERENCE_SRC, "src", "model.cpp")):
         targets += ["ref", "dropin"]
     subprocess.run(["make", "-s", "-C", HERE, f"REF={REFERENCE_SRC}", *targets], check=True)
 
