@@ -7,7 +7,7 @@
 // 2^(m_old - m_new) when it grows.
 //
 // paged_rows_kernel: a CTA takes its run of tiles (attn_schedule: RB query rows of
-// one KV head of one sequence against 8 keys a warp and tile); per piece its warps take
+// one KV head of one sequence against 8 keys of each warp); per piece its warps take
 // batches of 8 keys in turn and merge at the end.  K and V rows pass
 // through a ring of cp.async stages private to each warp, so no warp waits for
 // another while it streams; each lane owns head_dim / 32 dimensions.  The RB x 8
@@ -16,6 +16,7 @@
 #include "attn_paged.h"
 
 #include <algorithm>
+#include <climits>
 
 namespace tvb {
 
@@ -96,7 +97,7 @@ __device__ __forceinline__ void merge_warps(const PagedAttnArgs& a, const AttnPi
 #pragma unroll
         for (int w = 0; w < WARPS; ++w) {
             const float* x = red + (w * RB + r) * kW;
-            const float c = x[HD] == -INFINITY ? 0.f : exp2f(x[HD] - M);
+            const float c = x[HD] == -INFINITY ? (x[HD + 1] == 0.f ? 0.f : 1.f) : exp2f(x[HD] - M);   // no maximum but a sum: NaN
             if (c != 0.f) {
                 L = fmaf(x[HD + 1], c, L);
 #pragma unroll
@@ -280,8 +281,8 @@ __device__ __forceinline__ void rows_piece(const PagedAttnArgs& a, const AttnPie
 
 // ---- three to sixteen rows over an F16 cache: mma.sync ------------------------------
 // The rows are the 16-row operand of mma.sync m16n8k16 (a memory-bound product: the
-// legacy tensor path keeps up with memory where the FP32 pipe does not, 55 against
-// 52 us for 32 sequences).  q and p are split into F16 hi + lo planes, K and V rows
+// legacy tensor path keeps up with memory where the FP32 pipe does not, 48 against
+// 62 us for 32 sequences of up to 4096 keys with 20/5 heads).  q and p are split into F16 hi + lo planes, K and V rows
 // come from shared memory by ldmatrix.  Every 16 keys make a fresh product that is
 // added to F32 registers, so the tensor core's truncation does not add up.
 template <int HD, int RB>
@@ -653,7 +654,9 @@ extern "C" tvb_status tvb_attention_paged(float* out, int ldo, float* lse, const
     const int64_t span = window ? std::min<int64_t>(a.s.max_kv, (int64_t)window + a.s.max_new) : a.s.max_kv;
     // many sequences or row blocks fill the SMs evenly enough block by block
     const int64_t blocks = ((int64_t)a.s.n_tokens * a.group / (tensor ? 128 : 8) + a.s.n_seqs) * nkv;
-    a.balanced = a.s.n_seqs <= kAttnSeqs && span > kWholeKeys && blocks <= 64 * num_sms();
+    // (the schedule's sums are 32 bits; a tile is 48 keys or more)
+    a.balanced = a.s.n_seqs <= kAttnSeqs && span > kWholeKeys && blocks <= 64 * num_sms() &&
+                 blocks / nkv * (span / 48 + 4) < INT_MAX;
     if (tensor) {
         TVB_TRY(paged_attn_chunk(a, hd, f16, st));
     } else if (hd == 128) {

@@ -187,6 +187,10 @@ again:
 // neighbours never overlap and floor(T g / RB) + n of them are enough.
 template <int RB, int TK, int NT>
 __device__ __forceinline__ bool attn_block(const PagedAttnArgs& a, int align, AttnPiece* p) {
+    if ((blockIdx.x | blockIdx.y) == 0) {   // (a sequence that cannot be is no CTA's)
+        for (int b = threadIdx.x; b < a.s.n_seqs; b += NT)
+            if (!seq_view(a.s, b).ok) report_bad(a.status);
+    }
     int started = 0;
     for (int b0 = 0; b0 < a.s.n_seqs; b0 += NT) {
         const int b = b0 + (int)threadIdx.x;
@@ -199,11 +203,8 @@ __device__ __forceinline__ bool attn_block(const PagedAttnArgs& a, int align, At
     const int b = started - 1;
     const SeqView v = seq_view(a.s, b);
     const int i = (int)blockIdx.x - (int)(((int64_t)v.row0 * a.group) / RB) - b;
-    if (!v.ok) {
-        if (threadIdx.x == 0) report_bad(a.status);
-        return false;
-    }
-    if (i * RB >= v.n * a.group) return false;
+    if (!v.ok || i < 0) return false;   // i < 0: starts that go back
+    if ((int64_t)i * RB >= (int64_t)v.n * a.group) return false;
     p->b = b;
     p->tok0 = v.row0;
     p->pos0 = v.pos0;

@@ -11,8 +11,8 @@
 // is off by 1e-3).
 //
 // Memory bound: q is read and written once, k and v are read once and written
-// in the cache's type.  A CTA takes a few tokens: their cosines and sines go to
-// shared memory once (all heads share them), then every thread moves items of 8
+// in the cache's type.  A CTA takes a token: its cosines and sines go to shared
+// memory once (all heads share them), then every thread moves items of 8
 // dimensions as two float4.
 #include <cmath>
 
@@ -22,7 +22,6 @@ namespace tvb {
 
 constexpr int kRpThreads = 256;
 constexpr int kRpMaxPairs = 128;
-constexpr int kRpTokens = 4;   // tokens a CTA, at most
 
 struct RopeArgs {
     const float *q, *k, *v;
@@ -30,7 +29,6 @@ struct RopeArgs {
     int ldq, ldk, ldv, ldqo;
     int nh, nkv, hd;
     int rot, interleaved;
-    int tokens;      // a CTA
     int f16;         // cache type
     float m;
     unsigned* status;
@@ -52,54 +50,48 @@ __device__ __forceinline__ void rp_store(unsigned char* p, int elem, float4 x, b
 }
 
 __global__ void __launch_bounds__(kRpThreads) rope_append_kernel(const __grid_constant__ RopeArgs a) {
-    __shared__ float2 cs[kRpTokens][kRpMaxPairs];
-    __shared__ int64_t s_off[kRpTokens];   // the token's cache row; -1: skipped
-    __shared__ int s_pos[kRpTokens];
-    const int tid = threadIdx.x;
-    const int t0 = blockIdx.x * a.tokens;
-    const int nt = min(a.tokens, a.s.n_tokens - t0);
+    __shared__ float2 cs[kRpMaxPairs];
+    __shared__ int64_t s_off;   // the token's cache row; -1: skipped
+    __shared__ int s_pos;
+    const int tid = threadIdx.x, row = blockIdx.x;
 
-    // sequence of each token: how many sequences end at or before it
-    for (int j = 0; j < nt; ++j) {
-        int ended = 0;
-        for (int b0 = 0; b0 < a.s.n_seqs; b0 += kRpThreads) {
-            const int b = b0 + tid;
-            const int n = __syncthreads_count(b < a.s.n_seqs && __ldg(a.s.cu + b + 1) <= t0 + j);
-            ended += n;
-            if (n < kRpThreads) break;
+    // the token's sequence: how many end at or before it
+    int ended = 0;
+    for (int b0 = 0; b0 < a.s.n_seqs; b0 += kRpThreads) {
+        const int b = b0 + tid;
+        const int n = __syncthreads_count(b < a.s.n_seqs && __ldg(a.s.cu + b + 1) <= row);
+        ended += n;
+        if (n < kRpThreads) break;
+    }
+    if (tid == 0) {
+        int64_t off = -1;
+        int pos = 0;
+        if (ended < a.s.n_seqs) {   // else: behind the last sequence
+            const SeqView v = seq_view(a.s, ended);
+            pos = v.pos0 + (row - v.row0);
+            if (v.ok && row >= v.row0 && row - v.row0 < v.n)
+                off = paged_offset(a.kv, a.s.table + (size_t)ended * a.s.table_ld, pos);
+            if (off < 0) report_bad(a.status);
         }
-        if (tid == 0) {
-            int64_t off = -1;
-            int pos = 0;
-            if (ended < a.s.n_seqs) {   // else: behind the last sequence
-                const SeqView v = seq_view(a.s, ended);
-                pos = v.pos0 + (t0 + j - v.row0);
-                if (v.ok && t0 + j >= v.row0) off = paged_offset(a.kv, a.s.table + (size_t)ended * a.s.table_ld, pos);
-                if (off < 0) report_bad(a.status);
-            }
-            s_off[j] = off;
-            s_pos[j] = pos;
-        }
+        s_off = off;
+        s_pos = pos;
     }
     __syncthreads();
+    const int64_t off = s_off;
+    if (off < 0) return;
     const int pairs = a.rot >> 1;
-    for (int i = tid; i < nt * pairs; i += kRpThreads) {
-        const int j = i / pairs, p = i - j * pairs;
-        const double x = (double)s_pos[j] * a.turns[p];
+    for (int p = tid; p < pairs; p += kRpThreads) {
+        const double x = (double)s_pos * a.turns[p];
         float sn, c;
         sincospif(2.0f * (float)(x - rint(x)), &sn, &c);
-        cs[j][p] = make_float2(c * a.m, sn * a.m);
+        cs[p] = make_float2(c * a.m, sn * a.m);
     }
     __syncthreads();
 
     const int per_head = a.hd >> 3;
     const int items = (a.nh + 2 * a.nkv) * per_head;
-    for (int i = blockIdx.y * kRpThreads + tid; i < nt * items; i += gridDim.y * kRpThreads) {
-        const int j = i / items, it = i - j * items;
-        const int64_t off = s_off[j];
-        if (off < 0) continue;
+    for (int it = tid; it < items; it += kRpThreads) {
         const int h = it / per_head, c = it - h * per_head;
-        const int row = t0 + j;
         const bool is_q = h < a.nh, is_k = !is_q && h < a.nh + a.nkv;
         const bool turn = !(!is_q && !is_k) && c < (a.rot >> 3);
         const int o0 = turn && !a.interleaved ? 4 * c : 8 * c;
@@ -110,8 +102,8 @@ __global__ void __launch_bounds__(kRpThreads) rope_append_kernel(const __grid_co
         float4 x = *reinterpret_cast<const float4*>(src + o0);
         float4 y = *reinterpret_cast<const float4*>(src + o1);
         if (turn) {
-            const float4 p = *reinterpret_cast<const float4*>(&cs[j][4 * c]);
-            const float4 r = *reinterpret_cast<const float4*>(&cs[j][4 * c + 2]);
+            const float4 p = *reinterpret_cast<const float4*>(&cs[4 * c]);
+            const float4 r = *reinterpret_cast<const float4*>(&cs[4 * c + 2]);
             // cosines p.x p.z r.x r.z, sines p.y p.w r.y r.w of pairs 4c .. 4c + 3
             if (a.interleaved) {
                 x = make_float4(x.x * p.x - x.y * p.y, x.y * p.x + x.x * p.y, x.z * p.z - x.w * p.w,
@@ -224,11 +216,6 @@ extern "C" tvb_status tvb_rope_append_paged(float* q_out, int ldqo, const float*
     a.status = status;
     a.m = 1.0f;
     if (a.rot) rope_turns(*rope, a.turns, &a.m);
-    const int T = a.s.n_tokens;
-    const int items = (nh + 2 * nkv) * (hd / 8);
-    a.tokens = 1;
-    const dim3 grid((unsigned)((T + a.tokens - 1) / a.tokens), 1);
-    (void)items;
-    rope_append_kernel<<<grid, kRpThreads, 0, as_stream(stream)>>>(a);
+    rope_append_kernel<<<(unsigned)a.s.n_tokens, kRpThreads, 0, as_stream(stream)>>>(a);
     return check_launch("rope_append_kernel");
 }
