@@ -6,8 +6,9 @@
 //
 // lora_shrink_kernel: t[m] = scale_a A_a x[m], a warp a (row, rank index).
 // lora_rows_kernel: W streamed once for 16 rows through mma.sync m16n8k16 (rows
-// of x are the 16-row operand, 8 weight rows the other; a memory-bound product
-// that needs no more than the legacy tensor path).  More rows are blocks of 16 that
+// of x are the 16-row operand and 8 weight rows the other, or, up to 8 rows, 16
+// weight rows and x's; a memory-bound product that needs no more than the legacy
+// tensor path).  More rows are blocks of 16 that
 // share the GPU and walk the weights together, so that HBM gives them once and L2
 // the other times.  2560 -> 6912 with 8 adapters among 16, 64, 96 rows: 18.7, 42,
 // 57 us; the many-rows kernels take 80, 83, 84 us of rows mixed so (50 of them for
@@ -38,7 +39,13 @@ __host__ __device__ constexpr int lr_slice(bool w8, bool wide) { return w8 || !w
 // Weight rows a tile: what keeps enough loads under way (a warp's slice of an INT8
 // row is half as many bytes).
 __host__ __device__ constexpr int lr_cols(bool w8) { return w8 ? 32 : 16; }
+// Distance of x's rows in a warp's sums of a tile: no bank conflicts as they are stored.
+__host__ __device__ constexpr int lr_line(bool w8, bool wide) { return lr_cols(w8) + (wide ? 1 : 4); }
 __host__ __device__ constexpr int lr_batch(bool w8) { return w8 ? 2 : 4; }   // tiles between two barriers of the CTA
+// Tiles of weights under way in a warp's registers.  INT8 tiles are half the bytes;
+// where one CTA has the SM to itself there are registers for two (64 rows 6912 ->
+// 2560 51 -> 45 us, 16 rows 15.7 -> 14.2; F16 tiles gain nothing).
+__host__ __device__ constexpr int lr_depth(bool w8, bool wide) { return w8 && wide ? 2 : 1; }
 constexpr int kLrMaxSplit = 8;     // CTAs of a cluster
 constexpr int kLrRows = 16;        // rows of x a CTA
 constexpr int kLrMaxRows = 64;
@@ -157,8 +164,11 @@ lora_rows_kernel(const __grid_constant__ LoraArgs a, const __grid_constant__ Lor
     constexpr int kSteps = E / 4;                      // MMA steps a load
     constexpr int kHalves = WIDE ? 2 : 1;
     constexpr int kCols = lr_cols(W8), kGroups = kCols / 8, kBatch = lr_batch(W8), kRows = kLrRows / 2 * kHalves;
-    constexpr int kRed = kRows * (kCols + 1);          // a warp's sums of a tile
+    constexpr int kLine = lr_line(W8, WIDE);
+    constexpr int kRed = kRows * kLine;                // a warp's sums of a tile
     constexpr int kOut = kRows * kCols;
+    constexpr int kDepth = lr_depth(W8, WIDE);
+    static_assert(kBatch % kDepth == 0, "a tile keeps its registers");
     extern __shared__ __align__(16) float lr_smem[];   // [tile][rows][weight rows], then the warps' sums
     cg::cluster_group cl = cg::this_cluster();
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, q = lane & 3;
@@ -178,10 +188,10 @@ lora_rows_kernel(const __grid_constant__ LoraArgs a, const __grid_constant__ Lor
         for (int i = 0; i < kBlocks; ++i) in_k |= (unsigned)(i * kBlock < plan.slice && k0 + i * kBlock < a.K) << i;
 
         // this warp's weights of the tile's rows: 16 bytes of row g of each 8 a load
-        uint4 w[kGroups][kBlocks];
+        uint4 w[kDepth][kGroups][kBlocks];
         int n = group * kCols + g;
         const unsigned char* wp = static_cast<const unsigned char*>(a.w) + n * row_bytes + (int64_t)k0 * (W8 ? 1 : 2);
-        auto request = [&]() {
+        auto request = [&](uint4 (&w)[kGroups][kBlocks]) {
 #pragma unroll
             for (int h = 0; h < kGroups; ++h) {
                 const bool row = n + 8 * h < a.N;
@@ -193,7 +203,9 @@ lora_rows_kernel(const __grid_constant__ LoraArgs a, const __grid_constant__ Lor
             n += groups * kCols;
             wp += groups * kCols * row_bytes;
         };
-        if (my_tiles) request();
+#pragma unroll
+        for (int d = 0; d < kDepth; ++d)
+            if (d < my_tiles) request(w[d]);
 
         // x of rows g (and g + 8), this thread's k, as hi + lo with a factor a row
         uint32_t xh[kBlocks][kSteps][2 * kHalves], xl[kBlocks][kSteps][2 * kHalves];
@@ -235,48 +247,68 @@ lora_rows_kernel(const __grid_constant__ LoraArgs a, const __grid_constant__ Lor
                     }
         }
 
+        if constexpr (!WIDE) {   // D's columns are x's rows: their factors
+            const float mine = f[0];
+            f[0] = __shfl_sync(0xffffffffu, mine, 8 * q);
+            f[1] = __shfl_sync(0xffffffffu, mine, 8 * q + 4);
+        }
+        auto step = [&](const uint4& w, int s, uint32_t (&b)[2]) {   // a thread's fragment of 16 k
+            const uint32_t ww[4] = {w.x, w.y, w.z, w.w};
+            if constexpr (W8) i8x4_to_h2(ww[s], &b[0], &b[1]);
+            else b[0] = ww[2 * s], b[1] = ww[2 * s + 1];
+        };
+
         // kBatch tiles between barriers: the warps run apart as far as that
 #pragma unroll 1
         for (int it = 0; it < my_tiles; it += kBatch, ++batch) {
             float* half = warps + (batch & 1) * (kBatch * kLrWarps * kRed);
             const int nb = min(kBatch, my_tiles - it);
-#pragma unroll 1
-            for (int b = 0; b < nb; ++b) {
-                float hi[kGroups][4] = {}, lo[kGroups][4] = {};   // sums of the two planes apart: shorter chains
+            auto tile = [&](int b, uint4 (&w)[kGroups][kBlocks]) {
+                // sums of the two planes apart: shorter chains.  WIDE: D's 16 rows are x's, its 8 columns weight rows; else
+                // the other way round, 16 weight rows a product
+                constexpr int kProds = WIDE ? kGroups : kGroups / 2;
+                float hi[kProds][4] = {}, lo[kProds][4] = {};
 #pragma unroll
-                for (int h = 0; h < kGroups; ++h)
+                for (int h = 0; h < kProds; ++h)
 #pragma unroll
                     for (int i = 0; i < kBlocks; ++i) {
-                        const uint32_t ww[4] = {w[h][i].x, w[h][i].y, w[h][i].z, w[h][i].w};
 #pragma unroll
                         for (int s = 0; s < kSteps; ++s) {
-                            uint32_t b0, b1;
-                            if constexpr (W8) i8x4_to_h2(ww[s], &b0, &b1);
-                            else b0 = ww[2 * s], b1 = ww[2 * s + 1];
-                            uint32_t ah[4], al[4];
                             if constexpr (WIDE) {
-                                ah[0] = xh[i][s][0], ah[1] = xh[i][s][1], ah[2] = xh[i][s][2], ah[3] = xh[i][s][3];
-                                al[0] = xl[i][s][0], al[1] = xl[i][s][1], al[2] = xl[i][s][2], al[3] = xl[i][s][3];
+                                uint32_t b[2];
+                                step(w[h][i], s, b);
+                                mma_f16(hi[h], xh[i][s], b[0], b[1]);
+                                mma_f16(lo[h], xl[i][s], b[0], b[1]);
                             } else {
-                                ah[0] = xh[i][s][0], ah[1] = 0u, ah[2] = xh[i][s][1], ah[3] = 0u;
-                                al[0] = xl[i][s][0], al[1] = 0u, al[2] = xl[i][s][1], al[3] = 0u;
+                                uint32_t b[2], c[2];
+                                step(w[2 * h][i], s, b);
+                                step(w[2 * h + 1][i], s, c);
+                                const uint32_t rows[4] = {b[0], c[0], b[1], c[1]};
+                                mma_f16(hi[h], rows, xh[i][s][0], xh[i][s][1]);
+                                mma_f16(lo[h], rows, xl[i][s][0], xl[i][s][1]);
                             }
-                            mma_f16(hi[h], ah, b0, b1);
-                            mma_f16(lo[h], al, b0, b1);
                         }
                     }
-                if (it + b + 1 < my_tiles) request();
-                // D: rows g, g + 8; weight rows 2q, 2q + 1 of each 8
+                if (it + b + kDepth < my_tiles) request(w);
+                // D: rows g, g + 8; columns 2q, 2q + 1
                 float* red = half + (b * kLrWarps + warp) * kRed;
 #pragma unroll
-                for (int h = 0; h < kGroups; ++h)
+                for (int h = 0; h < kProds; ++h)
 #pragma unroll
-                    for (int e = 0; e < 4; ++e)
-                        if (WIDE || e < 2) red[(g + 8 * (e >> 1)) * (kCols + 1) + h * 8 + 2 * q + (e & 1)] = (hi[h][e] + lo[h][e]) * f[e >> 1];
+                    for (int e = 0; e < 4; ++e) {
+                        if constexpr (WIDE) red[(g + 8 * (e >> 1)) * kLine + h * 8 + 2 * q + (e & 1)] = (hi[h][e] + lo[h][e]) * f[e >> 1];
+                        else red[(2 * q + (e & 1)) * kLine + h * 16 + g + 8 * (e >> 1)] = (hi[h][e] + lo[h][e]) * f[e & 1];
+                    }
+            };
+#pragma unroll 1
+            for (int b = 0; b < nb; b += kDepth) {
+#pragma unroll
+                for (int d = 0; d < kDepth; ++d)
+                    if (b + d < nb) tile(b + d, w[d]);
             }
             __syncthreads();
             for (int i = threadIdx.x; i < nb * kOut; i += kLrThreads) {
-                const int b = i / kOut, at = i % kOut / kCols * (kCols + 1) + i % kCols;
+                const int b = i / kOut, at = i % kOut / kCols * kLine + i % kCols;
                 const float* r = half + b * kLrWarps * kRed + at;
                 float s = r[0];
 #pragma unroll
@@ -326,7 +358,7 @@ static tvb_status launch_rows_kernel(const LoraArgs& a, bool dependent, cudaStre
     plan.passes = (a.K + nsplit * kLrWarps * kMax - 1) / (nsplit * kLrWarps * kMax);
     const int per = (a.K + plan.passes * nsplit * kLrWarps - 1) / (plan.passes * nsplit * kLrWarps);
     plan.slice = (per + kBlock - 1) / kBlock * kBlock;
-    constexpr int kWarpSums = 2 * lr_batch(W8) * kLrWarps * (kOut / kCols) * (kCols + 1);
+    constexpr int kWarpSums = 2 * lr_batch(W8) * kLrWarps * (kOut / kCols) * lr_line(W8, WIDE);
 
     cudaLaunchConfig_t cfg = {};
     cfg.blockDim = dim3(kLrThreads);
