@@ -1,19 +1,20 @@
 // Adapters of many requests beside a shared projection (tvb_matmul_lora):
 //   y[m] = W x[m] + scale_a B_a (A_a x[m]),  a = adapter[m]
 //
-// Up to 64 rows (a decode batch) the call is bound by the bytes of W and of the
-// adapters in use, and by how fast weights reach the warps from L2:
+// A decode batch is bound by the bytes of W and of the adapters in use, and by how
+// fast weights reach the warps from L2:
 //
 // lora_shrink_kernel: t[m] = scale_a A_a x[m], a warp a (row, rank index).
 // lora_rows_kernel: W streamed once for 16 rows through mma.sync m16n8k16 (rows
 // of x are the 16-row operand and 8 weight rows the other, or, up to 8 rows, 16
 // weight rows and x's; a memory-bound product that needs no more than the legacy
-// tensor path).  More rows are blocks of 16 that
-// share the GPU and walk the weights together, so that HBM gives them once and L2
-// the other times.  2560 -> 6912 with 8 adapters among 16, 64, 96 rows: 18.7, 42,
-// 57 us; the many-rows kernels take 80, 83, 84 us of rows mixed so (50 of them for
-// what adapters cost there, less where a chunk's rows share one) and 29, 31, 31 us
-// without adapters against 13.7, 34, 47: hence 64.  x is split into F16 hi + lo
+// tensor path).  More rows are blocks of 16 that share
+// the GPU and walk the weights together, so that HBM gives them once and L2 the
+// other times.  The many-rows kernels (lora_gemm.cu) take over where that would be
+// more than 80 MB, or behind 256 rows: 2560 -> 6912 (35 MB) with 8 adapters of rank
+// 16 among 32, 48, 64 rows 26, 34, 43 against 47, 48, 49 us, without adapters 20,
+// 28, 36 against 28, 29, 29; 4096 -> 14336 (117 MB) 32 rows 113 against 67; 512 ->
+// 512 256 rows 13 against 40.  x is split into F16 hi + lo
 // planes with a power-of-two factor a row, so products are F32-faithful; each
 // warp keeps its K slice of x in registers for the whole kernel and weights come
 // straight from global memory in the operand's layout: with k permuted so that a
@@ -34,8 +35,9 @@ namespace cg = cooperative_groups;
 namespace tvb {
 
 constexpr int kLrWarps = 8, kLrThreads = 32 * kLrWarps;
-// Largest K slice of a warp: what two CTAs an SM (one, when WIDE) have registers for.
-__host__ __device__ constexpr int lr_slice(bool w8, bool wide) { return w8 || !wide ? 128 : 160; }
+// Largest K slice of a warp: what two CTAs an SM (one: INT8 and WIDE) have registers
+// for.  (F16 and WIDE with one CTA and 160: 16 rows 4096 -> 14336 38.8 against 35.4 us.)
+__host__ __device__ constexpr int lr_slice(bool w8, bool wide) { return w8 || !wide ? 128 : 96; }
 // Weight rows a tile: what keeps enough loads under way (a warp's slice of an INT8
 // row is half as many bytes).
 __host__ __device__ constexpr int lr_cols(bool w8) { return w8 ? 32 : 16; }
@@ -48,7 +50,8 @@ __host__ __device__ constexpr int lr_batch(bool w8) { return w8 ? 2 : 4; }   // 
 __host__ __device__ constexpr int lr_depth(bool w8, bool wide) { return w8 && wide ? 2 : 1; }
 constexpr int kLrMaxSplit = 8;     // CTAs of a cluster
 constexpr int kLrRows = 16;        // rows of x a CTA
-constexpr int kLrMaxRows = 64;
+constexpr int kLrMaxRows = 256;
+constexpr int64_t kLrMaxAgain = 80 << 20;   // bytes of W that blocks of 16 rows read from L2
 
 // A CTA takes 4 rank indexes of a row; its 8 warps cut K (8 k a lane), so that all
 // loads of a short K are in flight at once.
@@ -156,7 +159,7 @@ struct LoraRowsPlan {
 // W8: INT8 weights.  WIDE: 9 to 16 rows (else the upper half of the operand is
 // zero and takes no registers).
 template <bool W8, bool WIDE>
-__global__ void __launch_bounds__(kLrThreads, WIDE ? 1 : 2)
+__global__ void __launch_bounds__(kLrThreads, WIDE && W8 ? 1 : 2)
 lora_rows_kernel(const __grid_constant__ LoraArgs a, const __grid_constant__ LoraRowsPlan plan) {
     constexpr int E = W8 ? 16 : 8;                     // weights in 16 bytes
     constexpr int kBlock = 4 * E;                      // k a load of the warp
@@ -374,7 +377,7 @@ static tvb_status launch_rows_kernel(const LoraArgs& a, bool dependent, cudaStre
     // clusters that fit the GPU at once: one more would be a second wave
     static int resident[kMaxDevices][kLrMaxSplit + 1];
     static int set[kMaxDevices];
-    constexpr int kSmem = (WIDE ? 200 : 100) * 1024;   // one CTA an SM, or two
+    constexpr int kSmem = (WIDE && W8 ? 200 : 100) * 1024;   // one CTA an SM, or two
     TVB_TRY(allow_smem(reinterpret_cast<const void*>(kernel), kSmem, set));
     int dev = 0;
     TVB_CUDA(cudaGetDevice(&dev));
@@ -395,6 +398,13 @@ static tvb_status launch_rows_kernel(const LoraArgs& a, bool dependent, cudaStre
     cfg.numAttrs = dependent ? 2 : 1;
     TVB_CUDA(cudaLaunchKernelEx(&cfg, kernel, a, plan));
     return check_launch("lora_rows_kernel");
+}
+
+tvb_status lora_shrink_rows(const LoraArgs& a, cudaStream_t st) {
+    const dim3 grid((unsigned)a.M, (unsigned)((a.max_rank + kLsRanks - 1) / kLsRanks));
+    if (a.f16) lora_shrink_kernel<true><<<grid, 256, 0, st>>>(a);
+    else lora_shrink_kernel<false><<<grid, 256, 0, st>>>(a);
+    return check_launch("lora_shrink_kernel");
 }
 
 }  // namespace tvb
@@ -438,15 +448,13 @@ extern "C" tvb_status tvb_matmul_lora(float* y, const float* x, int M, int K, co
     a.scale = table->scale;
     a.adapter = adapter;
     a.status = status;
-    if (M > kLrMaxRows) return lora_many_rows(a, st);
+    const int64_t again = (int64_t)((M + kLrRows - 1) / kLrRows - 1) * N * K * (a.w8 ? 1 : 2);
+    if (M > kLrMaxRows || (again > kLrMaxAgain && K <= kLoraMaxK)) return lora_many_rows(a, st);
     Workspace ws(st);
     if (a.n) {
         TVB_TRY(ws.get((size_t)M * a.max_rank * 4));
         a.t = ws.at<float>();
-        const dim3 grid((unsigned)M, (unsigned)((a.max_rank + kLsRanks - 1) / kLsRanks));
-        if (a.f16) lora_shrink_kernel<true><<<grid, 256, 0, st>>>(a);
-        else lora_shrink_kernel<false><<<grid, 256, 0, st>>>(a);
-        TVB_TRY(check_launch("lora_shrink_kernel"));
+        TVB_TRY(lora_shrink_rows(a, st));
     }
     const bool wide = M > 8, dep = a.n > 0;
     if (a.w8) return wide ? launch_rows_kernel<true, true>(a, dep, st) : launch_rows_kernel<true, false>(a, dep, st);

@@ -7,6 +7,7 @@
 namespace tvb {
 
 constexpr int kLoraMaxRank = 256;
+constexpr int kLoraMaxK = 16384;   // of the many-rows kernels
 
 struct LoraArgs {
     const float* x;
@@ -23,7 +24,7 @@ struct LoraArgs {
     const int* rank;
     const float* scale;
     const int* adapter;
-    float* t;                  // [splits][M][max_rank]: scale_a A_a x[m], in parts of K
+    float* t;                  // [M][max_rank]: scale_a A_a x[m]
     unsigned* status;
 };
 
@@ -49,6 +50,7 @@ __device__ __forceinline__ float lora_elem(const void* p, size_t i, bool f16) {
     return f16 ? __half2float(static_cast<const __half*>(p)[i]) : static_cast<const float*>(p)[i];
 }
 
-tvb_status lora_many_rows(LoraArgs a, cudaStream_t st);   // lora_gemm.cu
+tvb_status lora_many_rows(LoraArgs a, cudaStream_t st);             // lora_gemm.cu
+tvb_status lora_shrink_rows(const LoraArgs& a, cudaStream_t st);   // lora.cu
 
 }  // namespace tvb

@@ -5,7 +5,8 @@
 // (pf_norm_split), so that F16 products are F32-faithful; the bound is the tensor
 // pipe at twice the FLOPs of the projection.
 //
-// lora_shrink_tile_kernel: t[m] = scale_a A_a x[m] for 16 rows a CTA.  x and A as
+// lora_shrink_tile_kernel (few values of t: lora_shrink_kernel, a CTA four of
+// them): t[m] = scale_a A_a x[m] for 16 rows a CTA.  x and A as
 // TF32 hi + lo planes (any magnitude), three products of mma.sync m16n8k8; 8
 // warps, and the CTAs of a cluster, cut K.  Small next to the projection (rank / N of it).
 // lora_gemm_kernel: 128 rows of x by 256 weight rows a tile, tcgen05 fed by TMA.
@@ -15,10 +16,11 @@
 // k-blocks a tile takes one more such product per adapter among its rows: t . B_a
 // as TF32 hi + lo planes (any magnitude, three products), added to that adapter's
 // rows alone, so one request's adapter never touches another's row, whatever it
-// holds.  Every CTA takes an equal run of the tiles' chunks; a tile that a cut
+// holds (few values of t: lora_expand_kernel does that, behind the join).  Every CTA takes an equal run of the tiles' chunks; a tile that a cut
 // divides leaves F32 partial sums and lora_join_kernel adds them.
 #include <algorithm>
 #include <cooperative_groups.h>
+#include <type_traits>
 
 #include "lora.h"
 #include "prefill.h"
@@ -44,11 +46,12 @@ __device__ __forceinline__ void tf32_planes(float x, uint32_t* hi, uint32_t* lo)
     *lo = __float_as_uint(x - __uint_as_float(*hi));
 }
 
-// The next adapter after `prev` among ids[] (4 a lane, -1 none), or INT_MAX.
-__device__ __forceinline__ int next_adapter(const int (&ids)[4], int prev) {
+// The next adapter after `prev` among ids[] (N a lane, -1 none), or INT_MAX.
+template <int N>
+__device__ __forceinline__ int next_adapter(const int (&ids)[N], int prev) {
     int v = 0x7fffffff;
 #pragma unroll
-    for (int i = 0; i < 4; ++i)
+    for (int i = 0; i < N; ++i)
         if (ids[i] > prev) v = min(v, ids[i]);
     return __reduce_min_sync(0xffffffffu, v);
 }
@@ -71,7 +74,7 @@ __global__ void __launch_bounds__(32 * kLtWarps, 2) lora_shrink_tile_kernel(cons
     cg::cluster_group cl = cg::this_cluster();   // its CTAs cut K
     const int rank = (int)cl.block_rank(), nsplit = (int)cl.num_blocks();
     const int m0 = blockIdx.y * kLtRows;
-    int ids[4] = {-1, -1, -1, -1}, rank_of = 0;
+    int ids[1] = {-1}, rank_of = 0;
     if (lane < kLtRows && m0 + lane < a.M) ids[0] = lora_of(a, m0 + lane, &rank_of, warp == 0 && rank == 0);
     if (rank_of == 0) ids[0] = -1;
     const int parts = kLtWarps * nsplit, part = rank * kLtWarps + warp;
@@ -176,6 +179,7 @@ struct LgPlan {
     int mt, tiles;      // tiles of rows, of both
     int nk, chunks;     // k-blocks, chunks a tile
     int ctas;
+    int fused;          // the adapters' products are lora_gemm_kernel's too
     const int* row_exp;
     float* part;        // [CTA][2][128][256]
 };
@@ -361,7 +365,7 @@ lora_gemm_kernel(const __grid_constant__ LgMaps maps, const __grid_constant__ Lo
                 }
                 chunk = __shfl_sync(0xffffffffu, chunk, 0);
                 ok = __shfl_sync(0xffffffffu, (int)ok, 0) != 0;
-                if (ok && a.n && p.c0 == 0) {
+                if (ok && plan.fused && p.c0 == 0) {
                     int ids[4];
                     lg_ids(a, p.m0, ids);
                     for (int ad = next_adapter(ids, -1); ok && ad != 0x7fffffff; ad = next_adapter(ids, ad), ++chunk) {
@@ -393,7 +397,7 @@ lora_gemm_kernel(const __grid_constant__ LgMaps maps, const __grid_constant__ Lo
                 mbar_wait_bounded(&sh.drained, 0u);
             }
             __syncwarp();
-        } else if (a.n) {
+        } else if (plan.fused) {
             // ---- adapters: 8 rank indexes of t and B a step, as TF32 hi + lo ------------
             const int tid = threadIdx.x - 320;   // 0 .. 63
             int ls = 0;
@@ -521,7 +525,7 @@ lora_gemm_kernel(const __grid_constant__ LgMaps maps, const __grid_constant__ Lo
                     acc[i] = lg_fma2(acc[i], lg_pack2(s0, s1), 0ull);
                 }
             }
-            if (ok && a.n && p.c0 == 0) {
+            if (ok && plan.fused && p.c0 == 0) {
                 int ids[4], rank;
                 lg_ids(a, p.m0, ids);
                 const int id = live ? lora_of(a, m, &rank, false) : -1;
@@ -593,10 +597,132 @@ __global__ void __launch_bounds__(256) lora_join_kernel(const __grid_constant__ 
     }
 }
 
+// ---- expand ------------------------------------------------------------------------
+// y[m] += B_a t[m] on the CUDA cores, a CTA `rows` rows (at most kLeRows) of 256
+// columns, two a thread: the rows' adapters one after another, 32 rank indexes of
+// their B rows in registers, t broadcast from shared memory.
+// For few values of t: lora_gemm_kernel's own products cost a step for every
+// adapter of a tile, this a pass over y for every 32 rank indexes.  2560 -> 6912,
+// 8 adapters of rank 16 mixed: 128 rows 58 against 85 us, 512 rows 94 against 120;
+// 2 of rank 64 in runs: 128 rows 66 against 56, 256 rows 93 against 65.
+constexpr int kLeMaxValues = 8192;   // rows x largest rank
+constexpr int kLeThreads = 128, kLeRows = 64, kLeRanks = 32, kLeGroup = 4, kLePerSm = 4;
+
+template <bool F16>
+__global__ void __launch_bounds__(kLeThreads, kLePerSm) lora_expand_kernel(const __grid_constant__ LoraArgs a, int rows) {
+    __shared__ __align__(16) float ts[kLeRows + 2 * kLeGroup][kLeRanks];   // (pairs of groups are read)
+    __shared__ int list[kLeRows], ids_s[kLeRows], count;
+    pdl_wait();
+    const int tid = threadIdx.x, m0 = blockIdx.y * rows, n0 = blockIdx.x * 2 * kLeThreads + tid;
+    {
+        int r = 0, id = -1;
+        if (tid < rows && m0 + tid < a.M) id = lora_of(a, m0 + tid, &r, false);
+        if (tid < kLeRows) ids_s[tid] = r > 0 ? id : -1;
+    }
+    __syncthreads();
+    int ids[kLeRows / 32];
+#pragma unroll
+    for (int i = 0; i < kLeRows / 32; ++i) ids[i] = ids_s[i * 32 + (tid & 31)];
+    for (int ad = next_adapter(ids, -1); ad != 0x7fffffff; ad = next_adapter(ids, ad)) {
+        const int r = __ldg(a.rank + ad);
+        const void* B = a.B[ad];
+        __syncthreads();   // the list was read
+        if (tid < 32) {    // the adapter's rows, in order
+            int n = 0;
+#pragma unroll
+            for (int i = 0; i < kLeRows / 32; ++i) {
+                const unsigned at = __ballot_sync(0xffffffffu, ids[i] == ad);
+                if (ids[i] == ad) list[n + __popc(at & ((1u << tid) - 1))] = i * 32 + tid;
+                n += __popc(at);
+            }
+            if (tid == 0) count = n;
+        }
+        for (int j0 = 0; j0 < r; j0 += kLeRanks) {
+            const int rj = min(kLeRanks, r - j0);
+            // 32 rank indexes of rows n0, n0 + 128 of B, as pairs
+            uint64_t b[2][kLeRanks / 2];
+#pragma unroll
+            for (int c = 0; c < 2; ++c) {
+                const int n = n0 + c * kLeThreads;
+                const size_t at = (size_t)n * r + j0;
+#pragma unroll
+                for (int j = 0; j < kLeRanks; j += 4) {
+                    float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
+                    if (n < a.N && j < rj) {
+                        if (r % 4 == 0) {
+                            x = lora_load4<F16>(B, at + j);
+                        } else {
+                            x.x = lora_elem(B, at + j, F16);
+                            if (j + 1 < rj) x.y = lora_elem(B, at + j + 1, F16);
+                            if (j + 2 < rj) x.z = lora_elem(B, at + j + 2, F16);
+                            if (j + 3 < rj) x.w = lora_elem(B, at + j + 3, F16);
+                        }
+                    }
+                    b[c][j / 2] = lg_pack2(x.x, x.y);
+                    b[c][j / 2 + 1] = lg_pack2(x.z, x.w);
+                }
+            }
+            __syncthreads();   // the list is there; t of the step before was read
+            const int n = count;
+            for (int i = tid; i < n * kLeRanks; i += kLeThreads) {
+                const int k = i / kLeRanks, j = i % kLeRanks;
+                ts[k][j] = j < rj ? a.t[(size_t)(m0 + list[k]) * a.max_rank + j0 + j] : 0.f;
+            }
+            __syncthreads();
+            // four rows at a time, the next four's y under way
+            float* const y = a.y + (size_t)m0 * a.N + n0;
+            const bool in[2] = {n0 < a.N, n0 + kLeThreads < a.N};
+            auto fetch = [&](int k, float (&v)[kLeGroup][2]) {
+#pragma unroll
+                for (int i = 0; i < kLeGroup; ++i)
+#pragma unroll
+                    for (int c = 0; c < 2; ++c) v[i][c] = k + i < n && in[c] ? y[(size_t)list[k + i] * a.N + c * kLeThreads] : 0.f;
+            };
+            // (ranks of t and B behind rj are zero)
+            auto add = [&](auto ranks, int k, const float (&v)[kLeGroup][2]) {
+                uint64_t s[kLeGroup][2];
+#pragma unroll
+                for (int i = 0; i < kLeGroup; ++i) s[i][0] = s[i][1] = 0ull;
+#pragma unroll
+                for (int j = 0; j < decltype(ranks)::value; j += 4) {
+#pragma unroll
+                    for (int i = 0; i < kLeGroup; ++i) {
+                        const float4 x = *reinterpret_cast<const float4*>(&ts[k + i][j]);
+                        const uint64_t x0 = lg_pack2(x.x, x.y), x1 = lg_pack2(x.z, x.w);
+#pragma unroll
+                        for (int c = 0; c < 2; ++c) s[i][c] = lg_fma2(b[c][j / 2 + 1], x1, lg_fma2(b[c][j / 2], x0, s[i][c]));
+                    }
+                }
+#pragma unroll
+                for (int i = 0; i < kLeGroup; ++i)
+#pragma unroll
+                    for (int c = 0; c < 2; ++c) {
+                        const float2 z = lg_unpack2(s[i][c]);
+                        if (k + i < n && in[c]) y[(size_t)list[k + i] * a.N + c * kLeThreads] = v[i][c] + (z.x + z.y);
+                    }
+            };
+            auto rows_of = [&](auto ranks) {
+                float u[kLeGroup][2], v[kLeGroup][2];
+                fetch(0, u);
+#pragma unroll 1
+                for (int k = 0; k < n; k += 2 * kLeGroup) {
+                    fetch(k + kLeGroup, v);
+                    add(ranks, k, u);
+                    fetch(k + 2 * kLeGroup, u);
+                    add(ranks, k + kLeGroup, v);
+                }
+            };
+            if (rj <= 8) rows_of(std::integral_constant<int, 8>());
+            else if (rj <= 16) rows_of(std::integral_constant<int, 16>());
+            else rows_of(std::integral_constant<int, kLeRanks>());
+        }
+    }
+}
+
 static size_t align256(size_t n) { return (n + 255) & ~(size_t)255; }
 
 tvb_status lora_many_rows(LoraArgs a, cudaStream_t st) {
-    TVB_REQUIRE(a.K <= 16384, "matmul_lora: K=%d with %d rows (at most 16384 above 64 rows)", a.K, a.M);
+    TVB_REQUIRE(a.K <= kLoraMaxK, "matmul_lora: K=%d with %d rows (at most %d above 256 rows)", a.K, a.M, kLoraMaxK);
     LgPlan plan = {};
     plan.mt = (a.M + kLgRows - 1) / kLgRows;
     plan.tiles = plan.mt * ((a.N + kLgCols - 1) / kLgCols);
@@ -616,7 +742,10 @@ tvb_status lora_many_rows(LoraArgs a, cudaStream_t st) {
     plan.part = ws.at<float>(2 * plane + wide + exps + ts);
     const uint16_t* w = a.w8 ? w16 : static_cast<const uint16_t*>(a.w);
     if (a.w8) TVB_TRY(pf_i8_to_f16(static_cast<const int8_t*>(a.w), (size_t)a.N * a.K, w16, st));
-    if (a.n) {
+    plan.fused = a.n && (int64_t)a.M * a.max_rank > kLeMaxValues;
+    if (a.n && !plan.fused) {
+        TVB_TRY(lora_shrink_rows(a, st));
+    } else if (a.n) {
         static int set[2][kMaxDevices];
         constexpr int smem = kLtWarps * kLtRows * (kLtRanks + 1) * 4;
         const auto kernel = a.f16 ? lora_shrink_tile_kernel<true> : lora_shrink_tile_kernel<false>;
@@ -650,7 +779,15 @@ tvb_status lora_many_rows(LoraArgs a, cudaStream_t st) {
     lora_gemm_kernel<<<(unsigned)plan.ctas, kLgThreads, kLgSmem, st>>>(maps, a, plan);
     TVB_TRY(check_launch("lora_gemm_kernel"));
     TVB_CUDA(launch_maybe_pdl(lora_join_kernel, dim3((unsigned)plan.ctas, kLgRows / 8), dim3(256), 0, st, true, a, plan));
-    return check_launch("lora_join_kernel");
+    TVB_TRY(check_launch("lora_join_kernel"));
+    if (!a.n || plan.fused) return TVB_OK;
+    const unsigned cols = (unsigned)((a.N + 2 * kLeThreads - 1) / (2 * kLeThreads));
+    // row blocks that fill the SMs once
+    const int blocks = std::max(1, std::min((a.M + kLeGroup - 1) / kLeGroup, kLePerSm * num_sms() / (int)cols));
+    const int rows = std::min(kLeRows, (a.M + blocks - 1) / blocks);
+    const auto expand = a.f16 ? lora_expand_kernel<true> : lora_expand_kernel<false>;
+    TVB_CUDA(launch_maybe_pdl(expand, dim3(cols, (unsigned)((a.M + rows - 1) / rows)), dim3(kLeThreads), 0, st, true, a, rows));
+    return check_launch("lora_expand_kernel");
 }
 
 }  // namespace tvb

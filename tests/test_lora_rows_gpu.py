@@ -327,3 +327,49 @@ assert float((y - ref).norm() / ref.norm()) < 4e-6
 """
     root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
     subprocess.run([sys.executable, "-c", code], check=True, cwd=root, timeout=300)
+
+
+# More than 256 rows, or weights too large to come several times from L2: the two ways of adding the adapters, few
+# values of t (rows x largest rank) and many.
+MANY = [
+    (257, 320, 512, "f16", [16, 3, 8], F32),
+    (400, 264, 333, "f16", [20, 7], F16),
+    (300, 128, 1000, "i8tensor", [1, 2, 5], F32),
+    (1000, 64, 70, "i8row", [8, 4], F16),
+    (48, 6144, 8000, "f16", [40, 100], F32),
+    (600, 320, 512, "f16", [16, 3, 8], F32),
+    (300, 272, 333, "i8row", [30, 7], F16),
+    (1000, 64, 70, "i8tensor", [9, 4], F32),
+    (40, 6144, 8000, "f16", [256, 33], F16),
+]
+
+
+@pytest.mark.parametrize("case", MANY, ids=lambda c: f"{c[0]}x{c[1]}x{c[2]}-{c[3]}-r{c[4][0]}x{len(c[4])}")
+@pytest.mark.parametrize("order", ["mixed", "runs"])
+def test_matmul_lora_many_rows(be, case, order):
+    test_matmul_lora(be, case, order)
+
+
+@pytest.mark.parametrize("M", [300, 600])
+def test_many_rows_each_way(be, M):
+    test_rows_of_any_magnitude(be, M)
+    test_ids_out_of_range_and_no_adapters(be, M)
+    test_a_row_that_is_not_finite_stays_alone(be, M)
+    for bad in (math.nan, math.inf):
+        test_an_adapter_that_is_not_finite_stays_alone(be, M, bad)
+    test_output_at_any_address(be, M)
+    test_an_adapter_of_misaligned_rows_is_reported(be, M)
+    test_first_call_inside_a_capture(M)
+
+
+def test_long_rows_of_few_and_many(be):
+    """K above what the many-rows kernels take: the few-rows ones up to 256 rows, a refusal behind."""
+    from ternative_b200 import TvbError
+    p = Projection(16400, 3000, "f16", [4], F32, seed=9)
+    x = torch.randn(40, 16400, generator=torch.Generator().manual_seed(1))
+    ids = torch.zeros(40, dtype=torch.long)
+    ref, tol = p(x, ids)
+    y = project(be, p, x.cuda(), ids.to(torch.int32).cuda()).cpu().double()
+    assert ((y - ref).abs() <= tol).all()
+    with pytest.raises(TvbError, match="16384"):
+        project(be, p, torch.zeros(257, 16400, device="cuda"), torch.zeros(257, dtype=torch.int32, device="cuda"))
