@@ -21,16 +21,18 @@
 namespace tvb {
 
 constexpr int kPrKeys = 8;   // keys a batch
-constexpr int kPrExtra = 1;   // what starting and leaving a block costs, in tiles
+// What starting and leaving a block costs, in tiles.  Decode of 32 sequences: 1, 4, 8
+// take 49.3, 46.1, 49.7 us, of 4 x 61000 keys 103, 100, 101.
+constexpr int kPrExtra = 4;
 // Rows of a KV head from which a call takes the tensor cores (paged_chunk_kernel):
-// below, its 128-row tiles are too empty.  Measured with 20/5 heads, 8 sequences of
-// 3000 keys: F16 24 rows 32 against 31 us, 48 rows 29 against 32; F32 32 rows 110
-// against 79 us, 64 rows 63 against 79.
-constexpr int kTensorRows16 = 32, kTensorRows32 = 64;
+// below, its 128-row tiles are too empty.  20/5 heads, 8 sequences of 3000 keys: F16
+// 24 rows 36 against 33 us there, 48 rows 46 against 33; F32 32 rows 127 against
+// 130, 64 rows 237 against 131.
+constexpr int kTensorRows16 = 24, kTensorRows32 = 40;
 // Keys up to which a CTA takes whole blocks: sharing tiles evenly costs a second
-// launch.  One token of one sequence, 130 keys 6.7 against 10.4 us, 400 keys 13.2
-// against 11.3.
-constexpr int kWholeKeys = 256;
+// launch.  One token, F16, 400 keys 14.2 against 16.4 us, 800 keys 20.9 against
+// 17.3; 128 sequences of 1000 keys 126 against 79.
+constexpr int kWholeKeys = 512;
 
 __device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, bool valid) {
     asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(valid ? 16 : 0) : "memory");
@@ -281,7 +283,7 @@ __device__ __forceinline__ void rows_piece(const PagedAttnArgs& a, const AttnPie
 
 // ---- three to sixteen rows over an F16 cache: mma.sync ------------------------------
 // The rows are the 16-row operand of mma.sync m16n8k16 (a memory-bound product: the
-// legacy tensor path keeps up with memory where the FP32 pipe does not, 48 against
+// legacy tensor path keeps up with memory where the FP32 pipe does not, 46 against
 // 62 us for 32 sequences of up to 4096 keys with 20/5 heads).  q and p are split into F16 hi + lo planes, K and V rows
 // come from shared memory by ldmatrix.  Every 16 keys make a fresh product that is
 // added to F32 registers, so the tensor core's truncation does not add up.

@@ -162,3 +162,57 @@ assert ((out.cpu().double() - ref).abs().amax(-1) <= tol).all()
 """
     root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
     subprocess.run([sys.executable, "-c", code], check=True, cwd=root, timeout=300)
+
+
+@pytest.mark.parametrize("dtype", [F32, F16])
+@pytest.mark.parametrize("new,kv,heads,hd,page,window", [
+    ([300, 40], [1500, 700], (4, 2), 128, 16, 0),
+    ([300, 40, 0, 1], [1500, 700, 9, 2000], (6, 2), 64, 24, 0),
+    ([129, 600], [129, 2100], (2, 2), 128, 5, 900),
+    ([700], [700], (8, 2), 64, 64, 0),
+    ([33, 1, 50], [3000, 40, 50], (3, 1), 128, 128, 0),
+    ([9, 3], [1700, 900], (4, 2), 128, 16, 0),
+    ([5, 3], [1700, 900], (4, 2), 64, 7, 600),
+    ([1, 1], [5000, 700], (2, 2), 128, 16, 0),
+])
+def test_attention_cut_into_runs(be, dtype, new, kv, heads, hd, page, window):
+    """Caches long enough that blocks are cut over several CTAs and joined."""
+    b = Batch(new, kv, *heads, hd, page, dtype, seed=11, tail=2)
+    out, lse, st = attend(be, b, window=window)
+    assert st == 0
+    check_attention(b, out, lse, window=window)
+
+
+@pytest.mark.parametrize("dtype", [F32, F16])
+@pytest.mark.parametrize("new", [1, 3, 9, 200])
+def test_attention_cut_into_runs_with_odd_values(be, dtype, new):
+    """Values that some rows do not see are not finite, a page in the middle does not exist: the other keys count, run
+    by run."""
+    b = Batch([new, new], [1500, 1300], 4, 2, 64, 16, dtype, seed=12)
+    out, lse, _ = attend(be, b)
+    limit = 1500 - new   # keys of the new tokens: seen by the later ones only
+    want = out[:1].clone()
+    if new > 1:
+        pg, at = b.where[0]
+        b.v[pg[limit + 1:].cuda(), at[limit + 1:].cuda()] = math.inf
+        out2, _, st = attend(be, b)
+        assert st == 0
+        # (the first row's keys are as they were; its sum may be taken in another order)
+        assert float((out2[:1] - want).abs().max()) < 1e-5 * float(b.v[torch.isfinite(b.v)].abs().max())
+        assert not torch.isfinite(out2[1:new]).any()
+        assert torch.equal(out2[new:], out[new:])
+    b = Batch([new, new], [1500, 1300], 4, 2, 64, 16, dtype, seed=12)
+    b.table[0, 40] = 1 << 30
+    out3, lse3, st = attend(be, b)
+    assert st == 2
+    assert torch.equal(out3[new:], out[new:])
+    keep = torch.ones(1500, dtype=torch.bool)
+    keep[640:656] = False
+    k, v = b.hk[b.where[0]].double(), b.hv[b.where[0]].double()
+    for j in range(0, new, max(1, new // 5)):
+        seen = keep & (torch.arange(1500) <= 1500 - new + j)
+        for h in range(4):
+            z = k[seen, h // 2] @ b.q[j, h].double() * 0.125
+            ref = torch.softmax(z, 0) @ v[seen, h // 2]
+            # (hd + 4) U S + n U with S < 64 and n = 1500, twice max |v| < 6: below 6e-5
+            assert float((out3[j, h].double() - ref).abs().max()) < 6e-5
