@@ -319,6 +319,89 @@ paged_chunk_kernel(const __grid_constant__ PcMaps maps, const __grid_constant__ 
             const int* table = a.s.table + (size_t)p.b * a.s.table_ld;
             const int p_first = p.pos0 + (int)a.gdiv.div((uint32_t)p.row);
             const int p_last = p.pos0 + (int)a.gdiv.div((uint32_t)(p.row + p.rows - 1));
+            if constexpr (kF32) {
+                // this warp's rows of the tile, every third, kBatch row loads (pairs of rows, HD 64) at a time into two sets
+                // of registers in turn, so that one is always under way: the next item's first too, before its slot is
+                // free, and its rows' pages.  Values that are not finite have no planes: their piece goes key by key
+                constexpr int kRowLanes = HD / 4, kPer = 32 / kRowLanes, kMine = (kPcKeys + Ty::kTeam - 1) / Ty::kTeam;
+                constexpr int kBatch = 6, kBatches = (kMine + kBatch * kPer - 1) / (kBatch * kPer);
+                static_assert(kBatches % 2 == 0 && kMine <= 32, "two sets of registers; a lane a row");
+                const int first = (warp - kPcSoft) % Ty::kTeam, sub = lane / kRowLanes, d = lane % kRowLanes * 4;
+                const int64_t head = (int64_t)p.kvh * a.kv.head_stride + d * 4;
+                bool bad = false, odd = false;
+                auto is_key = [&](int i) { return i != nitems - 1 && (i == 0 || (i & 1)); };
+                auto offsets = [&](int i) -> int64_t {   // of row first + lane * kTeam of item i
+                    const int tile = i == 0 ? 0 : is_key(i) ? (i + 1) >> 1 : i == nitems - 1 ? nt - 1 : (i >> 1) - 1;
+                    const int my = first + lane * Ty::kTeam, t = p.k0 + tile * kPcKeys + my;
+                    if (lane >= kMine || my >= kPcKeys || t >= p.k1) return -1;
+                    const int64_t off = paged_offset(a.kv, table, t);
+                    bad |= off < 0;
+                    if (off >= 0)
+                        asm volatile("cp.async.bulk.prefetch.L2.global [%0], %1;" ::"l"((is_key(i) ? a.kv.k : a.kv.v) + (int64_t)p.kvh * a.kv.head_stride + off), "n"(HD * 4) : "memory");
+                    return off;
+                };
+                auto load = [&](int i, int64_t off, int b, float4 (&x)[kBatch]) {
+                    const unsigned char* src = (is_key(i) ? a.kv.k : a.kv.v) + head;
+#pragma unroll
+                    for (int e = 0; e < kBatch; ++e) {
+                        const int64_t o = __shfl_sync(0xffffffffu, off, min((b * kBatch + e) * kPer + sub, 31));
+                        x[e] = o >= 0 ? *reinterpret_cast<const float4*>(src + o) : make_float4(0.f, 0.f, 0.f, 0.f);
+                    }
+                };
+                auto put = [&](unsigned char* dst, int b, const float4 (&x)[kBatch]) {
+#pragma unroll
+                    for (int e = 0; e < kBatch; ++e) {
+                        const int row = first + ((b * kBatch + e) * kPer + sub) * Ty::kTeam;
+                        uint2 u[3];
+                        bf16_planes(x[e].x, x[e].y, &u[0].x, &u[1].x, &u[2].x);
+                        bf16_planes(x[e].z, x[e].w, &u[0].y, &u[1].y, &u[2].y);
+                        const float big = fmaxf(fmaxf(fabsf(x[e].x), fabsf(x[e].y)), fmaxf(fabsf(x[e].z), fabsf(x[e].w)));
+                        const float all = x[e].x + x[e].y + x[e].z + x[e].w;
+                        odd |= !(big < 3.3e38f) || all != all;
+                        if (row < kPcKeys) {
+#pragma unroll
+                            for (int pl = 0; pl < 3; ++pl)
+                                *reinterpret_cast<uint2*>(dst + pl * Sm::kPlane + sw128_offset(row, (d >> 3) & 7)) = u[pl];
+                        }
+                    }
+                };
+                float4 x[kBatch], y[kBatch];
+                int i = (w - item0) & (kPcTeams - 1);
+                int64_t off = -1;
+                if (i < nitems) {
+                    off = offsets(i);
+                    load(i, off, 0, x);
+                }
+#pragma unroll 1
+                for (; i < nitems; i += kPcTeams) {
+                    const int gi = item0 + i, sl = gi % kPcSlots;
+                    const int64_t off2 = i + kPcTeams < nitems ? offsets(i + kPcTeams) : -1;
+                    const bool free_slot = landed(sh.empty + sl, gi / kPcSlots + 1);
+                    if (__any_sync(0xffffffffu, !free_slot || *abort_flag)) {
+                        fail();
+                        ok = false;
+                        break;
+                    }
+                    unsigned char* dst = smem + Sm::kSlots + sl * Sm::kSlot + (d >> 6) * Sm::kAtom + (d & 4) * 2;
+#pragma unroll 1
+                    for (int b = 0; b < kBatches; b += 2) {
+                        load(i, off, b + 1, y);
+                        put(dst, b, x);
+                        if (b + 2 < kBatches) load(i, off, b + 2, x);
+                        put(dst, b + 1, y);
+                    }
+                    if (bad || odd) *reinterpret_cast<volatile int*>(&sh.poison[pi & 7]) = pi + 1;
+                    if (bad) report_bad(a.status);
+                    fence_proxy_async_smem_cta();
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(sh.full + sl);
+                    off = off2;
+                    if (i + kPcTeams < nitems) load(i + kPcTeams, off, 0, x);
+                }
+                item0 += nitems;
+                done(pi);
+                continue;
+            }
             for (int i = 0; i < nitems; ++i) {
                 const int gi = item0 + i;
                 if (gi % kPcTeams != w) continue;
@@ -337,50 +420,6 @@ paged_chunk_kernel(const __grid_constant__ PcMaps maps, const __grid_constant__ 
                 const bool look = !is_k && (t1 - t0 < kPcKeys || t1 - 1 > p_first || t0 < p.first ||
                                             (a.window && t0 <= p_last - a.window));
                 bool bad = false;
-                if constexpr (kF32) {
-                    // this warp's rows of the tile, every third: loads of eight rows (pairs of rows, HD 64) before their
-                    // planes.  Values that are not finite have none: their piece goes key by key
-                    constexpr int kRowLanes = HD / 4, kPer = 32 / kRowLanes, kMine = (kPcKeys + Ty::kTeam - 1) / Ty::kTeam;
-                    const int first = (warp - kPcSoft) % Ty::kTeam, sub = lane / kRowLanes, d = lane % kRowLanes * 4;
-                    int64_t off = -1;
-                    const int my = first + lane * Ty::kTeam;
-                    if (lane < kMine && my < kPcKeys && t0 + my < p.k1) {
-                        off = paged_offset(a.kv, table, t0 + my);
-                        bad = off < 0;
-                    }
-                    const unsigned char* src = (is_k ? a.kv.k : a.kv.v) + (int64_t)p.kvh * a.kv.head_stride + d * 4;
-                    unsigned char* dst = smem + Sm::kSlots + sl * Sm::kSlot + (d >> 6) * Sm::kAtom + (d & 4) * 2;
-                    bool odd = false;
-#pragma unroll 1
-                    for (int r0 = 0; r0 < kMine; r0 += 8 * kPer) {
-                        float4 x[8];
-#pragma unroll
-                        for (int i = 0; i < 8; ++i) {
-                            const int64_t o = __shfl_sync(0xffffffffu, off, min(r0 + i * kPer + sub, 31));
-                            x[i] = o >= 0 ? *reinterpret_cast<const float4*>(src + o) : make_float4(0.f, 0.f, 0.f, 0.f);
-                        }
-#pragma unroll
-                        for (int i = 0; i < 8; ++i) {
-                            const int row = first + (r0 + i * kPer + sub) * Ty::kTeam;
-                            uint2 u[3];
-                            bf16_planes(x[i].x, x[i].y, &u[0].x, &u[1].x, &u[2].x);
-                            bf16_planes(x[i].z, x[i].w, &u[0].y, &u[1].y, &u[2].y);
-                            const float big = fmaxf(fmaxf(fabsf(x[i].x), fabsf(x[i].y)), fmaxf(fabsf(x[i].z), fabsf(x[i].w)));
-                            odd |= !(big < 3.3e38f) || x[i].x + x[i].y + x[i].z + x[i].w != x[i].x + x[i].y + x[i].z + x[i].w;
-                            if (row < kPcKeys) {
-#pragma unroll
-                                for (int pl = 0; pl < 3; ++pl)
-                                    *reinterpret_cast<uint2*>(dst + pl * Sm::kPlane + sw128_offset(row, (d >> 3) & 7)) = u[pl];
-                            }
-                        }
-                    }
-                    if (bad || odd) *reinterpret_cast<volatile int*>(&sh.poison[pi & 7]) = pi + 1;
-                    if (bad) report_bad(a.status);
-                    fence_proxy_async_smem_cta();
-                    __syncwarp();
-                    if (lane == 0) mbar_arrive(sh.full + sl);
-                    continue;
-                }
                 if (box) {
                     // one box a lane: `box` rows x 64 dimensions
                     const int per = kPcKeys / box, n = per * (HD / 64), row = (lane % per) * box, at = lane / per;
@@ -497,13 +536,23 @@ paged_chunk_kernel(const __grid_constant__ PcMaps maps, const __grid_constant__ 
         for (int pi = 0; ok && next(pi); ++pi) {
             const AttnPiece& p = sh.piece[pi & 3];
             if (lane == 0) {
+                // the products of two operands' planes, the small ones of all steps before the large: the sum is small
+                // while most are added.  F32: (0, 2) (1, 1) (2, 0) (0, 1) (1, 0) (0, 0), rolled for the instruction cache
+                auto products = [&](auto& product) {
+                    if constexpr (kF32) {
+#pragma unroll 1
+                        for (int i = 0; i < 6; ++i) product((0x010210 >> 4 * i) & 3, (0x001012 >> 4 * i) & 3, i == 0);
+                    } else {
+                        product(1, 0, true);
+                        product(0, 0, false);
+                    }
+                };
                 auto ready = [&]() { return landed(sh.full + item % kPcSlots, item / kPcSlots); };
                 auto mma_s = [&](int j) {   // tile j (of all) takes the buffer of P(j - 2)
                     const uint32_t d = tmem + (j & 1) * kSBuf;
                     const uint64_t qd = sw128_desc(base + Sm::kQ), kd = sw128_desc(base + Sm::kSlots + (item % kPcSlots) * Sm::kSlot);
                     tc_fence_after();
-                    // products of plane x of q and plane y of K, the small ones of all steps before the large: the sum is
-                    // small while most are added.  Addresses in a descriptor count 16 bytes
+                    // plane x of q, plane y of K; addresses in a descriptor count 16 bytes
                     auto product = [&](int x, int y, bool begin) {
 #pragma unroll
                         for (int kk = 0; kk < HD / 16; ++kk) {
@@ -512,16 +561,7 @@ paged_chunk_kernel(const __grid_constant__ PcMaps maps, const __grid_constant__ 
                             tc_mma(d, qd + qo, kd + ko, idesc_s, begin && kk == 0 ? 0u : 1u);
                         }
                     };
-                    if constexpr (kF32) {
-                        product(0, 2, true);
-                        product(1, 1, false);
-                        product(2, 0, false);
-                        product(0, 1, false);
-                        product(1, 0, false);
-                    } else {
-                        product(1, 0, true);
-                    }
-                    product(0, 0, false);
+                    products(product);
                     tc_commit(sh.s_full + (j & 1));
                     tc_commit(sh.empty + item % kPcSlots);
                     ++item;
@@ -544,16 +584,7 @@ paged_chunk_kernel(const __grid_constant__ PcMaps maps, const __grid_constant__ 
                             tc_mma_ts(ot, pt + kk * kPStep + 8 * x, vd + kk * (2048 >> 4) + y * (Sm::kPlane >> 4), idesc_o,
                                       begin && kk == 0 ? 0u : 1u);
                     };
-                    if constexpr (kF32) {
-                        product(0, 2, true);
-                        product(1, 1, false);
-                        product(2, 0, false);
-                        product(0, 1, false);
-                        product(1, 0, false);
-                    } else {
-                        product(1, 0, true);
-                    }
-                    product(0, 0, false);
+                    products(product);
                     tc_commit(sh.o_full + (j & 1));
                     tc_commit(sh.empty + item % kPcSlots);
                     ++item;
@@ -710,31 +741,41 @@ paged_chunk_kernel(const __grid_constant__ PcMaps maps, const __grid_constant__ 
                     mref = mn == -INFINITY ? 0.f : mn;
                 };
                 uint64_t sum[2] = {0ull, 0ull};
-                if constexpr (kF32) {
-                    // the whole tile in registers: the planes of p take more columns than its scores
-                    uint32_t s[kPcKeys];
-#pragma unroll
-                    for (int c = 0; c < kPcKeys; c += 32) tmem_ld32(sb + c, *reinterpret_cast<uint32_t(*)[32]>(s + c));
+                // loops rolled on purpose: what the three roles run between tiles fits the instruction cache
+#pragma unroll 1
+                for (int c = 0; c < kPcKeys; c += 32) {
+                    uint32_t s[32];
+                    tmem_ld32(sb + c, s);
                     tmem_wait_ld();
                     if (edge) {
+                        const uint32_t mk = seen(c);
 #pragma unroll
-                        for (int c = 0; c < kPcKeys; c += 32) {
-                            const uint32_t mk = seen(c);
-#pragma unroll
-                            for (int k = 0; k < 32; ++k)
-                                if (!(mk & (1u << k))) s[c + k] = 0xff800000u;   // -infinity
-                        }
+                        for (int k = 0; k < 32; ++k)
+                            if (!(mk & (1u << k))) s[k] = 0xff800000u;   // -infinity
                     }
 #pragma unroll
-                    for (int k = 0; k < kPcKeys; ++k) m4[k & 3] = fmaxf(m4[k & 3], __uint_as_float(s[k]));
-                    maximum();
+                    for (int k = 0; k < 32; ++k) m4[k & 3] = fmaxf(m4[k & 3], __uint_as_float(s[k]));
+                }
+                maximum();
+                if constexpr (kF32) {
+                    // the planes of p take more columns than its scores: from the last keys to the first they only cover
+                    // scores that were read
                     const uint64_t m2 = pack2(-mref, -mref);
+#pragma unroll 1
+                    for (int c = kPcKeys - 16; c >= 0; c -= 16) {   // 16 keys: 8 columns a plane
+                        uint32_t zc[16];
+                        tmem_ld16(sb + c, zc);
+                        tmem_wait_ld();
+                        if (edge) {
+                            const uint32_t mk = seen(c);
 #pragma unroll
-                    for (int c = 0; c < kPcKeys; c += 16) {   // 16 keys: 8 columns a plane
+                            for (int k = 0; k < 16; ++k)
+                                if (!(mk & (1u << k))) zc[k] = 0xff800000u;
+                        }
                         uint32_t p0[8], p1[8], p2[8];
 #pragma unroll
                         for (int k = 0; k < 8; ++k) {
-                            const float2 z = unpack2(add2(pack2(__uint_as_float(s[c + 2 * k]), __uint_as_float(s[c + 2 * k + 1])), m2));
+                            const float2 z = unpack2(add2(pack2(__uint_as_float(zc[2 * k]), __uint_as_float(zc[2 * k + 1])), m2));
                             const float x = ex2(z.x), y = ex2(z.y);
                             sum[k & 1] = add2(sum[k & 1], pack2(x, y));
                             bf16_planes(x, y, &p0[k], &p1[k], &p2[k]);
@@ -745,22 +786,6 @@ paged_chunk_kernel(const __grid_constant__ PcMaps maps, const __grid_constant__ 
                         tmem_st8(to + 16, p2);
                     }
                 } else {
-                    // loops rolled on purpose: what the three roles run between tiles fits the instruction cache
-#pragma unroll 1
-                    for (int c = 0; c < kPcKeys; c += 32) {
-                        uint32_t s[32];
-                        tmem_ld32(sb + c, s);
-                        tmem_wait_ld();
-                        if (edge) {
-                            const uint32_t mk = seen(c);
-#pragma unroll
-                            for (int k = 0; k < 32; ++k)
-                                if (!(mk & (1u << k))) s[k] = 0xff800000u;   // -infinity
-                        }
-#pragma unroll
-                        for (int k = 0; k < 32; ++k) m4[k & 3] = fmaxf(m4[k & 3], __uint_as_float(s[k]));
-                    }
-                    maximum();
                     const uint64_t f2 = pack2(f, f), m2 = pack2(-mref, -mref);
                     const uint64_t minus1 = pack2(-1.f, -1.f);
 #pragma unroll 1
