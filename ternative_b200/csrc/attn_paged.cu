@@ -26,9 +26,9 @@ constexpr int kPrKeys = 8;   // keys a batch
 constexpr int kPrExtra = 4;
 // Rows of a KV head from which a call takes the tensor cores (paged_chunk_kernel):
 // below, its 128-row tiles are too empty.  20/5 heads, 8 sequences of 3000 keys: F16
-// 24 rows 36 against 33 us there, 48 rows 46 against 33; F32 32 rows 127 against
-// 130, 64 rows 237 against 131.
-constexpr int kTensorRows16 = 24, kTensorRows32 = 40;
+// 24 rows 36 against 33 us there, 48 rows 46 against 33; F32 32 rows 126 against
+// 109 (24 rows 95), 64 rows 237 against 110.
+constexpr int kTensorRows16 = 24, kTensorRows32 = 25;
 // Keys up to which a CTA takes whole blocks: sharing tiles evenly costs a second
 // launch.  One token, F16, 400 keys 14.2 against 16.4 us, 800 keys 20.9 against
 // 17.3; 128 sequences of 1000 keys 126 against 79.
