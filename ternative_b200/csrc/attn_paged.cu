@@ -24,11 +24,17 @@ constexpr int kPrKeys = 8;   // keys a batch
 // What starting and leaving a block costs, in tiles.  Decode of 32 sequences: 1, 4, 8
 // take 49.3, 46.1, 49.7 us, of 4 x 61000 keys 103, 100, 101.
 constexpr int kPrExtra = 4;
-// Rows of a KV head from which a call takes the tensor cores (paged_chunk_kernel):
+// Rows of a KV head from which a call may take the tensor cores (paged_chunk_kernel):
 // below, its 128-row tiles are too empty.  20/5 heads, 8 sequences of 3000 keys: F16
-// 24 rows 36 against 33 us there, 48 rows 46 against 33; F32 32 rows 126 against
-// 109 (24 rows 95), 64 rows 237 against 110.
+// 24 rows 36 against 33 us there, 48 rows 46 against 33; F32 24 rows 95 against 100,
+// 32 rows 126 against 109.
 constexpr int kTensorRows16 = 24, kTensorRows32 = 25;
+// ... unless the few-rows kernels' blocks (16 rows, F32 8) are no more than a CTA (two)
+// an SM and short: more CTAs then share what one of 128 rows would do alone.  20/5
+// heads, F32: 64 tokens of one sequence over 300 keys 24 against 35 us, 8 x 7 over 600
+// keys 42 against 55, over 3000 126 against 109, 8 x 16 over 300 42 against 36; F16: 64
+// over 300 12.8 against 18.8, 8 x 7 over 600 21 against 27, 8 x 32 over 300 26 against 17.
+constexpr int kFewSpan = 1024;
 // Keys up to which a CTA takes whole blocks: sharing tiles evenly costs a second
 // launch.  One token, F16, 400 keys 14.2 against 16.4 us, 800 keys 20.9 against
 // 17.3; 128 sequences of 1000 keys 126 against 79.
@@ -652,8 +658,10 @@ extern "C" tvb_status tvb_attention_paged(float* out, int ldo, float* lse, const
     const int64_t rows64 = (int64_t)std::min(a.s.max_new, a.s.n_tokens) * a.group;
     const int rows = (int)std::min<int64_t>(rows64, 1 << 20);
     const bool f16 = kv->dtype == TVB_F16;
-    const bool tensor = rows >= (f16 ? kTensorRows16 : kTensorRows32);
     const int64_t span = window ? std::min<int64_t>(a.s.max_kv, (int64_t)window + a.s.max_new) : a.s.max_kv;
+    const int64_t few = (f16 ? 1 : 2) * num_sms();
+    const int64_t row_blocks = ((int64_t)a.s.n_tokens * a.group / (f16 ? 16 : 8) + a.s.n_seqs) * nkv;
+    const bool tensor = rows >= (f16 ? kTensorRows16 : kTensorRows32) && (row_blocks > few || row_blocks * span > few * kFewSpan);
     // many sequences or row blocks fill the SMs evenly enough block by block
     const int64_t blocks = ((int64_t)a.s.n_tokens * a.group / (tensor ? 128 : 8) + a.s.n_seqs) * nkv;
     // (the schedule's sums are 32 bits; a tile is 48 keys or more)
