@@ -6,9 +6,10 @@
 // pipe at twice the FLOPs of the projection.
 //
 // lora_shrink_tile_kernel (few values of t: lora_shrink_kernel, a CTA four of
-// them): t[m] = scale_a A_a x[m] for 16 rows a CTA.  x and A as
-// TF32 hi + lo planes (any magnitude), three products of mma.sync m16n8k8; 8
-// warps, and the CTAs of a cluster, cut K.  Small next to the projection (rank / N of it).
+// them): t[m] = scale_a A_a x[m] for 16 rows and 32 rank indexes a CTA.  x and A as
+// TF32 hi + lo planes (any magnitude), three products of mma.sync m16n8k8; 8 warps,
+// and the CTAs of a cluster, cut K.  Bound by the latency of its loads: 64 indexes
+// a CTA, two CTAs an SM, made a call of 1400 rows 165 us, these make it 162.
 // lora_gemm_kernel: 128 rows of x by 256 weight rows a tile, tcgen05 fed by TMA.
 // The tensor core truncates as it accumulates (about 2^-26 of the sum an MMA), so
 // four k-blocks (32 MMAs) are summed in TMEM and added to registers by the
@@ -31,7 +32,7 @@ namespace cg = cooperative_groups;
 namespace tvb {
 
 // ---- shrink -----------------------------------------------------------------------
-constexpr int kLtWarps = 8, kLtRows = 16, kLtRanks = 64;
+constexpr int kLtWarps = 8, kLtRows = 16, kLtRanks = 32, kLtPerSm = 3;
 
 __device__ __forceinline__ void mma_tf32(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
     asm volatile(
@@ -68,22 +69,22 @@ __device__ __forceinline__ float4 lora_load4(const void* p, size_t at) {
 }
 
 template <bool F16>
-__global__ void __launch_bounds__(32 * kLtWarps, 2) lora_shrink_tile_kernel(const __grid_constant__ LoraArgs a) {
+__global__ void __launch_bounds__(32 * kLtWarps, kLtPerSm) lora_shrink_tile_kernel(const __grid_constant__ LoraArgs a) {
     extern __shared__ float lt_red[];   // [warp][16 rows][kLtRanks + 1]
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, q = lane & 3;
     cg::cluster_group cl = cg::this_cluster();   // its CTAs cut K
     const int rank = (int)cl.block_rank(), nsplit = (int)cl.num_blocks();
     const int m0 = blockIdx.y * kLtRows;
     int ids[1] = {-1}, rank_of = 0;
-    if (lane < kLtRows && m0 + lane < a.M) ids[0] = lora_of(a, m0 + lane, &rank_of, warp == 0 && rank == 0);
+    if (lane < kLtRows && m0 + lane < a.M) ids[0] = lora_of(a, m0 + lane, &rank_of, warp == 0 && rank == 0 && blockIdx.z == 0);
     if (rank_of == 0) ids[0] = -1;
     const int parts = kLtWarps * nsplit, part = rank * kLtWarps + warp;
     const int steps = ((a.K + 15) / 16 + parts - 1) / parts;   // of 16 k, a warp
     const int s0 = part * steps, s1 = min(s0 + steps, (a.K + 15) / 16);
     for (int ad = next_adapter(ids, -1); ad != 0x7fffffff; ad = next_adapter(ids, ad)) {
-        const int r = __ldg(a.rank + ad);
+        const int r = __ldg(a.rank + ad), j0 = blockIdx.z * kLtRanks;
         const void* A = a.A[ad];
-        for (int j0 = 0; j0 < r; j0 += kLtRanks) {
+        if (j0 < r) {
             const int nt = min(kLtRanks / 8, (r - j0 + 7) / 8);
             float acc[kLtRanks / 8][4] = {};
             // the loads of a step (16 k) ahead of its arithmetic; k permuted so that a thread's fragments are 4
@@ -751,10 +752,11 @@ tvb_status lora_many_rows(LoraArgs a, cudaStream_t st) {
         const auto kernel = a.f16 ? lora_shrink_tile_kernel<true> : lora_shrink_tile_kernel<false>;
         TVB_TRY(allow_smem(reinterpret_cast<const void*>(kernel), smem, set[a.f16]));
         const int rows = (a.M + kLtRows - 1) / kLtRows;
-        int nsplit = 1;   // CTAs that cut K: while two an SM hold them all
-        while (nsplit < 8 && rows * nsplit * 2 <= 2 * num_sms()) nsplit *= 2;
+        const int slices = (a.max_rank + kLtRanks - 1) / kLtRanks;
+        int nsplit = 1;   // CTAs that cut K: while the SMs hold them all
+        while (nsplit < 8 && (int64_t)rows * slices * nsplit * 2 <= kLtPerSm * num_sms()) nsplit *= 2;
         cudaLaunchConfig_t cfg = {};
-        cfg.gridDim = dim3((unsigned)nsplit, (unsigned)rows);
+        cfg.gridDim = dim3((unsigned)nsplit, (unsigned)rows, (unsigned)slices);
         cfg.blockDim = dim3(32 * kLtWarps);
         cfg.dynamicSmemBytes = smem;
         cfg.stream = st;
