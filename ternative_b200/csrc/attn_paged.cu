@@ -287,7 +287,7 @@ __device__ __forceinline__ void rows_piece(const PagedAttnArgs& a, const AttnPie
     merge_warps<HD, RB, St::kWarps>(a, pc, red);
 }
 
-// ---- three to sixteen rows over an F16 cache: mma.sync ------------------------------
+// ---- three rows or more over an F16 cache, 8 or 16 a block: mma.sync ------------------
 // The rows are the 16-row operand of mma.sync m16n8k16 (a memory-bound product: the
 // legacy tensor path keeps up with memory where the FP32 pipe does not, 46 against
 // 62 us for 32 sequences of up to 4096 keys with 20/5 heads).  q and p are split into F16 hi + lo planes, K and V rows

@@ -152,3 +152,8 @@ def test_python_checks():
         LoraTable([z, z], [z], i, i, 4)
     with pytest.raises(ValueError, match="adapter type"):
         LoraTable([z.double()], [z.double()], i, i, 4)
+
+
+def test_lora_long_rows_of_many_are_refused(lib):
+    st, msg = lora(lib, M=257, K=16400)
+    assert st == 1 and b"16384" in msg, msg
