@@ -26,7 +26,7 @@ constexpr int kPrKeys = 8;   // keys a batch
 constexpr int kPrExtra = 4;
 // Rows of a KV head from which a call may take the tensor cores (paged_chunk_kernel):
 // below, its 128-row tiles are too empty.  20/5 heads, 8 sequences of 3000 keys: F16
-// 24 rows 36 against 33 us there, 48 rows 46 against 33; F32 24 rows 95 against 100,
+// 24 rows 36 against 33 us there, 48 rows 46 against 33; F32 24 rows 100 against 109,
 // 32 rows 126 against 109.
 constexpr int kTensorRows16 = 24, kTensorRows32 = 25;
 // ... unless the few-rows kernels' blocks (16 rows, F32 8) are no more than a CTA (two)
