@@ -3,6 +3,7 @@
 #pragma once
 
 #include "common.cuh"
+#include "paged_seq.h"
 
 namespace tvb {
 
@@ -43,22 +44,8 @@ __device__ __forceinline__ int64_t paged_offset(const PagedKV& kv, const int* ta
     return (int64_t)page * kv.page_stride + (int64_t)((uint32_t)t - p * kv.page.d) * kv.row_stride;
 }
 
-// One sequence of the batch: rows [row0, row0 + n) of the token buffers at
-// positions pos0 ... of a cache of kv tokens.
-struct SeqView {
-    int row0, n, kv, pos0;
-    bool ok;
-};
-
 __device__ __forceinline__ SeqView seq_view(const PagedSeqs& s, int b) {
-    SeqView v;
-    v.row0 = __ldg(s.cu + b);
-    const int end = __ldg(s.cu + b + 1);
-    v.n = end - v.row0;
-    v.kv = __ldg(s.kv_len + b);
-    v.pos0 = v.kv - v.n;
-    v.ok = v.row0 >= 0 && end <= s.n_tokens && v.n >= 0 && v.n <= s.max_new && v.kv <= s.max_kv && v.pos0 >= 0;
-    return v;
+    return seq_numbers(__ldg(s.cu + b), __ldg(s.cu + b + 1), __ldg(s.kv_len + b), s.n_tokens, s.max_new, s.max_kv);
 }
 
 __device__ __forceinline__ void report_bad(unsigned* status) {
