@@ -290,8 +290,8 @@ __device__ __forceinline__ void rows_piece(const PagedAttnArgs& a, const AttnPie
 // ---- three rows or more over an F16 cache, 8 or 16 a block: mma.sync ------------------
 // The rows are the 16-row operand of mma.sync m16n8k16 (a memory-bound product: the
 // legacy tensor path keeps up with memory where the FP32 pipe does not, 46 against
-// 62 us for 32 sequences of up to 4096 keys with 20/5 heads).  q and p are split into F16 hi + lo planes, K and V rows
-// come from shared memory by ldmatrix.  Every 16 keys make a fresh product that is
+// 62 us for 32 sequences of up to 4096 keys with 20/5 heads).  q and p (lifted, attn_lift)
+// are split into F16 hi + lo planes, K and V rows come from shared memory by ldmatrix.  Every 16 keys make a fresh product that is
 // added to F32 registers, so the tensor core's truncation does not add up.
 template <int HD, int RB>
 struct PmStage {
@@ -460,7 +460,7 @@ __device__ __forceinline__ void mma_piece(const PagedAttnArgs& a, const AttnPiec
             float mx = fmaxf(fmaxf(v[0], v[1]), fmaxf(v[2], v[3]));
             mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
             mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
-            const float mn = fmaxf(m[h], mx);
+            const float mn = fmaxf(m[h], attn_lift(mx));
             corr[h] = m[h] == mn ? 1.f : exp2f(m[h] - mn);
             m[h] = mn;
             const float ref = mn == -INFINITY ? 0.f : mn;

@@ -261,6 +261,14 @@ __device__ __forceinline__ void pr_load(const unsigned char* p, float (&f)[ND]) 
     }
 }
 
+// F16 planes of probabilities hold nothing below 2^-25: relative to the row's maximum
+// a key 17.4 nats below it would vanish from the output while the sum counted it.  So
+// the tensor-core kernels over F16 caches take powers relative to the maximum less 15:
+// 2^15 at most, 2^-40 of that at least.  (A maximum so large that subtracting rounds
+// stays as it is: neighbouring scores are then further apart than that.)  Sum, values
+// and what they refer to go together, so nothing after them knows.
+__device__ __forceinline__ float attn_lift(float mx) { return fabsf(mx) < 4194304.f ? mx - 15.f : mx; }
+
 // log of the sum of exponentials from the sum l of powers 2^(s - m)
 __device__ __forceinline__ float attn_lse(float l, float m) {
     return l == 0.f ? -INFINITY : (m + log2f(l)) * 0.69314718055994531f;

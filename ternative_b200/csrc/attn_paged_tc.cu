@@ -5,7 +5,7 @@
 // blocks of 128 query rows (new token x query head of the group) of one KV head
 // of one sequence against tiles of 128 keys (64, F32).  Products in F32 accuracy:
 // over an F16 cache q (times scale log2 e, with a power-of-two exponent a row) and
-// p are split into F16 hi + lo planes, K and V are F16 as they are, so every
+// p (relative to the maximum less 15, attn_lift) are split into F16 hi + lo planes, K and V are F16 as they are, so every
 // product takes two MMAs and the bound is the tensor pipe at twice the algorithmic
 // FLOPs; over an F32 cache q, K, p and V are split into three bf16 planes (24 bits
 // at any magnitude) and a product takes six MMAs.
@@ -74,7 +74,7 @@ struct PcShared {
     int gone[4];                // a warp of the pair gave up
     int poison[8];              // [piece % 8] = piece + 1: marked
     float f[128];               // q scale log2 e = (hi + lo) f
-    float m[4][128];            // row maxima that a tile's p refer to
+    float m[4][128];            // what a tile's p refer to, a row
     AttnRun run;
     uint64_t piece_full[4], piece_empty[4];
     AttnPiece piece[4];         // the pieces to come; tiles 0: no more
@@ -735,7 +735,8 @@ paged_chunk_kernel(const __grid_constant__ PcMaps maps, const __grid_constant__ 
                 float m4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
                 float mn, corr, mref;
                 auto maximum = [&]() {
-                    mn = fmaxf(m, fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3])) * f);
+                    const float mx = fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3])) * f;
+                    mn = fmaxf(m, kF32 ? mx : attn_lift(mx));   // (bf16 planes have F32's range)
                     corr = m == mn ? 1.f : ex2(m - mn);
                     mref = mn == -INFINITY ? 0.f : mn;
                 };
@@ -810,12 +811,14 @@ paged_chunk_kernel(const __grid_constant__ PcMaps maps, const __grid_constant__ 
                         }
 #pragma unroll
                         for (int k = 0; k < 8; ++k) sum[k & 1] = add2(sum[k & 1], x[k]);
-                        // hi: the upper 11 bits as they are; lo: the rest, rounded to F16
+                        // hi: rounded to F16; lo: the rest of that, rounded (of the value's upper 11 bits instead, it
+                        // would not make up for what hi loses below 2^-14, always to the same side)
 #pragma unroll
                         for (int k = 0; k < 8; ++k) {
-                            const uint64_t h = x[k] & 0xffffe000ffffe000ull;
-                            const float2 y = unpack2(h), w = unpack2(fma2(h, minus1, x[k]));
-                            const __half2 hi = __floats2half2_rn(y.x, y.y), lo = __floats2half2_rn(w.x, w.y);
+                            const float2 y = unpack2(x[k]);
+                            const __half2 hi = __floats2half2_rn(y.x, y.y);
+                            const float2 h = __half22float2(hi), w = unpack2(fma2(pack2(h.x, h.y), minus1, x[k]));
+                            const __half2 lo = __floats2half2_rn(w.x, w.y);
                             pl[k] = *reinterpret_cast<const uint32_t*>(&hi);
                             pl[8 + k] = *reinterpret_cast<const uint32_t*>(&lo);
                         }
