@@ -50,7 +50,7 @@ __device__ __forceinline__ void rp_store(unsigned char* p, int elem, float4 x, b
 }
 
 __global__ void __launch_bounds__(kRpThreads) rope_append_kernel(const __grid_constant__ RopeArgs a) {
-    __shared__ float2 cs[kRpMaxPairs];
+    __shared__ float4 cs[kRpMaxPairs / 2];   // cosine and sine of pairs 2i, 2i + 1; read 16 bytes at a time
     __shared__ int64_t s_off;   // the token's cache row; -1: skipped
     __shared__ int s_pos;
     const int tid = threadIdx.x, row = blockIdx.x;
@@ -84,7 +84,7 @@ __global__ void __launch_bounds__(kRpThreads) rope_append_kernel(const __grid_co
         const double x = (double)s_pos * a.turns[p];
         float sn, c;
         sincospif(2.0f * (float)(x - rint(x)), &sn, &c);
-        cs[p] = make_float2(c * a.m, sn * a.m);
+        reinterpret_cast<float2*>(cs)[p] = make_float2(c * a.m, sn * a.m);
     }
     __syncthreads();
 
@@ -102,8 +102,7 @@ __global__ void __launch_bounds__(kRpThreads) rope_append_kernel(const __grid_co
         float4 x = *reinterpret_cast<const float4*>(src + o0);
         float4 y = *reinterpret_cast<const float4*>(src + o1);
         if (turn) {
-            const float4 p = *reinterpret_cast<const float4*>(&cs[4 * c]);
-            const float4 r = *reinterpret_cast<const float4*>(&cs[4 * c + 2]);
+            const float4 p = cs[2 * c], r = cs[2 * c + 1];
             // cosines p.x p.z r.x r.z, sines p.y p.w r.y r.w of pairs 4c .. 4c + 3
             if (a.interleaved) {
                 x = make_float4(x.x * p.x - x.y * p.y, x.y * p.x + x.x * p.y, x.z * p.z - x.w * p.w,
