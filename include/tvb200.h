@@ -451,8 +451,9 @@ tvb_status tvb_gguf_close(tvb_gguf* gguf);
  * All buffers are device memory of the current device; lengths, tables and
  * adapter ids are read on the device, so a captured call replays with new ones.
  * What they hold is checked there: a sequence or token whose numbers are out of
- * range is skipped (its output rows stay as they were) and a key on a page out
- * of range is not read; `status` (optional device word, zeroed by the caller)
+ * range is skipped (its output rows stay as they were), so is a sequence that
+ * starts before the end of an earlier one (row starts that go back), and a key on
+ * a page out of range is not read; `status` (optional device word, zeroed by the caller)
  * then gets TVB_DEV_BAD_INPUT, and TVB_DEV_TIMEOUT when a bounded wait gave up.
  * The calls take workspaces from a pool of this library, ordered on `stream`,
  * so calls on different streams and captured graphs never share one. */

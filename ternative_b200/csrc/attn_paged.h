@@ -65,18 +65,30 @@ __device__ __forceinline__ int attn_tiles(const PagedAttnArgs& a, int n, int pos
     return (*k1 - *k0 + TK - 1) / TK;
 }
 
+// Whole warp: no rows for what is not in use.
+static __device__ __noinline__ void attn_drop_unused(const PagedSeqs& s, int* n) {
+    seq_scan(s, [&](int b, const SeqView&, bool used) {
+        if (b < s.n_seqs && !used) n[b] = 0;
+    });
+}
+
 // Whole CTA (NT threads): fills `s` and returns the units of one KV head.
 template <int RB, int TK, int EX, int NT>
 __device__ __forceinline__ int attn_schedule(const PagedAttnArgs& a, AttnSchedule& s, int align) {
     const int tid = threadIdx.x, lane = tid & 31;
+    bool back = false;
     for (int b = tid; b < a.s.n_seqs; b += NT) {
         const SeqView v = seq_view(a.s, b);
         if (!v.ok && blockIdx.x == 0) report_bad(a.status);
         s.row0[b] = v.row0;
-        s.n[b] = v.ok ? v.n : 0;
+        s.n[b] = v.n;
         s.kv[b] = v.kv;
+        back |= v.back;
     }
-    __syncthreads();
+    if (__syncthreads_or(back)) {   // what overlaps an earlier sequence has no rows of its own
+        if (tid < 32) attn_drop_unused(a.s, s.n);
+        __syncthreads();
+    }
     for (int b = tid >> 5; b < a.s.n_seqs; b += NT / 32) {
         const int n = s.n[b], blocks = (n * a.group + RB - 1) / RB;
         int t = 0, x, y, z;
@@ -182,29 +194,53 @@ again:
     return u;
 }
 
+// The first row block of a sequence in an unbalanced grid.
+template <int RB>
+struct AttnFirst {
+    int group;
+    __device__ __forceinline__ int64_t operator()(int b, int row0) const { return ((int64_t)row0 * group) / RB + b; }
+    // block x, at or behind the first, is one of the sequence's
+    __device__ __forceinline__ bool has(const SeqView& v, int b, int x) const {
+        return v.ok && (x - (*this)(b, v.row0)) * RB < (int64_t)v.n * group;
+    }
+};
+
+// Whole CTA: the sequence of a block where starts go back (between the first `next`, or
+// further on), or -1.
+template <int RB, int NT>
+__device__ __noinline__ int attn_odd_block(const PagedAttnArgs& a, int next, bool back) {
+    if (!back && !seq_back<NT>(a.s, next)) return -1;
+    const AttnFirst<RB> first = {a.group};
+    const int x = (int)blockIdx.x, b = seq_last(a.s, x, first);
+    return b >= 0 && first.has(seq_view(a.s, b), b, x) ? b : -1;
+}
+
 // The piece of a CTA of an unbalanced grid: row block blockIdx.x of the batch,
-// whole.  Block floor(cu[b] g / RB) + b is the first of sequence b, so blocks of
-// neighbours never overlap and floor(T g / RB) + n of them are enough.
+// whole.  Block floor(row0 g / RB) + b is the first of sequence b, so blocks of
+// sequences in use never overlap and floor(T g / RB) + n of them are enough.
 template <int RB, int TK, int NT>
 __device__ __forceinline__ bool attn_block(const PagedAttnArgs& a, int align, AttnPiece* p) {
     if ((blockIdx.x | blockIdx.y) == 0) {   // (a sequence that cannot be is no CTA's)
         for (int b = threadIdx.x; b < a.s.n_seqs; b += NT)
             if (!seq_view(a.s, b).ok) report_bad(a.status);
     }
-    int started = 0;
-    for (int b0 = 0; b0 < a.s.n_seqs; b0 += NT) {
-        const int b = b0 + (int)threadIdx.x;
-        const bool at = b < a.s.n_seqs && (int)(((int64_t)__ldg(a.s.cu + b) * a.group) / RB) + b <= (int)blockIdx.x;
-        const int n = __syncthreads_count(at);
-        started += n;
-        if (n < NT) break;
+    const AttnFirst<RB> first = {a.group};
+    const int x = (int)blockIdx.x;
+    int next;
+    bool back;
+    int b = seq_count<NT>(a.s, x, first, &next, &back) - 1;
+    back = __syncthreads_or(back);
+    SeqView v = {};
+    if (b >= 0) v = seq_view(a.s, b);
+    if (!back && v.ok && v.n) {
+        // a later sequence that starts in front of the next one starts before this one's end: it cannot claim the block
+        if (!first.has(v, b, x)) return false;
+    } else {
+        b = attn_odd_block<RB, NT>(a, next, back);
+        if (b < 0) return false;
+        v = seq_view(a.s, b);
     }
-    if (!started) return false;
-    const int b = started - 1;
-    const SeqView v = seq_view(a.s, b);
-    const int i = (int)blockIdx.x - (int)(((int64_t)v.row0 * a.group) / RB) - b;
-    if (!v.ok || i < 0) return false;   // i < 0: starts that go back
-    if ((int64_t)i * RB >= (int64_t)v.n * a.group) return false;
+    const int i = x - (int)first(b, v.row0);
     p->b = b;
     p->tok0 = v.row0;
     p->pos0 = v.pos0;

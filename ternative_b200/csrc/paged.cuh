@@ -48,6 +48,87 @@ __device__ __forceinline__ SeqView seq_view(const PagedSeqs& s, int b) {
     return seq_numbers(__ldg(s.cu + b), __ldg(s.cu + b + 1), __ldg(s.kv_len + b), s.n_tokens, s.max_new, s.max_kv);
 }
 
+// A sequence is in use when its own numbers fit (SeqView::ok) and it starts at or
+// behind the end of every earlier one that has rows and whose numbers fit: rows then
+// belong to one sequence at most.  Where starts never go back the numbers alone
+// decide; else a whole warp walks through the sequences, 32 a turn: f(b, view, in
+// use) with a lane's b, which may lie behind the last.
+template <class F>
+__device__ __forceinline__ void seq_scan(const PagedSeqs& s, F f) {
+    const int lane = threadIdx.x & 31;
+    int ends = 0;   // the largest so far
+    for (int b0 = 0; b0 < s.n_seqs; b0 += 32) {
+        const int b = b0 + lane;
+        SeqView v = {};
+        if (b < s.n_seqs) v = seq_view(s, b);
+        int end = v.n ? v.row0 + v.n : 0;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const int u = __shfl_up_sync(0xffffffffu, end, o);
+            if (lane >= o) end = max(end, u);
+        }
+        const int before = __shfl_up_sync(0xffffffffu, end, 1);
+        f(b, v, v.ok && v.row0 >= (lane ? max(ends, before) : ends));
+        ends = max(ends, __shfl_sync(0xffffffffu, end, 31));
+    }
+}
+
+// Whole warp: the last sequence in use with rows whose key(b, row0) is at most x, or -1.
+template <class F>
+__device__ __noinline__ int seq_last(const PagedSeqs& s, int x, F key) {
+    int last = -1;
+    seq_scan(s, [&](int b, const SeqView& v, bool used) {
+        const unsigned at = __ballot_sync(0xffffffffu, used && v.n && key(b, v.row0) <= x);
+        if (at) last = (b & ~31) + 31 - __clz(at);
+    });
+    return last;
+}
+
+// Whole CTA (NT threads): do starts go back from sequence b0 on?
+template <int NT>
+__device__ __forceinline__ bool seq_back(const PagedSeqs& s, int b0) {
+    bool back = false;
+#pragma unroll 4
+    for (int b = b0 + (int)threadIdx.x; b < s.n_seqs; b += NT) back |= __ldg(s.cu + b + 1) < __ldg(s.cu + b);
+    return __syncthreads_or(back);
+}
+
+// Whole CTA (NT threads): how many sequences have key(b, cu[b]) at or before x, if starts
+// do not go back (keys then do not either).  *next: the first one not looked at; *back:
+// starts go back between those this thread looked at.
+template <int NT, class K>
+__device__ __forceinline__ int seq_count(const PagedSeqs& s, int x, K key, int* next, bool* back) {
+    constexpr int kAhead = 4;   // loads of as many rounds under way: 20,000 sequences of a token 2558 -> 2208 us
+    int started = 0, b0 = 0;
+    *back = false;
+    while (b0 < s.n_seqs) {
+        int row0[kAhead], end[kAhead];
+#pragma unroll
+        for (int i = 0; i < kAhead; ++i) {
+            const int b = b0 + i * NT + (int)threadIdx.x;
+            if (b < s.n_seqs) row0[i] = __ldg(s.cu + b), end[i] = __ldg(s.cu + b + 1);
+        }
+#pragma unroll
+        for (int i = 0; i < kAhead; ++i) {
+            const int b = b0 + (int)threadIdx.x;
+            bool at = false;
+            if (b < s.n_seqs) {
+                at = key(b, row0[i]) <= x;
+                *back |= end[i] < row0[i];
+            }
+            const int n = __syncthreads_count(at);
+            started += n;
+            b0 += NT;
+            if (n < NT) {
+                *next = b0;
+                return started;
+            }
+        }
+    }
+    *next = b0;
+    return started;
+}
+
 __device__ __forceinline__ void report_bad(unsigned* status) {
     if (status) atomicOr(status, TVB_DEV_BAD_INPUT);
 }

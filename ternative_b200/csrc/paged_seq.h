@@ -14,7 +14,8 @@ namespace tvb {
 // kv tokens.
 struct SeqView {
     int row0, n, kv, pos0;
-    bool ok;   // else n and pos0 are 0
+    bool ok;     // else n and pos0 are 0
+    bool back;   // it ends before it starts: starts that go back
 };
 
 // The arrays hold anything: every difference is taken after its operands were
@@ -26,6 +27,7 @@ TVB_HOST_DEVICE SeqView seq_numbers(int row0, int end, int kv, int n_tokens, int
     v.ok = row0 >= 0 && end >= row0 && end <= n_tokens;
     v.n = v.ok ? end - row0 : 0;
     v.ok = v.ok && v.n <= max_new && kv >= v.n && kv <= max_kv;
+    v.back = end < row0;
     if (!v.ok) v.n = 0;
     v.pos0 = v.ok ? kv - v.n : 0;
     return v;

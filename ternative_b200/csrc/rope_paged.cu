@@ -14,6 +14,7 @@
 // in the cache's type.  A CTA takes a token: its cosines and sines go to shared
 // memory once (all heads share them), then every thread moves items of 8
 // dimensions as two float4.
+#include <climits>
 #include <cmath>
 
 #include "paged.cuh"
@@ -49,39 +50,68 @@ __device__ __forceinline__ void rp_store(unsigned char* p, int elem, float4 x, b
     }
 }
 
+// The cache row and position of token `row` if it is sequence b's (one thread).  (Both
+// ends are checked: before starts are known to be in order, b may begin behind the row.)
+__device__ __forceinline__ bool rope_place(const RopeArgs& a, int row, int b, int64_t* off, int* pos) {
+    *off = -1;
+    if (b < 0) return false;
+    const SeqView v = seq_view(a.s, b);
+    if (!v.ok || row < v.row0 || row - v.row0 >= v.n) return false;
+    *pos = v.pos0 + (row - v.row0);
+    *off = paged_offset(a.kv, a.s.table + (size_t)b * a.s.table_ld, *pos);
+    return *off >= 0;
+}
+
+// Whole CTA: a row that is nobody's, or whose page does not exist, or starts that go back.
+__device__ __noinline__ void rope_odd_row(const RopeArgs& a, int row, int64_t* off, int* pos) {
+    const bool back = seq_back<kRpThreads>(a.s, 0);
+    if (back) {
+        const int b = seq_last(a.s, row, [](int, int row0) { return row0; });
+        __syncthreads();
+        if (threadIdx.x == 0) rope_place(a, row, b, off, pos);
+        __syncthreads();
+    }
+    // (a row behind the last sequence is nobody's, and no fault)
+    if (threadIdx.x == 0 && (back || row < __ldg(a.s.cu + a.s.n_seqs))) report_bad(a.status);
+}
+
+// Whole CTA: reports sequences that cannot be; they may have no row of their own to do so.
+__device__ __noinline__ void rope_report(const RopeArgs& a) {
+    for (int b = threadIdx.x; b < a.s.n_seqs; b += kRpThreads)
+        if (!seq_view(a.s, b).ok) report_bad(a.status);
+}
+
 __global__ void __launch_bounds__(kRpThreads) rope_append_kernel(const __grid_constant__ RopeArgs a) {
     __shared__ float4 cs[kRpMaxPairs / 2];   // cosine and sine of pairs 2i, 2i + 1; read 16 bytes at a time
     __shared__ int64_t s_off;   // the token's cache row; -1: skipped
     __shared__ int s_pos;
     const int tid = threadIdx.x, row = blockIdx.x;
 
-    // the token's sequence: how many end at or before it
-    int ended = 0;
-    for (int b0 = 0; b0 < a.s.n_seqs; b0 += kRpThreads) {
-        const int b = b0 + tid;
-        const int n = __syncthreads_count(b < a.s.n_seqs && __ldg(a.s.cu + b + 1) <= row);
+    if (row == a.s.n_tokens) {   // one CTA more
+        if (a.status) rope_report(a);
+        return;
+    }
+    // the token's sequence: how many end at or before it, where starts are in order
+    int ended = 0, next = 0;
+    bool odd = false;   // starts go back, or the row is nobody's
+    for (; next < a.s.n_seqs;) {
+        const int b = next + tid;
+        int row0 = INT_MIN, end = INT_MAX;
+        if (b < a.s.n_seqs) row0 = __ldg(a.s.cu + b), end = __ldg(a.s.cu + b + 1);
+        odd |= end < row0;
+        const int n = __syncthreads_count(end <= row);
         ended += n;
+        next += kRpThreads;
         if (n < kRpThreads) break;
     }
-    if (tid == 0) {
-        int64_t off = -1;
-        int pos = 0;
-        if (ended < a.s.n_seqs) {   // else: behind the last sequence
-            const SeqView v = seq_view(a.s, ended);
-            pos = v.pos0 + (row - v.row0);
-            if (v.ok && row >= v.row0 && row - v.row0 < v.n)
-                off = paged_offset(a.kv, a.s.table + (size_t)ended * a.s.table_ld, pos);
-            if (off < 0) report_bad(a.status);
-        }
-        s_off = off;
-        s_pos = pos;
-    }
-    __syncthreads();
+    if (tid == 0) odd |= !rope_place(a, row, ended < a.s.n_seqs ? ended : -1, &s_off, &s_pos);
+    if (__syncthreads_or(odd)) rope_odd_row(a, row, &s_off, &s_pos);
     const int64_t off = s_off;
     if (off < 0) return;
+    const int pos = s_pos;
     const int pairs = a.rot >> 1;
     for (int p = tid; p < pairs; p += kRpThreads) {
-        const double x = (double)s_pos * a.turns[p];
+        const double x = (double)pos * a.turns[p];
         float sn, c;
         sincospif(2.0f * (float)(x - rint(x)), &sn, &c);
         reinterpret_cast<float2*>(cs)[p] = make_float2(c * a.m, sn * a.m);
@@ -215,6 +245,6 @@ extern "C" tvb_status tvb_rope_append_paged(float* q_out, int ldqo, const float*
     a.status = status;
     a.m = 1.0f;
     if (a.rot) rope_turns(*rope, a.turns, &a.m);
-    rope_append_kernel<<<(unsigned)a.s.n_tokens, kRpThreads, 0, as_stream(stream)>>>(a);
+    rope_append_kernel<<<(unsigned)a.s.n_tokens + 1u, kRpThreads, 0, as_stream(stream)>>>(a);
     return check_launch("rope_append_kernel");
 }
