@@ -537,7 +537,8 @@ tvb_status tvb_rope_append_paged(float* q_out, int ldqo, const float* q, int ldq
  * [n_tokens][n_heads] the natural logarithm of the sum of exponentials; a row
  * that sees no key gets zeros and -infinity.  One token a sequence (decode) and
  * long chunks alike; head_dim 64 or 128.  Values of keys that a row does not
- * see never reach it, whatever they hold. */
+ * see never reach it, whatever they hold; infinities that it does see count as in
+ * the formula (a score of -infinity weighs nothing). */
 tvb_status tvb_attention_paged(float* out, int ldo, float* lse, const float* q, int ldq, const tvb_kv_pages* kv,
                                const tvb_paged_batch* batch, int n_heads, int n_kv_heads, int head_dim, float scale,
                                int window, unsigned* status, void* stream);

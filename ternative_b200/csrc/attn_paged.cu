@@ -90,8 +90,11 @@ __host__ __device__ constexpr int rows_smem() {
     return St::kSmem > St::kWarps * RB * (HD + 2) * 4 ? St::kSmem : St::kWarps * RB * (HD + 2) * 4;
 }
 
-// Joins the warps' sums of a piece: [warp][row][HD + 2], maximum and sum last.
-template <int HD, int RB, int WARPS>
+// Joins the warps' sums of a piece: [warp][row][HD + 2], maximum and sum last.  PLANES:
+// the products were of two planes, where an infinity times the small one (zero, or of
+// the other sign) is NaN: a row that is not finite is computed key by key, unless its
+// query is not (NaN whatever the keys are).
+template <int HD, int RB, int WARPS, bool PLANES>
 __device__ __forceinline__ void merge_warps(const PagedAttnArgs& a, const AttnPiece& pc, const float* red) {
     constexpr int ND = HD / 32, kW = HD + 2;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -110,6 +113,22 @@ __device__ __forceinline__ void merge_warps(const PagedAttnArgs& a, const AttnPi
                 L = fmaf(x[HD + 1], c, L);
 #pragma unroll
                 for (int d = 0; d < ND; ++d) o[d] = fmaf(x[lane * ND + d], c, o[d]);
+            }
+        }
+        if constexpr (PLANES) {
+            bool odd = !(L < INFINITY);
+#pragma unroll
+            for (int d = 0; d < ND; ++d) odd |= !(fabsf(o[d]) < INFINITY);
+            if (__any_sync(0xffffffffu, odd)) {
+                const int t = (int)a.gdiv.div((uint32_t)(pc.row + r));
+                const float* q = a.q + (size_t)(pc.tok0 + t) * a.ldq + (pc.kvh * a.group + pc.row + r - t * a.group) * HD + lane * ND;
+                bool finite = true;
+#pragma unroll
+                for (int d = 0; d < ND; ++d) finite = finite && fabsf(q[d] * a.scale2) < INFINITY;
+                if (__all_sync(0xffffffffu, finite)) {
+                    attn_row_slow<__half, RB, HD>(a, pc, r);
+                    continue;
+                }
             }
         }
         attn_row_store<RB, HD, ND>(a, pc, r, L, M, o);
@@ -284,7 +303,7 @@ __device__ __forceinline__ void rows_piece(const PagedAttnArgs& a, const AttnPie
 #pragma unroll
         for (int d = 0; d < ND; ++d) red[(warp * RB + r) * kW + lane * ND + d] = acc[r][d];
     __syncthreads();
-    merge_warps<HD, RB, St::kWarps>(a, pc, red);
+    merge_warps<HD, RB, St::kWarps, false>(a, pc, red);
 }
 
 // ---- three rows or more over an F16 cache, 8 or 16 a block: mma.sync ------------------
@@ -513,7 +532,7 @@ __device__ __forceinline__ void mma_piece(const PagedAttnArgs& a, const AttnPiec
         if (q == 0) *reinterpret_cast<float2*>(w + HD) = make_float2(m[h], l[h]);
     }
     __syncthreads();
-    merge_warps<HD, RB, St::kWarps>(a, pc, red);
+    merge_warps<HD, RB, St::kWarps, true>(a, pc, red);
 }
 
 template <int HD, int RB>

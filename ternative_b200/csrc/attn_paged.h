@@ -334,7 +334,8 @@ __device__ __forceinline__ void attn_row_store(const PagedAttnArgs& a, const Att
 }
 
 // One row by one warp, key by key: for tiles whose masked values are not finite
-// or whose pages do not exist, which the tensor cores cannot skip.
+// or whose pages do not exist, which the tensor cores cannot skip, and for rows that
+// see something that planes cannot hold.
 template <typename T, int RB, int HD>
 __device__ __noinline__ void attn_row_slow(const PagedAttnArgs& a, const AttnPiece& p, int r) {
     constexpr int ND = HD / 32;

@@ -73,7 +73,7 @@ struct PcShared {
     int slow, slow_done;        // warps that compute rows key by key now; how many have done so
     int gone[4];                // a warp of the pair gave up
     int poison[8];              // [piece % 8] = piece + 1: marked
-    float f[128];               // q scale log2 e = (hi + lo) f
+    float f[128];               // q scale log2 e = (hi + lo) f; NaN where it is not finite
     float m[4][128];            // what a tile's p refer to, a row
     AttnRun run;
     uint64_t piece_full[4], piece_empty[4];
@@ -648,6 +648,7 @@ paged_chunk_kernel(const __grid_constant__ PcMaps maps, const __grid_constant__ 
                     const int qr = warp * 16 + k * kPer + sub;
                     const float4 y = make_float4(x[k].x * a.scale2, x[k].y * a.scale2, x[k].z * a.scale2, x[k].w * a.scale2);
                     int e = 0;
+                    uint32_t mx = 0;
                     unsigned char* dst = smem + Sm::kQ + (d >> 6) * Sm::kQAtom + sw128_offset(qr, (d >> 3) & 7) + (d & 4) * 2;
                     if constexpr (kF32) {
                         uint2 u[3];
@@ -657,8 +658,8 @@ paged_chunk_kernel(const __grid_constant__ PcMaps maps, const __grid_constant__ 
                         for (int pl = 0; pl < 3; ++pl) *reinterpret_cast<uint2*>(dst + pl * Sm::kQPlane) = u[pl];
                     } else {
                         // the largest magnitude by its bits, infinities and NaN apart
-                        uint32_t mx = max(max(__float_as_uint(fabsf(y.x)), __float_as_uint(fabsf(y.y))),
-                                          max(__float_as_uint(fabsf(y.z)), __float_as_uint(fabsf(y.w))));
+                        mx = max(max(__float_as_uint(fabsf(y.x)), __float_as_uint(fabsf(y.y))),
+                                 max(__float_as_uint(fabsf(y.z)), __float_as_uint(fabsf(y.w))));
                         if constexpr (HD == 128) {
                             mx = __reduce_max_sync(0xffffffffu, mx);
                         } else {
@@ -679,7 +680,7 @@ paged_chunk_kernel(const __grid_constant__ PcMaps maps, const __grid_constant__ 
                         *reinterpret_cast<uint2*>(dst) = *reinterpret_cast<const uint2*>(hi);
                         *reinterpret_cast<uint2*>(dst + Sm::kQPlane) = *reinterpret_cast<const uint2*>(lo);
                     }
-                    if (d == 0) sh.f[qr] = __uint_as_float((uint32_t)(127 + e) << 23);
+                    if (d == 0) sh.f[qr] = !kF32 && mx >= 0x7f800000u ? NAN : __uint_as_float((uint32_t)(127 + e) << 23);
                 }
                 fence_proxy_async_smem_cta();
                 warp_arrive(&sh.q_full);
@@ -851,6 +852,8 @@ paged_chunk_kernel(const __grid_constant__ PcMaps maps, const __grid_constant__ 
             m = mo;
             begun = begun || p.slot == 1;
             const bool poisoned = *reinterpret_cast<volatile int*>(&sh.poison[pi & 7]) == pi + 1;
+            const int rows0 = (warp & 3) * 32 + half * 16;   // of the sixteen rows that this warp stores
+            float z = 0.f;   // NaN where something stored is not finite
             if (ok && !poisoned) {
                 // rows through shared memory (the planes of q, all read), so that a warp stores whole rows: chunk c of row
                 // r (16 bytes) at c ^ (r % 32), without bank conflicts either way
@@ -871,19 +874,33 @@ paged_chunk_kernel(const __grid_constant__ PcMaps maps, const __grid_constant__ 
                 const int sub = lane / (HD / 4), c = lane % (HD / 4);
 #pragma unroll 4
                 for (int k = 0; k < 16; k += kPer) {
-                    const int rr = (warp & 3) * 32 + half * 16 + k + sub;
+                    const int rr = rows0 + k + sub;
                     if (rr < p.rows) {
                         const float4 v = *reinterpret_cast<const float4*>(smem + Sm::kQ + rr * (HD * 4) + ((c ^ (rr & (HD / 4 - 1))) * 16));
                         const int rt = (int)a.gdiv.div((uint32_t)(p.row + rr));
                         float* to = p.slot >= 0 ? attn_part<kPcRows, HD>(a, blockIdx.x, p.slot, rr)
                                                 : a.out + (size_t)(p.tok0 + rt) * a.ldo + (p.kvh * a.group + p.row + rr - rt * a.group) * HD;
                         *reinterpret_cast<float4*>(to + c * 4) = v;
+                        if constexpr (!kF32) z = fmaf(v.x, 0.f, fmaf(v.y, 0.f, fmaf(v.z, 0.f, fmaf(v.w, 0.f, z))));
                     }
                 }
             }
-            if (ok && poisoned) {
+            // an infinity times a small plane (zero, or of the other sign) is NaN: rows that are not finite though their
+            // queries are go key by key as well (F32: their tiles were marked)
+            const bool odd = !kF32 && __any_sync(0xffffffffu, z != 0.f);
+            if (ok && (poisoned || odd)) {
                 if (lane == 0) atomicAdd(&sh.slow, 1);
-                for (int k = warp; k < p.rows; k += kPcSoft) attn_row_slow<T, kPcRows, HD>(a, p, k);
+                if (poisoned) {
+                    for (int k = warp; k < p.rows; k += kPcSoft) attn_row_slow<T, kPcRows, HD>(a, p, k);
+                } else {
+#pragma unroll 1
+                    for (int k = rows0; k < min(rows0 + 16, p.rows); ++k) {
+                        bool bad = false;
+                        for (int d = lane; d < HD; d += 32)
+                            bad |= !(fabsf(*reinterpret_cast<const float*>(smem + Sm::kQ + k * (HD * 4) + d * 4)) < INFINITY);
+                        if (__any_sync(0xffffffffu, bad) && sh.f[k] > 0.f) attn_row_slow<T, kPcRows, HD>(a, p, k);
+                    }
+                }
                 if (lane == 0) {
                     atomicAdd(&sh.slow_done, 1);
                     atomicSub(&sh.slow, 1);
