@@ -418,7 +418,7 @@ __device__ __forceinline__ void mma_piece(const PagedAttnArgs& a, const AttnPiec
         mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
         mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
         int e = 0;
-        if (mx > 0.f && mx < INFINITY) e = max(-100, min(100, (int)((__float_as_uint(mx) >> 23) & 255) - 127 - 13));
+        if (mx > 0.f && mx < INFINITY) e = max(-100, min(114, (int)((__float_as_uint(mx) >> 23) & 255) - 127 - 13));
         f[h] = __uint_as_float((uint32_t)(127 + e) << 23);
         const float inv = __uint_as_float((uint32_t)(127 - e) << 23);
 #pragma unroll

@@ -667,7 +667,7 @@ paged_chunk_kernel(const __grid_constant__ PcMaps maps, const __grid_constant__ 
                             for (int o = 8; o > 0; o >>= 1) mx = max(mx, __shfl_xor_sync(0xffffffffu, mx, o));
                         }
                         // 2^e with the largest / 2^e in [2^13, 2^14): both planes of every value that matters are normal F16
-                        if (mx > 0u && mx < 0x7f800000u) e = max(-100, min(100, (int)(mx >> 23) - 127 - 13));
+                        if (mx > 0u && mx < 0x7f800000u) e = max(-100, min(114, (int)(mx >> 23) - 127 - 13));
                         const float g = __uint_as_float((uint32_t)(127 - e) << 23);
                         const float v[4] = {y.x * g, y.y * g, y.z * g, y.w * g};
                         __half2 hi[2], lo[2];

@@ -232,7 +232,7 @@ lora_rows_kernel(const __grid_constant__ LoraArgs a, const __grid_constant__ Lor
             mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
             mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
             int e2 = 0;   // the largest / 2^e2 in [2^13, 2^14)
-            if (mx > 0.f && mx < INFINITY) e2 = max(-100, min(100, (int)((__float_as_uint(mx) >> 23) & 255) - 127 - 13));
+            if (mx > 0.f && mx < INFINITY) e2 = max(-100, min(114, (int)((__float_as_uint(mx) >> 23) & 255) - 127 - 13));
             f[hf] = __uint_as_float((uint32_t)(127 + e2) << 23);
             const float inv = __uint_as_float((uint32_t)(127 - e2) << 23);
 #pragma unroll
