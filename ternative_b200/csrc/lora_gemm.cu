@@ -11,11 +11,12 @@
 // and the CTAs of a cluster, cut K.  Bound by the latency of its loads: 64 indexes
 // a CTA, two CTAs an SM, made a call of 1400 rows 165 us, these make it 162.
 // lora_gemm_kernel: 128 rows of x by 256 weight rows a tile, tcgen05 fed by TMA.
-// The tensor core truncates as it accumulates (about 2^-26 of the sum an MMA), so
-// four k-blocks (32 MMAs) are summed in TMEM and added to registers by the
+// The tensor core truncates to 24 bits as it accumulates (where all products are of
+// one sign, 2^-25.4 of what a chain ends with, an MMA: 6e-7 in 30), so no chain is
+// longer than 32: four k-blocks are summed in TMEM and added to registers by the
 // epilogue warps while the next four go to the other half of TMEM.  After its
-// k-blocks a tile takes one more such product per adapter among its rows: t . B_a
-// as TF32 hi + lo planes (any magnitude, three products), added to that adapter's
+// k-blocks a tile takes one more such product per adapter among its rows (and 80
+// rank indexes): t . B_a as TF32 hi + lo planes (any magnitude, three products), added to that adapter's
 // rows alone, so one request's adapter never touches another's row, whatever it
 // holds (few values of t: lora_expand_kernel does that, behind the join).  Every CTA takes an equal run of the tiles' chunks; a tile that a cut
 // divides leaves F32 partial sums and lora_join_kernel adds them.
@@ -33,6 +34,10 @@ namespace tvb {
 
 // ---- shrink -----------------------------------------------------------------------
 constexpr int kLtWarps = 8, kLtRows = 16, kLtRanks = 32, kLtPerSm = 3;
+// Steps of 16 k (6 products each) that the tensor core sums before the warp's sums in
+// shared memory take them.  In one chain K 16384 lost 2e-5 of an adapter's product (now
+// 1.3e-6); 1400 rows 2560 -> 6912 166.4 -> 168.5 us.
+constexpr int kLtChain = 5;
 
 __device__ __forceinline__ void mma_tf32(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
     asm volatile(
@@ -87,6 +92,17 @@ __global__ void __launch_bounds__(32 * kLtWarps, kLtPerSm) lora_shrink_tile_kern
         if (j0 < r) {
             const int nt = min(kLtRanks / 8, (r - j0 + 7) / 8);
             float acc[kLtRanks / 8][4] = {};
+            float* red = lt_red + warp * kLtRows * (kLtRanks + 1);
+            auto put = [&](bool more) {   // to (more of) this warp's sums
+#pragma unroll
+                for (int n = 0; n < kLtRanks / 8; ++n)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        float* to = red + (g + 8 * (e >> 1)) * (kLtRanks + 1) + n * 8 + 2 * q + (e & 1);
+                        *to = more ? *to + acc[n][e] : acc[n][e];
+                        acc[n][e] = 0.f;
+                    }
+            };
             // the loads of a step (16 k) ahead of its arithmetic; k permuted so that a thread's fragments are 4
             // consecutive k
             float4 x[2], w[kLtRanks / 8];
@@ -103,7 +119,11 @@ __global__ void __launch_bounds__(32 * kLtWarps, kLtPerSm) lora_shrink_tile_kern
             for (int n = 0; n < kLtRanks / 8; ++n)
                 if (n < nt) w[n] = load_w(s0, n);
 #pragma unroll 1
-            for (int s = s0; s < s1; ++s) {
+            for (int s = s0, end = s0 + kLtChain; s < s1; ++s) {
+                if (s == end) {   // what the tensor core has summed goes to F32
+                    put(end > s0 + kLtChain);
+                    end += kLtChain;
+                }
                 uint32_t xh[2][4], xl[2][4];   // [8 k][fragment]
 #pragma unroll
                 for (int h = 0; h < 2; ++h) {
@@ -129,11 +149,7 @@ __global__ void __launch_bounds__(32 * kLtWarps, kLtPerSm) lora_shrink_tile_kern
                     }
                 }
             }
-            float* red = lt_red + warp * kLtRows * (kLtRanks + 1);
-#pragma unroll
-            for (int n = 0; n < kLtRanks / 8; ++n)
-#pragma unroll
-                for (int e = 0; e < 4; ++e) red[(g + 8 * (e >> 1)) * (kLtRanks + 1) + n * 8 + 2 * q + (e & 1)] = acc[n][e];
+            put(s1 - s0 > kLtChain);
             if (nsplit > 1) cl.sync();
             else __syncthreads();
             // the cluster's CTAs share the rows; sums in the order of K
@@ -254,6 +270,10 @@ __device__ __forceinline__ void lg_arrive(uint64_t* bar) {
     asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_u32(bar)) : "memory");
 }
 
+// Steps of 8 rank indexes of an adapter, and how many the tensor core sums (3 products each).
+constexpr int kLgRankSteps = 10;
+__device__ __forceinline__ int lg_steps(const LoraArgs& a, int ad) { return (__ldg(a.rank + ad) + 7) / 8; }
+
 // The adapters of rows [m0, m0 + 128): 4 rows a lane.
 __device__ __forceinline__ void lg_ids(const LoraArgs& a, int m0, int (&ids)[4]) {
     const int lane = threadIdx.x & 31;
@@ -369,25 +389,27 @@ lora_gemm_kernel(const __grid_constant__ LgMaps maps, const __grid_constant__ Lo
                 if (ok && plan.fused && p.c0 == 0) {
                     int ids[4];
                     lg_ids(a, p.m0, ids);
-                    for (int ad = next_adapter(ids, -1); ok && ad != 0x7fffffff; ad = next_adapter(ids, ad), ++chunk) {
-                        const int steps = (__ldg(a.rank + ad) + 7) / 8;
+                    for (int ad = next_adapter(ids, -1); ok && ad != 0x7fffffff; ad = next_adapter(ids, ad)) {
+                        const int steps = lg_steps(a, ad);
                         if (lane == 0) {
-                            const uint32_t d = tmem + (chunk & 1) * kLgCols;
-                            ok = chunk < 2 || mbar_wait_bounded(sh.acc_empty + (chunk & 1), (uint32_t)(((chunk - 2) >> 1) & 1));
                             for (int s = 0; ok && s < steps; ++s) {
-                                ok = mbar_wait_bounded(&sh.l_full, (uint32_t)((ls + s) & 1));
+                                const uint32_t d = tmem + (chunk & 1) * kLgCols;
+                                const bool begin = s % kLgRankSteps == 0;
+                                if (begin) ok = chunk < 2 || mbar_wait_bounded(sh.acc_empty + (chunk & 1), (uint32_t)(((chunk - 2) >> 1) & 1));
+                                ok = ok && mbar_wait_bounded(&sh.l_full, (uint32_t)((ls + s) & 1));
                                 if (!ok) break;
                                 tc_fence_after();
                                 const uint64_t th = sw32_desc(lora_s), tl = th + (kLgRows * 32 >> 4);
                                 const uint64_t bh = th + (2 * kLgRows * 32 >> 4), bl = bh + (kLgCols * 32 >> 4);
-                                tc_mma_tf32(d, th, bh, idesc_l, s ? 1u : 0u);
+                                tc_mma_tf32(d, th, bh, idesc_l, begin ? 0u : 1u);
                                 tc_mma_tf32(d, th, bl, idesc_l, 1u);
                                 tc_mma_tf32(d, tl, bh, idesc_l, 1u);
                                 tc_commit(&sh.l_empty);
+                                if (s + 1 == steps || (s + 1) % kLgRankSteps == 0) tc_commit(sh.acc_full + (chunk++ & 1));
                             }
-                            if (ok) tc_commit(sh.acc_full + (chunk & 1));
                         }
                         ls += steps;
+                        chunk = __shfl_sync(0xffffffffu, chunk, 0);
                         ok = __shfl_sync(0xffffffffu, (int)ok, 0) != 0;
                     }
                 }
@@ -531,7 +553,8 @@ lora_gemm_kernel(const __grid_constant__ LgMaps maps, const __grid_constant__ Lo
                 lg_ids(a, p.m0, ids);
                 const int id = live ? lora_of(a, m, &rank, false) : -1;
 #pragma unroll 1
-                for (int ad = next_adapter(ids, -1); ok && ad != 0x7fffffff; ad = next_adapter(ids, ad)) add(one, ad == id);
+                for (int ad = next_adapter(ids, -1); ok && ad != 0x7fffffff; ad = next_adapter(ids, ad))
+                    for (int left = lg_steps(a, ad); ok && left > 0; left -= kLgRankSteps) add(one, ad == id);
             }
             if (!ok) break;
             if (p.slot >= 0) {

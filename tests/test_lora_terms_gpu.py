@@ -1,4 +1,7 @@
-"""tvb_matmul_lora, one term at a time: the projection of rows up to the largest float."""
+"""tvb_matmul_lora, one term at a time: the adapters' products alone over long rows
+and large ranks, and rows up to the largest float."""
+import math
+
 import pytest
 import torch
 
@@ -23,6 +26,27 @@ def project(be, x, w, A, B, ids):
     y = torch.empty(x.shape[0], w.shape[0], device="cuda")
     be.matmul_lora_d(y, x.cuda(), x.shape[0], x.shape[1], DeviceWeight(dw.data_ptr(), TVB_F16), w.shape[0], table, ids.cuda())
     return y.cpu().double()
+
+
+@pytest.mark.parametrize("M,K,rank", [(5, 16384, 16), (300, 6912, 24), (300, 16384, 250), (520, 6912, 256), (520, 16384, 256),
+                                      (3600, 16384, 32), (520, 64, 256)])
+def test_adapters_of_one_sign(be, M, K, rank):
+    """A zero weight leaves the adapter's term alone; with everything positive, what each step of a sum loses adds up.
+
+    Tensor cores truncate to 24 bits, at most 30 products before the sum goes to F32: together 30 x 2^-26 to 2^-25 of it
+    in each of the two products; the planes 2^-22 each; and 2^-24 at most an addition: K / 640 + 16 of them in the first
+    where a CTA's eight warps cut K, 8 in the second.  (The CUDA-core kernels add K / 2048 + 14 and rank values.)"""
+    g = torch.Generator().manual_seed(M + K)
+    x = torch.rand(M, K, generator=g) + 0.5
+    A = [torch.rand(rank, K, generator=g) + 0.5]
+    B = [torch.rand(40, rank, generator=g) + 0.5]
+    y = project(be, x, torch.zeros(40, K, dtype=F16), A, B, torch.zeros(M, dtype=torch.int32))
+    want = (x.double() @ A[0].double().T) @ B[0].double().T
+    rel = (y - want) / want
+    # what the additions lose is of either sign: their root mean square; the rest in full
+    adds = math.sqrt(K / 640 + 24 + rank) * U
+    assert float(rel.mean().abs()) < 2 * 30 * 2.0 ** -26 + 2 * 2.0 ** -22 + adds, float(rel.mean())
+    assert float(rel.abs().max()) < 2 * 30 * 2.0 ** -25 + 2 * 2.0 ** -22 + 4 * adds, float(rel.abs().max())
 
 
 @pytest.mark.parametrize("M", [1, 12, 40, 300])
