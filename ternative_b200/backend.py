@@ -126,6 +126,7 @@ class PagedCache:
             raise ValueError("k and v must have the same type, shape and strides")
         self.k, self.v = k, v
         n_pages, page_size, self.n_kv_heads, self.head_dim = k.shape
+        self.page_size = page_size
         ps, rs, hs, _ = k.stride()
         self.desc = KvPages(k.data_ptr(), v.data_ptr(), TVB_F32 if k.dtype == torch.float32 else TVB_F16, n_pages,
                             page_size, ps, rs, hs)
@@ -145,7 +146,7 @@ class PagedBatch:
         if cu_tokens.shape[0] != n + 1 or block_table.shape[0] != n:
             raise ValueError(f"{n} lengths, {cu_tokens.shape[0]} row offsets, {block_table.shape[0]} tables")
         self.tensors = (cu_tokens, kv_len, block_table)
-        self.n_tokens = n_tokens
+        self.n_tokens, self.max_kv, self.pages = n_tokens, max_kv, block_table.shape[1]
         self.desc = PagedBatchDesc(n, n_tokens, max_new, max_kv, cu_tokens.data_ptr(), kv_len.data_ptr(),
                                    block_table.data_ptr(), block_table.stride(0) if n > 1 else block_table.shape[1])
         self.address = C.addressof(self.desc)
@@ -197,6 +198,14 @@ class LoraTable:
         self.desc = LoraTableDesc(len(A), max_rank, TVB_F32 if dtype == torch.float32 else TVB_F16,
                                   ptrs[0].data_ptr(), ptrs[1].data_ptr(), rank.data_ptr(), scale.data_ptr())
         self.address = C.addressof(self.desc)
+
+
+def _paged(cache: PagedCache, batch: PagedBatch, n_kv_heads: int, head_dim: int) -> None:
+    """What a cache and a batch have to be to each other and to a call."""
+    if cache.n_kv_heads != n_kv_heads or cache.head_dim != head_dim:
+        raise ValueError(f"a cache of {cache.n_kv_heads} heads of {cache.head_dim}")
+    if batch.max_kv > batch.pages * cache.page_size:   # rows of a slice may be further apart than they are long
+        raise ValueError(f"block_table: {batch.pages} pages of {cache.page_size} tokens a sequence, max_kv {batch.max_kv}")
 
 
 class CUDABackend:
@@ -339,8 +348,7 @@ class CUDABackend:
         (tvb_rope_append_paged).  Token buffers are float32 tensors [rows][heads *
         head_dim] or [rows][heads][head_dim]; rows may be a slice of a wider buffer."""
         import torch
-        if cache.n_kv_heads != n_kv_heads or cache.head_dim != head_dim:
-            raise ValueError(f"a cache of {cache.n_kv_heads} heads of {cache.head_dim}")
+        _paged(cache, batch, n_kv_heads, head_dim)
         T, dev = batch.n_tokens, torch.cuda.current_device()
         _lib.check(self.lib.tvb_rope_append_paged(
             d_q_out.data_ptr(), _rows(d_q_out, "q_out", T, n_heads, head_dim, torch, dev),
@@ -355,8 +363,7 @@ class CUDABackend:
         """Causal attention of the new tokens over the cache (tvb_attention_paged),
         window keys back at most when window > 0; lse: float32 [rows][n_heads]."""
         import torch
-        if cache.n_kv_heads != n_kv_heads or cache.head_dim != head_dim:
-            raise ValueError(f"a cache of {cache.n_kv_heads} heads of {cache.head_dim}")
+        _paged(cache, batch, n_kv_heads, head_dim)
         T, dev = batch.n_tokens, torch.cuda.current_device()
         if lse is not None and lse.shape[-1] != n_heads:
             raise ValueError(f"lse: shape {tuple(lse.shape)} for {n_heads} heads")

@@ -1,0 +1,60 @@
+"""The Python layer's checks of what the paged operators would read or write out of
+range, on the CPU: the library is a recorder and the current device is the CPU's."""
+import pytest
+import torch
+
+import ternative_b200.backend as backend
+from ternative_b200 import CUDABackend, PagedBatch, PagedCache, RopeConfig
+
+
+class Recorder:
+    """Stands in for the library: takes every call."""
+
+    def __init__(self):
+        self.calls = []
+
+    def __getattr__(self, name):
+        def call(*args):
+            self.calls.append(name)
+            return 0
+        return call
+
+
+@pytest.fixture
+def be(monkeypatch):
+    monkeypatch.setattr(backend, "_tensor", lambda x, name, dtype, ndim: x)
+    monkeypatch.setattr(torch.cuda, "current_device", lambda: -1)   # what get_device() says of CPU tensors
+    b = CUDABackend.__new__(CUDABackend)
+    b.lib, b.ctx = Recorder(), None
+    return b
+
+
+def ints(*values):
+    return torch.tensor(values, dtype=torch.int32)
+
+
+def cache(pages=8, page=16):
+    k = torch.zeros(pages, page, 2, 64)
+    return PagedCache(k, torch.zeros_like(k))
+
+
+def both(be, c, b, **kw):
+    """Each of the two calls over a cache."""
+    q, k = torch.zeros(b.n_tokens, 4, 64), torch.zeros(b.n_tokens, 2, 64)
+    yield lambda: be.attention_paged_d(torch.zeros_like(q), q, c, b, 4, 2, 64, 0.125, **kw)
+    yield lambda: be.rope_append_paged_d(torch.zeros_like(q), q, k, k, c, b, RopeConfig(64), 4, 2, 64, **kw)
+
+
+def test_a_table_that_is_a_slice(be):
+    """Rows of a wider table are far enough apart for max_kv, but the slice has not the pages for it: the last row would
+    be read behind its end."""
+    wide = torch.zeros(2, 8, dtype=torch.int32)
+    for pages, max_kv, ok in ((4, 64, True), (4, 65, False), (8, 128, True), (1, 17, False), (1, 16, True)):
+        b = PagedBatch(ints(0, 1, 2), ints(max_kv, max_kv), wide[:, 8 - pages:], 2, 1, max_kv)
+        for call in both(be, cache(), b):
+            if ok:
+                call()
+            else:
+                with pytest.raises(ValueError, match="block_table"):
+                    call()
+    assert len(be.lib.calls) == 6
