@@ -126,7 +126,7 @@ class PagedCache:
             raise ValueError("k and v must have the same type, shape and strides")
         self.k, self.v = k, v
         n_pages, page_size, self.n_kv_heads, self.head_dim = k.shape
-        self.page_size = page_size
+        self.page_size, self.device = page_size, k.get_device()
         ps, rs, hs, _ = k.stride()
         self.desc = KvPages(k.data_ptr(), v.data_ptr(), TVB_F32 if k.dtype == torch.float32 else TVB_F16, n_pages,
                             page_size, ps, rs, hs)
@@ -147,6 +147,7 @@ class PagedBatch:
             raise ValueError(f"{n} lengths, {cu_tokens.shape[0]} row offsets, {block_table.shape[0]} tables")
         self.tensors = (cu_tokens, kv_len, block_table)
         self.n_tokens, self.max_kv, self.pages = n_tokens, max_kv, block_table.shape[1]
+        self.device = kv_len.get_device()
         self.desc = PagedBatchDesc(n, n_tokens, max_new, max_kv, cu_tokens.data_ptr(), kv_len.data_ptr(),
                                    block_table.data_ptr(), block_table.stride(0) if n > 1 else block_table.shape[1])
         self.address = C.addressof(self.desc)
@@ -195,13 +196,16 @@ class LoraTable:
             raise ValueError(f"{len(A)} adapters, {rank.shape[0]} ranks, {scale.shape[0]} scales")
         ptrs = [torch.tensor([t.data_ptr() for t in f], dtype=torch.int64, device=rank.device) for f in (A, B)]
         self.tensors = (list(A), list(B), rank, scale, ptrs)   # kept alive with the descriptor
+        self.device = rank.get_device()
         self.desc = LoraTableDesc(len(A), max_rank, TVB_F32 if dtype == torch.float32 else TVB_F16,
                                   ptrs[0].data_ptr(), ptrs[1].data_ptr(), rank.data_ptr(), scale.data_ptr())
         self.address = C.addressof(self.desc)
 
 
-def _paged(cache: PagedCache, batch: PagedBatch, n_kv_heads: int, head_dim: int) -> None:
+def _paged(cache: PagedCache, batch: PagedBatch, n_kv_heads: int, head_dim: int, device: int) -> None:
     """What a cache and a batch have to be to each other and to a call."""
+    if cache.device != device or batch.device != device:
+        raise ValueError(f"a cache on device {cache.device} and a batch on device {batch.device}, not on the current one ({device})")
     if cache.n_kv_heads != n_kv_heads or cache.head_dim != head_dim:
         raise ValueError(f"a cache of {cache.n_kv_heads} heads of {cache.head_dim}")
     if batch.max_kv > batch.pages * cache.page_size:   # rows of a slice may be further apart than they are long
@@ -348,8 +352,8 @@ class CUDABackend:
         (tvb_rope_append_paged).  Token buffers are float32 tensors [rows][heads *
         head_dim] or [rows][heads][head_dim]; rows may be a slice of a wider buffer."""
         import torch
-        _paged(cache, batch, n_kv_heads, head_dim)
         T, dev = batch.n_tokens, torch.cuda.current_device()
+        _paged(cache, batch, n_kv_heads, head_dim, dev)
         _lib.check(self.lib.tvb_rope_append_paged(
             d_q_out.data_ptr(), _rows(d_q_out, "q_out", T, n_heads, head_dim, torch, dev),
             d_q.data_ptr(), _rows(d_q, "q", T, n_heads, head_dim, torch, dev),
@@ -363,8 +367,8 @@ class CUDABackend:
         """Causal attention of the new tokens over the cache (tvb_attention_paged),
         window keys back at most when window > 0; lse: float32 [rows][n_heads]."""
         import torch
-        _paged(cache, batch, n_kv_heads, head_dim)
         T, dev = batch.n_tokens, torch.cuda.current_device()
+        _paged(cache, batch, n_kv_heads, head_dim, dev)
         if lse is not None and lse.shape[-1] != n_heads:
             raise ValueError(f"lse: shape {tuple(lse.shape)} for {n_heads} heads")
         _lib.check(self.lib.tvb_attention_paged(
@@ -380,6 +384,8 @@ class CUDABackend:
         (tvb_matmul_lora)."""
         import torch
         dev = torch.cuda.current_device()
+        if table.device != dev:
+            raise ValueError(f"adapters on device {table.device}, not on the current one ({dev})")
         if table.K is not None and (table.K != K or table.N != N):
             raise ValueError(f"adapters of a projection {table.K} -> {table.N}, not {K} -> {N}")
         _lib.check(self.lib.tvb_matmul_lora(

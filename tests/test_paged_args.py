@@ -4,7 +4,7 @@ import pytest
 import torch
 
 import ternative_b200.backend as backend
-from ternative_b200 import CUDABackend, PagedBatch, PagedCache, RopeConfig
+from ternative_b200 import CUDABackend, DeviceWeight, LoraTable, PagedBatch, PagedCache, RopeConfig
 
 
 class Recorder:
@@ -45,6 +45,15 @@ def both(be, c, b, **kw):
     yield lambda: be.rope_append_paged_d(torch.zeros_like(q), q, k, k, c, b, RopeConfig(64), 4, 2, 64, **kw)
 
 
+def table(ranks, K=64, N=32, values=None):
+    return LoraTable([torch.zeros(r, K) for r in ranks], [torch.zeros(N, r) for r in ranks],
+                     ints(*(ranks if values is None else values)), torch.ones(len(ranks)), 8)
+
+
+def project(be, t, K=64, N=32, adapter=ints(0, 0), **kw):
+    be.matmul_lora_d(torch.zeros(2, N), torch.zeros(2, K), 2, K, DeviceWeight(4096), N, t, adapter, **kw)
+
+
 def test_a_table_that_is_a_slice(be):
     """Rows of a wider table are far enough apart for max_kv, but the slice has not the pages for it: the last row would
     be read behind its end."""
@@ -58,3 +67,21 @@ def test_a_table_that_is_a_slice(be):
                 with pytest.raises(ValueError, match="block_table"):
                     call()
     assert len(be.lib.calls) == 6
+
+
+def test_descriptors_of_another_device(be, monkeypatch):
+    """A cache, a batch or adapters made on another device than the current one."""
+    b = PagedBatch(ints(0, 1), ints(5), torch.zeros(1, 1, dtype=torch.int32), 1, 1, 5)
+    c, t = cache(), table([4])
+    for call in both(be, c, b):
+        call()
+    project(be, t)
+    done = len(be.lib.calls)
+    for d in (c, b, t):
+        d.device = 3
+        calls = [lambda: project(be, t)] if d is t else list(both(be, c, b))
+        for call in calls:
+            with pytest.raises(ValueError, match="device"):
+                call()
+        d.device = -1
+    assert len(be.lib.calls) == done
