@@ -111,6 +111,18 @@ def _flat(x, name: str, dtype, n: int, device: int) -> int:
     return x.data_ptr()
 
 
+def _status(x, torch, device: int) -> Optional[int]:
+    """Address of a status word: none, a device address, or a tensor of 32 bits or
+    more on the current device."""
+    if x is None or isinstance(x, int):
+        return x
+    if not isinstance(x, torch.Tensor):
+        raise TypeError(f"status: {type(x)!r} (an int32 tensor on the current CUDA device)")
+    if x.get_device() != device or x.numel() * x.element_size() < 4 or x.data_ptr() & 3:
+        raise ValueError(f"status: {x.dtype} on {x.device}, shape {tuple(x.shape)}; want an int32 on the current CUDA device")
+    return x.data_ptr()
+
+
 class PagedCache:
     """One layer's paged KV cache (tvb_kv_pages) over two torch tensors of the
     same type (float32, float16) and strides, indexed [page][row][head][dim];
@@ -359,7 +371,7 @@ class CUDABackend:
             d_q.data_ptr(), _rows(d_q, "q", T, n_heads, head_dim, torch, dev),
             d_k.data_ptr(), _rows(d_k, "k", T, n_kv_heads, head_dim, torch, dev),
             d_v.data_ptr(), _rows(d_v, "v", T, n_kv_heads, head_dim, torch, dev),
-            cache.address, batch.address, rope.address, n_heads, n_kv_heads, head_dim, _ptr(status),
+            cache.address, batch.address, rope.address, n_heads, n_kv_heads, head_dim, _status(status, torch, dev),
             self.stream if stream is None else stream), "tvb_rope_append_paged")
 
     def attention_paged_d(self, d_out, d_q, cache: PagedCache, batch: PagedBatch, n_heads, n_kv_heads, head_dim, scale,
@@ -375,7 +387,7 @@ class CUDABackend:
             d_out.data_ptr(), _rows(d_out, "out", T, n_heads, head_dim, torch, dev),
             None if lse is None else _flat(lse, "lse", torch.float32, T * n_heads, dev),
             d_q.data_ptr(), _rows(d_q, "q", T, n_heads, head_dim, torch, dev),
-            cache.address, batch.address, n_heads, n_kv_heads, head_dim, scale, window, _ptr(status),
+            cache.address, batch.address, n_heads, n_kv_heads, head_dim, scale, window, _status(status, torch, dev),
             self.stream if stream is None else stream), "tvb_attention_paged")
 
     def matmul_lora_d(self, d_y, d_x, M, K, weight: DeviceWeight, N, table: LoraTable, d_adapter, status=None,
@@ -390,7 +402,7 @@ class CUDABackend:
             raise ValueError(f"adapters of a projection {table.K} -> {table.N}, not {K} -> {N}")
         _lib.check(self.lib.tvb_matmul_lora(
             _flat(d_y, "y", torch.float32, M * N, dev), _flat(d_x, "x", torch.float32, M * K, dev), M, K,
-            C.byref(weight.to_c()), N, table.address, _flat(d_adapter, "adapter", torch.int32, M, dev), _ptr(status),
+            C.byref(weight.to_c()), N, table.address, _flat(d_adapter, "adapter", torch.int32, M, dev), _status(status, torch, dev),
             self.stream if stream is None else stream), "tvb_matmul_lora")
 
     # ---- load-time merge (replaces apply_lora, src/model.cpp:205-258) ----------

@@ -85,3 +85,19 @@ def test_descriptors_of_another_device(be, monkeypatch):
                 call()
         d.device = -1
     assert len(be.lib.calls) == done
+
+
+@pytest.mark.parametrize("word", [torch.zeros(8, dtype=torch.uint8)[1:], torch.zeros(1, dtype=torch.int16),
+                                  torch.zeros(0, dtype=torch.int32), torch.zeros(1, dtype=torch.int32).numpy(), "status"],
+                         ids=lambda w: str(getattr(w, "dtype", w)))
+def test_status_words_that_are_none(be, word):
+    """The kernels write 32 bits of device memory."""
+    b = PagedBatch(ints(0, 1), ints(5), torch.zeros(1, 1, dtype=torch.int32), 1, 1, 5)
+    calls = list(both(be, cache(), b, status=word)) + [lambda: project(be, table([4]), status=word)]
+    for call in calls:
+        with pytest.raises((ValueError, TypeError), match="status"):
+            call()
+    assert not be.lib.calls
+    for ok in (None, 4096, ints(0), ints(0, 0)[1:]):
+        for call in list(both(be, cache(), b, status=ok)) + [lambda: project(be, table([4]), status=ok)]:
+            call()
