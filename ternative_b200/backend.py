@@ -183,7 +183,8 @@ class RopeConfig:
 class LoraTable:
     """The adapters of one projection (tvb_lora_table): A [rank][K] and B
     [N][rank] of each, float32 or float16 alike, with their ranks (int32) and
-    scales alpha / rank (float32) as device tensors.  No rank is above max_rank."""
+    scales alpha / rank (float32) as device tensors.  No rank is above max_rank;
+    a rank of 0 switches its adapter off."""
 
     def __init__(self, A: Sequence, B: Sequence, rank, scale, max_rank: int):
         import torch
@@ -206,6 +207,9 @@ class LoraTable:
         _tensor(scale, "scale", "float32", 1)
         if rank.shape[0] != len(A) or scale.shape[0] != len(A):
             raise ValueError(f"{len(A)} adapters, {rank.shape[0]} ranks, {scale.shape[0]} scales")
+        for i, (r, x) in enumerate(zip(rank.tolist(), A)):   # (0: an adapter that adds nothing)
+            if r not in (0, x.shape[0]):
+                raise ValueError(f"adapter {i}: rank {r}, A {tuple(x.shape)}")
         ptrs = [torch.tensor([t.data_ptr() for t in f], dtype=torch.int64, device=rank.device) for f in (A, B)]
         self.tensors = (list(A), list(B), rank, scale, ptrs)   # kept alive with the descriptor
         self.device = rank.get_device()

@@ -101,3 +101,12 @@ def test_status_words_that_are_none(be, word):
     for ok in (None, 4096, ints(0), ints(0, 0)[1:]):
         for call in list(both(be, cache(), b, status=ok)) + [lambda: project(be, table([4]), status=ok)]:
             call()
+
+
+def test_ranks_that_contradict_the_factors(be):
+    """The kernels read rank[i] rows of A[i] and rows of B[i] rank[i] apart."""
+    project(be, table([4, 8]))
+    project(be, table([4, 8], values=[0, 8]))   # an adapter that is switched off
+    for values in ([4, 7], [8, 8], [4, -8], [5, 8]):
+        with pytest.raises(ValueError, match="rank"):
+            table([4, 8], values=values)
