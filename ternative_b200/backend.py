@@ -396,17 +396,20 @@ class CUDABackend:
 
     def matmul_lora_d(self, d_y, d_x, M, K, weight: DeviceWeight, N, table: LoraTable, d_adapter, status=None,
                       stream=None):
-        """y[m] = W x[m] + scale_a B_a A_a x[m], a = adapter[m] (int32, -1: none)
-        (tvb_matmul_lora)."""
+        """y[m] = W x[m] + scale_a B_a A_a x[m], a = adapter[m] (int32, -1: none;
+        None for a table without adapters) (tvb_matmul_lora)."""
         import torch
         dev = torch.cuda.current_device()
         if table.device != dev:
             raise ValueError(f"adapters on device {table.device}, not on the current one ({dev})")
         if table.K is not None and (table.K != K or table.N != N):
             raise ValueError(f"adapters of a projection {table.K} -> {table.N}, not {K} -> {N}")
+        if d_adapter is None and table.K is not None:
+            raise ValueError(f"adapter: none for {M} rows and a table of {len(table.tensors[0])}")
         _lib.check(self.lib.tvb_matmul_lora(
             _flat(d_y, "y", torch.float32, M * N, dev), _flat(d_x, "x", torch.float32, M * K, dev), M, K,
-            C.byref(weight.to_c()), N, table.address, _flat(d_adapter, "adapter", torch.int32, M, dev), _status(status, torch, dev),
+            C.byref(weight.to_c()), N, table.address,
+            None if d_adapter is None else _flat(d_adapter, "adapter", torch.int32, M, dev), _status(status, torch, dev),
             self.stream if stream is None else stream), "tvb_matmul_lora")
 
     # ---- load-time merge (replaces apply_lora, src/model.cpp:205-258) ----------

@@ -110,3 +110,9 @@ def test_ranks_that_contradict_the_factors(be):
     for values in ([4, 7], [8, 8], [4, -8], [5, 8]):
         with pytest.raises(ValueError, match="rank"):
             table([4, 8], values=values)
+
+
+def test_no_adapters_need_no_ids(be):
+    project(be, table([]), adapter=None)
+    with pytest.raises(ValueError, match="adapter"):
+        project(be, table([4]), adapter=None)
