@@ -485,7 +485,7 @@ typedef struct {
     int n_seqs;
     int n_tokens;            /* rows of the token buffers */
     int max_new;             /* no sequence brings more new tokens */
-    int max_kv;              /* no sequence is longer */
+    int max_kv;              /* no sequence is longer; at most 2^30 */
     const int* cu_tokens;    /* device [n_seqs + 1] */
     const int* kv_len;       /* device [n_seqs] */
     const int* block_table;  /* device [n_seqs][table_ld] */

@@ -32,6 +32,8 @@ tvb_status paged_batch_arg(const char* who, const tvb_paged_batch* b, const tvb_
     TVB_REQUIRE(b->n_seqs == 0 || (b->cu_tokens && b->kv_len && b->block_table), "%s: null batch pointer", who);
     TVB_REQUIRE(b->n_seqs <= 65535, "%s: %d sequences (at most 65535)", who, b->n_seqs);
     TVB_REQUIRE(b->max_new >= 0 && b->max_kv >= 0, "%s: max_new %d, max_kv %d", who, b->max_new, b->max_kv);
+    // a kernel's last step ends behind the longest sequence: positions stay in 32 bits
+    TVB_REQUIRE(b->max_kv <= 1 << 30, "%s: max_kv %d (at most 2^30)", who, b->max_kv);
     TVB_REQUIRE(b->n_seqs == 0 || (int64_t)b->table_ld * kv->page_size >= b->max_kv,
                 "%s: block_table rows of %d pages of %d tokens do not hold max_kv %d", who, b->table_ld, kv->page_size,
                 b->max_kv);
