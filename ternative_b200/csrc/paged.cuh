@@ -137,8 +137,8 @@ __device__ __forceinline__ void report_bad(unsigned* status) {
 tvb_status paged_cache_arg(const char* who, const tvb_kv_pages* kv, int n_kv_heads, int head_dim, PagedKV* out);
 tvb_status paged_batch_arg(const char* who, const tvb_paged_batch* b, const tvb_kv_pages* kv, PagedSeqs* out);
 
-// A workspace of this call on `st`, from a pool of the library that keeps its
-// memory between calls (the driver orders reuse across streams; inside a
+// A workspace of this call on `st`, from a pool of the library that keeps some of
+// its memory between calls (the driver orders reuse across streams; inside a
 // capture it becomes the graph's own).  Freed on `st` when it goes out of scope,
 // after the kernels launched until then.
 class Workspace {
