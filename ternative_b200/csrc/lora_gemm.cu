@@ -36,7 +36,7 @@ namespace tvb {
 constexpr int kLtWarps = 8, kLtRows = 16, kLtRanks = 32, kLtPerSm = 3;
 // Steps of 16 k (6 products each) that the tensor core sums before the warp's sums in
 // shared memory take them.  In one chain K 16384 lost 2e-5 of an adapter's product (now
-// 1.3e-6); 1400 rows 2560 -> 6912 166.4 -> 168.5 us.
+// 1.3e-6); 1400 rows 2560 -> 6912 162.7 -> 164.1 us.
 constexpr int kLtChain = 5;
 
 __device__ __forceinline__ void mma_tf32(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
@@ -91,18 +91,6 @@ __global__ void __launch_bounds__(32 * kLtWarps, kLtPerSm) lora_shrink_tile_kern
         const void* A = a.A[ad];
         if (j0 < r) {
             const int nt = min(kLtRanks / 8, (r - j0 + 7) / 8);
-            float acc[kLtRanks / 8][4] = {};
-            float* red = lt_red + warp * kLtRows * (kLtRanks + 1);
-            auto put = [&](bool more) {   // to (more of) this warp's sums
-#pragma unroll
-                for (int n = 0; n < kLtRanks / 8; ++n)
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) {
-                        float* to = red + (g + 8 * (e >> 1)) * (kLtRanks + 1) + n * 8 + 2 * q + (e & 1);
-                        *to = more ? *to + acc[n][e] : acc[n][e];
-                        acc[n][e] = 0.f;
-                    }
-            };
             // the loads of a step (16 k) ahead of its arithmetic; k permuted so that a thread's fragments are 4
             // consecutive k
             float4 x[2], w[kLtRanks / 8];
@@ -118,38 +106,48 @@ __global__ void __launch_bounds__(32 * kLtWarps, kLtPerSm) lora_shrink_tile_kern
 #pragma unroll
             for (int n = 0; n < kLtRanks / 8; ++n)
                 if (n < nt) w[n] = load_w(s0, n);
+            float* red = lt_red + warp * kLtRows * (kLtRanks + 1);
+            int c = s0;
 #pragma unroll 1
-            for (int s = s0, end = s0 + kLtChain; s < s1; ++s) {
-                if (s == end) {   // what the tensor core has summed goes to F32
-                    put(end > s0 + kLtChain);
-                    end += kLtChain;
-                }
-                uint32_t xh[2][4], xl[2][4];   // [8 k][fragment]
+            do {
+                float acc[kLtRanks / 8][4] = {};
+#pragma unroll 1
+                for (int s = c; s < min(c + kLtChain, s1); ++s) {
+                    uint32_t xh[2][4], xl[2][4];   // [8 k][fragment]
 #pragma unroll
-                for (int h = 0; h < 2; ++h) {
-                    const float v[4] = {x[h].x, x[h].y, x[h].z, x[h].w};
+                    for (int h = 0; h < 2; ++h) {
+                        const float v[4] = {x[h].x, x[h].y, x[h].z, x[h].w};
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) tf32_planes(v[e], &xh[e >> 1][h + 2 * (e & 1)], &xl[e >> 1][h + 2 * (e & 1)]);
-                    x[h] = load_x(s + 1, h);
-                }
+                        for (int e = 0; e < 4; ++e) tf32_planes(v[e], &xh[e >> 1][h + 2 * (e & 1)], &xl[e >> 1][h + 2 * (e & 1)]);
+                        x[h] = load_x(s + 1, h);
+                    }
 #pragma unroll
-                for (int n = 0; n < kLtRanks / 8; ++n) {
-                    if (n < nt) {
-                        const float v[4] = {w[n].x, w[n].y, w[n].z, w[n].w};
-                        uint32_t wh[4], wl[4];
+                    for (int n = 0; n < kLtRanks / 8; ++n) {
+                        if (n < nt) {
+                            const float v[4] = {w[n].x, w[n].y, w[n].z, w[n].w};
+                            uint32_t wh[4], wl[4];
 #pragma unroll
-                        for (int e = 0; e < 4; ++e) tf32_planes(v[e], &wh[e], &wl[e]);
-                        w[n] = load_w(s + 1, n);
+                            for (int e = 0; e < 4; ++e) tf32_planes(v[e], &wh[e], &wl[e]);
+                            w[n] = load_w(s + 1, n);
 #pragma unroll
-                        for (int i = 0; i < 2; ++i) {
-                            mma_tf32(acc[n], xl[i], wh[2 * i], wh[2 * i + 1]);
-                            mma_tf32(acc[n], xh[i], wl[2 * i], wl[2 * i + 1]);
-                            mma_tf32(acc[n], xh[i], wh[2 * i], wh[2 * i + 1]);
+                            for (int i = 0; i < 2; ++i) {
+                                mma_tf32(acc[n], xl[i], wh[2 * i], wh[2 * i + 1]);
+                                mma_tf32(acc[n], xh[i], wl[2 * i], wl[2 * i + 1]);
+                                mma_tf32(acc[n], xh[i], wh[2 * i], wh[2 * i + 1]);
+                            }
                         }
                     }
                 }
-            }
-            put(s1 - s0 > kLtChain);
+                // to this warp's sums
+#pragma unroll
+                for (int n = 0; n < kLtRanks / 8; ++n)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        float* to = red + (g + 8 * (e >> 1)) * (kLtRanks + 1) + n * 8 + 2 * q + (e & 1);
+                        *to = c > s0 ? *to + acc[n][e] : acc[n][e];
+                    }
+                c += kLtChain;
+            } while (c < s1);
             if (nsplit > 1) cl.sync();
             else __syncthreads();
             // the cluster's CTAs share the rows; sums in the order of K
