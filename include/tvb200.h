@@ -454,7 +454,8 @@ tvb_status tvb_gguf_close(tvb_gguf* gguf);
  * range is skipped (its output rows stay as they were), so is a sequence that
  * starts before the end of an earlier one (row starts that go back), and a key on
  * a page out of range is not read; `status` (optional device word, zeroed by the caller)
- * then gets TVB_DEV_BAD_INPUT, and TVB_DEV_TIMEOUT when a bounded wait gave up.
+ * then gets TVB_DEV_BAD_INPUT, and TVB_DEV_TIMEOUT when a bounded wait gave up:
+ * what that left unfinished is NaN, with or without a status word.
  * The calls take workspaces from a pool of this library, ordered on `stream`,
  * so calls on different streams and captured graphs never share one. */
 #define TVB_DEV_TIMEOUT 1u

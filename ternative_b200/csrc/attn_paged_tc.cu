@@ -216,6 +216,33 @@ __device__ __noinline__ void pc_rows_slow(const PagedAttnArgs& a, const AttnPiec
     }
 }
 
+// One warp, when a wait gave up: every row of the CTA's run is NaN.
+template <typename T, int HD>
+__device__ __noinline__ void pc_give_up(const PagedAttnArgs& a, const AttnSchedule& sched, const AttnRun& run, AttnPiece* piece,
+                                        int align) {
+    constexpr int ND = HD / 32;
+    float o[ND];
+#pragma unroll
+    for (int d = 0; d < ND; ++d) o[d] = NAN;
+    auto rows = [&](const AttnPiece& p) {
+        for (int r = 0; r < p.rows; ++r) attn_row_store<kPcRows, HD, ND>(a, p, r, NAN, -INFINITY, o);
+    };
+    if (!a.balanced) {
+        rows(*piece);   // the only one
+        return;
+    }
+    bool begun = false;
+    for (int64_t at = run.u; (at = attn_next<kPcRows, PcType<T>::kKeys, kPcExtra>(a, sched, run, at, align, piece)) != 0;) {
+        rows(*piece);
+        if (piece->slot == 1) {
+            begun = true;
+            if ((threadIdx.x & 31) == 0) attn_header(a, piece);
+        }
+        __syncwarp();
+    }
+    if (!begun && (threadIdx.x & 31) == 0) attn_header(a, nullptr);
+}
+
 template <typename T, int HD>
 __global__ void __launch_bounds__(PcType<T>::kThreads, 1)
 paged_chunk_kernel(const __grid_constant__ PcMaps maps, const __grid_constant__ PagedAttnArgs a, int box) {
@@ -931,6 +958,7 @@ paged_chunk_kernel(const __grid_constant__ PcMaps maps, const __grid_constant__ 
         tc_fence_after();
         tmem_dealloc(tmem, 512);
     }
+    if (warp == 0 && *abort_flag) pc_give_up<T, HD>(a, sched, sh.run, sh.piece, align);
 }
 
 // Pool as a tensor map, or false where its strides do not make one.

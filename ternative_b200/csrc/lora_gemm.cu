@@ -506,7 +506,7 @@ lora_gemm_kernel(const __grid_constant__ LgMaps maps, const __grid_constant__ Lo
         const uint32_t lanes = tmem + ((uint32_t)(32 * (warp & 3)) << 16) + half * 128;
         int chunk = 0;
         bool ok = true;
-        while (ok && lg_next(plan, &u, end, &p)) {
+        while (lg_next(plan, &u, end, &p)) {   // (after a wait that gave up: NaN)
             const int m = p.m0 + r;
             const bool live = m < a.M;
             const float f = live ? ldexpf(1.0f, __ldg(plan.row_exp + m)) : 0.f;
@@ -554,7 +554,10 @@ lora_gemm_kernel(const __grid_constant__ LgMaps maps, const __grid_constant__ Lo
                 for (int ad = next_adapter(ids, -1); ok && ad != 0x7fffffff; ad = next_adapter(ids, ad))
                     for (int left = lg_steps(a, ad); ok && left > 0; left -= kLgRankSteps) add(one, ad == id);
             }
-            if (!ok) break;
+            if (!ok) {
+#pragma unroll
+                for (int i = 0; i < 64; ++i) acc[i] = lg_pack2(NAN, NAN);
+            }
             if (p.slot >= 0) {
                 float* to = plan.part + ((size_t)(blockIdx.x * 2 + p.slot) * kLgRows + r) * kLgCols + half * 128;
 #pragma unroll
