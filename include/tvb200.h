@@ -561,7 +561,9 @@ typedef struct {
 /* tvb_matmul with an adapter for each row: y[m] = W x[m] + scale_a B_a A_a x[m],
  * a = adapter[m] (device [M]; -1: none).  K is a multiple of 8 (16 for INT8
  * weights) and at most 16384 above 256 rows, M at most 65535; x and y rows are
- * contiguous, x, W 16-byte aligned. */
+ * contiguous, x, W 16-byte aligned.  What an infinity or NaN in x[m] or a row of W
+ * reaches is not finite (either of them, products are of two planes), and no other
+ * row of y or column. */
 tvb_status tvb_matmul_lora(float* y, const float* x, int M, int K, const tvb_weight* w, int N,
                            const tvb_lora_table* table, const int* adapter, unsigned* status, void* stream);
 
