@@ -61,3 +61,25 @@ def test_rows_up_to_the_largest_float(be, M, size):
     tol = (x.double().abs() @ w.double().abs().T) * ((512 + 4) * U + 2.0 ** -21) + 512 * 2.0 ** -140
     assert torch.isfinite(y).all()
     assert ((y - want).abs() <= tol).all()
+
+
+@pytest.mark.parametrize("M", [1, 12, 40, 300])
+@pytest.mark.parametrize("bad", [math.inf, -math.inf, math.nan])
+def test_what_is_not_finite_reaches_its_own_row_and_column(be, M, bad):
+    g = torch.Generator().manual_seed(M)
+    x = torch.randn(M, 512, generator=g)
+    w = (torch.randn(96, 512, generator=g) * 0.02).half()
+    A, B = [torch.randn(4, 512, generator=g)], [torch.randn(96, 4, generator=g)]
+    ids = torch.zeros(M, dtype=torch.int32)
+    want = project(be, x, w, A, B, ids)
+    xb, wb = x.clone(), w.clone()
+    xb[M // 2, 77] = bad
+    wb[50, 300] = bad
+    y = project(be, xb, w, A, B, ids)
+    assert not torch.isfinite(y[M // 2]).any()
+    rest = [m for m in range(M) if m != M // 2]
+    assert torch.equal(y[rest], want[rest])
+    y = project(be, x, wb, A, B, ids)
+    assert not torch.isfinite(y[:, 50]).any()
+    rest = [n for n in range(96) if n != 50]
+    assert torch.equal(y[:, rest], want[:, rest])
